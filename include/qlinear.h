@@ -337,6 +337,117 @@ int ql_allgather_f16(const void* src, int64_t lds, void* out, int64_t ldo, int64
                      int64_t block, int rank, int world, int max_m, void* const* peers, unsigned flags,
                      void* stream);
 
+/* ------------------------------------------------------------ rotary positions */
+/* The four entry points below take their arguments in a structure of 8-byte
+ * fields.  x, k, v and q are 16-bit tensors [tokens][heads][head_dim] with
+ * strides in elements and unit inner stride, so that the column slices of a
+ * fused projection's output go in as they are.  No counterpart of the
+ * reference's quantized linears: they sit between qkv_proj and o_proj
+ * (src/engine/paged_engine.py:98-146). */
+#define QL_ROTARY_HALF         0   /* pair i = elements i and i + rotary_dim / 2 */
+#define QL_ROTARY_INTERLEAVED  1   /* pair i = elements 2i and 2i + 1            */
+/*
+ * out[t, h] = x[t, h] with its first rotary_dim elements turned by the angles
+ * of positions[t]; out may be x.  table fp32 [max_positions][rotary_dim / 2][2]
+ * holds each pair's cosine and sine (and any factor on both).  rotary_dim is
+ * a multiple of 8, head_dim too.  inverse != 0 turns back (the direction of
+ * the gradient).  A position outside the table takes its nearest row and
+ * records QL_DEVICE_ERROR_BAD_INDEX.
+ */
+typedef struct {
+  const void* x;
+  void* out;
+  const void* table;
+  const void* positions;                 /* int32 or int64 [tokens] */
+  int64_t tokens, heads, head_dim, rotary_dim, max_positions;
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  int64_t dtype, layout, position_bytes, inverse, flags;
+} ql_rotary_args;
+int ql_rotary(const ql_rotary_args* args, void* stream);
+
+/* ------------------------------------------------- quantised paged key/value cache */
+/* One row = one token of one key/value head: codes [head_dim * bits / 8 bytes]
+ * and a bf16 scale per group (bits 8: the row; bits 4: 64 elements),
+ *   scale = bf16(max|x| * (1 / top)),  code = clamp(rne(x / scale), -top, top)
+ * with top 127 or 7, computed in fp32.  8-bit codes are int8; 4-bit codes are
+ * stored + 8, two to a byte, the even element in the low nibble.  A group of
+ * zeros reads back as zeros, one with an infinity or NaN as NaN.
+ *   codes  [num_pages][kv_heads][page_size][row bytes]
+ *   scales [num_pages][kv_heads][page_size][groups]
+ * contiguous within a page; page strides in bytes (codes) and elements
+ * (scales).  page_size is a power of two from 16 to 65536; head_dim is 64,
+ * 128 or 256.  Token t of page p is slot p * page_size + t.  Pointers and page
+ * strides are multiples of 16 bytes. */
+typedef struct {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int64_t num_pages, page_size, kv_heads, head_dim, bits;
+  int64_t k_page_stride, v_page_stride, k_scale_page_stride, v_scale_page_stride;
+} ql_kv_cache;
+/*
+ * Writes k[t, h] and v[t, h] to slot slots[t] of every head.  With rotary_dim
+ * > 0, k is turned first (in fp32, unrounded) and, with q_heads > 0, q is
+ * turned into q_out (which may be q).  A slot of -1 (any negative) writes
+ * nothing, but its q is turned; one past the pool writes nothing and records
+ * QL_DEVICE_ERROR_BAD_INDEX.  Two tokens with one slot leave either's row or
+ * a mixture of both.
+ */
+typedef struct {
+  ql_kv_cache cache;
+  const void *k, *v, *q;
+  void* q_out;
+  const void* slots;                     /* int32 or int64 [tokens] */
+  const void* table;
+  const void* positions;
+  int64_t tokens, q_heads;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+  int64_t dtype, slot_bytes, rotary_dim, max_positions, layout, position_bytes, flags;
+} ql_kv_append_args;
+int ql_kv_append(const ql_kv_append_args* args, void* stream);
+/*
+ * k[t, h], v[t, h] = the values at slots[t], rounded once to dtype, into
+ * contiguous 16-byte aligned [tokens][kv_heads][head_dim]; zeros where the
+ * slot is negative, or past the pool (recorded as above).
+ */
+typedef struct {
+  ql_kv_cache cache;
+  const void* slots;
+  void *k, *v;
+  int64_t tokens, dtype, slot_bytes, flags;
+} ql_kv_read_args;
+int ql_kv_read(const ql_kv_read_args* args, void* stream);
+
+/* ------------------------------------------------ attention over the cache */
+/*
+ * out[i, h] = sum_j softmax_j(scale * q[i, h] . k_j) v_j over the cached
+ * positions j of i's request that row i sees, for the new tokens of `batch`
+ * requests: request b has the rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q NULL:
+ * total_q / batch each).  Its keys are positions 0 .. kv_lens[b] - 1, position
+ * j in page page_table[b][j / page_size]; its own new tokens are the last of
+ * them and already written.  Row i sees every position before the new tokens
+ * and, of those, new token d when d <= i (mask NULL) or when bit d of mask
+ * row i (mask_words 64-bit words, bit d % 64 of word d / 64) is set; bits past
+ * the mask's words count as clear.  A row that sees nothing gives zeros and
+ * lse -inf.  lse[i, h] (optional, fp32) = log of the softmax's denominator.
+ * Rows that cu_q does not cover are not written.  kv_lens is clamped to the
+ * table; a page outside the pool hides its keys and records
+ * QL_DEVICE_ERROR_BAD_INDEX.  max_q and max_kv bound the requests' tokens and
+ * lengths and only choose the launch.
+ * q_heads is a multiple of kv_heads; query head h reads key/value head
+ * h / (q_heads / kv_heads).
+ */
+typedef struct {
+  ql_kv_cache cache;
+  const void* q;
+  void *out, *lse;
+  const void *page_table, *kv_lens, *cu_q, *mask;
+  int64_t batch, total_q, q_heads, q_token_stride, q_head_stride;
+  int64_t table_width, table_stride, mask_words, max_q, max_kv, dtype;
+  double scale;
+  int64_t flags;
+} ql_tree_attention_args;
+int ql_tree_attention(const ql_tree_attention_args* args, void* stream);
+
 /* ------------------------------------------------------------- diagnostics */
 const char* ql_strerror(int status);
 /* Version as (major << 16) | (minor << 8) | patch. */
@@ -347,6 +458,7 @@ int ql_version(void);
 #define QL_DEVICE_ERROR_MMA_WAIT    3   /* a tensor-core completion wait ran out          */
 #define QL_DEVICE_ERROR_TMEM        4   /* tensor-memory allocation failed                */
 #define QL_DEVICE_ERROR_PEER_WAIT   5   /* another rank's keys / columns never arrived    */
+#define QL_DEVICE_ERROR_BAD_INDEX   6   /* a position, slot or page outside its table      */
 /* Kernels never trap: a bounded wait that runs out records a code in a
  * device-global word, and the kernel lets its copies in flight land and
  * returns early.  These read (and clear)

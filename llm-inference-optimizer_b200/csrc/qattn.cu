@@ -1,0 +1,265 @@
+// qattn.cu — C ABI of the attention side of libqlinear.so (declared in
+// include/qlinear.h): rotary positions, the quantised paged cache and
+// attention over it.  Argument checks, variant choice and launches; every
+// entry point returns a status and allocates nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "../../include/qlinear.h"
+#include "ql_host.h"
+#include "qattend.cuh"
+#include "qcache.cuh"
+
+namespace {
+
+using ql::kvc::Pool;
+using ql::kvc::Rows;
+using ql::kvc::Turn;
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+template <typename Kern, typename... Args>
+int launch(Kern kernel, dim3 grid, dim3 block, size_t smem, void* stream, int64_t flags, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = (flags & QL_FLAG_PDL) ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return QL_ERR_CUDA;
+  }
+  return QL_OK;
+}
+
+bool act_dtype(int64_t d) { return d == QL_DTYPE_F16 || d == QL_DTYPE_BF16; }
+bool index_bytes(int64_t n) { return n == 4 || n == 8; }
+
+// A [tokens][heads][head_dim] tensor of 16-bit elements.
+int make_rows(Rows* r, const void* p, int64_t token_stride, int64_t head_stride, int64_t head_dim) {
+  if (!p) return QL_ERR_NULL_POINTER;
+  if (!aligned(p, 2)) return QL_ERR_UNSUPPORTED;
+  if (token_stride < 0 || head_stride < 0) return QL_ERR_BAD_STRIDE;
+  r->p = p;
+  r->token_stride = token_stride;
+  r->head_stride = head_stride;
+  r->vec = aligned(p, 16) && token_stride % 8 == 0 && head_stride % 8 == 0 && head_dim % 8 == 0;
+  return QL_OK;
+}
+
+int make_turn(Turn* t, const void* table, const void* positions, int64_t position_bytes, int64_t max_positions,
+              int64_t rotary_dim, int64_t head_dim, int64_t layout, int64_t inverse) {
+  if (rotary_dim <= 0 || rotary_dim % 8 != 0 || rotary_dim > head_dim || max_positions <= 0)
+    return QL_ERR_BAD_SHAPE;
+  if (!table || !positions) return QL_ERR_NULL_POINTER;
+  if (!index_bytes(position_bytes) || !aligned(table, 16) || !aligned(positions, (size_t)position_bytes) ||
+      (layout != QL_ROTARY_HALF && layout != QL_ROTARY_INTERLEAVED))
+    return QL_ERR_UNSUPPORTED;
+  t->table = static_cast<const float2*>(table);
+  t->positions = positions;
+  t->max_positions = max_positions;
+  t->wide = position_bytes == 8;
+  t->rotary_dim = (int)rotary_dim;
+  t->interleaved = layout == QL_ROTARY_INTERLEAVED;
+  t->inverse = inverse != 0;
+  return QL_OK;
+}
+
+int make_pool(Pool* c, const ql_kv_cache& a) {
+  if (!a.k_codes || !a.k_scales || !a.v_codes || !a.v_scales) return QL_ERR_NULL_POINTER;
+  if (a.bits != 8 && a.bits != 4) return QL_ERR_UNSUPPORTED;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return QL_ERR_UNSUPPORTED;
+  if (a.page_size < 16 || a.page_size > 65536 || (a.page_size & (a.page_size - 1)) != 0) return QL_ERR_UNSUPPORTED;
+  if (a.num_pages <= 0 || a.kv_heads <= 0 || a.num_pages > INT_MAX || a.kv_heads > 65536 ||
+      a.kv_heads * a.page_size > INT_MAX)
+    return QL_ERR_BAD_SHAPE;
+  const int64_t row = a.head_dim * a.bits / 8, groups = a.bits == 8 ? 1 : a.head_dim / ql::kvc::kGroup4;
+  const int64_t rows = a.kv_heads * a.page_size;
+  if (a.k_page_stride < rows * row || a.v_page_stride < rows * row || a.k_scale_page_stride < rows * groups ||
+      a.v_scale_page_stride < rows * groups)
+    return QL_ERR_BAD_STRIDE;
+  // rows are read and written in 16-byte words
+  if (!aligned(a.k_codes, 16) || !aligned(a.v_codes, 16) || !aligned(a.k_scales, 16) || !aligned(a.v_scales, 16) ||
+      a.k_page_stride % 16 || a.v_page_stride % 16 || a.k_scale_page_stride % 8 || a.v_scale_page_stride % 8)
+    return QL_ERR_UNSUPPORTED;
+  c->k_codes = static_cast<unsigned char*>(a.k_codes);
+  c->v_codes = static_cast<unsigned char*>(a.v_codes);
+  c->k_scales = static_cast<unsigned short*>(a.k_scales);
+  c->v_scales = static_cast<unsigned short*>(a.v_scales);
+  c->k_page = a.k_page_stride;
+  c->v_page = a.v_page_stride;
+  c->ks_page = a.k_scale_page_stride;
+  c->vs_page = a.v_scale_page_stride;
+  c->slots = a.num_pages * a.page_size;
+  c->page_shift = __builtin_ctzll((unsigned long long)a.page_size);
+  c->heads = (int)a.kv_heads;
+  c->row_bytes = (int)row;
+  c->groups = (int)groups;
+  c->bits = (int)a.bits;
+  return QL_OK;
+}
+
+template <typename T>
+int run_append(const ql::kvc::AppendParams& p, int64_t head_dim, void* stream, int64_t flags) {
+  const int lanes = (int)head_dim / 8, rows = p.q_heads + 2 * p.cache.heads;
+  const int threads = (int)std::min<int64_t>(256, cdiv((int64_t)rows * lanes, 32) * 32);
+  const dim3 grid((unsigned)p.tokens), block((unsigned)threads);
+  switch (lanes) {
+    case 8: return launch(ql::kvc::append_kernel<T, 8>, grid, block, 0, stream, flags, p);
+    case 16: return launch(ql::kvc::append_kernel<T, 16>, grid, block, 0, stream, flags, p);
+    default: return launch(ql::kvc::append_kernel<T, 32>, grid, block, 0, stream, flags, p);
+  }
+}
+
+template <typename T>
+int run_attention(const ql::att::Params& p, int64_t head_dim, void* stream, int64_t flags) {
+  const dim3 grid((unsigned)p.q_heads, (unsigned)p.total_q), block(ql::att::kTile);
+  switch (head_dim) {
+    case 64: return launch(ql::att::simple_kernel<T, 64>, grid, block, 0, stream, flags, p);
+    case 128: return launch(ql::att::simple_kernel<T, 128>, grid, block, 0, stream, flags, p);
+    default: return launch(ql::att::simple_kernel<T, 256>, grid, block, 0, stream, flags, p);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int ql_rotary(const ql_rotary_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->tokens < 0 || a->heads < 0 || a->tokens > INT_MAX || a->head_dim <= 0 || a->head_dim % 8 != 0 ||
+      a->head_dim > 65536 || a->heads > 65536 || a->heads * a->head_dim > INT_MAX)
+    return QL_ERR_BAD_SHAPE;
+  if (!act_dtype(a->dtype)) return QL_ERR_UNSUPPORTED;
+  if (a->tokens == 0 || a->heads == 0) return QL_OK;
+  ql::kvc::RotaryParams p = {};
+  int st = make_rows(&p.x, a->x, a->x_token_stride, a->x_head_stride, a->head_dim);
+  if (st == QL_OK) st = make_rows(&p.out, a->out, a->out_token_stride, a->out_head_stride, a->head_dim);
+  if (st == QL_OK)
+    st = make_turn(&p.turn, a->table, a->positions, a->position_bytes, a->max_positions, a->rotary_dim, a->head_dim,
+                   a->layout, a->inverse);
+  if (st != QL_OK) return st;
+  ql_host::Device dev;
+  if ((st = ql_host::current(&dev)) != QL_OK) return st;
+  p.tokens = a->tokens;
+  p.heads = (int)a->heads;
+  p.chunks = (int)(a->head_dim / 8);
+  p.err = dev.err_word;
+  const int threads = (int)std::min<int64_t>(256, cdiv((int64_t)p.heads * p.chunks, 32) * 32);
+  const dim3 grid((unsigned)a->tokens), block((unsigned)threads);
+  return a->dtype == QL_DTYPE_F16
+             ? launch(ql::kvc::rotary_kernel<__half>, grid, block, 0, stream, a->flags, p)
+             : launch(ql::kvc::rotary_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p);
+}
+
+int ql_kv_append(const ql_kv_append_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->tokens < 0 || a->tokens > INT_MAX || a->q_heads < 0 || a->q_heads > 65536) return QL_ERR_BAD_SHAPE;
+  if (!act_dtype(a->dtype) || !index_bytes(a->slot_bytes)) return QL_ERR_UNSUPPORTED;
+  ql::kvc::AppendParams p = {};
+  int st = make_pool(&p.cache, a->cache);
+  if (st != QL_OK) return st;
+  if (a->tokens == 0) return QL_OK;
+  const int64_t d = a->cache.head_dim;
+  if (!a->slots) return QL_ERR_NULL_POINTER;
+  if (!aligned(a->slots, (size_t)a->slot_bytes)) return QL_ERR_UNSUPPORTED;
+  if ((st = make_rows(&p.k, a->k, a->k_token_stride, a->k_head_stride, d)) != QL_OK) return st;
+  if ((st = make_rows(&p.v, a->v, a->v_token_stride, a->v_head_stride, d)) != QL_OK) return st;
+  if (a->q_heads > 0) {
+    if ((st = make_rows(&p.q, a->q, a->q_token_stride, a->q_head_stride, d)) != QL_OK) return st;
+    if ((st = make_rows(&p.q_out, a->q_out, a->q_out_token_stride, a->q_out_head_stride, d)) != QL_OK) return st;
+  }
+  if (a->rotary_dim != 0) {
+    st = make_turn(&p.turn, a->table, a->positions, a->position_bytes, a->max_positions, a->rotary_dim, d, a->layout,
+                   0);
+    if (st != QL_OK) return st;
+  }
+  ql_host::Device dev;
+  if ((st = ql_host::current(&dev)) != QL_OK) return st;
+  p.slots = a->slots;
+  p.wide_slots = a->slot_bytes == 8;
+  p.tokens = a->tokens;
+  p.q_heads = (int)a->q_heads;
+  p.err = dev.err_word;
+  return a->dtype == QL_DTYPE_F16 ? run_append<__half>(p, d, stream, a->flags)
+                                  : run_append<__nv_bfloat16>(p, d, stream, a->flags);
+}
+
+int ql_kv_read(const ql_kv_read_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->tokens < 0 || a->tokens > INT_MAX) return QL_ERR_BAD_SHAPE;
+  if (!act_dtype(a->dtype) || !index_bytes(a->slot_bytes)) return QL_ERR_UNSUPPORTED;
+  ql::kvc::ReadParams p = {};
+  int st = make_pool(&p.cache, a->cache);
+  if (st != QL_OK) return st;
+  if (a->tokens == 0) return QL_OK;
+  if (!a->slots || !a->k || !a->v) return QL_ERR_NULL_POINTER;
+  if (!aligned(a->slots, (size_t)a->slot_bytes) || !aligned(a->k, 16) || !aligned(a->v, 16))
+    return QL_ERR_UNSUPPORTED;
+  const int64_t chunks = a->cache.head_dim / 8, blocks = cdiv(a->tokens * a->cache.kv_heads * chunks, 256);
+  if (blocks > INT_MAX) return QL_ERR_BAD_SHAPE;
+  ql_host::Device dev;
+  if ((st = ql_host::current(&dev)) != QL_OK) return st;
+  p.slots = a->slots;
+  p.wide_slots = a->slot_bytes == 8;
+  p.tokens = a->tokens;
+  p.k = a->k;
+  p.v = a->v;
+  p.err = dev.err_word;
+  const dim3 grid((unsigned)blocks, 2), block(256);
+  return a->dtype == QL_DTYPE_F16
+             ? launch(ql::kvc::read_kernel<__half>, grid, block, 0, stream, a->flags, p, (int)chunks)
+             : launch(ql::kvc::read_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p, (int)chunks);
+}
+
+int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->batch < 0 || a->total_q < 0 || a->batch > 65535 || a->total_q > INT_MAX || a->q_heads < 0 ||
+      a->q_heads > 65536 || a->table_width < 0 || a->table_width > INT_MAX || a->mask_words < 0 ||
+      a->mask_words > 1024)
+    return QL_ERR_BAD_SHAPE;
+  if (!act_dtype(a->dtype)) return QL_ERR_UNSUPPORTED;
+  ql::att::Params p = {};
+  int st = make_pool(&p.cache, a->cache);
+  if (st != QL_OK) return st;
+  if (a->q_heads % a->cache.kv_heads != 0) return QL_ERR_BAD_SHAPE;
+  if (a->batch == 0 || a->total_q == 0 || a->q_heads == 0) return QL_OK;
+  if (!a->cu_q && a->total_q % a->batch != 0) return QL_ERR_BAD_SHAPE;
+  if (!a->out || !a->kv_lens || (!a->page_table && a->table_width > 0)) return QL_ERR_NULL_POINTER;
+  if ((st = make_rows(&p.q, a->q, a->q_token_stride, a->q_head_stride, a->cache.head_dim)) != QL_OK) return st;
+  if (a->table_stride < a->table_width) return QL_ERR_BAD_STRIDE;
+  if (!aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->page_table, 4) || !aligned(a->kv_lens, 4) ||
+      !aligned(a->cu_q, 4) || !aligned(a->mask, 8))
+    return QL_ERR_UNSUPPORTED;
+  ql_host::Device dev;
+  if ((st = ql_host::current(&dev)) != QL_OK) return st;
+  p.out = a->out;
+  p.lse = static_cast<float*>(a->lse);
+  p.page_table = static_cast<const int*>(a->page_table);
+  p.kv_lens = static_cast<const int*>(a->kv_lens);
+  p.cu_q = static_cast<const int*>(a->cu_q);
+  p.mask = static_cast<const unsigned long long*>(a->mask);
+  p.table_stride = a->table_stride;
+  p.table_width = (int)a->table_width;
+  p.num_pages = (int)a->cache.num_pages;
+  p.batch = (int)a->batch;
+  p.total_q = (int)a->total_q;
+  p.q_heads = (int)a->q_heads;
+  p.group = (int)(a->q_heads / a->cache.kv_heads);
+  p.mask_words = (int)a->mask_words;
+  p.scale = (float)a->scale;
+  p.err = dev.err_word;
+  return a->dtype == QL_DTYPE_F16 ? run_attention<__half>(p, a->cache.head_dim, stream, a->flags)
+                                  : run_attention<__nv_bfloat16>(p, a->cache.head_dim, stream, a->flags);
+}
+
+}  // extern "C"

@@ -22,6 +22,7 @@ enum DeviceError : unsigned {
   kDevErrMmaWait = 3,       // tensor-core completion wait ran out
   kDevErrTmem = 4,          // TMEM allocation failed
   kDevErrPeerWait = 5,      // another rank's exchange data never arrived
+  kDevErrBadIndex = 6,      // a position, slot or page outside its table
 };
 
 // Budget of any single bounded wait, in SM clock cycles.  %clock64 is

@@ -19,6 +19,7 @@
 
 #include "../../include/qlinear.h"
 #include "ql_common.cuh"
+#include "ql_host.h"
 #include "qargmax.cuh"
 #include "qxchg.cuh"
 #include "qgather.cuh"
@@ -1233,6 +1234,15 @@ int run_linear_argmax(const LinearArgs& a0, int64_t col_offset, int rank, int wo
 }  // namespace
 
 // ======================================================================
+int ql_host::current(Device* out) {
+  int st;
+  const DeviceInfo* d = current_device(&st);
+  if (!d) return st;
+  out->sms = d->sms;
+  out->err_word = d->err_word;
+  return QL_OK;
+}
+
 extern "C" {
 
 int ql_w8a16_linear(const void* x, int x_dtype, const void* w_q, const void* scale, int scale_dtype,

@@ -2,9 +2,10 @@
 
     python -m qlinear._build            (from llm-inference-optimizer_b200/)
 
-The library is a single translation unit (csrc/qlinear.cu includes the
-kernel headers) linked against a static CUDA runtime, so the .so next to
-this file is all a GPU machine needs.
+The library is two translation units (csrc/qlinear.cu, the linear layers, and
+csrc/qattn.cu, the attention side; both include their kernel headers) linked
+against a static CUDA runtime, so the .so next to this file is all a GPU
+machine needs.
 """
 from __future__ import annotations
 
@@ -28,7 +29,7 @@ def nvcc_path() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [HERE.parent.parent / "include" / "qlinear.h"]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [HERE.parent.parent / "include" / "qlinear.h"]
 
 
 def up_to_date() -> bool:
@@ -43,10 +44,9 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return OUT
     cmd = [nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17",
            "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
-           "-o", str(OUT) + ".tmp", str(CSRC / "qlinear.cu")]
+           "--threads", "0", "-o", str(OUT) + ".tmp", *(str(s) for s in sorted(CSRC.glob("*.cu")))]
     if verbose:
-        cmd.insert(-3, "-Xptxas")
-        cmd.insert(-3, "-v")
+        cmd[1:1] = ["-Xptxas", "-v"]
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=not verbose, text=True)
     if res.returncode != 0:

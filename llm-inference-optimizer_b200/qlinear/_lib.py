@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -37,10 +38,14 @@ QL_DEVICE_ERROR_EMPTY_WAIT = 2
 QL_DEVICE_ERROR_MMA_WAIT = 3
 QL_DEVICE_ERROR_TMEM = 4
 QL_DEVICE_ERROR_PEER_WAIT = 5
+QL_DEVICE_ERROR_BAD_INDEX = 6
 QL_XCHG_MAX_RANKS = 8
 
 QL_W4_LAYOUT_SPLIT_HALF = 0
 QL_W4_LAYOUT_ADJACENT = 1
+
+QL_ROTARY_HALF = 0
+QL_ROTARY_INTERLEAVED = 1
 
 QL_FLAG_PDL = 0x1
 QL_FLAG_FORCE_GEMM = 0x2
@@ -94,11 +99,25 @@ SIGNATURES = {
     "ql_gather_buffer_bytes": (_sz, [_int, _i64]),
     "ql_allgather_f16": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _i64, _int, _int, _int,
                                 ctypes.POINTER(_vp), _uint, _vp]),
+    # the attention side: packed argument structures (ARGS below), then the stream
+    "ql_rotary": (_int, [ctypes.c_char_p, _vp]),
+    "ql_kv_append": (_int, [ctypes.c_char_p, _vp]),
+    "ql_kv_read": (_int, [ctypes.c_char_p, _vp]),
+    "ql_tree_attention": (_int, [ctypes.c_char_p, _vp]),
     "ql_strerror": (ctypes.c_char_p, [_int]),
     "ql_version": (_int, []),
     "ql_device_error": (_int, [ctypes.POINTER(_int)]),
     "ql_clear_device_error": (_int, []),
 }
+
+# Layouts of the argument structures: every field is 8 bytes (pointers and
+# int64 as q, double as d), in the order of include/qlinear.h.  Packing one
+# bytes object costs a third of converting as many ctypes arguments.
+KV_CACHE_FIELDS = 13
+ROTARY_ARGS = struct.Struct("18q")
+KV_APPEND_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 24}q")
+KV_READ_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 7}q")
+TREE_ATTENTION_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 18}qdq")
 
 _lock = threading.Lock()
 _lib = None

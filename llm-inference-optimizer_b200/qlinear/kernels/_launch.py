@@ -81,3 +81,32 @@ class on_device:
         if self.prev is not None:
             torch.cuda.set_device(self.prev)
         return False
+
+
+def index_bytes(t: torch.Tensor, what: str) -> int:
+    """4 or 8 for an int32 / int64 index tensor."""
+    if t.dtype == torch.int64:
+        return 8
+    if t.dtype == torch.int32:
+        return 4
+    raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+
+
+def activation_code(t: torch.Tensor, what: str) -> int:
+    """dtype code of a 16-bit activation tensor."""
+    if t.dtype == torch.float16:
+        return _lib.QL_DTYPE_F16
+    if t.dtype == torch.bfloat16:
+        return _lib.QL_DTYPE_BF16
+    raise TypeError(f"{what} must be fp16 or bf16, got {t.dtype}")
+
+
+def call(entry, packed: bytes, device: torch.device) -> None:
+    """entry(packed arguments, current stream) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        status = entry(packed, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with on_device(device):
+            status = entry(packed, torch.cuda.current_stream(device).cuda_stream)
+    if status != _lib.QL_OK:
+        _lib.check(status)

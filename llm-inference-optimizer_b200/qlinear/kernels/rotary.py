@@ -1,0 +1,156 @@
+"""Rotary positions for query and key heads (libqlinear).
+
+The reference's engines rotate q and k between the projections and the
+attention with the model's cos / sin tensors (src/engine/paged_engine.py:98-126).
+``RotaryTable`` holds those angles for every position once, with any scaling
+for long contexts folded in; ``apply_rotary`` turns heads by them in one
+launch, reading the column slices of a fused projection's output as they are.
+Turning q and k while k is written to a cache is ``kv_cache.append_kv``.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _lib
+from ._launch import activation_code, call, default_flags, index_bytes
+
+LAYOUTS = {"half": _lib.QL_ROTARY_HALF, "interleaved": _lib.QL_ROTARY_INTERLEAVED}
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None,
+                       max_positions: int | None = None) -> tuple[torch.Tensor, float]:
+    """Radians per position of each pair (float64 [rotary_dim / 2]) and the
+    factor on cos and sin.  `scaling` follows the model configurations:
+    ``{"rope_type": name, ...}`` with
+
+    * ``default``: base ** (-2i / rotary_dim);
+    * ``linear``: all of them divided by ``factor``;
+    * ``dynamic``: the base grown so that ``max_positions`` positions span what
+      ``original_max_position_embeddings`` did (times ``factor``);
+    * ``llama3``: wavelengths longer than original / low_freq_factor divided by
+      ``factor``, shorter than original / high_freq_factor kept, and a linear
+      step in original / wavelength between;
+    * ``yarn``: pairs that turn less than ``beta_slow`` times over the original
+      length divided by ``factor``, more than ``beta_fast`` times kept, a ramp
+      over the pair index between, and cos / sin times
+      ``attention_factor`` (0.1 ln(factor) + 1 unless given).
+    """
+    s = dict(scaling or {})
+    kind = s.get("rope_type", s.get("type", "default"))
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+
+    def need(name):
+        if s.get(name) is None:
+            raise ValueError(f"rotary scaling {kind!r} needs {name!r}")
+        return float(s[name])
+
+    if kind == "dynamic":
+        old, factor = need("original_max_position_embeddings"), need("factor")
+        if max_positions is not None and max_positions > old:
+            base = base * (factor * max_positions / old - (factor - 1.0)) ** (rotary_dim / (rotary_dim - 2.0))
+    f = float(base) ** (-2.0 * i / rotary_dim)
+    if kind in ("default", "dynamic"):
+        return f, 1.0
+    if kind == "linear":
+        return f / need("factor"), 1.0
+    if kind == "llama3":
+        old, low, high = (need("original_max_position_embeddings"), need("low_freq_factor"),
+                          need("high_freq_factor"))
+        kept = ((old * f / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        return f * (kept + (1.0 - kept) / need("factor")), 1.0
+    if kind == "yarn":
+        old, factor = need("original_max_position_embeddings"), need("factor")
+
+        def pair_with(turns):            # the (fractional) pair that turns so often over the original length
+            return rotary_dim * math.log(old / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+
+        fast, slow = s.get("beta_fast") or 32.0, s.get("beta_slow") or 1.0
+        lo, hi = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), rotary_dim - 1)
+        kept = 1.0 - ((i - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+        factor_on = s.get("attention_factor")
+        if factor_on is None:
+            factor_on = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        return f * (kept + (1.0 - kept) / factor), float(factor_on)
+    raise ValueError(f"unknown rotary scaling {kind!r}")
+
+
+class RotaryTable:
+    """cos and sin of every position: fp32 [max_positions, rotary_dim / 2, 2]."""
+
+    def __init__(self, table: torch.Tensor, layout: str = "half"):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout must be one of {sorted(LAYOUTS)}, got {layout!r}")
+        if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2:
+            raise TypeError(f"table must be fp32 [max_positions, rotary_dim / 2, 2], got {table.dtype} "
+                            f"{tuple(table.shape)}")
+        if table.shape[0] == 0 or table.shape[1] == 0 or table.shape[1] % 4 != 0:
+            raise ValueError(f"rotary_dim must be a positive multiple of 8 and the table not empty, got "
+                             f"{tuple(table.shape)}")
+        self.table = table.contiguous()
+        self.layout = layout
+        self.rotary_dim = 2 * table.shape[1]
+        self.max_positions = table.shape[0]
+
+    @classmethod
+    def build(cls, rotary_dim: int, max_positions: int, base: float = 10000.0, layout: str = "half",
+              scaling: dict | None = None, device="cuda") -> "RotaryTable":
+        """The table of `rotary_frequencies`, computed in float64 and rounded once."""
+        f, factor = rotary_frequencies(rotary_dim, base, scaling, max_positions)
+        angles = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
+        return cls((torch.stack([angles.cos(), angles.sin()], dim=-1) * factor).float(), layout)
+
+    @classmethod
+    def from_config(cls, config, max_positions: int | None = None, layout: str = "half",
+                    device="cuda") -> "RotaryTable":
+        """From a decoder model's configuration (``rope_parameters``, or
+        ``rope_theta`` and ``rope_scaling``)."""
+        s = dict(getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {})
+        base = s.get("rope_theta") or getattr(config, "rope_theta", None) or 10000.0
+        if s.get("rope_type", "default") not in ("default", "linear"):
+            s.setdefault("original_max_position_embeddings", config.max_position_embeddings)
+        head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+        part = s.get("partial_rotary_factor") or getattr(config, "partial_rotary_factor", None) or 1.0
+        return cls.build(int(head_dim * part), max_positions or config.max_position_embeddings, base, layout, s,
+                         device)
+
+
+def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, out: torch.Tensor = None,
+                 inverse: bool = False) -> torch.Tensor:
+    """Turns x (tokens, heads, head_dim) fp16 / bf16 by the angles of
+    positions (tokens,): the first ``rotary.rotary_dim`` elements of each head
+    in ``rotary.layout``'s pairs, the rest unchanged, one rounding.  x and
+    `out` may have any strides with unit stride along head_dim; ``out=x``
+    turns in place.  ``inverse=True`` turns back: it undoes the call, and maps
+    the gradient of its result to that of x."""
+    assert x.is_cuda and x.dim() == 3, f"x must be a CUDA tensor (tokens, heads, head_dim), got {tuple(x.shape)}"
+    tokens, heads, head_dim = x.shape
+    dtype = activation_code(x, "apply_rotary: x")
+    assert positions.shape == (tokens,) and positions.device == x.device, \
+        f"positions must be ({tokens},) on {x.device}, got {tuple(positions.shape)} on {positions.device}"
+    assert rotary.table.device == x.device, f"the rotary table is on {rotary.table.device}, x on {x.device}"
+    assert rotary.rotary_dim <= head_dim and head_dim % 8 == 0, \
+        f"head_dim {head_dim} must be a multiple of 8 and at least rotary_dim {rotary.rotary_dim}"
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), dtype=x.dtype, device=x.device)
+    else:
+        assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, \
+            f"out must be {tuple(x.shape)} {x.dtype} on {x.device}"
+        assert out.stride(-1) == 1, "out must have unit stride along head_dim"
+    if tokens == 0 or heads == 0:
+        return out
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    xs, os_ = x.stride(), out.stride()
+    packed = _lib.ROTARY_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), rotary.table.data_ptr(), positions.data_ptr(), tokens, heads, head_dim,
+        rotary.rotary_dim, rotary.max_positions, xs[0], xs[1], os_[0], os_[1], dtype, LAYOUTS[rotary.layout],
+        index_bytes(positions, "positions"), int(inverse), default_flags())
+    call(_lib.load().ql_rotary, packed, x.device)
+    return out
+
+
+__all__ = ["RotaryTable", "apply_rotary", "rotary_frequencies"]
