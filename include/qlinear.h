@@ -435,6 +435,9 @@ int ql_kv_read(const ql_kv_read_args* args, void* stream);
  * lengths and only choose the launch.
  * q_heads is a multiple of kv_heads; query head h reads key/value head
  * h / (q_heads / kv_heads).
+ *   workspace: ql_tree_attention_workspace_size(head_dim) bytes of the current
+ *   device, 16-byte aligned, zeroed before its first use (a call leaves what
+ *   the next one needs zero); calls that share one must not overlap.
  */
 typedef struct {
   ql_kv_cache cache;
@@ -444,8 +447,10 @@ typedef struct {
   int64_t batch, total_q, q_heads, q_token_stride, q_head_stride;
   int64_t table_width, table_stride, mask_words, max_q, max_kv, dtype;
   double scale;
-  int64_t flags;
+  void* workspace;
+  int64_t workspace_bytes, flags;
 } ql_tree_attention_args;
+size_t ql_tree_attention_workspace_size(int64_t head_dim);
 int ql_tree_attention(const ql_tree_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------- diagnostics */

@@ -8,6 +8,8 @@
 // A row that sees nothing gives zeros and a log-sum of minus infinity.
 #pragma once
 
+#include <type_traits>
+
 #include "qcache.cuh"
 
 namespace ql {
@@ -25,7 +27,7 @@ struct Params {
   long long table_stride;
   int table_width, num_pages;
   int batch, total_q, q_heads, group, mask_words;
-  float scale;
+  float scale_log2;              // scale * log2(e): scores in units of log2
   unsigned* err;
 };
 
@@ -52,88 +54,683 @@ __device__ __forceinline__ bool sees(const Params& p, const Request& r, int i, i
   return d < 64 * p.mask_words && ((p.mask[(long long)(r.q0 + i) * p.mask_words + (d >> 6)] >> (d & 63)) & 1);
 }
 
-constexpr int kTile = 128;
+// ------------------------------------------------------------ work of a launch
+// Work is counted in units of 128 keys of one item: one request, one
+// key/value head, one tile of ROWS = 8 NT rows (row r of a request is new
+// token r / group under query head r % group of the key/value head).  Items
+// lie one behind another, each rounded up to a multiple of kMinUnits, and
+// the CTAs take equal runs of units, whatever the requests' lengths are: a
+// CTA may end one item, do some whole and begin another.  Lengths are read
+// on the device, so a captured launch serves other lengths later.
+constexpr int kUnitKeys = 128;
+constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMinUnits = 2;               // keys worth a CTA of their own: 256
+constexpr int kMaxCtas = 1024;             // counters in the workspace's first 4 KB
+constexpr int kHeaderBytes = 4 * kMaxCtas;
 
-// One CTA per (query head, new token): each thread scores one key of a tile of
-// 128, then sums one element of the output over the tile.
-template <typename T, int D>
-__global__ void __launch_bounds__(kTile) simple_kernel(const Params p) {
+struct Work {
+  long long total;     // units of the launch
+  int ctas;            // CTAs that take part
+  __device__ long long first_unit(int cta) const { return total * cta / ctas; }
+  __device__ int cta_of(long long u) const { return (int)(((u + 1) * ctas - 1) / total); }
+};
+
+__device__ __forceinline__ int item_units(const Request& r) {
+  const int n = (r.kv_len + kUnitKeys - 1) / kUnitKeys;
+  return max((n + kMinUnits - 1) / kMinUnits, 1) * kMinUnits;
+}
+template <int ROWS>
+__device__ __forceinline__ long long request_units(const Params& p, const Request& r) {
+  const long long tiles = ((long long)r.q_len * p.group + ROWS - 1) / ROWS;
+  return tiles * p.cache.heads * item_units(r);
+}
+
+// Sums the requests' units and finds the request that holds this CTA's first
+// unit: *b and the unit at which it begins.  All threads call it.
+template <int ROWS>
+__device__ __forceinline__ Work find_work(const Params& p, int* b, long long* base) {
+  __shared__ long long warp_sum[kWarps];
+  __shared__ long long found_base;
+  __shared__ int found_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto scan = [&](long long v, long long* sum) {      // inclusive, and the CTA's sum
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = v;
+    __syncthreads();
+    long long before = 0, all = 0;
+    #pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    *sum = all;
+    return v + before;
+  };
+  Work w = {0, 0};
+  long long mine = 0, incl = 0, sum;
+  for (int i = 0; i < p.batch; i += kThreads) {
+    const int at = i + threadIdx.x;
+    mine = at < p.batch ? request_units<ROWS>(p, request(p, at)) : 0;
+    incl = scan(mine, &sum);
+    w.total += sum;
+  }
+  w.ctas = (int)min((long long)gridDim.x, w.total / kMinUnits);
+  if ((int)blockIdx.x >= w.ctas) return w;
+  const long long u = w.first_unit(blockIdx.x);
+  long long before = 0;
+  for (int i = 0; i < p.batch; i += kThreads) {
+    if (p.batch > kThreads) {                          // else mine, incl and sum are still these
+      const int at = i + threadIdx.x;
+      mine = at < p.batch ? request_units<ROWS>(p, request(p, at)) : 0;
+      incl = scan(mine, &sum);
+    }
+    const long long from = before + incl - mine;
+    if (u >= from && u < from + mine) {
+      found_b = i + threadIdx.x;
+      found_base = from;
+    }
+    before += sum;
+  }
+  __syncthreads();
+  *b = found_b;
+  *base = found_base;
+  return w;
+}
+
+// ---------------------------------------------------------------- primitives
+// 2^x; subnormal results only where a 16-bit type can show them (bf16).
+template <bool SUBNORMAL>
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  if constexpr (SUBNORMAL)
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Transpose of an 8x8 matrix of 16-bit elements held two to a lane by rows.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// A row's factor brings its largest weight just under 2^kTopWeight, and again
+// when one passes kMostWeight: high in fp16's range, and in bf16's neither so
+// low that a small one's remainder is lost, nor so high that the matrix
+// unit, which aligns a large weight times a code of 0 by the weight's
+// exponent, drops a small one beside it.
+constexpr int kTopWeight = 11;
+constexpr float kMostWeight = 0x1p15f;
+// The 16-bit type of the products: the codes are exact in both.  fp16 takes
+// the weights rounded once (11 bits); bf16, whose outputs have fp32's range,
+// as a sum of two (16 bits).
+template <typename T> struct Num;
+template <> struct Num<__half> {
+  static constexpr bool kSplit = false;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  // 4 signed bytes -> (0, 1), (2, 3)
+  static __device__ __forceinline__ void dec8(uint32_t u, uint32_t& p01, uint32_t& p23) { dec_w8(u, p01, p23); }
+  // 16-bit lanes of 4 nibbles (codes + 8) -> nibble i of both lanes
+  static __device__ __forceinline__ void dec4(uint32_t u, uint32_t (&v)[4]) {
+    const uint32_t w = u >> 8;
+    v[0] = h2_sub(lop3_and_or(u, 0x000F000Fu, kH2Magic), kH2_1032);
+    v[1] = h2_fma(lop3_and_or(u, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
+    v[2] = h2_sub(lop3_and_or(w, 0x000F000Fu, kH2Magic), kH2_1032);
+    v[3] = h2_fma(lop3_and_or(w, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    mma_16816(d, a0, a1, a2, a3, b0, b1);
+  }
+};
+template <> struct Num<__nv_bfloat16> {
+  static constexpr bool kSplit = true;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  // 0x43bb with the byte's sign bit cleared is 128 + its low 7 bits; with the
+  // low 7 bits cleared it is 128, or 256 where the sign bit is set: their
+  // difference is the signed byte
+  static __device__ __forceinline__ uint32_t signed_bytes(uint32_t t) { return sub(t & 0xFF7FFF7Fu, t & 0xFF80FF80u); }
+  static __device__ __forceinline__ void dec8(uint32_t u, uint32_t& p01, uint32_t& p23) {
+    p01 = signed_bytes(__byte_perm(u, 0x43434343u, 0x4140));
+    p23 = signed_bytes(__byte_perm(u, 0x43434343u, 0x4342));
+  }
+  static __device__ __forceinline__ void dec4(uint32_t u, uint32_t (&v)[4]) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sub(lop3_and_or(u >> (4 * i), 0x000F000Fu, 0x43004300u), 0x43084308u);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+// Cache codes: read once by this CTA, so not kept in L1.
+template <int WORDS>
+__device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const unsigned char* p) {
+  static_assert(WORDS == 1 || WORDS == 2 || WORDS == 4 || WORDS == 8, "4 to 32 bytes");
+  if constexpr (WORDS == 1) {
+    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+  } else if constexpr (WORDS == 2) {
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+  } else {
+    #pragma unroll
+    for (int i = 0; i < WORDS; i += 4)
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "l"(p + 4 * i));
+  }
+}
+
+// ------------------------------------------------- the kernel for a few rows
+// Bound by reading the cache (one unit of keys and values, 33 KB at 8 bits
+// and head_dim 128, serves 8 NT rows), so everything else is arranged around
+// the loads: keys and values go from global memory straight into the
+// registers that the matrix instructions take them from.
+//
+// Keys are the M side of both products, rows the N side (m16n8k16):
+//   S^T[key, row] = K Q^T: lane (g, t) = (lane / 4, lane % 4) holds keys g and
+//     g + 8.  The order of the sum over head_dim is free, so a lane reads 16
+//     neighbouring elements of a key from each 64 and Q is laid out alike.
+//   O^T[d, row] = V^T P: lane (g, t) holds keys 2t, 2t + 1, 2t + 8, 2t + 9 and
+//     an eighth of head_dim; pairs of keys are joined by byte permutes, and
+//     the order of d within a tile of 16 is free (it only names the outputs).
+// The codes enter as exact integers of the calls' 16-bit type.  Key scales
+// multiply the scores afterwards; value scales multiply the weights, against
+// a factor per row that keeps the largest weight * scale seen high in the
+// type's range, so that the scales' size does not matter.
+//
+// The running maximum of a row moves only when a score passes it by 6 (weights
+// up to 2^6): one vote per 16 keys stands for the reductions and the
+// rescaling, which become rare.
+//
+// A key's scale is read by its own lanes; hidden keys are removed by
+// selection, never by multiplication, so what unused rows of a page hold
+// does not matter.
+template <int D, int BITS, int NT>
+struct Shape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kGroups = BITS == 8 ? 1 : kChunks;
+  static constexpr int kKeyWords = BITS == 8 ? 4 : 2;                // of a 64-element chunk
+  static constexpr int kValWords = BITS == 8 ? D / 32 : D / 64;      // of a lane's eighth of a row
+  static constexpr int kTiles = D / 16;
+  static constexpr int kCtas = D == 256 ? 1 : NT == 1 ? 2 : 1;       // per SM, by registers
+  // partial of an item: per row its maximum, its sum and D outputs
+  static constexpr int kPartial = kRows * (D + 2);
+  static constexpr size_t kSmem = (size_t)kWarps * kRows * (D + 2) * sizeof(float);
+};
+
+template <typename T, int D, int BITS, int NT>
+__global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
+    stream_kernel(const Params p, unsigned* counters, float* partials) {
+  using S = Shape<D, BITS, NT>;
+  using N = Num<T>;
   griddep_launch_dependents();
   griddep_wait();
-  __shared__ float q[D], w[kTile], red[4];
-  const int head = blockIdx.x, token = blockIdx.y, t = threadIdx.x;
+  extern __shared__ float smem[];
+  float* sm_o = smem;                                   // [warp][row][D]
+  float* sm_m = smem + kWarps * S::kRows * D;           // [warp][row]
+  float* sm_l = sm_m + kWarps * S::kRows;
+  __shared__ int last_one;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
   const kvc::Pool& kv = p.cache;
-  Request r;
-  int b = 0;
-  for (; b < p.batch; ++b) {
-    r = request(p, b);
-    if (token >= r.q0 && token < r.q0 + r.q_len) break;
-  }
-  if (b == p.batch) return;
-  const int row = token - r.q0, kv_head = head / p.group;
-  for (int d = t; d < D; d += kTile)
-    q[d] = kvc::to_f(static_cast<const T*>(p.q.p)[(long long)token * p.q.token_stride + head * p.q.head_stride + d]);
-  __syncthreads();
-  const int span = kv.groups > 1 ? kvc::kGroup4 : D;
-  constexpr int E = (D + kTile - 1) / kTile;
-  float m = -INFINITY, l = 0.f, o[E] = {};
-  for (int j0 = 0; j0 < r.kv_len; j0 += kTile) {
-    const int j = j0 + t;
-    float s = -INFINITY;
-    if (j < r.kv_len && sees(p, r, row, j)) {
-      const int page = p.page_table[b * p.table_stride + (j >> kv.page_shift)];
-      if (page >= 0 && page < p.num_pages) {
-        const kvc::RowAt k = kvc::row_at(kv, ((long long)page << kv.page_shift) + (j & ((1 << kv.page_shift) - 1)),
-                                         kv_head, false);
-        s = 0.f;
-        for (int g = 0; g < kv.groups; ++g) {
-          float sum = 0.f, f[8];
-          for (int d = g * span; d < g * span + span; d += 8) {
-            kvc::codes8(f, k.codes + d / 8 * kv.bits, kv.bits);
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(f[i], q[d + i], sum);
+  int b;
+  long long base;
+  const Work work = find_work<S::kRows>(p, &b, &base);
+  if ((int)blockIdx.x >= work.ctas) return;
+  long long u = work.first_unit(blockIdx.x);
+  const long long u_end = work.first_unit(blockIdx.x + 1);
+  Request r = request(p, b);
+
+  while (u < u_end) {
+    // ------------------------------------------------------ the next segment
+    long long mine = request_units<S::kRows>(p, r);
+    while (u >= base + mine) {
+      base += mine;
+      r = request(p, ++b);
+      mine = request_units<S::kRows>(p, r);
+    }
+    const int per_item = item_units(r);
+    const int tiles = (int)(((long long)r.q_len * p.group + S::kRows - 1) / S::kRows);
+    const long long item = (u - base) / per_item;
+    const int k_begin = (int)((u - base) - item * per_item);
+    const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
+    const int head = (int)(item / tiles), row0 = (int)(item - (long long)head * tiles) * S::kRows;
+    const int rows = min(S::kRows, r.q_len * p.group - row0);
+    const int context = r.kv_len - r.q_len;             // positions that every row sees
+
+    // ------------------------------------------------------------- queries
+    uint32_t qb[NT][S::kTiles][2];
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + 8 * n + g;
+      const bool live = 8 * n + g < rows;
+      const int token = live ? row / p.group : 0, qh = head * p.group + (live ? row - token * p.group : 0);
+      const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
+      float f[S::kChunks][16];
+      #pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+        #pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+          float x[4] = {}, y[4] = {};
+          if (live) kvc::load8(x, y, src + c * 64 + t * 16 + i, p.q.vec);
+          #pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[c][i + e] = x[e];
+            f[c][i + 4 + e] = y[e];
           }
-          s = fmaf(sum, kvc::bf16_bits_to_f(k.scales[g]), s);
         }
-        s *= p.scale;
-      } else {
+      #pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+        #pragma unroll
+        for (int w = 0; w < 4; ++w)
+          #pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            // 8 bits: steps of 4 neighbours; 4 bits: elements i and i + 4 of 8 share a word
+            const int i = BITS == 8 ? 4 * w + 2 * x : 8 * (w >> 1) + 2 * (w & 1) + x;
+            const int j = BITS == 8 ? i + 1 : i + 4;
+            qb[n][4 * c + w][x] = N::pack(f[c][i], f[c][j]);
+          }
+    }
+
+    // ---------------------------------------------------------- running state
+    float acc[NT][S::kTiles][4];
+    float m[NT][2], l[NT][2], fac[NT][2];
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      #pragma unroll
+      for (int i = 0; i < S::kTiles; ++i)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[n][x] = -INFINITY;
+        l[n][x] = 0.f;
+        fac[n][x] = 1.f;
+      }
+    }
+
+    // --------------------------------------------- this warp's tiles of 16 keys
+    // tile i: keys j0(i) .. j0(i) + 15, within one page
+    const int j_first = k_begin * kUnitKeys + warp * 16;
+    const int j_stop = min(k_end * kUnitKeys, r.kv_len);
+    const int n_tiles = j_first < j_stop ? (j_stop - j_first + kUnitKeys - 1) / kUnitKeys : 0;
+    const int* pages = p.page_table + b * p.table_stride;
+    auto fetch_pages = [&](int i) {                     // page of tile i + lane
+      const int j = j_first + (i + lane) * kUnitKeys;
+      int page = i + lane < n_tiles ? pages[j >> kv.page_shift] : 0;
+      if (page < 0 || page >= p.num_pages) {
         atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+        page = -1;
+      }
+      return page;
+    };
+    int page_now = fetch_pages(0), page_next = fetch_pages(32);
+
+    uint32_t kw[2][S::kChunks][S::kKeyWords], vw[4][S::kValWords];
+    unsigned short ks[2][S::kGroups], vs[2][S::kGroups];
+    int page_k = -1, page_v = -1;                       // of the tiles in kw and vw
+    auto rows_of = [&](int page, int i) {               // row index within the page of tile i's first key
+      return (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
+    };
+    auto load_keys = [&](int i) {
+      if (i > 0 && (i & 31) == 0) {
+        page_now = page_next;
+        page_next = fetch_pages(i + 32);
+      }
+      page_k = __shfl_sync(0xffffffffu, page_now, i & 31);
+      if (page_k < 0) return;
+      const int at = rows_of(page_k, i);
+      const unsigned char* code = kv.k_codes + page_k * kv.k_page + (long long)(at + g) * (D * BITS / 8) + t * 4 * S::kKeyWords;
+      const unsigned short* sc = kv.k_scales + page_k * kv.ks_page + (long long)(at + g) * S::kGroups;
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        #pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+          load_codes<S::kKeyWords>(kw[x][c], code + x * 8 * (D * BITS / 8) + c * 8 * BITS);
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q) ks[x][q] = sc[x * 8 * S::kGroups + q];
+      }
+    };
+    auto load_values = [&]() {                          // of the tile whose page is page_k
+      page_v = page_k;
+    };
+    auto load_values_at = [&](int i) {
+      if (page_v < 0) return;
+      const int at = rows_of(page_v, i);
+      const unsigned char* code = kv.v_codes + page_v * kv.v_page + (long long)(at + 2 * t) * (D * BITS / 8);
+      const unsigned short* sc = kv.v_scales + page_v * kv.vs_page + (long long)(at + g) * S::kGroups;
+      #pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const unsigned char* row = code + ((x & 1) + (x >> 1) * 8) * (D * BITS / 8);
+        if constexpr (BITS == 8) {
+          load_codes<S::kValWords>(vw[x], row + g * (D / 8));
+        } else {
+          #pragma unroll
+          for (int c = 0; c < S::kChunks; ++c) {
+            uint32_t w[1];
+            load_codes<1>(w, row + c * 32 + g * 4);
+            vw[x][c] = w[0];
+          }
+        }
+      }
+      #pragma unroll
+      for (int x = 0; x < 2; ++x)
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q) vs[x][q] = sc[x * 8 * S::kGroups + q];
+    };
+
+    if (n_tiles > 0) {
+      load_keys(0);
+      load_values();
+      load_values_at(0);
+    }
+    #pragma unroll 1
+    for (int i = 0; i < n_tiles; ++i) {
+      const int j0 = j_first + i * kUnitKeys;
+      const bool hidden = page_k < 0;
+      // ------------------------------------------------------------- scores
+      float s[NT][4];
+      #pragma unroll
+      for (int n = 0; n < NT; ++n)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      #pragma unroll
+      for (int c = 0; c < S::kChunks; ++c) {
+        float part[NT][4];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+          #pragma unroll
+          for (int e = 0; e < 4; ++e) part[n][e] = BITS == 8 ? s[n][e] : 0.f;
+        #pragma unroll
+        for (int w = 0; w < S::kKeyWords; ++w) {
+          if constexpr (BITS == 8) {
+            uint32_t a0, a1, a2, a3;
+            N::dec8(kw[0][c][w], a0, a2);
+            N::dec8(kw[1][c][w], a1, a3);
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) N::mma(part[n], a0, a1, a2, a3, qb[n][4 * c + w][0], qb[n][4 * c + w][1]);
+          } else {
+            uint32_t x[4], y[4];
+            N::dec4(kw[0][c][w], x);
+            N::dec4(kw[1][c][w], y);
+            #pragma unroll
+            for (int h = 0; h < 2; ++h)
+              #pragma unroll
+              for (int n = 0; n < NT; ++n)
+                N::mma(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * c + 2 * w + h][0],
+                          qb[n][4 * c + 2 * w + h][1]);
+          }
+        }
+        if constexpr (BITS == 8) {
+          #pragma unroll
+          for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = part[n][e];
+        } else {
+          const float k0 = kvc::bf16_bits_to_f(ks[0][c]), k1 = kvc::bf16_bits_to_f(ks[1][c]);
+          #pragma unroll
+          for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(part[n][e], (e < 2 ? k0 : k1) * p.scale_log2, s[n][e]);
+        }
+      }
+      if constexpr (BITS == 8) {
+        const float k0 = kvc::bf16_bits_to_f(ks[0][0]), k1 = kvc::bf16_bits_to_f(ks[1][0]);
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+          #pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] *= (e < 2 ? k0 : k1) * p.scale_log2;
+      }
+      if (i + 1 < n_tiles) load_keys(i + 1);
+
+      // ------------------------------------------------- what the rows see
+      if (hidden || j0 + 15 >= context) {
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+          #pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + g + (e >> 1) * 8, row = 8 * n + 2 * t + (e & 1);
+            const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, (row0 + row) / p.group, j);
+            if (!see) s[n][e] = -INFINITY;
+          }
+      }
+
+      // ------------------------------------------------------------ weights
+      float v_top[2], v_sc[2][S::kGroups];
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        v_top[x] = 0.f;
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q) {
+          v_sc[x][q] = kvc::bf16_bits_to_f(vs[x][q]);
+          v_top[x] = fmaxf(v_top[x], v_sc[x][q]);
+        }
+      }
+      float w[NT][4];
+      bool move[NT][2] = {}, any_move = false;
+      #pragma unroll
+      for (int n = 0; n < NT; ++n)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float top = m[n][e & 1];
+          w[n][e] = s[n][e] == -INFINITY ? 0.f : ex2<N::kSplit>(s[n][e] - (top == -INFINITY ? 0.f : top));
+          move[n][e & 1] |= s[n][e] > top + 6.f || (w[n][e] != 0.f && w[n][e] * v_top[e >> 1] * fac[n][e & 1] > kMostWeight);
+          any_move |= move[n][e & 1];
+        }
+      if (__any_sync(0xffffffffu, any_move)) {
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+          #pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            // a row's own lanes alone move it, so that its bits do not depend on the other rows
+            const bool row_moves = __ballot_sync(0xffffffffu, move[n][x]) & (0x11111111u << t);
+            float top = fmaxf(s[n][x], s[n][2 + x]);
+            #pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m[n][x]);
+            const float keep = m[n][x] == top ? 1.f : ex2<N::kSplit>(m[n][x] - top);
+            float most = 0.f;
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float sv = s[n][2 * h + x];
+              const float moved = sv == -INFINITY ? 0.f : ex2<N::kSplit>(sv - (top == -INFINITY ? 0.f : top));
+              const float wv = moved * v_top[h];
+              if (row_moves) w[n][2 * h + x] = moved;
+              if (wv > 0.f && wv < INFINITY) most = fmaxf(most, wv);
+            }
+            #pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // the factor that brings the largest weight just under 2^kTopWeight, and none of the earlier ones above that
+            const int e = (int)(__float_as_uint(most) >> 23) - 126;
+            float next = keep > 0.f ? fminf(fac[n][x] / keep, 0x1p100f) : 0x1p100f;
+            if (most > 0.f) next = fminf(next, __uint_as_float((unsigned)min(max(kTopWeight - e + 127, 1), 227) << 23));
+            const float adjust = keep > 0.f ? keep * (next / fac[n][x]) : 0.f;
+            if (!row_moves) continue;
+            #pragma unroll
+            for (int q = 0; q < S::kTiles; ++q) {
+              acc[n][q][x] *= adjust;
+              acc[n][q][2 + x] *= adjust;
+            }
+            l[n][x] *= keep;
+            m[n][x] = top;
+            fac[n][x] = next;
+          }
+      }
+      uint32_t pb[S::kGroups][NT][2], pb_lo[S::kGroups][NT][2];
+      #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) l[n][e & 1] += w[n][e];
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool z0 = s[n][2 * h] == -INFINITY, z1 = s[n][2 * h + 1] == -INFINITY;
+            const float a = z0 ? 0.f : w[n][2 * h] * v_sc[h][q] * fac[n][0];
+            const float c = z1 ? 0.f : w[n][2 * h + 1] * v_sc[h][q] * fac[n][1];
+            const uint32_t hi = N::pack(a, c);
+            pb[q][n][h] = transpose8(hi);
+            if constexpr (N::kSplit)
+              pb_lo[q][n][h] = transpose8(N::pack(a - __uint_as_float(hi << 16), c - __uint_as_float(hi & 0xFFFF0000u)));
+          }
+      }
+
+      // -------------------------------------------------------------- values
+      if (!hidden) {
+        auto tile = [&](int at, int q, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+          #pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            N::mma(acc[n][at], a0, a1, a2, a3, pb[q][n][0], pb[q][n][1]);
+            if constexpr (N::kSplit) N::mma(acc[n][at], a0, a1, a2, a3, pb_lo[q][n][0], pb_lo[q][n][1]);
+          }
+        };
+        if constexpr (BITS == 8) {
+          #pragma unroll
+          for (int q = 0; q < S::kValWords; ++q)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sel = h == 0 ? 0x5140 : 0x7362;
+              uint32_t a0, a1, a2, a3;
+              N::dec8(__byte_perm(vw[0][q], vw[1][q], sel), a0, a1);
+              N::dec8(__byte_perm(vw[2][q], vw[3][q], sel), a2, a3);
+              tile(2 * q + h, 0, a0, a1, a2, a3);
+            }
+        } else {
+          #pragma unroll
+          for (int c = 0; c < S::kChunks; ++c)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sel = h == 0 ? 0x5410 : 0x7632;
+              uint32_t x[4], y[4];
+              N::dec4(__byte_perm(vw[0][c], vw[1][c], sel), x);
+              N::dec4(__byte_perm(vw[2][c], vw[3][c], sel), y);
+              tile(4 * c + 2 * h, c, x[0], x[1], y[0], y[1]);
+              tile(4 * c + 2 * h + 1, c, x[2], x[3], y[2], y[3]);
+            }
+        }
+      }
+      if (i + 1 < n_tiles) {
+        load_values();
+        load_values_at(i + 1);
       }
     }
-    float top = s;
+
+    // -------------------------------------------- join the warps of the CTA
     #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    if ((t & 31) == 0) red[t >> 5] = top;
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        #pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], o);
+        if (g == 0) {
+          sm_m[warp * S::kRows + 8 * n + 2 * t + x] = m[n][x];
+          sm_l[warp * S::kRows + 8 * n + 2 * t + x] = l[n][x];
+        }
+      }
     __syncthreads();
-    const float mn = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-    const float keep = m == -INFINITY ? 0.f : __expf(m - mn);
-    w[t] = s == -INFINITY ? 0.f : expf(s - mn);
-    __syncthreads();
-    m = mn;
-    l *= keep;
-    for (int i = 0; i < kTile; ++i) l += w[i];
     #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = e * kTile + t;
-      o[e] *= keep;
-      for (int i = 0; i < kTile && d < D; ++i) {
-        if (w[i] == 0.f) continue;
-        const int jj = j0 + i, page = p.page_table[b * p.table_stride + (jj >> kv.page_shift)];
-        const kvc::RowAt v = kvc::row_at(kv, ((long long)page << kv.page_shift) + (jj & ((1 << kv.page_shift) - 1)),
-                                         kv_head, true);
-        const float c = kv.bits == 8 ? (float)(signed char)v.codes[d]
-                                     : (float)((int)((v.codes[d >> 1] >> (4 * (d & 1))) & 15) - 8);
-        o[e] = fmaf(w[i] * kvc::bf16_bits_to_f(v.scales[kv.groups > 1 ? d / kvc::kGroup4 : 0]), c, o[e]);
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = 8 * n + 2 * t + x;
+        float top = -INFINITY;
+        #pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
+        // one after the other: their product can be too small for fp32
+        const float f = m[n][x] == top ? 1.f : ex2<N::kSplit>(m[n][x] - top), unit = 1.f / fac[n][x];
+        float* dst = sm_o + (warp * S::kRows + row) * D;
+        #pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) {
+          // elements 2i, 2i + 1 of the lane's eighth (8 bits), or of its 8 in each 64 (4 bits)
+          const int d = BITS == 8 ? g * (D / 8) + 2 * i : (i / 4) * 64 + g * 8 + 2 * (i % 4);
+          *reinterpret_cast<float2*>(dst + d) = make_float2(acc[n][i][x] * unit * f, acc[n][i][2 + x] * unit * f);
+        }
+      }
+    __syncthreads();
+
+    const long long item_begin = base + item * per_item;
+    const bool whole = k_begin == 0 && k_end == per_item;
+    const int c_first = whole ? 0 : work.cta_of(item_begin);
+    float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
+    // a row's sum and output over the warps, in warp order; whole items end here
+    for (int e = threadIdx.x; e < rows * D; e += kThreads) {
+      const int row = e / D, d = e - row * D;
+      float top = -INFINITY, sum = 0.f, o = 0.f;
+      #pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
+      #pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = sm_m[w * S::kRows + row];
+        sum += sm_l[w * S::kRows + row] * (mw == top ? 1.f : ex2<N::kSplit>(mw - top));
+        o += sm_o[(w * S::kRows + row) * D + d];
+      }
+      if (whole) {
+        const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
+        const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
+        static_cast<T*>(p.out)[at * D + d] = kvc::from_f<T>(sum == 0.f ? 0.f : o / sum);
+        if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+      } else {
+        mine_out[2 * S::kRows + row * D + d] = o;
+        if (d == 0) {
+          mine_out[row] = top;
+          mine_out[S::kRows + row] = sum;
+        }
       }
     }
-    __syncthreads();
+
+    if (!whole) {
+      // ---------------------------- the last CTA of the item joins its parts
+      const int c_last = work.cta_of(item_begin + per_item - 1), parts = c_last - c_first + 1;
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) last_one = atomic_add_acq_rel_gpu(counters + c_first, 1u) == (unsigned)parts - 1;
+      __syncthreads();
+      if (last_one) {
+        if (threadIdx.x == 0) counters[c_first] = 0;
+        auto part = [&](int q) {                        // the first begins the item: its CTA's second slot
+          return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
+        };
+        for (int e = threadIdx.x; e < rows * D; e += kThreads) {
+          const int row = e / D, d = e - row * D;
+          float top = -INFINITY, sum = 0.f, o = 0.f;
+          for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(part(q) + row));
+          for (int q = 0; q < parts; ++q) {
+            const float* src = part(q);
+            const float mq = __ldcg(src + row), f = mq == top ? 1.f : ex2<N::kSplit>(mq - top);
+            sum += __ldcg(src + S::kRows + row) * f;
+            o += __ldcg(src + 2 * S::kRows + row * D + d) * f;
+          }
+          const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
+          const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
+          static_cast<T*>(p.out)[at * D + d] = kvc::from_f<T>(sum == 0.f ? 0.f : o / sum);
+          if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+        }
+      }
+    }
+    __syncthreads();                                    // before the next segment reuses shared memory
+    u += k_end - k_begin;
   }
-  #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e * kTile + t < D)
-      static_cast<T*>(p.out)[((long long)token * p.q_heads + head) * D + e * kTile + t] =
-          kvc::from_f<T>(l == 0.f ? 0.f : o[e] / l);
-  if (p.lse && t == 0) p.lse[(long long)token * p.q_heads + head] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 }  // namespace att

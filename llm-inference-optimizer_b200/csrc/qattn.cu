@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
@@ -18,6 +19,8 @@ namespace {
 using ql::kvc::Pool;
 using ql::kvc::Rows;
 using ql::kvc::Turn;
+
+constexpr int kMaxDevices = 64;
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -120,13 +123,70 @@ int run_append(const ql::kvc::AppendParams& p, int64_t head_dim, void* stream, i
   }
 }
 
+// Raise the dynamic shared-memory limit of a kernel once per device.
+template <typename Kern>
+int allow_smem(Kern kernel, size_t bytes, std::atomic<unsigned char>* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    cudaGetLastError();
+    return QL_ERR_DEVICE;
+  }
+  if (done[dev].load(std::memory_order_acquire)) return QL_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return QL_ERR_CUDA;
+  }
+  done[dev].store(1, std::memory_order_release);
+  return QL_OK;
+}
+
+struct Attention {
+  ql::att::Params p;
+  int64_t max_q, max_kv, flags;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+  int sms;
+};
+
+template <int D, int BITS, int NT>
+size_t stream_workspace(int sms) {
+  using S = ql::att::Shape<D, BITS, NT>;
+  const size_t ctas = std::min(ql::att::kMaxCtas, S::kCtas * sms);
+  return ql::att::kHeaderBytes + 2 * ctas * S::kPartial * sizeof(float);
+}
+
+template <typename T, int D, int BITS, int NT>
+int run_stream(const Attention& a) {
+  using S = ql::att::Shape<D, BITS, NT>;
+  if (a.workspace_bytes < stream_workspace<D, BITS, NT>(a.sms)) return QL_ERR_WORKSPACE;
+  auto kernel = ql::att::stream_kernel<T, D, BITS, NT>;
+  static std::atomic<unsigned char> done[kMaxDevices];
+  const int st = allow_smem(kernel, S::kSmem, done);
+  if (st != QL_OK) return st;
+  // as many CTAs as the SMs hold at once, and no more than the bounds on the work can use
+  const int64_t tiles = cdiv(std::max<int64_t>(a.max_q, 1) * a.p.group, S::kRows);
+  const int64_t runs = cdiv(std::max<int64_t>(a.max_kv, 1), ql::att::kUnitKeys * ql::att::kMinUnits);
+  int64_t ctas = std::min<int64_t>(ql::att::kMaxCtas, (int64_t)S::kCtas * a.sms);
+  const double bound = (double)a.p.batch * a.p.cache.heads * (double)tiles * (double)runs;
+  if (bound < (double)ctas) ctas = std::max<int64_t>((int64_t)bound, 1);
+  return launch(kernel, dim3((unsigned)ctas), dim3(ql::att::kThreads), S::kSmem, a.stream, a.flags, a.p,
+                static_cast<unsigned*>(a.workspace),
+                reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes));
+}
+
+template <typename T, int D, int BITS>
+int run_rows(const Attention& a) {
+  return a.max_q * a.p.group <= 8 ? run_stream<T, D, BITS, 1>(a) : run_stream<T, D, BITS, 2>(a);
+}
+
 template <typename T>
-int run_attention(const ql::att::Params& p, int64_t head_dim, void* stream, int64_t flags) {
-  const dim3 grid((unsigned)p.q_heads, (unsigned)p.total_q), block(ql::att::kTile);
+int run_attention(const Attention& a, int64_t head_dim) {
+  const bool eight = a.p.cache.bits == 8;
   switch (head_dim) {
-    case 64: return launch(ql::att::simple_kernel<T, 64>, grid, block, 0, stream, flags, p);
-    case 128: return launch(ql::att::simple_kernel<T, 128>, grid, block, 0, stream, flags, p);
-    default: return launch(ql::att::simple_kernel<T, 256>, grid, block, 0, stream, flags, p);
+    case 64: return eight ? run_rows<T, 64, 8>(a) : run_rows<T, 64, 4>(a);
+    case 128: return eight ? run_rows<T, 128, 8>(a) : run_rows<T, 128, 4>(a);
+    default: return eight ? run_rows<T, 256, 8>(a) : run_rows<T, 256, 4>(a);
   }
 }
 
@@ -234,11 +294,11 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   if (a->q_heads % a->cache.kv_heads != 0) return QL_ERR_BAD_SHAPE;
   if (a->batch == 0 || a->total_q == 0 || a->q_heads == 0) return QL_OK;
   if (!a->cu_q && a->total_q % a->batch != 0) return QL_ERR_BAD_SHAPE;
-  if (!a->out || !a->kv_lens || (!a->page_table && a->table_width > 0)) return QL_ERR_NULL_POINTER;
+  if (!a->out || !a->kv_lens || !a->workspace || (!a->page_table && a->table_width > 0)) return QL_ERR_NULL_POINTER;
   if ((st = make_rows(&p.q, a->q, a->q_token_stride, a->q_head_stride, a->cache.head_dim)) != QL_OK) return st;
   if (a->table_stride < a->table_width) return QL_ERR_BAD_STRIDE;
   if (!aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->page_table, 4) || !aligned(a->kv_lens, 4) ||
-      !aligned(a->cu_q, 4) || !aligned(a->mask, 8))
+      !aligned(a->cu_q, 4) || !aligned(a->mask, 8) || !aligned(a->workspace, 16))
     return QL_ERR_UNSUPPORTED;
   ql_host::Device dev;
   if ((st = ql_host::current(&dev)) != QL_OK) return st;
@@ -256,10 +316,23 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   p.q_heads = (int)a->q_heads;
   p.group = (int)(a->q_heads / a->cache.kv_heads);
   p.mask_words = (int)a->mask_words;
-  p.scale = (float)a->scale;
+  p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   p.err = dev.err_word;
-  return a->dtype == QL_DTYPE_F16 ? run_attention<__half>(p, a->cache.head_dim, stream, a->flags)
-                                  : run_attention<__nv_bfloat16>(p, a->cache.head_dim, stream, a->flags);
+  const Attention work = {p, a->max_q, a->max_kv, a->flags, a->workspace, (size_t)std::max<int64_t>(a->workspace_bytes, 0),
+                          stream, dev.sms};
+  return a->dtype == QL_DTYPE_F16 ? run_attention<__half>(work, a->cache.head_dim)
+                                  : run_attention<__nv_bfloat16>(work, a->cache.head_dim);
+}
+
+size_t ql_tree_attention_workspace_size(int64_t head_dim) {
+  ql_host::Device dev;
+  if (ql_host::current(&dev) != QL_OK) return 0;
+  switch (head_dim) {   // the largest of the variants' (equal for 8 and 4 bits)
+    case 64: return std::max(stream_workspace<64, 8, 1>(dev.sms), stream_workspace<64, 8, 2>(dev.sms));
+    case 128: return std::max(stream_workspace<128, 8, 1>(dev.sms), stream_workspace<128, 8, 2>(dev.sms));
+    case 256: return std::max(stream_workspace<256, 8, 1>(dev.sms), stream_workspace<256, 8, 2>(dev.sms));
+    default: return 0;
+  }
 }
 
 }  // extern "C"

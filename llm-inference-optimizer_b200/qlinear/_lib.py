@@ -103,6 +103,7 @@ SIGNATURES = {
     "ql_rotary": (_int, [ctypes.c_char_p, _vp]),
     "ql_kv_append": (_int, [ctypes.c_char_p, _vp]),
     "ql_kv_read": (_int, [ctypes.c_char_p, _vp]),
+    "ql_tree_attention_workspace_size": (_sz, [_i64]),
     "ql_tree_attention": (_int, [ctypes.c_char_p, _vp]),
     "ql_strerror": (ctypes.c_char_p, [_int]),
     "ql_version": (_int, []),
@@ -117,7 +118,7 @@ KV_CACHE_FIELDS = 13
 ROTARY_ARGS = struct.Struct("18q")
 KV_APPEND_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 24}q")
 KV_READ_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 7}q")
-TREE_ATTENTION_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 18}qdq")
+TREE_ATTENTION_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 18}qd3q")
 
 _lock = threading.Lock()
 _lib = None

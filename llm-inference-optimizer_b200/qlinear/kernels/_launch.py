@@ -41,6 +41,29 @@ def workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> t
     return buf
 
 
+_scratches: dict[tuple[int, int], torch.Tensor] = {}
+_SCRATCH_HEADER = 4096
+
+
+def scratch(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> torch.Tensor:
+    """Scratch whose head alone is kept zero by the kernels, one per (device,
+    stream) as `workspace`.  A stream that has none while it is being captured
+    gets one of the graph's own, whose head the graph clears."""
+    key = (device.index, stream.cuda_stream)
+    buf = _scratches.get(key)
+    if buf is None or buf.numel() < nbytes:
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buf[:_SCRATCH_HEADER].zero_()
+            return buf
+        with _ws_lock:
+            buf = _scratches.get(key)
+            if buf is None or buf.numel() < nbytes:
+                buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+                _scratches[key] = buf
+    return buf
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -102,7 +125,7 @@ def activation_code(t: torch.Tensor, what: str) -> int:
 
 
 def call(entry, packed: bytes, device: torch.device) -> None:
-    """entry(packed arguments, current stream) with `device` current."""
+    """entry(packed arguments, current stream) with `device` current (the ABI uses the current device)."""
     if torch.cuda.current_device() == device.index:
         status = entry(packed, torch.cuda.current_stream(device).cuda_stream)
     else:

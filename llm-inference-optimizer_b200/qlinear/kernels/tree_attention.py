@@ -12,8 +12,20 @@ import math
 import torch
 
 from .. import _lib
-from ._launch import activation_code, call, default_flags
+from ._launch import activation_code, call, default_flags, on_device, scratch
 from .kv_cache import QuantizedKVCache
+
+
+_workspace_bytes: dict[tuple[int, int], int] = {}
+
+
+def _workspace(device: torch.device, head_dim: int) -> torch.Tensor:
+    nbytes = _workspace_bytes.get((device.index, head_dim))
+    if nbytes is None:
+        with on_device(device):
+            nbytes = _lib.load().ql_tree_attention_workspace_size(head_dim)
+        _workspace_bytes[device.index, head_dim] = nbytes
+    return scratch(device, torch.cuda.current_stream(device), nbytes)
 
 
 def pack_tree_mask(visible: torch.Tensor) -> torch.Tensor:
@@ -112,11 +124,13 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
             max_q = total_q // batch if cu_q is None else total_q
         if max_kv is None:
             max_kv = width * cache.page_size
+        ws = _workspace(dev, head_dim)
         packed = _lib.TREE_ATTENTION_ARGS.pack(
             *cache.fields, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(),
             kv_lens.data_ptr(), cu_ptr, mask_ptr, batch, total_q, q_heads, qs[0], qs[1], width,
             page_table.stride(0) if batch > 1 else width, words, max_q, max_kv, dtype,
-            1.0 / math.sqrt(head_dim) if scale is None else scale, default_flags())
+            1.0 / math.sqrt(head_dim) if scale is None else scale, ws.data_ptr(),
+            ws.numel(), default_flags())
         call(_lib.load().ql_tree_attention, packed, dev)
     return (out, lse) if return_lse else out
 

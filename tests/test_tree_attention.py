@@ -43,7 +43,7 @@ def test_host_checks_without_gpu():
                  kps=2048, vps=2048, ksps=32, vsps=32,
                  q=64, out=64, lse=0, page_table=64, kv_lens=64, cu_q=0, mask=0, batch=2, total_q=2, q_heads=4,
                  qt=256, qh=64, table_width=2, table_stride=2, mask_words=0, max_q=1, max_kv=32,
-                 dtype=_lib.QL_DTYPE_F16, scale=0.1, flags=0)
+                 dtype=_lib.QL_DTYPE_F16, scale=0.1, ws=1024, ws_bytes=1 << 30, flags=0)
         f.update(change)
         return lib.ql_tree_attention(_lib.TREE_ATTENTION_ARGS.pack(*f.values()), None)
 
@@ -55,6 +55,8 @@ def test_host_checks_without_gpu():
     assert call(kv_lens=0) == _lib.QL_ERR_NULL_POINTER
     assert call(page_table=0) == _lib.QL_ERR_NULL_POINTER
     assert call(kc=0) == _lib.QL_ERR_NULL_POINTER
+    assert call(ws=0) == _lib.QL_ERR_NULL_POINTER
+    assert call(ws=1032) == _lib.QL_ERR_UNSUPPORTED
     assert call(total_q=3) == _lib.QL_ERR_BAD_SHAPE                 # uneven without cu_q
     assert call(q_heads=5) == _lib.QL_ERR_BAD_SHAPE
     assert call(batch=-1) == _lib.QL_ERR_BAD_SHAPE
