@@ -62,6 +62,7 @@ __device__ __forceinline__ bool sees(const Params& p, const Request& r, int i, i
 // the CTAs take equal runs of units, whatever the requests' lengths are: a
 // CTA may end one item, do some whole and begin another.  Lengths are read
 // on the device, so a captured launch serves other lengths later.
+constexpr float kLow = -1e30f;             // below every score: a maximum of nothing, finite so that differences are
 constexpr int kUnitKeys = 128;
 constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
 constexpr int kThreads = 32 * kWarps;
@@ -160,68 +161,48 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// A row's factor brings its largest weight just under 2^kTopWeight, and again
-// when one passes kMostWeight: high in fp16's range, and in bf16's neither so
-// low that a small one's remainder is lost, nor so high that the matrix
-// unit, which aligns a large weight times a code of 0 by the weight's
-// exponent, drops a small one beside it.
-constexpr int kTopWeight = 11;
-constexpr float kMostWeight = 0x1p15f;
-// The 16-bit type of the products: the codes are exact in both.  fp16 takes
-// the weights rounded once (11 bits); bf16, whose outputs have fp32's range,
-// as a sum of two (16 bits).
-template <typename T> struct Num;
-template <> struct Num<__half> {
-  static constexpr bool kSplit = false;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  // 4 signed bytes -> (0, 1), (2, 3)
-  static __device__ __forceinline__ void dec8(uint32_t u, uint32_t& p01, uint32_t& p23) { dec_w8(u, p01, p23); }
-  // 16-bit lanes of 4 nibbles (codes + 8) -> nibble i of both lanes
-  static __device__ __forceinline__ void dec4(uint32_t u, uint32_t (&v)[4]) {
-    const uint32_t w = u >> 8;
-    v[0] = h2_sub(lop3_and_or(u, 0x000F000Fu, kH2Magic), kH2_1032);
-    v[1] = h2_fma(lop3_and_or(u, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
-    v[2] = h2_sub(lop3_and_or(w, 0x000F000Fu, kH2Magic), kH2_1032);
-    v[3] = h2_fma(lop3_and_or(w, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    mma_16816(d, a0, a1, a2, a3, b0, b1);
-  }
-};
-template <> struct Num<__nv_bfloat16> {
-  static constexpr bool kSplit = true;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  // 0x43bb with the byte's sign bit cleared is 128 + its low 7 bits; with the
-  // low 7 bits cleared it is 128, or 256 where the sign bit is set: their
-  // difference is the signed byte
-  static __device__ __forceinline__ uint32_t signed_bytes(uint32_t t) { return sub(t & 0xFF7FFF7Fu, t & 0xFF80FF80u); }
-  static __device__ __forceinline__ void dec8(uint32_t u, uint32_t& p01, uint32_t& p23) {
-    p01 = signed_bytes(__byte_perm(u, 0x43434343u, 0x4140));
-    p23 = signed_bytes(__byte_perm(u, 0x43434343u, 0x4342));
-  }
-  static __device__ __forceinline__ void dec4(uint32_t u, uint32_t (&v)[4]) {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = sub(lop3_and_or(u >> (4 * i), 0x000F000Fu, 0x43004300u), 0x43084308u);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
+// The codes are exact in both 16-bit types.
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t b2_sub(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// 16-bit lanes of 4 nibbles (codes + 8) -> nibble i of both lanes, fp16
+__device__ __forceinline__ void dec4_h(uint32_t u, uint32_t (&v)[4]) {
+  const uint32_t w = u >> 8;
+  v[0] = h2_sub(lop3_and_or(u, 0x000F000Fu, kH2Magic), kH2_1032);
+  v[1] = h2_fma(lop3_and_or(u, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
+  v[2] = h2_sub(lop3_and_or(w, 0x000F000Fu, kH2Magic), kH2_1032);
+  v[3] = h2_fma(lop3_and_or(w, 0x00F000F0u, kH2Magic), kH2_1_16, kH2_m72);
+}
+// the same in bf16: 0x430n is 128 + n
+__device__ __forceinline__ void dec4_b(uint32_t u, uint32_t (&v)[4]) {
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = b2_sub(lop3_and_or(u >> (4 * i), 0x000F000Fu, 0x43004300u), 0x43084308u);
+}
+// 4 signed bytes -> (0, 1), (2, 3) in bf16.  0x43bb with the byte's sign bit
+// cleared is 128 + its low 7 bits; with the low 7 bits cleared it is 128, or
+// 256 where the sign bit is set: their difference is the signed byte.
+__device__ __forceinline__ void dec8_b(uint32_t u, uint32_t& p01, uint32_t& p23) {
+  const uint32_t x = __byte_perm(u, 0x43434343u, 0x4140), y = __byte_perm(u, 0x43434343u, 0x4342);
+  p01 = b2_sub(x & 0xFF7FFF7Fu, x & 0xFF80FF80u);
+  p23 = b2_sub(y & 0xFF7FFF7Fu, y & 0xFF80FF80u);
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 // Cache codes: read once by this CTA, so not kept in L1.
 template <int WORDS>
 __device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const unsigned char* p) {
@@ -252,13 +233,17 @@ __device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const unsigned 
 //   O^T[d, row] = V^T P: lane (g, t) holds keys 2t, 2t + 1, 2t + 8, 2t + 9 and
 //     an eighth of head_dim; pairs of keys are joined by byte permutes, and
 //     the order of d within a tile of 16 is free (it only names the outputs).
-// The codes enter as exact integers of the calls' 16-bit type.  Key scales
-// multiply the scores afterwards; value scales multiply the weights, against
-// a factor per row that keeps the largest weight * scale seen high in the
-// type's range, so that the scales' size does not matter.
+// The codes enter as exact fp16 integers.  Key scales multiply the scores
+// afterwards; bf16 queries become fp16 by a power of two per row (their 8
+// significant bits fit).  Value scales multiply the weights, which are rounded
+// to fp16 once, against a power of two that follows the largest scale seen.
+// A tile with a weight below fp16's normal range (or a hidden key) takes the
+// product in bf16 instead, the weights as a sum of two: 16 bits and fp32's
+// range, so that no score far below the largest and no mixture of scales
+// costs precision; it needs twice the decoding and products.
 //
-// The running maximum of a row moves only when a score passes it by 6 (weights
-// up to 2^6): one vote per 16 keys stands for the reductions and the
+// The running maximum of a row moves only when a score passes it by 4 (weights
+// up to 2^4): one vote per 16 keys stands for the reductions and the
 // rescaling, which become rare.
 //
 // A key's scale is read by its own lanes; hidden keys are removed by
@@ -282,7 +267,7 @@ template <typename T, int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     stream_kernel(const Params p, unsigned* counters, float* partials) {
   using S = Shape<D, BITS, NT>;
-  using N = Num<T>;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ float smem[];
@@ -321,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
 
     // ------------------------------------------------------------- queries
     uint32_t qb[NT][S::kTiles][2];
+    float rs[NT][2];                                    // on the scores of rows 2t, 2t + 1, in units of log2
     #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + g;
@@ -328,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       const int token = live ? row / p.group : 0, qh = head * p.group + (live ? row - token * p.group : 0);
       const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
       float f[S::kChunks][16];
+      unsigned top = 0;
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
         #pragma unroll
@@ -338,8 +325,17 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           for (int e = 0; e < 4; ++e) {
             f[c][i + e] = x[e];
             f[c][i + 4 + e] = y[e];
+            top = max(top, max(__float_as_uint(x[e]) & 0x7FFFFFFFu, __float_as_uint(y[e]) & 0x7FFFFFFFu));
           }
         }
+      float down = 1.f, up = 1.f;
+      if constexpr (kBf16) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top >= 0x7F800000u ? 0 : min(max((int)(top >> 23) - 127, -126), 126);
+        down = pow2(-e);
+        up = pow2(e);
+      }
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
         #pragma unroll
@@ -349,13 +345,17 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             // 8 bits: steps of 4 neighbours; 4 bits: elements i and i + 4 of 8 share a word
             const int i = BITS == 8 ? 4 * w + 2 * x : 8 * (w >> 1) + 2 * (w & 1) + x;
             const int j = BITS == 8 ? i + 1 : i + 4;
-            qb[n][4 * c + w][x] = N::pack(f[c][i], f[c][j]);
+            qb[n][4 * c + w][x] = pack_h2(f[c][i] * down, f[c][j] * down);
           }
+      #pragma unroll
+      for (int x = 0; x < 2; ++x)
+        rs[n][x] = kBf16 ? __shfl_sync(0xffffffffu, up, (2 * t + x) * 4) * p.scale_log2 : p.scale_log2;
     }
 
     // ---------------------------------------------------------- running state
     float acc[NT][S::kTiles][4];
-    float m[NT][2], l[NT][2], fac[NT][2];
+    float m[NT][2], l[NT][2];
+    float v_ref = 0.f, fac = 1.f;                       // power of two at least every value scale seen; on the weights
     #pragma unroll
     for (int n = 0; n < NT; ++n) {
       #pragma unroll
@@ -364,9 +364,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
       #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        m[n][x] = -INFINITY;
+        m[n][x] = kLow;
         l[n][x] = 0.f;
-        fac[n][x] = 1.f;
       }
     }
 
@@ -466,19 +465,19 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         for (int w = 0; w < S::kKeyWords; ++w) {
           if constexpr (BITS == 8) {
             uint32_t a0, a1, a2, a3;
-            N::dec8(kw[0][c][w], a0, a2);
-            N::dec8(kw[1][c][w], a1, a3);
+            dec_w8(kw[0][c][w], a0, a2);
+            dec_w8(kw[1][c][w], a1, a3);
             #pragma unroll
-            for (int n = 0; n < NT; ++n) N::mma(part[n], a0, a1, a2, a3, qb[n][4 * c + w][0], qb[n][4 * c + w][1]);
+            for (int n = 0; n < NT; ++n) mma_16816(part[n], a0, a1, a2, a3, qb[n][4 * c + w][0], qb[n][4 * c + w][1]);
           } else {
             uint32_t x[4], y[4];
-            N::dec4(kw[0][c][w], x);
-            N::dec4(kw[1][c][w], y);
+            dec4_h(kw[0][c][w], x);
+            dec4_h(kw[1][c][w], y);
             #pragma unroll
             for (int h = 0; h < 2; ++h)
               #pragma unroll
               for (int n = 0; n < NT; ++n)
-                N::mma(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * c + 2 * w + h][0],
+                mma_16816(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * c + 2 * w + h][0],
                           qb[n][4 * c + 2 * w + h][1]);
           }
         }
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           #pragma unroll
           for (int n = 0; n < NT; ++n)
             #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(part[n][e], (e < 2 ? k0 : k1) * p.scale_log2, s[n][e]);
+            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(part[n][e], (e < 2 ? k0 : k1) * rs[n][e & 1], s[n][e]);
         }
       }
       if constexpr (BITS == 8) {
@@ -500,12 +499,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         #pragma unroll
         for (int n = 0; n < NT; ++n)
           #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] *= (e < 2 ? k0 : k1) * p.scale_log2;
+          for (int e = 0; e < 4; ++e) s[n][e] *= (e < 2 ? k0 : k1) * rs[n][e & 1];
       }
       if (i + 1 < n_tiles) load_keys(i + 1);
 
       // ------------------------------------------------- what the rows see
-      if (hidden || j0 + 15 >= context) {
+      const bool some_hidden = hidden || j0 + 15 >= context;
+      if (some_hidden) {
         #pragma unroll
         for (int n = 0; n < NT; ++n)
           #pragma unroll
@@ -517,94 +517,67 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       }
 
       // ------------------------------------------------------------ weights
-      float v_top[2], v_sc[2][S::kGroups];
+      float v_top = 0.f, v_sc[2][S::kGroups];
       #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        v_top[x] = 0.f;
+      for (int x = 0; x < 2; ++x)
         #pragma unroll
         for (int q = 0; q < S::kGroups; ++q) {
           v_sc[x][q] = kvc::bf16_bits_to_f(vs[x][q]);
-          v_top[x] = fmaxf(v_top[x], v_sc[x][q]);
+          v_top = fmaxf(v_top, v_sc[x][q]);
         }
-      }
-      float w[NT][4];
-      bool move[NT][2] = {}, any_move = false;
+      bool move = v_top > v_ref;
       #pragma unroll
       for (int n = 0; n < NT; ++n)
         #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float top = m[n][e & 1];
-          w[n][e] = s[n][e] == -INFINITY ? 0.f : ex2<N::kSplit>(s[n][e] - (top == -INFINITY ? 0.f : top));
-          move[n][e & 1] |= s[n][e] > top + 6.f || (w[n][e] != 0.f && w[n][e] * v_top[e >> 1] * fac[n][e & 1] > kMostWeight);
-          any_move |= move[n][e & 1];
+        for (int e = 0; e < 4; ++e) move |= s[n][e] > m[n][e & 1] + 4.f;
+      if (__any_sync(0xffffffffu, move)) {
+        const unsigned bits = __float_as_uint(v_top);
+        const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, some_hidden || bits >= 0x7F800000u ? 0u : bits));
+        float adjust = 1.f;
+        if (most > v_ref) {
+          const int e = max((int)((__float_as_uint(most) + 0x007FFFFFu) >> 23) - 127, -100);   // 2^e >= most
+          v_ref = e > 127 ? INFINITY : pow2(e);
+          adjust = pow2(11 - e) / fac;
+          fac = pow2(11 - e);
         }
-      if (__any_sync(0xffffffffu, any_move)) {
         #pragma unroll
         for (int n = 0; n < NT; ++n)
           #pragma unroll
           for (int x = 0; x < 2; ++x) {
             // a row's own lanes alone move it, so that its bits do not depend on the other rows
-            const bool row_moves = __ballot_sync(0xffffffffu, move[n][x]) & (0x11111111u << t);
+            const bool moves = s[n][x] > m[n][x] + 4.f || s[n][2 + x] > m[n][x] + 4.f;
+            const bool row_moves = __ballot_sync(0xffffffffu, moves) & (0x11111111u << t);
             float top = fmaxf(s[n][x], s[n][2 + x]);
             #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m[n][x]);
-            const float keep = m[n][x] == top ? 1.f : ex2<N::kSplit>(m[n][x] - top);
-            float most = 0.f;
-            #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float sv = s[n][2 * h + x];
-              const float moved = sv == -INFINITY ? 0.f : ex2<N::kSplit>(sv - (top == -INFINITY ? 0.f : top));
-              const float wv = moved * v_top[h];
-              if (row_moves) w[n][2 * h + x] = moved;
-              if (wv > 0.f && wv < INFINITY) most = fmaxf(most, wv);
-            }
-            #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // the factor that brings the largest weight just under 2^kTopWeight, and none of the earlier ones above that
-            const int e = (int)(__float_as_uint(most) >> 23) - 126;
-            float next = keep > 0.f ? fminf(fac[n][x] / keep, 0x1p100f) : 0x1p100f;
-            if (most > 0.f) next = fminf(next, __uint_as_float((unsigned)min(max(kTopWeight - e + 127, 1), 227) << 23));
-            const float adjust = keep > 0.f ? keep * (next / fac[n][x]) : 0.f;
-            if (!row_moves) continue;
+            const float keep = row_moves ? ex2<kBf16>(m[n][x] - top) : 1.f;
+            if (row_moves) m[n][x] = top;
             #pragma unroll
             for (int q = 0; q < S::kTiles; ++q) {
-              acc[n][q][x] *= adjust;
-              acc[n][q][2 + x] *= adjust;
+              acc[n][q][x] *= keep * adjust;
+              acc[n][q][2 + x] *= keep * adjust;
             }
             l[n][x] *= keep;
-            m[n][x] = top;
-            fac[n][x] = next;
           }
       }
-      uint32_t pb[S::kGroups][NT][2], pb_lo[S::kGroups][NT][2];
+      float least = INFINITY, a[S::kGroups][NT][4];
       #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n)
         #pragma unroll
-        for (int e = 0; e < 4; ++e) l[n][e & 1] += w[n][e];
-        #pragma unroll
-        for (int q = 0; q < S::kGroups; ++q)
+        for (int e = 0; e < 4; ++e) {
+          const float w = ex2<kBf16>(s[n][e] - m[n][e & 1]);
+          l[n][e & 1] += w;
           #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const bool z0 = s[n][2 * h] == -INFINITY, z1 = s[n][2 * h + 1] == -INFINITY;
-            const float a = z0 ? 0.f : w[n][2 * h] * v_sc[h][q] * fac[n][0];
-            const float c = z1 ? 0.f : w[n][2 * h + 1] * v_sc[h][q] * fac[n][1];
-            const uint32_t hi = N::pack(a, c);
-            pb[q][n][h] = transpose8(hi);
-            if constexpr (N::kSplit)
-              pb_lo[q][n][h] = transpose8(N::pack(a - __uint_as_float(hi << 16), c - __uint_as_float(hi & 0xFFFF0000u)));
+          for (int q = 0; q < S::kGroups; ++q) {
+            a[q][n][e] = w * (v_sc[e >> 1][q] * fac);
+            least = fminf(least, a[q][n][e]);
           }
-      }
+        }
+      const bool wide = some_hidden || __any_sync(0xffffffffu, least < 0x1p-14f);
 
       // -------------------------------------------------------------- values
-      if (!hidden) {
-        auto tile = [&](int at, int q, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-          #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            N::mma(acc[n][at], a0, a1, a2, a3, pb[q][n][0], pb[q][n][1]);
-            if constexpr (N::kSplit) N::mma(acc[n][at], a0, a1, a2, a3, pb_lo[q][n][0], pb_lo[q][n][1]);
-          }
-        };
+      // products of 16 keys' values, decoded by dec8 / dec4, tile by tile of 16 elements
+      auto products = [&](auto dec8, auto dec4, auto tile) {
         if constexpr (BITS == 8) {
           #pragma unroll
           for (int q = 0; q < S::kValWords; ++q)
@@ -612,8 +585,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             for (int h = 0; h < 2; ++h) {
               const uint32_t sel = h == 0 ? 0x5140 : 0x7362;
               uint32_t a0, a1, a2, a3;
-              N::dec8(__byte_perm(vw[0][q], vw[1][q], sel), a0, a1);
-              N::dec8(__byte_perm(vw[2][q], vw[3][q], sel), a2, a3);
+              dec8(__byte_perm(vw[0][q], vw[1][q], sel), a0, a1);
+              dec8(__byte_perm(vw[2][q], vw[3][q], sel), a2, a3);
               tile(2 * q + h, 0, a0, a1, a2, a3);
             }
         } else {
@@ -623,12 +596,50 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             for (int h = 0; h < 2; ++h) {
               const uint32_t sel = h == 0 ? 0x5410 : 0x7632;
               uint32_t x[4], y[4];
-              N::dec4(__byte_perm(vw[0][c], vw[1][c], sel), x);
-              N::dec4(__byte_perm(vw[2][c], vw[3][c], sel), y);
+              dec4(__byte_perm(vw[0][c], vw[1][c], sel), x);
+              dec4(__byte_perm(vw[2][c], vw[3][c], sel), y);
               tile(4 * c + 2 * h, c, x[0], x[1], y[0], y[1]);
               tile(4 * c + 2 * h + 1, c, x[2], x[3], y[2], y[3]);
             }
         }
+      };
+      if (!wide) {
+        uint32_t pb[S::kGroups][NT][2];
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q)
+          #pragma unroll
+          for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) pb[q][n][h] = transpose8(pack_h2(a[q][n][2 * h], a[q][n][2 * h + 1]));
+        products([](uint32_t u, uint32_t& x, uint32_t& y) { dec_w8(u, x, y); },
+                 [](uint32_t u, uint32_t (&v)[4]) { dec4_h(u, v); },
+                 [&](int at, int q, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                   #pragma unroll
+                   for (int n = 0; n < NT; ++n) mma_16816(acc[n][at], a0, a1, a2, a3, pb[q][n][0], pb[q][n][1]);
+                 });
+      } else if (!hidden) {
+        uint32_t hi[S::kGroups][NT][2], lo[S::kGroups][NT][2];
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q)
+          #pragma unroll
+          for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = s[n][2 * h] == -INFINITY ? 0.f : a[q][n][2 * h];
+              const float y = s[n][2 * h + 1] == -INFINITY ? 0.f : a[q][n][2 * h + 1];
+              const uint32_t u = pack_b2(x, y);
+              hi[q][n][h] = transpose8(u);
+              lo[q][n][h] = transpose8(pack_b2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
+            }
+        products([](uint32_t u, uint32_t& x, uint32_t& y) { dec8_b(u, x, y); },
+                 [](uint32_t u, uint32_t (&v)[4]) { dec4_b(u, v); },
+                 [&](int at, int q, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                   #pragma unroll
+                   for (int n = 0; n < NT; ++n) {
+                     mma_bf16(acc[n][at], a0, a1, a2, a3, hi[q][n][0], hi[q][n][1]);
+                     mma_bf16(acc[n][at], a0, a1, a2, a3, lo[q][n][0], lo[q][n][1]);
+                   }
+                 });
       }
       if (i + 1 < n_tiles) {
         load_values();
@@ -654,11 +665,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int row = 8 * n + 2 * t + x;
-        float top = -INFINITY;
+        float top = kLow;
         #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
         // one after the other: their product can be too small for fp32
-        const float f = m[n][x] == top ? 1.f : ex2<N::kSplit>(m[n][x] - top), unit = 1.f / fac[n][x];
+        const float f = ex2<kBf16>(m[n][x] - top), unit = 1.f / fac;
         float* dst = sm_o + (warp * S::kRows + row) * D;
         #pragma unroll
         for (int i = 0; i < S::kTiles; ++i) {
@@ -676,13 +687,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     // a row's sum and output over the warps, in warp order; whole items end here
     for (int e = threadIdx.x; e < rows * D; e += kThreads) {
       const int row = e / D, d = e - row * D;
-      float top = -INFINITY, sum = 0.f, o = 0.f;
+      float top = kLow, sum = 0.f, o = 0.f;
       #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
       #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float mw = sm_m[w * S::kRows + row];
-        sum += sm_l[w * S::kRows + row] * (mw == top ? 1.f : ex2<N::kSplit>(mw - top));
+        sum += sm_l[w * S::kRows + row] * ex2<kBf16>(mw - top);
         o += sm_o[(w * S::kRows + row) * D + d];
       }
       if (whole) {
@@ -713,11 +724,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         };
         for (int e = threadIdx.x; e < rows * D; e += kThreads) {
           const int row = e / D, d = e - row * D;
-          float top = -INFINITY, sum = 0.f, o = 0.f;
+          float top = kLow, sum = 0.f, o = 0.f;
           for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(part(q) + row));
           for (int q = 0; q < parts; ++q) {
             const float* src = part(q);
-            const float mq = __ldcg(src + row), f = mq == top ? 1.f : ex2<N::kSplit>(mq - top);
+            const float mq = __ldcg(src + row), f = ex2<kBf16>(mq - top);
             sum += __ldcg(src + S::kRows + row) * f;
             o += __ldcg(src + 2 * S::kRows + row * D + d) * f;
           }

@@ -45,11 +45,11 @@ _scratches: dict[tuple[int, int], torch.Tensor] = {}
 _SCRATCH_HEADER = 4096
 
 
-def scratch(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> torch.Tensor:
+def scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch whose head alone is kept zero by the kernels, one per (device,
-    stream) as `workspace`.  A stream that has none while it is being captured
-    gets one of the graph's own, whose head the graph clears."""
-    key = (device.index, stream.cuda_stream)
+    stream handle) as `workspace`.  A stream that has none while it is being
+    captured gets one of the graph's own, whose head the graph clears."""
+    key = (device.index, stream)
     buf = _scratches.get(key)
     if buf is None or buf.numel() < nbytes:
         if torch.cuda.is_current_stream_capturing():
@@ -106,30 +106,38 @@ class on_device:
         return False
 
 
+_INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
+_ACTIVATION_CODES = {torch.float16: _lib.QL_DTYPE_F16, torch.bfloat16: _lib.QL_DTYPE_BF16}
+
+
 def index_bytes(t: torch.Tensor, what: str) -> int:
     """4 or 8 for an int32 / int64 index tensor."""
-    if t.dtype == torch.int64:
-        return 8
-    if t.dtype == torch.int32:
-        return 4
-    raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    n = _INDEX_BYTES.get(t.dtype)
+    if n is None:
+        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    return n
 
 
-def activation_code(t: torch.Tensor, what: str) -> int:
+def activation_code(dtype: torch.dtype, what: str) -> int:
     """dtype code of a 16-bit activation tensor."""
-    if t.dtype == torch.float16:
-        return _lib.QL_DTYPE_F16
-    if t.dtype == torch.bfloat16:
-        return _lib.QL_DTYPE_BF16
-    raise TypeError(f"{what} must be fp16 or bf16, got {t.dtype}")
+    code = _ACTIVATION_CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"{what} must be fp16 or bf16, got {dtype}")
+    return code
+
+
+# The current stream's handle of a device, without building a Stream object
+# (2 us of the host's time, as much as a launch).
+current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def call(entry, packed: bytes, device: torch.device) -> None:
     """entry(packed arguments, current stream) with `device` current (the ABI uses the current device)."""
-    if torch.cuda.current_device() == device.index:
-        status = entry(packed, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = entry(packed, current_raw_stream(index))
     else:
         with on_device(device):
-            status = entry(packed, torch.cuda.current_stream(device).cuda_stream)
+            status = entry(packed, current_raw_stream(index))
     if status != _lib.QL_OK:
         _lib.check(status)

@@ -16,7 +16,7 @@ import torch
 
 from .. import _lib
 from ._launch import activation_code, call, default_flags, index_bytes
-from .rotary import LAYOUTS, RotaryTable
+from .rotary import RotaryTable
 
 GROUP4 = 64                     # elements that share a scale at 4 bits
 
@@ -94,55 +94,63 @@ def append_kv(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: 
     turned by the same angles and returned (in `q_out`, which may be q).
     Tensors may have any strides with unit stride along head_dim, such as
     the column slices of a fused projection's output."""
-    tokens, heads, head_dim = k.shape
-    assert k.is_cuda and k.device == cache.device, f"k is on {k.device}, the cache on {cache.device}"
-    assert (heads, head_dim) == (cache.kv_heads, cache.head_dim), \
-        f"k must be (tokens, {cache.kv_heads}, {cache.head_dim}), got {tuple(k.shape)}"
-    dtype = activation_code(k, "append_kv: k")
-    assert v.shape == k.shape and v.dtype == k.dtype and v.device == k.device, \
-        f"v must be {tuple(k.shape)} {k.dtype} on {k.device}"
-    assert slots.shape == (tokens,) and slots.device == k.device, \
-        f"slots must be ({tokens},) on {k.device}, got {tuple(slots.shape)} on {slots.device}"
-    assert (rotary is None) == (positions is None), "rotary and positions go together"
-    assert q is None or rotary is not None, "q is taken to be turned: pass rotary and positions"
-    if k.stride(-1) != 1:
+    shape, dev = k.shape, cache.device
+    tokens = shape[0]
+    assert k.device == dev and k.is_cuda, f"k is on {k.device}, the cache on {dev}"
+    assert shape == (tokens, cache.kv_heads, cache.head_dim), \
+        f"k must be (tokens, {cache.kv_heads}, {cache.head_dim}), got {tuple(shape)}"
+    dtype = k.dtype
+    code = activation_code(dtype, "append_kv: k")
+    assert v.shape == shape and v.dtype == dtype and v.device == dev, f"v must be {tuple(shape)} {dtype} on {dev}"
+    assert slots.shape == (tokens,) and slots.device == dev, \
+        f"slots must be ({tokens},) on {dev}, got {tuple(slots.shape)} on {slots.device}"
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1:
         k = k.contiguous()
-    if v.stride(-1) != 1:
+        ks = k.stride()
+    if vs[2] != 1:
         v = v.contiguous()
+        vs = v.stride()
     if not slots.is_contiguous():
         slots = slots.contiguous()
-    turn = (0, 0, 0, 0, 0, 8)
+    table, position_ptr, turn = 0, 0, (0, 0, 0, 8)
     if rotary is not None:
-        assert rotary.table.device == k.device, f"the rotary table is on {rotary.table.device}, k on {k.device}"
-        assert rotary.rotary_dim <= head_dim, f"rotary_dim {rotary.rotary_dim} > head_dim {head_dim}"
-        assert positions.shape == (tokens,) and positions.device == k.device, \
-            f"positions must be ({tokens},) on {k.device}, got {tuple(positions.shape)} on {positions.device}"
+        assert positions is not None, "rotary and positions go together"
+        assert rotary.device == dev, f"the rotary table is on {rotary.device}, k on {dev}"
+        assert rotary.rotary_dim <= cache.head_dim, f"rotary_dim {rotary.rotary_dim} > head_dim {cache.head_dim}"
+        assert positions.shape == (tokens,) and positions.device == dev, \
+            f"positions must be ({tokens},) on {dev}, got {tuple(positions.shape)} on {positions.device}"
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        turn = (rotary.table.data_ptr(), positions.data_ptr(), rotary.rotary_dim, rotary.max_positions,
-                LAYOUTS[rotary.layout], index_bytes(positions, "positions"))
+        table, position_ptr = rotary.ptr, positions.data_ptr()
+        turn = (rotary.rotary_dim, rotary.max_positions, rotary.layout_code, index_bytes(positions, "positions"))
+    else:
+        assert positions is None, "rotary and positions go together"
     q_heads, q_ptr, q_out_ptr, qs, os_ = 0, 0, 0, (0, 0), (0, 0)
     if q is not None:
-        assert q.dim() == 3 and q.shape[0] == tokens and q.shape[2] == head_dim and q.dtype == k.dtype \
-            and q.device == k.device, f"q must be ({tokens}, q_heads, {head_dim}) {k.dtype} on {k.device}"
+        assert rotary is not None, "q is taken to be turned: pass rotary and positions"
+        q_shape = q.shape
+        assert len(q_shape) == 3 and q_shape[0] == tokens and q_shape[2] == shape[2] and q.dtype == dtype \
+            and q.device == dev, f"q must be ({tokens}, q_heads, {shape[2]}) {dtype} on {dev}"
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = q.new_empty(q_shape)
         else:
-            assert q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.device == q.device \
-                and q_out.stride(-1) == 1, f"q_out must be {tuple(q.shape)} {q.dtype} with unit inner stride"
-        if q.stride(-1) != 1:
+            assert q_out.shape == q_shape and q_out.dtype == dtype and q_out.device == dev \
+                and q_out.stride(-1) == 1, f"q_out must be {tuple(q_shape)} {dtype} with unit inner stride"
+        qs, os_ = q.stride(), q_out.stride()
+        if qs[2] != 1:
             q = q.contiguous()
-        q_heads, q_ptr, q_out_ptr, qs, os_ = q.shape[1], q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride()
+            qs = q.stride()
+        q_heads, q_ptr, q_out_ptr = q_shape[1], q.data_ptr(), q_out.data_ptr()
     else:
         assert q_out is None, "q_out without q"
     if tokens == 0:
         return q_out
-    ks, vs = k.stride(), v.stride()
     packed = _lib.KV_APPEND_ARGS.pack(
-        *cache.fields, k.data_ptr(), v.data_ptr(), q_ptr, q_out_ptr, slots.data_ptr(), turn[0], turn[1], tokens,
-        q_heads, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], dtype, index_bytes(slots, "slots"),
-        *turn[2:], default_flags())
-    call(_lib.load().ql_kv_append, packed, cache.device)
+        *cache.fields, k.data_ptr(), v.data_ptr(), q_ptr, q_out_ptr, slots.data_ptr(), table, position_ptr, tokens,
+        q_heads, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], code, index_bytes(slots, "slots"),
+        *turn, default_flags())
+    call(_lib.load().ql_kv_append, packed, dev)
     return q_out
 
 
@@ -150,16 +158,18 @@ def read_kv(cache: QuantizedKVCache, slots: torch.Tensor,
             dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows at `slots` (tokens,) as k, v (tokens, kv_heads, head_dim) in
     fp16 or bf16, one rounding; zeros where a slot is negative."""
-    assert slots.dim() == 1 and slots.device == cache.device, f"slots must be (tokens,) on {cache.device}"
-    k, v = torch.empty((2, slots.shape[0], cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
-    code = activation_code(k, "read_kv: dtype")
-    if slots.shape[0] == 0:
+    dev = cache.device
+    assert slots.dim() == 1 and slots.device == dev, f"slots must be (tokens,) on {dev}"
+    code = activation_code(dtype, "read_kv: dtype")
+    tokens = slots.shape[0]
+    k, v = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev).unbind(0)
+    if tokens == 0:
         return k, v
     if not slots.is_contiguous():
         slots = slots.contiguous()
-    packed = _lib.KV_READ_ARGS.pack(*cache.fields, slots.data_ptr(), k.data_ptr(), v.data_ptr(), slots.shape[0],
-                                    code, index_bytes(slots, "slots"), default_flags())
-    call(_lib.load().ql_kv_read, packed, cache.device)
+    packed = _lib.KV_READ_ARGS.pack(*cache.fields, slots.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, code,
+                                    index_bytes(slots, "slots"), default_flags())
+    call(_lib.load().ql_kv_read, packed, dev)
     return k, v
 
 

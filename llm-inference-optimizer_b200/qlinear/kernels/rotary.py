@@ -90,6 +90,7 @@ class RotaryTable:
                              f"{tuple(table.shape)}")
         self.table = table.contiguous()
         self.layout = layout
+        self.device, self.ptr, self.layout_code = self.table.device, self.table.data_ptr(), LAYOUTS[layout]
         self.rotary_dim = 2 * table.shape[1]
         self.max_positions = table.shape[0]
 
@@ -124,32 +125,34 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     `out` may have any strides with unit stride along head_dim; ``out=x``
     turns in place.  ``inverse=True`` turns back: it undoes the call, and maps
     the gradient of its result to that of x."""
-    assert x.is_cuda and x.dim() == 3, f"x must be a CUDA tensor (tokens, heads, head_dim), got {tuple(x.shape)}"
-    tokens, heads, head_dim = x.shape
-    dtype = activation_code(x, "apply_rotary: x")
-    assert positions.shape == (tokens,) and positions.device == x.device, \
-        f"positions must be ({tokens},) on {x.device}, got {tuple(positions.shape)} on {positions.device}"
-    assert rotary.table.device == x.device, f"the rotary table is on {rotary.table.device}, x on {x.device}"
+    shape, dev = x.shape, x.device
+    assert x.is_cuda and len(shape) == 3, f"x must be a CUDA tensor (tokens, heads, head_dim), got {tuple(shape)}"
+    tokens, heads, head_dim = shape
+    dtype = activation_code(x.dtype, "apply_rotary: x")
+    assert positions.shape == (tokens,) and positions.device == dev, \
+        f"positions must be ({tokens},) on {dev}, got {tuple(positions.shape)} on {positions.device}"
+    assert rotary.device == dev, f"the rotary table is on {rotary.device}, x on {dev}"
     assert rotary.rotary_dim <= head_dim and head_dim % 8 == 0, \
         f"head_dim {head_dim} must be a multiple of 8 and at least rotary_dim {rotary.rotary_dim}"
     if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
     else:
-        assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, \
-            f"out must be {tuple(x.shape)} {x.dtype} on {x.device}"
+        assert out.shape == shape and out.dtype == x.dtype and out.device == dev, \
+            f"out must be {tuple(shape)} {x.dtype} on {dev}"
         assert out.stride(-1) == 1, "out must have unit stride along head_dim"
     if tokens == 0 or heads == 0:
         return out
-    if x.stride(-1) != 1:
+    xs, os_ = x.stride(), out.stride()
+    if xs[2] != 1:
         x = x.contiguous()
+        xs = x.stride()
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    xs, os_ = x.stride(), out.stride()
     packed = _lib.ROTARY_ARGS.pack(
-        x.data_ptr(), out.data_ptr(), rotary.table.data_ptr(), positions.data_ptr(), tokens, heads, head_dim,
-        rotary.rotary_dim, rotary.max_positions, xs[0], xs[1], os_[0], os_[1], dtype, LAYOUTS[rotary.layout],
-        index_bytes(positions, "positions"), int(inverse), default_flags())
-    call(_lib.load().ql_rotary, packed, x.device)
+        x.data_ptr(), out.data_ptr(), rotary.ptr, positions.data_ptr(), tokens, heads, head_dim, rotary.rotary_dim,
+        rotary.max_positions, xs[0], xs[1], os_[0], os_[1], dtype, rotary.layout_code,
+        index_bytes(positions, "positions"), 1 if inverse else 0, default_flags())
+    call(_lib.load().ql_rotary, packed, dev)
     return out
 
 

@@ -7,12 +7,10 @@ all of them attending in one call to the 8- or 4-bit cache in place.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .. import _lib
-from ._launch import activation_code, call, default_flags, on_device, scratch
+from ._launch import activation_code, call, current_raw_stream, default_flags, on_device, scratch
 from .kv_cache import QuantizedKVCache
 
 
@@ -25,7 +23,7 @@ def _workspace(device: torch.device, head_dim: int) -> torch.Tensor:
         with on_device(device):
             nbytes = _lib.load().ql_tree_attention_workspace_size(head_dim)
         _workspace_bytes[device.index, head_dim] = nbytes
-    return scratch(device, torch.cuda.current_stream(device), nbytes)
+    return scratch(device, current_raw_stream(device.index), nbytes)
 
 
 def pack_tree_mask(visible: torch.Tensor) -> torch.Tensor:
@@ -74,63 +72,67 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
     Returns (total_q, q_heads, head_dim) in q's dtype, and with
     ``return_lse`` the rows' log-sums (total_q, q_heads) fp32 (minus infinity
     where nothing is seen)."""
-    assert q.is_cuda and q.dim() == 3, f"q must be a CUDA tensor (total_q, q_heads, head_dim), got {tuple(q.shape)}"
-    total_q, q_heads, head_dim = q.shape
-    dev = cache.device
-    dtype = activation_code(q, "tree_attention: q")
+    shape, dev, dtype = q.shape, cache.device, q.dtype
+    assert q.is_cuda and len(shape) == 3, f"q must be a CUDA tensor (total_q, q_heads, head_dim), got {tuple(shape)}"
+    total_q, q_heads, head_dim = shape
+    code = activation_code(dtype, "tree_attention: q")
     assert q.device == dev and head_dim == cache.head_dim, \
-        f"q must be (total_q, q_heads, {cache.head_dim}) on {dev}, got {tuple(q.shape)} on {q.device}"
+        f"q must be (total_q, q_heads, {cache.head_dim}) on {dev}, got {tuple(shape)} on {q.device}"
     assert q_heads % cache.kv_heads == 0, f"q_heads {q_heads} must be a multiple of kv_heads {cache.kv_heads}"
-    batch = kv_lens.shape[0]
     if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32:
         raise TypeError(f"page_table and kv_lens must be int32, got {page_table.dtype} and {kv_lens.dtype}")
-    assert page_table.dim() == 2 and page_table.shape[0] == batch and page_table.device == dev, \
-        f"page_table must be ({batch}, pages) on {dev}, got {tuple(page_table.shape)} on {page_table.device}"
-    assert kv_lens.dim() == 1 and kv_lens.device == dev, f"kv_lens must be (batch,) on {dev}"
-    if page_table.stride(-1) != 1:
-        page_table = page_table.contiguous()
+    table_shape, lens_shape = page_table.shape, kv_lens.shape
+    assert len(lens_shape) == 1 and kv_lens.device == dev, f"kv_lens must be (batch,) on {dev}"
+    batch = lens_shape[0]
+    assert len(table_shape) == 2 and table_shape[0] == batch and page_table.device == dev, \
+        f"page_table must be ({batch}, pages) on {dev}, got {tuple(table_shape)} on {page_table.device}"
     if not kv_lens.is_contiguous():
         kv_lens = kv_lens.contiguous()
     cu_ptr, mask_ptr, words = 0, 0, 0
     if cu_q is not None:
         if cu_q.dtype != torch.int32:
             raise TypeError(f"cu_q must be int32, got {cu_q.dtype}")
-        assert cu_q.shape == (batch + 1,) and cu_q.device == dev and cu_q.is_contiguous(), \
-            f"cu_q must be ({batch + 1},) on {dev}"
+        assert cu_q.shape == (batch + 1,) and cu_q.device == dev, f"cu_q must be ({batch + 1},) on {dev}"
+        if not cu_q.is_contiguous():
+            cu_q = cu_q.contiguous()
         cu_ptr = cu_q.data_ptr()
-    else:
-        assert batch > 0 or total_q == 0, "q has rows but there is no request"
-        assert batch == 0 or total_q % batch == 0, f"{total_q} rows do not divide among {batch} requests: pass cu_q"
+        if max_q is None:
+            max_q = total_q
+    elif total_q > 0:
+        assert batch > 0, "q has rows but there is no request"
+        assert total_q % batch == 0, f"{total_q} rows do not divide among {batch} requests: pass cu_q"
+        max_q = total_q // batch
     if mask is not None:
         if mask.dtype != torch.int64:
             raise TypeError(f"mask must be int64, got {mask.dtype}")
         assert mask.dim() == 2 and mask.shape[0] == total_q and mask.device == dev, \
             f"mask must be ({total_q}, words) on {dev}, got {tuple(mask.shape)} on {mask.device}"
-        assert 1 <= mask.shape[1] <= 1024, f"mask must have 1 to 1024 words a row, got {mask.shape[1]}"
+        words = mask.shape[1]
+        assert 1 <= words <= 1024, f"mask must have 1 to 1024 words a row, got {words}"
         mask = mask.contiguous()
-        mask_ptr, words = mask.data_ptr(), mask.shape[1]
+        mask_ptr = mask.data_ptr()
     if out is None:
-        out = torch.empty((total_q, q_heads, head_dim), dtype=q.dtype, device=dev)
+        out = q.new_empty(shape)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous(), \
-            f"out must be contiguous {tuple(q.shape)} {q.dtype} on {dev}"
+        assert out.shape == shape and out.dtype == dtype and out.device == dev and out.is_contiguous(), \
+            f"out must be contiguous {tuple(shape)} {dtype} on {dev}"
     lse = torch.empty((total_q, q_heads), dtype=torch.float32, device=dev) if return_lse else None
     if total_q > 0 and batch > 0:
-        if q.stride(-1) != 1:
+        qs, ts, width = q.stride(), page_table.stride(), table_shape[1]
+        if qs[2] != 1:
             q = q.contiguous()
-        qs = q.stride()
-        width = page_table.shape[1]
-        if max_q is None:
-            max_q = total_q // batch if cu_q is None else total_q
+            qs = q.stride()
+        if ts[1] != 1:
+            page_table = page_table.contiguous()
+            ts = page_table.stride()
         if max_kv is None:
             max_kv = width * cache.page_size
         ws = _workspace(dev, head_dim)
         packed = _lib.TREE_ATTENTION_ARGS.pack(
             *cache.fields, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(),
             kv_lens.data_ptr(), cu_ptr, mask_ptr, batch, total_q, q_heads, qs[0], qs[1], width,
-            page_table.stride(0) if batch > 1 else width, words, max_q, max_kv, dtype,
-            1.0 / math.sqrt(head_dim) if scale is None else scale, ws.data_ptr(),
-            ws.numel(), default_flags())
+            ts[0] if batch > 1 else width, words, max_q, max_kv, code,
+            head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), default_flags())
         call(_lib.load().ql_tree_attention, packed, dev)
     return (out, lse) if return_lse else out
 
