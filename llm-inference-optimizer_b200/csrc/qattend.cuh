@@ -67,8 +67,9 @@ constexpr int kUnitKeys = 128;
 constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMinUnits = 2;               // keys worth a CTA of their own: 256
-constexpr int kMaxCtas = 1024;             // counters in the workspace's first 4 KB
-constexpr int kHeaderBytes = 4 * kMaxCtas;
+constexpr int kJoin = 16;                  // parts of an item that are joined at once
+constexpr int kMaxCtas = 1024;
+constexpr int kHeaderBytes = 2 * 4 * kMaxCtas;   // counters of items and of groups of parts
 
 struct Work {
   long long total;     // units of the launch
@@ -680,64 +681,108 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       }
     __syncthreads();
 
+    // a row's maximum, sum and output over the warps, in warp order
     const long long item_begin = base + item * per_item;
     const bool whole = k_begin == 0 && k_end == per_item;
-    const int c_first = whole ? 0 : work.cta_of(item_begin);
     float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
-    // a row's sum and output over the warps, in warp order; whole items end here
-    for (int e = threadIdx.x; e < rows * D; e += kThreads) {
+    auto finish = [&](int row, int d, const float4& o, float top, float sum) {
+      const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
+      const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
+      const float f[4] = {o.x, o.y, o.z, o.w};
+      kvc::Vec4<T> v;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) v.v[i] = kvc::from_f<T>(sum == 0.f ? 0.f : f[i] / sum);
+      *reinterpret_cast<kvc::Vec4<T>*>(static_cast<T*>(p.out) + at * D + d) = v;
+      if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+    };
+    auto park = [&](float* dst, int row, int d, const float4& o, float top, float sum) {
+      *reinterpret_cast<float4*>(dst + 2 * S::kRows + row * D + d) = o;
+      if (d == 0) {
+        dst[row] = top;
+        dst[S::kRows + row] = sum;
+      }
+    };
+    for (int e = threadIdx.x * 4; e < rows * D; e += kThreads * 4) {
       const int row = e / D, d = e - row * D;
-      float top = kLow, sum = 0.f, o = 0.f;
+      float top = kLow, sum = 0.f;
+      float4 o = {0.f, 0.f, 0.f, 0.f};
       #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
       #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = sm_m[w * S::kRows + row];
-        sum += sm_l[w * S::kRows + row] * ex2<kBf16>(mw - top);
-        o += sm_o[(w * S::kRows + row) * D + d];
+        sum += sm_l[w * S::kRows + row] * ex2<kBf16>(sm_m[w * S::kRows + row] - top);
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * S::kRows + row) * D + d);
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
       }
-      if (whole) {
-        const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
-        const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
-        static_cast<T*>(p.out)[at * D + d] = kvc::from_f<T>(sum == 0.f ? 0.f : o / sum);
-        if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
-      } else {
-        mine_out[2 * S::kRows + row * D + d] = o;
-        if (d == 0) {
-          mine_out[row] = top;
-          mine_out[S::kRows + row] = sum;
-        }
-      }
+      if (whole)
+        finish(row, d, o, top, sum);
+      else
+        park(mine_out, row, d, o, top, sum);
     }
 
     if (!whole) {
-      // ---------------------------- the last CTA of the item joins its parts
-      const int c_last = work.cta_of(item_begin + per_item - 1), parts = c_last - c_first + 1;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) last_one = atomic_add_acq_rel_gpu(counters + c_first, 1u) == (unsigned)parts - 1;
-      __syncthreads();
-      if (last_one) {
-        if (threadIdx.x == 0) counters[c_first] = 0;
-        auto part = [&](int q) {                        // the first begins the item: its CTA's second slot
-          return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
-        };
-        for (int e = threadIdx.x; e < rows * D; e += kThreads) {
-          const int row = e / D, d = e - row * D;
-          float top = kLow, sum = 0.f, o = 0.f;
-          for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(part(q) + row));
-          for (int q = 0; q < parts; ++q) {
-            const float* src = part(q);
-            const float mq = __ldcg(src + row), f = ex2<kBf16>(mq - top);
-            sum += __ldcg(src + S::kRows + row) * f;
-            o += __ldcg(src + 2 * S::kRows + row * D + d) * f;
-          }
-          const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
-          const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
-          static_cast<T*>(p.out)[at * D + d] = kvc::from_f<T>(sum == 0.f ? 0.f : o / sum);
-          if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+      // The item's parts, one a CTA, are joined by its last CTA.  Many parts
+      // are joined in groups of kJoin first, each by its last CTA, so that no
+      // CTA reads more than a few dozen: with 74 parts a single one took
+      // longer than the keys had.
+      const int c_first = work.cta_of(item_begin), parts = work.cta_of(item_begin + per_item - 1) - c_first + 1;
+      const int groups = (parts + kJoin - 1) / kJoin, me = (int)blockIdx.x - c_first, group = me / kJoin;
+      auto part = [&](int q) {                          // the first begins the item: its CTA's second slot
+        return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
+      };
+      auto arrive = [&](unsigned* counter, int n) {     // true in the last of n CTAs, which sees the others' parts
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          last_one = atomic_add_acq_rel_gpu(counter, 1u) == (unsigned)n - 1;
+          if (last_one) *counter = 0;
         }
+        __syncthreads();
+        return last_one != 0;
+      };
+      auto join = [&](int first, int step, int n, auto out) {
+        float* f_m = smem;                              // [part][row], then the factors
+        float* f_l = smem + n * S::kRows;
+        for (int i = threadIdx.x; i < n * S::kRows; i += kThreads) {
+          const int q = i / S::kRows, row = i - q * S::kRows;
+          if (row < rows) {
+            f_m[i] = __ldcg(part(first + q * step) + row);
+            f_l[i] = __ldcg(part(first + q * step) + S::kRows + row);
+          }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x * 4; e < rows * D; e += kThreads * 4) {
+          const int row = e / D, d = e - row * D;
+          float top = kLow, sum = 0.f;
+          float4 o = {0.f, 0.f, 0.f, 0.f};
+          for (int q = 0; q < n; ++q) top = fmaxf(top, f_m[q * S::kRows + row]);
+          #pragma unroll 8
+          for (int q = 0; q < n; ++q) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(first + q * step) + 2 * S::kRows + row * D + d));
+            const float f = ex2<kBf16>(f_m[q * S::kRows + row] - top);
+            sum += f_l[q * S::kRows + row] * f;
+            o.x += v.x * f;
+            o.y += v.y * f;
+            o.z += v.z * f;
+            o.w += v.w * f;
+          }
+          out(row, d, o, top, sum);
+        }
+      };
+      bool last = true;
+      if (groups > 1) {
+        const int n = min(kJoin, parts - group * kJoin);
+        last = arrive(counters + kMaxCtas + c_first + group * kJoin, n);
+        if (last)
+          join(group * kJoin, 1, n, [&](int row, int d, const float4& o, float top, float sum) {
+            park(part(group * kJoin), row, d, o, top, sum);   // read by this thread alone; the row's m and l are in shared memory
+          });
       }
+      if (last && arrive(counters + c_first, groups > 1 ? groups : parts))
+        join(0, groups > 1 ? kJoin : 1, groups > 1 ? groups : parts, finish);
     }
     __syncthreads();                                    // before the next segment reuses shared memory
     u += k_end - k_begin;

@@ -42,7 +42,7 @@ def workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> t
 
 
 _scratches: dict[tuple[int, int], torch.Tensor] = {}
-_SCRATCH_HEADER = 4096
+_SCRATCH_HEADER = 8192           # ql_tree_attention's counters
 
 
 def scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
