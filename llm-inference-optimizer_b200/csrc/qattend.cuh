@@ -204,27 +204,47 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
-// Cache codes: read once by this CTA, so not kept in L1.
+// 16 bytes from global to shared memory, past L1, in the thread's current group.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {           // all but the newest LEFT groups have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 template <int WORDS>
-__device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const unsigned char* p) {
-  static_assert(WORDS == 1 || WORDS == 2 || WORDS == 4 || WORDS == 8, "4 to 32 bytes");
-  if constexpr (WORDS == 1) {
-    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-  } else if constexpr (WORDS == 2) {
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-    #pragma unroll
-    for (int i = 0; i < WORDS; i += 4)
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
-                   : "l"(p + 4 * i));
-  }
+__device__ __forceinline__ void load_shared(uint32_t (&w)[WORDS], uint32_t addr) {
+  if constexpr (WORDS == 1)
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+}
+
+// Where 16-byte chunk `chunk` of row `row` (of 16) of a tile lies in shared
+// memory.  The lanes of a quarter, half or whole warp that read together take
+// either neighbouring rows at one place (keys) or every second row at one
+// place (values); the order below puts both on different banks.
+template <int ROW_BYTES, int BITS>
+__device__ __forceinline__ int tile_offset(int row, int chunk) {
+  const int u0 = (row ^ (row >> 2)) & 1, u1 = (row >> 1) & 1;      // distinct over rows 4i.., over 0 2 4 6, over 1 3 5 7
+  if constexpr (ROW_BYTES == 32) return (row >> 2) * 128 + u1 * 64 + u0 * 32 + chunk * 16;
+  if constexpr (ROW_BYTES == 64) return (row >> 1) * 128 + u0 * 64 + (chunk ^ (u1 << 1)) * 16;
+  if constexpr (ROW_BYTES == 128 && BITS == 4) return row * 128 + (chunk ^ (u1 << 2) ^ (u0 << 1)) * 16;
+  if constexpr (ROW_BYTES == 128 && BITS == 8) return row * 128 + (chunk ^ (row & 6) ^ ((row & 1) << 2)) * 16;
+  const int f = ((row >> 1) & 1) ^ ((row & 4)) ^ ((row & 1) << 2);
+  return row * 256 + (chunk ^ f) * 16;
 }
 
 // ------------------------------------------------- the kernel for a few rows
 // Bound by reading the cache (one unit of keys and values, 33 KB at 8 bits
-// and head_dim 128, serves 8 NT rows), so everything else is arranged around
-// the loads: keys and values go from global memory straight into the
+// and head_dim 128, serves 8 NT rows).  Each warp copies its own tiles of 16
+// keys to shared memory some tiles ahead (16-byte asynchronous copies, no
+// barrier beyond the warp), and reads them from there straight into the
 // registers that the matrix instructions take them from.
 //
 // Keys are the M side of both products, rows the N side (m16n8k16):
@@ -255,13 +275,22 @@ struct Shape {
   static constexpr int kRows = 8 * NT;
   static constexpr int kChunks = D / 64;
   static constexpr int kGroups = BITS == 8 ? 1 : kChunks;
+  static constexpr int kRowBytes = D * BITS / 8;
   static constexpr int kKeyWords = BITS == 8 ? 4 : 2;                // of a 64-element chunk
   static constexpr int kValWords = BITS == 8 ? D / 32 : D / 64;      // of a lane's eighth of a row
   static constexpr int kTiles = D / 16;
   static constexpr int kCtas = D == 256 ? 1 : NT == 1 ? 2 : 1;       // per SM, by registers
   // partial of an item: per row its maximum, its sum and D outputs
   static constexpr int kPartial = kRows * (D + 2);
-  static constexpr size_t kSmem = (size_t)kWarps * kRows * (D + 2) * sizeof(float);
+  // a warp's ring: 16 rows of keys, of values, and their scales, a stage
+  static constexpr int kTileBytes = 16 * kRowBytes, kScaleBytes = 16 * kGroups * 2;
+  static constexpr int kStageBytes = (2 * (kTileBytes + kScaleBytes) + 127) / 128 * 128;
+  static constexpr int kBudget = (kCtas == 2 ? 108 : 216) * 1024;
+  static constexpr int kStages = kBudget / (kWarps * kStageBytes) < 6 ? kBudget / (kWarps * kStageBytes) : 6;
+  static_assert(kStages >= 2 && 4 * kGroups <= 32, "");
+  static constexpr size_t kRing = (size_t)kWarps * kStages * kStageBytes;
+  static constexpr size_t kJoined = (size_t)kWarps * kRows * (D + 2) * sizeof(float);   // takes the ring's place
+  static constexpr size_t kSmem = 128 + (kRing > kJoined ? kRing : kJoined);
 };
 
 template <typename T, int D, int BITS, int NT>
@@ -271,7 +300,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   griddep_launch_dependents();
   griddep_wait();
-  extern __shared__ float smem[];
+  extern __shared__ float smem_raw[];
+  float* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u) / 4;
   float* sm_o = smem;                                   // [warp][row][D]
   float* sm_m = smem + kWarps * S::kRows * D;           // [warp][row]
   float* sm_l = sm_m + kWarps * S::kRows;
@@ -385,70 +415,90 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       }
       return page;
     };
-    int page_now = fetch_pages(0), page_next = fetch_pages(32);
+    int page_now = fetch_pages(0), page_next = fetch_pages(32), pages_at = 0;   // of tiles 32 pages_at ..
 
-    uint32_t kw[2][S::kChunks][S::kKeyWords], vw[4][S::kValWords];
-    unsigned short ks[2][S::kGroups], vs[2][S::kGroups];
-    int page_k = -1, page_v = -1;                       // of the tiles in kw and vw
-    auto rows_of = [&](int page, int i) {               // row index within the page of tile i's first key
-      return (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
-    };
-    auto load_keys = [&](int i) {
-      if (i > 0 && (i & 31) == 0) {
-        page_now = page_next;
-        page_next = fetch_pages(i + 32);
-      }
-      page_k = __shfl_sync(0xffffffffu, page_now, i & 31);
-      if (page_k < 0) return;
-      const int at = rows_of(page_k, i);
-      const unsigned char* code = kv.k_codes + page_k * kv.k_page + (long long)(at + g) * (D * BITS / 8) + t * 4 * S::kKeyWords;
-      const unsigned short* sc = kv.k_scales + page_k * kv.ks_page + (long long)(at + g) * S::kGroups;
+    // copies of tile i into its stage; a tile in no page leaves the stage as it is
+    const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+    auto page_of = [&](int i) { return __shfl_sync(0xffffffffu, (i >> 5) == pages_at ? page_now : page_next, i & 31); };
+    auto copy_tile = [&](int i, int stage) {
+      const int page = page_of(i);
+      if (page < 0) return;
+      const int at = (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
+      const uint32_t dst = ring + stage * S::kStageBytes;
+      const unsigned char* k = kv.k_codes + page * kv.k_page + (long long)at * S::kRowBytes + lane * 16;
+      const unsigned char* v = kv.v_codes + page * kv.v_page + (long long)at * S::kRowBytes + lane * 16;
+      constexpr int kRowChunks = S::kRowBytes / 16;
       #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c)
-          load_codes<S::kKeyWords>(kw[x][c], code + x * 8 * (D * BITS / 8) + c * 8 * BITS);
-        #pragma unroll
-        for (int q = 0; q < S::kGroups; ++q) ks[x][q] = sc[x * 8 * S::kGroups + q];
+      for (int c = 0; c < kRowChunks / 2; ++c) {
+        const int chunk = c * 32 + lane;
+        const uint32_t to = dst + tile_offset<S::kRowBytes, BITS>(chunk / kRowChunks, chunk % kRowChunks);
+        copy16(to, k + c * 512);
+        copy16(to + S::kTileBytes, v + c * 512);
+      }
+      if (lane < 4 * S::kGroups) {
+        const bool value = lane >= 2 * S::kGroups;
+        const unsigned short* sc = value ? kv.v_scales + page * kv.vs_page : kv.k_scales + page * kv.ks_page;
+        copy16(dst + 2 * S::kTileBytes + lane * 16, sc + (long long)at * S::kGroups + (lane - (value ? 2 * S::kGroups : 0)) * 8);
       }
     };
-    auto load_values = [&]() {                          // of the tile whose page is page_k
-      page_v = page_k;
-    };
-    auto load_values_at = [&](int i) {
-      if (page_v < 0) return;
-      const int at = rows_of(page_v, i);
-      const unsigned char* code = kv.v_codes + page_v * kv.v_page + (long long)(at + 2 * t) * (D * BITS / 8);
-      const unsigned short* sc = kv.v_scales + page_v * kv.vs_page + (long long)(at + g) * S::kGroups;
-      #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const unsigned char* row = code + ((x & 1) + (x >> 1) * 8) * (D * BITS / 8);
-        if constexpr (BITS == 8) {
-          load_codes<S::kValWords>(vw[x], row + g * (D / 8));
-        } else {
-          #pragma unroll
-          for (int c = 0; c < S::kChunks; ++c) {
-            uint32_t w[1];
-            load_codes<1>(w, row + c * 32 + g * 4);
-            vw[x][c] = w[0];
-          }
-        }
-      }
-      #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        #pragma unroll
-        for (int q = 0; q < S::kGroups; ++q) vs[x][q] = sc[x * 8 * S::kGroups + q];
-    };
-
-    if (n_tiles > 0) {
-      load_keys(0);
-      load_values();
-      load_values_at(0);
+    __syncwarp();
+    #pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      if (i < n_tiles) copy_tile(i, i);
+      copy_commit();
     }
+    int stage = 0;
     #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int j0 = j_first + i * kUnitKeys;
-      const bool hidden = page_k < 0;
+      copy_wait<S::kStages - 2>();
+      __syncwarp();
+      const uint32_t here = ring + stage * S::kStageBytes;
+      if ((i >> 5) > pages_at) {
+        ++pages_at;
+        page_now = page_next;
+        page_next = fetch_pages(32 * pages_at + 32);
+      }
+      const bool hidden = page_of(i) < 0;
+      if (++stage == S::kStages) stage = 0;
+      // the stage before this one, read to its end by all lanes, takes the next tile
+      {
+        const int next = i + S::kStages - 1;
+        if (next < n_tiles) {
+          copy_tile(next, stage == 0 ? S::kStages - 2 : stage == 1 ? S::kStages - 1 : stage - 2);
+        }
+        copy_commit();
+      }
+      uint32_t kw[2][S::kChunks][S::kKeyWords];
+      float ks[2][S::kGroups];
+      #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        #pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+          if constexpr (BITS == 8)
+            load_shared<4>(kw[x][c], here + tile_offset<S::kRowBytes, BITS>(g + 8 * x, 4 * c + t));
+          else
+            load_shared<2>(kw[x][c], here + tile_offset<S::kRowBytes, BITS>(g + 8 * x, 2 * c + (t >> 1)) + (t & 1) * 8);
+        }
+      }
+      auto load_scales = [&](float (&sc)[2][S::kGroups], uint32_t at) {
+        #pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t addr = at + (g + 8 * x) * S::kGroups * 2;
+          if constexpr (S::kGroups == 1) {
+            unsigned short h;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr));
+            sc[x][0] = kvc::bf16_bits_to_f(h);
+          } else {
+            uint32_t w[S::kGroups / 2];
+            load_shared<S::kGroups / 2>(w, addr);
+            #pragma unroll
+            for (int q = 0; q < S::kGroups; ++q)
+              sc[x][q] = __uint_as_float(q & 1 ? w[q / 2] & 0xFFFF0000u : w[q / 2] << 16);
+          }
+        }
+      };
+      load_scales(ks, here + 2 * S::kTileBytes);
       // ------------------------------------------------------------- scores
       float s[NT][4];
       #pragma unroll
@@ -488,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = part[n][e];
         } else {
-          const float k0 = kvc::bf16_bits_to_f(ks[0][c]), k1 = kvc::bf16_bits_to_f(ks[1][c]);
+          const float k0 = ks[0][c], k1 = ks[1][c];
           #pragma unroll
           for (int n = 0; n < NT; ++n)
             #pragma unroll
@@ -496,13 +546,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         }
       }
       if constexpr (BITS == 8) {
-        const float k0 = kvc::bf16_bits_to_f(ks[0][0]), k1 = kvc::bf16_bits_to_f(ks[1][0]);
+        const float k0 = ks[0][0], k1 = ks[1][0];
         #pragma unroll
         for (int n = 0; n < NT; ++n)
           #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][e] *= (e < 2 ? k0 : k1) * rs[n][e & 1];
       }
-      if (i + 1 < n_tiles) load_keys(i + 1);
 
       // ------------------------------------------------- what the rows see
       const bool some_hidden = hidden || j0 + 15 >= context;
@@ -519,13 +568,35 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
 
       // ------------------------------------------------------------ weights
       float v_top = 0.f, v_sc[2][S::kGroups];
+      load_scales(v_sc, here + 2 * S::kTileBytes + S::kScaleBytes);
       #pragma unroll
       for (int x = 0; x < 2; ++x)
         #pragma unroll
-        for (int q = 0; q < S::kGroups; ++q) {
-          v_sc[x][q] = kvc::bf16_bits_to_f(vs[x][q]);
-          v_top = fmaxf(v_top, v_sc[x][q]);
+        for (int q = 0; q < S::kGroups; ++q) v_top = fmaxf(v_top, v_sc[x][q]);
+      uint32_t vw[4][S::kValWords];
+      #pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = 2 * t + (x & 1) + (x >> 1) * 8;
+        const uint32_t values = here + S::kTileBytes;
+        if constexpr (BITS == 4) {
+          #pragma unroll
+          for (int c = 0; c < S::kChunks; ++c) {
+            uint32_t w[1];
+            load_shared<1>(w, values + tile_offset<S::kRowBytes, BITS>(row, 2 * c + (g >> 2)) + (g & 3) * 4);
+            vw[x][c] = w[0];
+          }
+        } else if constexpr (D == 64) {
+          load_shared<2>(vw[x], values + tile_offset<S::kRowBytes, BITS>(row, g >> 1) + (g & 1) * 8);
+        } else {
+          #pragma unroll
+          for (int c = 0; c < D / 128; ++c) {
+            uint32_t w[4];
+            load_shared<4>(w, values + tile_offset<S::kRowBytes, BITS>(row, g * (D / 128) + c));
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) vw[x][4 * c + q] = w[q];
+          }
         }
+      }
       bool move = v_top > v_ref;
       #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -642,11 +713,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
                    }
                  });
       }
-      if (i + 1 < n_tiles) {
-        load_values();
-        load_values_at(i + 1);
-      }
     }
+    copy_wait<0>();
+    __syncthreads();                                    // the ring gives way to the joined rows
 
     // -------------------------------------------- join the warps of the CTA
     #pragma unroll
