@@ -62,7 +62,7 @@ __device__ __forceinline__ bool sees(const Params& p, const Request& r, int i, i
 // the CTAs take equal runs of units, whatever the requests' lengths are: a
 // CTA may end one item, do some whole and begin another.  Lengths are read
 // on the device, so a captured launch serves other lengths later.
-constexpr float kLow = -1e30f;             // below every score: a maximum of nothing, finite so that differences are
+constexpr float kLow = -1e30f;             // the maximum of nothing: below every score, and finite
 constexpr int kUnitKeys = 128;
 constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
 constexpr int kThreads = 32 * kWarps;
@@ -74,8 +74,12 @@ constexpr int kHeaderBytes = 2 * 4 * kMaxCtas;   // counters of items and of gro
 struct Work {
   long long total;     // units of the launch
   int ctas;            // CTAs that take part
-  __device__ long long first_unit(int cta) const { return total * cta / ctas; }
-  __device__ int cta_of(long long u) const { return (int)(((u + 1) * ctas - 1) / total); }
+  __device__ long long first_unit(int cta) const { return quotient(total * cta, ctas); }
+  __device__ int cta_of(long long u) const { return (int)quotient((u + 1) * ctas - 1, total); }
+  // of non-negative numbers, by the short division where it does (nearly always)
+  static __device__ long long quotient(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+  }
 };
 
 __device__ __forceinline__ int item_units(const Request& r) {
@@ -239,6 +243,26 @@ __device__ __forceinline__ int tile_offset(int row, int chunk) {
   const int f = ((row >> 1) & 1) ^ ((row & 4)) ^ ((row & 1) << 2);
   return row * 256 + (chunk ^ f) * 16;
 }
+// tile_offset of a row and chunk that are `drow` and `dchunk` further on,
+// where these change no bit that the lane's own row and chunk have set: as a
+// constant to xor to the lane's address (tiles are 128-byte aligned) and one
+// to add.
+template <int ROW_BYTES, int BITS>
+__host__ __device__ constexpr int step_xor(int drow, int dchunk) {
+  const int r0 = drow & 1, r1 = (drow >> 1) & 1, r2 = (drow >> 2) & 1;
+  int x = (dchunk & 7) * 16;
+  if (ROW_BYTES == 32) return x ^ r1 * 64 ^ (r0 ^ r2) * 32;
+  if (ROW_BYTES == 64) return x ^ (r0 ^ r2) * 64 ^ r1 * 32;
+  if (ROW_BYTES == 128 && BITS == 4) return x ^ r1 * 64 ^ (r0 ^ r2) * 32;
+  if (ROW_BYTES == 128) return x ^ r1 * 32 ^ r2 * 64 ^ r0 * 64;
+  return x ^ r1 * 16 ^ r2 * 64 ^ r0 * 64;
+}
+template <int ROW_BYTES, int BITS>
+__host__ __device__ constexpr int step_add(int drow, int dchunk) {
+  if (ROW_BYTES == 32) return (drow >> 2) * 128;
+  if (ROW_BYTES == 64) return (drow >> 1) * 128;
+  return drow * ROW_BYTES + (dchunk & 8) * 16;
+}
 
 // ------------------------------------------------- the kernel for a few rows
 // Bound by reading the cache (one unit of keys and values, 33 KB at 8 bits
@@ -264,8 +288,8 @@ __device__ __forceinline__ int tile_offset(int row, int chunk) {
 // costs precision; it needs twice the decoding and products.
 //
 // The running maximum of a row moves only when a score passes it by 4 (weights
-// up to 2^4): one vote per 16 keys stands for the reductions and the
-// rescaling, which become rare.
+// up to 2^4): one vote per 16 keys stands for the reductions, the rescaling
+// and the look for hidden keys and small weights, which become rare.
 //
 // A key's scale is read by its own lanes; hidden keys are removed by
 // selection, never by multiplication, so what unused rows of a page hold
@@ -328,16 +352,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     }
     const int per_item = item_units(r);
     const int tiles = (int)(((long long)r.q_len * p.group + S::kRows - 1) / S::kRows);
-    const long long item = (u - base) / per_item;
+    const long long item = Work::quotient(u - base, per_item);
     const int k_begin = (int)((u - base) - item * per_item);
     const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
-    const int head = (int)(item / tiles), row0 = (int)(item - (long long)head * tiles) * S::kRows;
+    const int head = (int)Work::quotient(item, tiles), row0 = (int)(item - (long long)head * tiles) * S::kRows;
     const int rows = min(S::kRows, r.q_len * p.group - row0);
     const int context = r.kv_len - r.q_len;             // positions that every row sees
 
     // ------------------------------------------------------------- queries
     uint32_t qb[NT][S::kTiles][2];
-    float rs[NT][2];                                    // on the scores of rows 2t, 2t + 1, in units of log2
+    float rs[NT][2];                                    // on the scores of rows 2t, 2t + 1
     #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + g;
@@ -380,13 +404,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           }
       #pragma unroll
       for (int x = 0; x < 2; ++x)
-        rs[n][x] = kBf16 ? __shfl_sync(0xffffffffu, up, (2 * t + x) * 4) * p.scale_log2 : p.scale_log2;
+        rs[n][x] = kBf16 ? __shfl_sync(0xffffffffu, up, (2 * t + x) * 4) : 1.f;
     }
 
     // ---------------------------------------------------------- running state
     float acc[NT][S::kTiles][4];
     float m[NT][2], l[NT][2];
     float v_ref = 0.f, fac = 1.f;                       // power of two at least every value scale seen; on the weights
+    bool open = true;                                   // some row has seen nothing yet
     #pragma unroll
     for (int n = 0; n < NT; ++n) {
       #pragma unroll
@@ -395,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
       #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        m[n][x] = kLow;
+        m[n][x] = 0.f;
         l[n][x] = 0.f;
       }
     }
@@ -406,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     const int j_stop = min(k_end * kUnitKeys, r.kv_len);
     const int n_tiles = j_first < j_stop ? (j_stop - j_first + kUnitKeys - 1) / kUnitKeys : 0;
     const int* pages = p.page_table + b * p.table_stride;
+    bool any_bad = false;                               // some page so far lies outside the pool
     auto fetch_pages = [&](int i) {                     // page of tile i + lane
       const int j = j_first + (i + lane) * kUnitKeys;
       int page = i + lane < n_tiles ? pages[j >> kv.page_shift] : 0;
@@ -413,32 +439,40 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
         page = -1;
       }
+      any_bad |= __any_sync(0xffffffffu, page < 0);
       return page;
     };
     int page_now = fetch_pages(0), page_next = fetch_pages(32), pages_at = 0;   // of tiles 32 pages_at ..
 
     // copies of tile i into its stage; a tile in no page leaves the stage as it is
     const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+    constexpr int kRowChunks = S::kRowBytes / 16;
+    const uint32_t copy_at = tile_offset<S::kRowBytes, BITS>(lane / kRowChunks, lane % kRowChunks);
+    const uint32_t key_at = BITS == 8 ? tile_offset<S::kRowBytes, BITS>(g, t)
+                                      : tile_offset<S::kRowBytes, BITS>(g, t >> 1) + (t & 1) * 8;
+    const uint32_t value_at = S::kTileBytes +
+        (BITS == 4 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 2) + (g & 3) * 4
+         : D == 64 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 1) + (g & 1) * 8
+                   : tile_offset<S::kRowBytes, BITS>(2 * t, g * (D / 128)));
     auto page_of = [&](int i) { return __shfl_sync(0xffffffffu, (i >> 5) == pages_at ? page_now : page_next, i & 31); };
     auto copy_tile = [&](int i, int stage) {
       const int page = page_of(i);
       if (page < 0) return;
       const int at = (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
-      const uint32_t dst = ring + stage * S::kStageBytes;
+      const uint32_t dst = ring + stage * S::kStageBytes + copy_at;
       const unsigned char* k = kv.k_codes + page * kv.k_page + (long long)at * S::kRowBytes + lane * 16;
       const unsigned char* v = kv.v_codes + page * kv.v_page + (long long)at * S::kRowBytes + lane * 16;
-      constexpr int kRowChunks = S::kRowBytes / 16;
       #pragma unroll
       for (int c = 0; c < kRowChunks / 2; ++c) {
-        const int chunk = c * 32 + lane;
-        const uint32_t to = dst + tile_offset<S::kRowBytes, BITS>(chunk / kRowChunks, chunk % kRowChunks);
+        const uint32_t to = (dst ^ step_xor<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0)) +
+                            step_add<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0);
         copy16(to, k + c * 512);
         copy16(to + S::kTileBytes, v + c * 512);
       }
       if (lane < 4 * S::kGroups) {
         const bool value = lane >= 2 * S::kGroups;
         const unsigned short* sc = value ? kv.v_scales + page * kv.vs_page : kv.k_scales + page * kv.ks_page;
-        copy16(dst + 2 * S::kTileBytes + lane * 16, sc + (long long)at * S::kGroups + (lane - (value ? 2 * S::kGroups : 0)) * 8);
+        copy16(ring + stage * S::kStageBytes + 2 * S::kTileBytes + lane * 16, sc + (long long)at * S::kGroups + (lane - (value ? 2 * S::kGroups : 0)) * 8);
       }
     };
     __syncwarp();
@@ -459,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         page_now = page_next;
         page_next = fetch_pages(32 * pages_at + 32);
       }
-      const bool hidden = page_of(i) < 0;
+      const bool hidden = any_bad && page_of(i) < 0;
       if (++stage == S::kStages) stage = 0;
       // the stage before this one, read to its end by all lanes, takes the next tile
       {
@@ -475,10 +509,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       for (int x = 0; x < 2; ++x) {
         #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
-          if constexpr (BITS == 8)
-            load_shared<4>(kw[x][c], here + tile_offset<S::kRowBytes, BITS>(g + 8 * x, 4 * c + t));
-          else
-            load_shared<2>(kw[x][c], here + tile_offset<S::kRowBytes, BITS>(g + 8 * x, 2 * c + (t >> 1)) + (t & 1) * 8);
+          constexpr int kStep = BITS == 8 ? 4 : 2;
+          load_shared<S::kKeyWords>(kw[x][c], ((here + key_at) ^ step_xor<S::kRowBytes, BITS>(0, kStep * c)) +
+                                                  step_add<S::kRowBytes, BITS>(8 * x, kStep * c));
         }
       }
       auto load_scales = [&](float (&sc)[2][S::kGroups], uint32_t at) {
@@ -499,111 +532,98 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         }
       };
       load_scales(ks, here + 2 * S::kTileBytes);
-      // ------------------------------------------------------------- scores
-      float s[NT][4];
+      // ---------------------- scores, less the rows' maxima, in units of log2
+      float d[NT][4];
       #pragma unroll
       for (int n = 0; n < NT; ++n)
         #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) d[n][e] = -m[n][e & 1];
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c) {
-        float part[NT][4];
+        if (BITS == 8 && c > 0) break;                  // one sum over all chunks
+        float part[NT][4] = {};
         #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int cc = c; cc < (BITS == 8 ? S::kChunks : c + 1); ++cc)
           #pragma unroll
-          for (int e = 0; e < 4; ++e) part[n][e] = BITS == 8 ? s[n][e] : 0.f;
-        #pragma unroll
-        for (int w = 0; w < S::kKeyWords; ++w) {
-          if constexpr (BITS == 8) {
-            uint32_t a0, a1, a2, a3;
-            dec_w8(kw[0][c][w], a0, a2);
-            dec_w8(kw[1][c][w], a1, a3);
-            #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816(part[n], a0, a1, a2, a3, qb[n][4 * c + w][0], qb[n][4 * c + w][1]);
-          } else {
-            uint32_t x[4], y[4];
-            dec4_h(kw[0][c][w], x);
-            dec4_h(kw[1][c][w], y);
-            #pragma unroll
-            for (int h = 0; h < 2; ++h)
+          for (int w = 0; w < S::kKeyWords; ++w) {
+            if constexpr (BITS == 8) {
+              uint32_t a0, a1, a2, a3;
+              dec_w8(kw[0][cc][w], a0, a2);
+              dec_w8(kw[1][cc][w], a1, a3);
               #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_16816(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * c + 2 * w + h][0],
-                          qb[n][4 * c + 2 * w + h][1]);
+                mma_16816(part[n], a0, a1, a2, a3, qb[n][4 * cc + w][0], qb[n][4 * cc + w][1]);
+            } else {
+              uint32_t x[4], y[4];
+              dec4_h(kw[0][cc][w], x);
+              dec4_h(kw[1][cc][w], y);
+              #pragma unroll
+              for (int h = 0; h < 2; ++h)
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_16816(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * cc + 2 * w + h][0],
+                            qb[n][4 * cc + 2 * w + h][1]);
+            }
           }
-        }
-        if constexpr (BITS == 8) {
-          #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = part[n][e];
-        } else {
-          const float k0 = ks[0][c], k1 = ks[1][c];
-          #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(part[n][e], (e < 2 ? k0 : k1) * rs[n][e & 1], s[n][e]);
-        }
-      }
-      if constexpr (BITS == 8) {
-        const float k0 = ks[0][0], k1 = ks[1][0];
+        const float k0 = ks[0][c] * p.scale_log2, k1 = ks[1][c] * p.scale_log2;
         #pragma unroll
         for (int n = 0; n < NT; ++n)
           #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] *= (e < 2 ? k0 : k1) * rs[n][e & 1];
+          for (int e = 0; e < 4; ++e)
+            d[n][e] = fmaf(part[n][e], (e < 2 ? k0 : k1) * rs[n][e & 1], d[n][e]);
       }
 
-      // ------------------------------------------------- what the rows see
-      const bool some_hidden = hidden || j0 + 15 >= context;
-      if (some_hidden) {
-        #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = j0 + g + (e >> 1) * 8, row = 8 * n + 2 * t + (e & 1);
-            const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, (row0 + row) / p.group, j);
-            if (!see) s[n][e] = -INFINITY;
-          }
-      }
-
-      // ------------------------------------------------------------ weights
-      float v_top = 0.f, v_sc[2][S::kGroups];
+      float v_sc[2][S::kGroups];
       load_scales(v_sc, here + 2 * S::kTileBytes + S::kScaleBytes);
-      #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        #pragma unroll
-        for (int q = 0; q < S::kGroups; ++q) v_top = fmaxf(v_top, v_sc[x][q]);
       uint32_t vw[4][S::kValWords];
       #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int row = 2 * t + (x & 1) + (x >> 1) * 8;
-        const uint32_t values = here + S::kTileBytes;
-        if constexpr (BITS == 4) {
+        constexpr int kLoads = BITS == 4 ? S::kChunks : D == 64 ? 1 : D / 128;
+        constexpr int kWords = S::kValWords / kLoads, kStep = BITS == 4 ? 2 : 1;
+        #pragma unroll
+        for (int c = 0; c < kLoads; ++c) {
+          uint32_t w[kWords];
+          load_shared<kWords>(w, ((here + value_at) ^ step_xor<S::kRowBytes, BITS>(x & 1, kStep * c)) +
+                                     step_add<S::kRowBytes, BITS>((x & 1) + (x >> 1) * 8, kStep * c));
           #pragma unroll
-          for (int c = 0; c < S::kChunks; ++c) {
-            uint32_t w[1];
-            load_shared<1>(w, values + tile_offset<S::kRowBytes, BITS>(row, 2 * c + (g >> 2)) + (g & 3) * 4);
-            vw[x][c] = w[0];
-          }
-        } else if constexpr (D == 64) {
-          load_shared<2>(vw[x], values + tile_offset<S::kRowBytes, BITS>(row, g >> 1) + (g & 1) * 8);
-        } else {
-          #pragma unroll
-          for (int c = 0; c < D / 128; ++c) {
-            uint32_t w[4];
-            load_shared<4>(w, values + tile_offset<S::kRowBytes, BITS>(row, g * (D / 128) + c));
-            #pragma unroll
-            for (int q = 0; q < 4; ++q) vw[x][4 * c + q] = w[q];
-          }
+          for (int q = 0; q < kWords; ++q) vw[x][kWords * c + q] = w[q];
         }
       }
-      bool move = v_top > v_ref;
+
+      // One vote finds what the plain course below cannot take: hidden keys, a
+      // score past its row's maximum by more than 4, one below it by more than
+      // 20, a value scale above the reference or under a 32nd of it.
+      const bool some_hidden = hidden || j0 + 15 >= context;
+      float v_top = v_sc[0][0], v_low = v_sc[0][0], d_top = d[0][0], d_low = d[0][0];
+      #pragma unroll
+      for (int x = 0; x < 2; ++x)
+        #pragma unroll
+        for (int q = 0; q < S::kGroups; ++q) {
+          v_top = fmaxf(v_top, v_sc[x][q]);
+          v_low = fminf(v_low, v_sc[x][q]);
+        }
       #pragma unroll
       for (int n = 0; n < NT; ++n)
         #pragma unroll
-        for (int e = 0; e < 4; ++e) move |= s[n][e] > m[n][e & 1] + 4.f;
-      if (__any_sync(0xffffffffu, move)) {
-        const unsigned bits = __float_as_uint(v_top);
+        for (int e = 0; e < 4; ++e) {
+          d_top = fmaxf(d_top, d[n][e]);
+          d_low = fminf(d_low, d[n][e]);
+        }
+      const bool plain = d_top <= 4.f && d_low >= -20.f && v_top <= v_ref && v_low >= v_ref * 0.03125f;
+      const bool rare = some_hidden || open || !__all_sync(0xffffffffu, plain);
+      if (rare) {
+        open = false;
+        if (some_hidden) {
+          #pragma unroll
+          for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = j0 + g + (e >> 1) * 8, row = 8 * n + 2 * t + (e & 1);
+              const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, (row0 + row) / p.group, j);
+              if (!see) d[n][e] = -INFINITY;
+            }
+        }
+        const unsigned bits = __float_as_uint(fmaxf(v_top, 0.f));
         const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, some_hidden || bits >= 0x7F800000u ? 0u : bits));
         float adjust = 1.f;
         if (most > v_ref) {
@@ -617,13 +637,21 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           #pragma unroll
           for (int x = 0; x < 2; ++x) {
             // a row's own lanes alone move it, so that its bits do not depend on the other rows
-            const bool moves = s[n][x] > m[n][x] + 4.f || s[n][2 + x] > m[n][x] + 4.f;
-            const bool row_moves = __ballot_sync(0xffffffffu, moves) & (0x11111111u << t);
-            float top = fmaxf(s[n][x], s[n][2 + x]);
+            const unsigned lanes = 0x11111111u << t;
+            float top = fmaxf(d[n][x], d[n][2 + x]);
             #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float keep = row_moves ? ex2<kBf16>(m[n][x] - top) : 1.f;
-            if (row_moves) m[n][x] = top;
+            const bool fresh = !(__ballot_sync(0xffffffffu, l[n][x] > 0.f) & lanes);   // it has seen nothing yet
+            float keep = 1.f;
+            if (top > 4.f || (fresh && top > -INFINITY)) {
+              const float moved = m[n][x] + top, by = moved - m[n][x];
+              m[n][x] = moved;
+              d[n][x] -= by;
+              d[n][2 + x] -= by;
+              keep = fresh ? 1.f : ex2<kBf16>(-by);
+            } else if (fresh) {
+              open = true;
+            }
             #pragma unroll
             for (int q = 0; q < S::kTiles; ++q) {
               acc[n][q][x] *= keep * adjust;
@@ -631,21 +659,30 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             }
             l[n][x] *= keep;
           }
+        open = __any_sync(0xffffffffu, open);
       }
-      float least = INFINITY, a[S::kGroups][NT][4];
+      // ------------------------------------------------------------ weights
+      float a[S::kGroups][NT][4];
       #pragma unroll
       for (int n = 0; n < NT; ++n)
         #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float w = ex2<kBf16>(s[n][e] - m[n][e & 1]);
+          const float w = ex2<kBf16>(d[n][e]);
           l[n][e & 1] += w;
           #pragma unroll
-          for (int q = 0; q < S::kGroups; ++q) {
-            a[q][n][e] = w * (v_sc[e >> 1][q] * fac);
-            least = fminf(least, a[q][n][e]);
-          }
+          for (int q = 0; q < S::kGroups; ++q) a[q][n][e] = w * (v_sc[e >> 1][q] * fac);
         }
-      const bool wide = some_hidden || __any_sync(0xffffffffu, least < 0x1p-14f);
+      bool wide = false;
+      if (rare) {
+        float least = INFINITY;
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+          #pragma unroll
+          for (int e = 0; e < 4; ++e)
+            #pragma unroll
+            for (int q = 0; q < S::kGroups; ++q) least = fminf(least, a[q][n][e]);
+        wide = some_hidden || __any_sync(0xffffffffu, least < 0x1p-14f);
+      }
 
       // -------------------------------------------------------------- values
       // products of 16 keys' values, decoded by dec8 / dec4, tile by tile of 16 elements
@@ -697,8 +734,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           for (int n = 0; n < NT; ++n)
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float x = s[n][2 * h] == -INFINITY ? 0.f : a[q][n][2 * h];
-              const float y = s[n][2 * h + 1] == -INFINITY ? 0.f : a[q][n][2 * h + 1];
+              const float x = d[n][2 * h] == -INFINITY ? 0.f : a[q][n][2 * h];
+              const float y = d[n][2 * h + 1] == -INFINITY ? 0.f : a[q][n][2 * h + 1];
               const uint32_t u = pack_b2(x, y);
               hi[q][n][h] = transpose8(u);
               lo[q][n][h] = transpose8(pack_b2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
@@ -724,6 +761,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       for (int x = 0; x < 2; ++x) {
         #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], o);
+        if (l[n][x] == 0.f) m[n][x] = kLow;             // nothing seen
         if (g == 0) {
           sm_m[warp * S::kRows + 8 * n + 2 * t + x] = m[n][x];
           sm_l[warp * S::kRows + 8 * n + 2 * t + x] = l[n][x];
