@@ -377,7 +377,7 @@ int ql_rotary(const ql_rotary_args* args, void* stream);
  * contiguous within a page; page strides in bytes (codes) and elements
  * (scales).  page_size is a power of two from 16 to 65536; head_dim is 64,
  * 128 or 256.  Token t of page p is slot p * page_size + t.  Pointers and page
- * strides are multiples of 16 bytes. */
+ * strides are multiples of 16 bytes, strides below 2^32. */
 typedef struct {
   void *k_codes, *k_scales, *v_codes, *v_scales;
   int64_t num_pages, page_size, kv_heads, head_dim, bits;

@@ -15,6 +15,14 @@
 namespace ql {
 namespace att {
 
+// Division of numbers below 2^31 by one known on the host: with s the
+// smallest power of two at least d and m = ceil(2^31 s / d), n m / (2^31 s)
+// exceeds n / d by less than 1 / d, so its whole part is n / d's.
+struct Divisor {
+  unsigned m, shift;
+  __device__ __forceinline__ int of(int n) const { return (int)(((unsigned long long)(unsigned)n * m) >> shift); }
+};
+
 struct Params {
   kvc::Pool cache;
   kvc::Rows q;                   // [total_q][q_heads][head_dim]
@@ -27,6 +35,7 @@ struct Params {
   long long table_stride;
   int table_width, num_pages;
   int batch, total_q, q_heads, group, mask_words;
+  Divisor by_group;
   float scale_log2;              // scale * log2(e): scores in units of log2
   unsigned* err;
 };
@@ -88,37 +97,62 @@ __device__ __forceinline__ int item_units(const Request& r) {
 }
 template <int ROWS>
 __device__ __forceinline__ long long request_units(const Params& p, const Request& r) {
-  const long long tiles = ((long long)r.q_len * p.group + ROWS - 1) / ROWS;
-  return tiles * p.cache.heads * item_units(r);
+  const unsigned tiles = (unsigned)(r.q_len * p.group + ROWS - 1) / ROWS;
+  return (long long)tiles * p.cache.heads * item_units(r);
 }
 
 // Sums the requests' units and finds the request that holds this CTA's first
-// unit: *b and the unit at which it begins.  All threads call it.
+// unit: *b, the unit at which it begins, and its lengths.  All threads call
+// it; up to 32 requests each warp does so by itself.
 template <int ROWS>
-__device__ __forceinline__ Work find_work(const Params& p, int* b, long long* base) {
+__device__ __forceinline__ Work find_work(const Params& p, int* b, long long* base, Request* r) {
   __shared__ long long warp_sum[kWarps];
   __shared__ long long found_base;
   __shared__ int found_b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto scan = [&](long long v, long long* sum) {      // inclusive, and the CTA's sum
+  auto warp_scan = [&](long long v) {
     #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
+    return v;
+  };
+  Work w = {0, 0};
+  if (p.batch <= 32) {
+    Request mine = {0, 0, 0};
+    long long units = 0;
+    if (lane < p.batch) {
+      mine = request(p, lane);
+      units = request_units<ROWS>(p, mine);
+    }
+    const long long incl = warp_scan(units);
+    w.total = __shfl_sync(0xffffffffu, incl, 31);
+    w.ctas = (int)min((long long)gridDim.x, w.total / kMinUnits);
+    if ((int)blockIdx.x >= w.ctas) return w;
+    const long long u = w.first_unit(blockIdx.x);
+    const int at = __ffs(__ballot_sync(0xffffffffu, u < incl)) - 1;      // some lane: u < total
+    *b = at;
+    *base = __shfl_sync(0xffffffffu, incl - units, at);
+    r->q0 = __shfl_sync(0xffffffffu, mine.q0, at);
+    r->q_len = __shfl_sync(0xffffffffu, mine.q_len, at);
+    r->kv_len = __shfl_sync(0xffffffffu, mine.kv_len, at);
+    return w;
+  }
+  auto scan = [&](long long v, long long* sum) {      // inclusive over the CTA, and its sum
+    v = warp_scan(v);
     __syncthreads();
     if (lane == 31) warp_sum[warp] = v;
     __syncthreads();
     long long before = 0, all = 0;
     #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += warp_sum[w];
-      all += warp_sum[w];
+    for (int x = 0; x < kWarps; ++x) {
+      if (x < warp) before += warp_sum[x];
+      all += warp_sum[x];
     }
     *sum = all;
     return v + before;
   };
-  Work w = {0, 0};
   long long mine = 0, incl = 0, sum;
   for (int i = 0; i < p.batch; i += kThreads) {
     const int at = i + threadIdx.x;
@@ -146,6 +180,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
   __syncthreads();
   *b = found_b;
   *base = found_base;
+  *r = request(p, *b);
   return w;
 }
 
@@ -207,10 +242,26 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = a b (+ d unless this begins the sum)
+__device__ __forceinline__ void mma_from(float (&d)[4], bool begin, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if (begin)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    mma_16816(d, a0, a1, a2, a3, b0, b1);
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 // 16 bytes from global to shared memory, past L1, in the thread's current group.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_if(bool yes, uint32_t dst, const void* src) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst),
+               "l"(src), "r"((int)yes)
+               : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -313,7 +364,10 @@ struct Shape {
   static constexpr int kStages = kBudget / (kWarps * kStageBytes) < 6 ? kBudget / (kWarps * kStageBytes) : 6;
   static_assert(kStages >= 2 && 4 * kGroups <= 32, "");
   static constexpr size_t kRing = (size_t)kWarps * kStages * kStageBytes;
-  static constexpr size_t kJoined = (size_t)kWarps * kRows * (D + 2) * sizeof(float);   // takes the ring's place
+  // rows of the warps to be joined take the ring's place; their stride puts the rows that a quarter warp writes
+  // together on different banks
+  static constexpr int kRowStride = D + 4;
+  static constexpr size_t kJoined = (size_t)kWarps * kRows * (kRowStride + 2) * sizeof(float);
   static constexpr size_t kSmem = 128 + (kRing > kJoined ? kRing : kJoined);
 };
 
@@ -326,8 +380,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
   griddep_wait();
   extern __shared__ float smem_raw[];
   float* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u) / 4;
-  float* sm_o = smem;                                   // [warp][row][D]
-  float* sm_m = smem + kWarps * S::kRows * D;           // [warp][row]
+  float* sm_o = smem;                                   // [warp][row][kRowStride]
+  float* sm_m = smem + kWarps * S::kRows * S::kRowStride;   // [warp][row]
   float* sm_l = sm_m + kWarps * S::kRows;
   __shared__ int last_one;
 
@@ -336,11 +390,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
   const kvc::Pool& kv = p.cache;
   int b;
   long long base;
-  const Work work = find_work<S::kRows>(p, &b, &base);
+  Request r;
+  const Work work = find_work<S::kRows>(p, &b, &base, &r);
   if ((int)blockIdx.x >= work.ctas) return;
   long long u = work.first_unit(blockIdx.x);
   const long long u_end = work.first_unit(blockIdx.x + 1);
-  Request r = request(p, b);
 
   while (u < u_end) {
     // ------------------------------------------------------ the next segment
@@ -351,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       mine = request_units<S::kRows>(p, r);
     }
     const int per_item = item_units(r);
-    const int tiles = (int)(((long long)r.q_len * p.group + S::kRows - 1) / S::kRows);
+    const int tiles = (int)((unsigned)(r.q_len * p.group + S::kRows - 1) / S::kRows);
     const long long item = Work::quotient(u - base, per_item);
     const int k_begin = (int)((u - base) - item * per_item);
     const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
@@ -359,31 +413,101 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     const int rows = min(S::kRows, r.q_len * p.group - row0);
     const int context = r.kv_len - r.q_len;             // positions that every row sees
 
+    // --------------------------------------------- this warp's tiles of 16 keys
+    // tile i: keys j0(i) .. j0(i) + 15, within one page
+    const int j_first = k_begin * kUnitKeys + warp * 16;
+    const int j_stop = min(k_end * kUnitKeys, r.kv_len);
+    const int n_tiles = j_first < j_stop ? (j_stop - j_first + kUnitKeys - 1) / kUnitKeys : 0;
+    const int* pages = p.page_table + b * p.table_stride;
+    bool any_bad = false;                               // some page so far lies outside the pool
+    auto fetch_page = [&](int i) {                      // of tile i + lane
+      return i + lane < n_tiles ? pages[(j_first + (i + lane) * kUnitKeys) >> kv.page_shift] : 0;
+    };
+    auto check_page = [&](int page) {
+      const bool bad = page < 0 || page >= p.num_pages;
+      if (__any_sync(0xffffffffu, bad)) {
+        any_bad = true;
+        if (bad) atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+      }
+      return bad ? -1 : page;
+    };
+    int page_now = fetch_page(0), page_next = fetch_page(32), pages_at = 0;   // of tiles 32 pages_at ..
+    // rows g of the queries, on their way while the pages are looked up and the first tiles copied
+    kvc::Vec8<T> q_raw[NT][S::kChunks][2];
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + 8 * n + g;
+      const bool live = 8 * n + g < rows;
+      const int token = live ? p.by_group.of(row) : 0, qh = head * p.group + (live ? row - token * p.group : 0);
+      const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
+      #pragma unroll
+      for (int c = 0; c < S::kChunks; ++c)
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const T* at = src + c * 64 + t * 16 + h * 8;
+          if (live && p.q.vec) {
+            q_raw[n][c][h] = *reinterpret_cast<const kvc::Vec8<T>*>(at);
+          } else {
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) q_raw[n][c][h].v[i] = live ? at[i] : kvc::from_f<T>(0.f);
+          }
+        }
+    }
+    page_now = check_page(page_now);
+    page_next = check_page(page_next);
+
+    const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+    constexpr int kRowChunks = S::kRowBytes / 16;
+    const uint32_t copy_at = tile_offset<S::kRowBytes, BITS>(lane / kRowChunks, lane % kRowChunks);
+    const uint32_t key_at = BITS == 8 ? tile_offset<S::kRowBytes, BITS>(g, t)
+                                      : tile_offset<S::kRowBytes, BITS>(g, t >> 1) + (t & 1) * 8;
+    const uint32_t value_at = S::kTileBytes +
+        (BITS == 4 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 2) + (g & 3) * 4
+         : D == 64 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 1) + (g & 1) * 8
+                   : tile_offset<S::kRowBytes, BITS>(2 * t, g * (D / 128)));
+    auto page_of = [&](int i) { return __shfl_sync(0xffffffffu, (i >> 5) == pages_at ? page_now : page_next, i & 31); };
+    // Copies of tile i to the stage at `dst` (of a page outside the pool, any rows: its keys are hidden).  A lane's
+    // part of a tile, and of the scales: the first lanes take those of the keys, the next of the values.
+    const unsigned char *lane_k = kv.k_codes + lane * 16, *lane_v = kv.v_codes + lane * 16;
+    const bool of_values = lane >= 2 * S::kGroups;
+    const unsigned short* lane_s = (of_values ? kv.v_scales : kv.k_scales) + (lane - (of_values ? 2 * S::kGroups : 0)) * 8;
+    const unsigned scale_page = of_values ? kv.vs_page : kv.ks_page;
+    auto copy_tile = [&](int i, uint32_t dst) {
+      const unsigned page = (unsigned)max(page_of(i), 0);
+      const unsigned at = (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
+      const unsigned char* k = lane_k + (unsigned long long)page * kv.k_page + (unsigned long long)at * S::kRowBytes;
+      const unsigned char* v = lane_v + (unsigned long long)page * kv.v_page + (unsigned long long)at * S::kRowBytes;
+      const unsigned short* sc = lane_s + (unsigned long long)page * scale_page + (unsigned long long)at * S::kGroups;
+      #pragma unroll
+      for (int c = 0; c < kRowChunks / 2; ++c) {
+        const uint32_t to = ((dst + copy_at) ^ step_xor<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0)) +
+                            step_add<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0);
+        copy16(to, k + c * 512);
+        copy16(to + S::kTileBytes, v + c * 512);
+      }
+      copy16_if(lane < 4 * S::kGroups, dst + 2 * S::kTileBytes + lane * 16, sc);
+    };
+    __syncwarp();
+    #pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      if (i < n_tiles) copy_tile(i, ring + i * S::kStageBytes);
+      copy_commit();
+    }
+
     // ------------------------------------------------------------- queries
     uint32_t qb[NT][S::kTiles][2];
     float rs[NT][2];                                    // on the scores of rows 2t, 2t + 1
     #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 8 * n + g;
-      const bool live = 8 * n + g < rows;
-      const int token = live ? row / p.group : 0, qh = head * p.group + (live ? row - token * p.group : 0);
-      const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
-      float f[S::kChunks][16];
+      float f[S::kChunks][16], down = 1.f, up = 1.f;
       unsigned top = 0;
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
         #pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-          float x[4] = {}, y[4] = {};
-          if (live) kvc::load8(x, y, src + c * 64 + t * 16 + i, p.q.vec);
-          #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[c][i + e] = x[e];
-            f[c][i + 4 + e] = y[e];
-            top = max(top, max(__float_as_uint(x[e]) & 0x7FFFFFFFu, __float_as_uint(y[e]) & 0x7FFFFFFFu));
-          }
+        for (int i = 0; i < 16; ++i) {
+          f[c][i] = kvc::to_f(q_raw[n][c][i / 8].v[i % 8]);
+          if (kBf16) top = max(top, __float_as_uint(f[c][i]) & 0x7FFFFFFFu);
         }
-      float down = 1.f, up = 1.f;
       if constexpr (kBf16) {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -403,8 +527,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             qb[n][4 * c + w][x] = pack_h2(f[c][i] * down, f[c][j] * down);
           }
       #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        rs[n][x] = kBf16 ? __shfl_sync(0xffffffffu, up, (2 * t + x) * 4) : 1.f;
+      for (int x = 0; x < 2; ++x) rs[n][x] = kBf16 ? __shfl_sync(0xffffffffu, up, (2 * t + x) * 4) : 1.f;
     }
 
     // ---------------------------------------------------------- running state
@@ -425,84 +548,22 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       }
     }
 
-    // --------------------------------------------- this warp's tiles of 16 keys
-    // tile i: keys j0(i) .. j0(i) + 15, within one page
-    const int j_first = k_begin * kUnitKeys + warp * 16;
-    const int j_stop = min(k_end * kUnitKeys, r.kv_len);
-    const int n_tiles = j_first < j_stop ? (j_stop - j_first + kUnitKeys - 1) / kUnitKeys : 0;
-    const int* pages = p.page_table + b * p.table_stride;
-    bool any_bad = false;                               // some page so far lies outside the pool
-    auto fetch_pages = [&](int i) {                     // page of tile i + lane
-      const int j = j_first + (i + lane) * kUnitKeys;
-      int page = i + lane < n_tiles ? pages[j >> kv.page_shift] : 0;
-      if (page < 0 || page >= p.num_pages) {
-        atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
-        page = -1;
-      }
-      any_bad |= __any_sync(0xffffffffu, page < 0);
-      return page;
-    };
-    int page_now = fetch_pages(0), page_next = fetch_pages(32), pages_at = 0;   // of tiles 32 pages_at ..
-
-    // copies of tile i into its stage; a tile in no page leaves the stage as it is
-    const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
-    constexpr int kRowChunks = S::kRowBytes / 16;
-    const uint32_t copy_at = tile_offset<S::kRowBytes, BITS>(lane / kRowChunks, lane % kRowChunks);
-    const uint32_t key_at = BITS == 8 ? tile_offset<S::kRowBytes, BITS>(g, t)
-                                      : tile_offset<S::kRowBytes, BITS>(g, t >> 1) + (t & 1) * 8;
-    const uint32_t value_at = S::kTileBytes +
-        (BITS == 4 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 2) + (g & 3) * 4
-         : D == 64 ? tile_offset<S::kRowBytes, BITS>(2 * t, g >> 1) + (g & 1) * 8
-                   : tile_offset<S::kRowBytes, BITS>(2 * t, g * (D / 128)));
-    auto page_of = [&](int i) { return __shfl_sync(0xffffffffu, (i >> 5) == pages_at ? page_now : page_next, i & 31); };
-    auto copy_tile = [&](int i, int stage) {
-      const int page = page_of(i);
-      if (page < 0) return;
-      const int at = (head << kv.page_shift) + ((j_first + i * kUnitKeys) & ((1 << kv.page_shift) - 1));
-      const uint32_t dst = ring + stage * S::kStageBytes + copy_at;
-      const unsigned char* k = kv.k_codes + page * kv.k_page + (long long)at * S::kRowBytes + lane * 16;
-      const unsigned char* v = kv.v_codes + page * kv.v_page + (long long)at * S::kRowBytes + lane * 16;
-      #pragma unroll
-      for (int c = 0; c < kRowChunks / 2; ++c) {
-        const uint32_t to = (dst ^ step_xor<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0)) +
-                            step_add<S::kRowBytes, BITS>(c * 32 / kRowChunks, 0);
-        copy16(to, k + c * 512);
-        copy16(to + S::kTileBytes, v + c * 512);
-      }
-      if (lane < 4 * S::kGroups) {
-        const bool value = lane >= 2 * S::kGroups;
-        const unsigned short* sc = value ? kv.v_scales + page * kv.vs_page : kv.k_scales + page * kv.ks_page;
-        copy16(ring + stage * S::kStageBytes + 2 * S::kTileBytes + lane * 16, sc + (long long)at * S::kGroups + (lane - (value ? 2 * S::kGroups : 0)) * 8);
-      }
-    };
-    __syncwarp();
-    #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      if (i < n_tiles) copy_tile(i, i);
-      copy_commit();
-    }
-    int stage = 0;
+    uint32_t here = ring + (S::kStages - 1) * S::kStageBytes;
     #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int j0 = j_first + i * kUnitKeys;
       copy_wait<S::kStages - 2>();
       __syncwarp();
-      const uint32_t here = ring + stage * S::kStageBytes;
       if ((i >> 5) > pages_at) {
         ++pages_at;
         page_now = page_next;
-        page_next = fetch_pages(32 * pages_at + 32);
+        page_next = check_page(fetch_page(32 * pages_at + 32));
       }
       const bool hidden = any_bad && page_of(i) < 0;
-      if (++stage == S::kStages) stage = 0;
       // the stage before this one, read to its end by all lanes, takes the next tile
-      {
-        const int next = i + S::kStages - 1;
-        if (next < n_tiles) {
-          copy_tile(next, stage == 0 ? S::kStages - 2 : stage == 1 ? S::kStages - 1 : stage - 2);
-        }
-        copy_commit();
-      }
+      if (i + S::kStages - 1 < n_tiles) copy_tile(i + S::kStages - 1, here);
+      copy_commit();
+      here = here == ring + (S::kStages - 1) * S::kStageBytes ? ring : here + S::kStageBytes;
       uint32_t kw[2][S::kChunks][S::kKeyWords];
       float ks[2][S::kGroups];
       #pragma unroll
@@ -541,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c) {
         if (BITS == 8 && c > 0) break;                  // one sum over all chunks
-        float part[NT][4] = {};
+        float part[NT][4];
         #pragma unroll
         for (int cc = c; cc < (BITS == 8 ? S::kChunks : c + 1); ++cc)
           #pragma unroll
@@ -552,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
               dec_w8(kw[1][cc][w], a1, a3);
               #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_16816(part[n], a0, a1, a2, a3, qb[n][4 * cc + w][0], qb[n][4 * cc + w][1]);
+                mma_from(part[n], cc == c && w == 0, a0, a1, a2, a3, qb[n][4 * cc + w][0], qb[n][4 * cc + w][1]);
             } else {
               uint32_t x[4], y[4];
               dec4_h(kw[0][cc][w], x);
@@ -561,8 +622,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
               for (int h = 0; h < 2; ++h)
                 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                  mma_16816(part[n], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1], qb[n][4 * cc + 2 * w + h][0],
-                            qb[n][4 * cc + 2 * w + h][1]);
+                  mma_from(part[n], w == 0 && h == 0, x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1],
+                           qb[n][4 * cc + 2 * w + h][0], qb[n][4 * cc + 2 * w + h][1]);
             }
           }
         const float k0 = ks[0][c] * p.scale_log2, k1 = ks[1][c] * p.scale_log2;
@@ -619,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = j0 + g + (e >> 1) * 8, row = 8 * n + 2 * t + (e & 1);
-              const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, (row0 + row) / p.group, j);
+              const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, p.by_group.of(row0 + row), j);
               if (!see) d[n][e] = -INFINITY;
             }
         }
@@ -778,13 +839,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
         // one after the other: their product can be too small for fp32
         const float f = ex2<kBf16>(m[n][x] - top), unit = 1.f / fac;
-        float* dst = sm_o + (warp * S::kRows + row) * D;
+        float* dst = sm_o + (warp * S::kRows + row) * S::kRowStride + g * 4;
         #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
-          // elements 2i, 2i + 1 of the lane's eighth (8 bits), or of its 8 in each 64 (4 bits)
-          const int d = BITS == 8 ? g * (D / 8) + 2 * i : (i / 4) * 64 + g * 8 + 2 * (i % 4);
-          *reinterpret_cast<float2*>(dst + d) = make_float2(acc[n][i][x] * unit * f, acc[n][i][2 + x] * unit * f);
-        }
+        for (int i = 0; i < S::kTiles; i += 2)
+          *reinterpret_cast<float4*>(dst + i * 16) =
+              make_float4(acc[n][i][x] * unit * f, acc[n][i][2 + x] * unit * f, acc[n][i + 1][x] * unit * f,
+                          acc[n][i + 1][2 + x] * unit * f);
       }
     __syncthreads();
 
@@ -792,15 +852,19 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     const long long item_begin = base + item * per_item;
     const bool whole = k_begin == 0 && k_end == per_item;
     float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
-    auto finish = [&](int row, int d, const float4& o, float top, float sum) {
-      const int token = (row0 + row) / p.group, qh = head * p.group + (row0 + row) - token * p.group;
+    // Four neighbouring elements of a row are parked at `at`: those of lane group g = at / 4 % 8 and tiles 2 j,
+    // 2 j + 1, j = at / 32, which are elements 4 j.. of its eighth (8 bits), or 4 (j % 2).. of its 8 in 64 j / 2 (4 bits).
+    auto finish = [&](int row, int place, const float4& o, float top, float sum) {
+      const int pg = (place >> 2) & 7, j = place >> 5;
+      const int d = BITS == 8 ? pg * (D / 8) + 4 * j : (j >> 1) * 64 + pg * 8 + 4 * (j & 1);
+      const int token = p.by_group.of(row0 + row), qh = head * p.group + (row0 + row) - token * p.group;
       const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
       const float f[4] = {o.x, o.y, o.z, o.w};
       kvc::Vec4<T> v;
       #pragma unroll
       for (int i = 0; i < 4; ++i) v.v[i] = kvc::from_f<T>(sum == 0.f ? 0.f : f[i] / sum);
       *reinterpret_cast<kvc::Vec4<T>*>(static_cast<T*>(p.out) + at * D + d) = v;
-      if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
+      if (p.lse && place == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718056f;
     };
     auto park = [&](float* dst, int row, int d, const float4& o, float top, float sum) {
       *reinterpret_cast<float4*>(dst + 2 * S::kRows + row * D + d) = o;
@@ -818,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         sum += sm_l[w * S::kRows + row] * ex2<kBf16>(sm_m[w * S::kRows + row] - top);
-        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * S::kRows + row) * D + d);
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * S::kRows + row) * S::kRowStride + d);
         o.x += v.x;
         o.y += v.y;
         o.z += v.z;

@@ -90,6 +90,8 @@ int make_pool(Pool* c, const ql_kv_cache& a) {
   if (a.k_page_stride < rows * row || a.v_page_stride < rows * row || a.k_scale_page_stride < rows * groups ||
       a.v_scale_page_stride < rows * groups)
     return QL_ERR_BAD_STRIDE;
+  if (std::max(a.k_page_stride, a.v_page_stride) > UINT_MAX || std::max(a.k_scale_page_stride, a.v_scale_page_stride) > UINT_MAX)
+    return QL_ERR_UNSUPPORTED;
   // rows are read and written in 16-byte words
   if (!aligned(a.k_codes, 16) || !aligned(a.v_codes, 16) || !aligned(a.k_scales, 16) || !aligned(a.v_scales, 16) ||
       a.k_page_stride % 16 || a.v_page_stride % 16 || a.k_scale_page_stride % 8 || a.v_scale_page_stride % 8)
@@ -98,10 +100,10 @@ int make_pool(Pool* c, const ql_kv_cache& a) {
   c->v_codes = static_cast<unsigned char*>(a.v_codes);
   c->k_scales = static_cast<unsigned short*>(a.k_scales);
   c->v_scales = static_cast<unsigned short*>(a.v_scales);
-  c->k_page = a.k_page_stride;
-  c->v_page = a.v_page_stride;
-  c->ks_page = a.k_scale_page_stride;
-  c->vs_page = a.v_scale_page_stride;
+  c->k_page = (unsigned)a.k_page_stride;
+  c->v_page = (unsigned)a.v_page_stride;
+  c->ks_page = (unsigned)a.k_scale_page_stride;
+  c->vs_page = (unsigned)a.v_scale_page_stride;
   c->slots = a.num_pages * a.page_size;
   c->page_shift = __builtin_ctzll((unsigned long long)a.page_size);
   c->heads = (int)a.kv_heads;
@@ -291,7 +293,7 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   ql::att::Params p = {};
   int st = make_pool(&p.cache, a->cache);
   if (st != QL_OK) return st;
-  if (a->q_heads % a->cache.kv_heads != 0) return QL_ERR_BAD_SHAPE;
+  if (a->q_heads % a->cache.kv_heads != 0 || a->total_q * a->q_heads > INT_MAX) return QL_ERR_BAD_SHAPE;
   if (a->batch == 0 || a->total_q == 0 || a->q_heads == 0) return QL_OK;
   if (!a->cu_q && a->total_q % a->batch != 0) return QL_ERR_BAD_SHAPE;
   if (!a->out || !a->kv_lens || !a->workspace || (!a->page_table && a->table_width > 0)) return QL_ERR_NULL_POINTER;
@@ -315,6 +317,9 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   p.total_q = (int)a->total_q;
   p.q_heads = (int)a->q_heads;
   p.group = (int)(a->q_heads / a->cache.kv_heads);
+  unsigned log = 0;
+  while ((1ll << log) < p.group) ++log;
+  p.by_group = {(unsigned)cdiv(1ll << (31 + log), p.group), 31 + log};
   p.mask_words = (int)a->mask_words;
   p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   p.err = dev.err_word;

@@ -229,10 +229,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
 }
 
 // --------------------------------------------------------------------- cache
-struct Pool {              // strides between pages in bytes (codes) and elements (scales)
+struct Pool {              // strides between pages in bytes (codes) and elements (scales), below 2^32
   unsigned char *k_codes, *v_codes;
   unsigned short *k_scales, *v_scales;
-  long long k_page, v_page, ks_page, vs_page;
+  unsigned k_page, v_page, ks_page, vs_page;
   long long slots;         // pages * page_size
   int page_shift;          // log2(page_size)
   int heads, row_bytes, groups, bits;
