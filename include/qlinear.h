@@ -350,7 +350,7 @@ int ql_allgather_f16(const void* src, int64_t lds, void* out, int64_t ldo, int64
  * out[t, h] = x[t, h] with its first rotary_dim elements turned by the angles
  * of positions[t]; out may be x.  table fp32 [max_positions][rotary_dim / 2][2]
  * holds each pair's cosine and sine (and any factor on both).  rotary_dim is
- * a multiple of 8, head_dim too.  inverse != 0 turns back (the direction of
+ * a multiple of 8, head_dim too (at most 2048).  inverse != 0 turns back (the direction of
  * the gradient).  A position outside the table takes its nearest row and
  * records QL_DEVICE_ERROR_BAD_INDEX.
  */

@@ -15,14 +15,6 @@
 namespace ql {
 namespace att {
 
-// Division of numbers below 2^31 by one known on the host: with s the
-// smallest power of two at least d and m = ceil(2^31 s / d), n m / (2^31 s)
-// exceeds n / d by less than 1 / d, so its whole part is n / d's.
-struct Divisor {
-  unsigned m, shift;
-  __device__ __forceinline__ int of(int n) const { return (int)(((unsigned long long)(unsigned)n * m) >> shift); }
-};
-
 struct Params {
   kvc::Pool cache;
   kvc::Rows q;                   // [total_q][q_heads][head_dim]
@@ -35,7 +27,7 @@ struct Params {
   long long table_stride;
   int table_width, num_pages;
   int batch, total_q, q_heads, group, mask_words;
-  Divisor by_group;
+  kvc::Divisor by_group;
   float scale_log2;              // scale * log2(e): scores in units of log2
   unsigned* err;
 };

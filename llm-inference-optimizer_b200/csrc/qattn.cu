@@ -113,18 +113,6 @@ int make_pool(Pool* c, const ql_kv_cache& a) {
   return QL_OK;
 }
 
-template <typename T>
-int run_append(const ql::kvc::AppendParams& p, int64_t head_dim, void* stream, int64_t flags) {
-  const int lanes = (int)head_dim / 8, rows = p.q_heads + 2 * p.cache.heads;
-  const int threads = (int)std::min<int64_t>(256, cdiv((int64_t)rows * lanes, 32) * 32);
-  const dim3 grid((unsigned)p.tokens), block((unsigned)threads);
-  switch (lanes) {
-    case 8: return launch(ql::kvc::append_kernel<T, 8>, grid, block, 0, stream, flags, p);
-    case 16: return launch(ql::kvc::append_kernel<T, 16>, grid, block, 0, stream, flags, p);
-    default: return launch(ql::kvc::append_kernel<T, 32>, grid, block, 0, stream, flags, p);
-  }
-}
-
 // Raise the dynamic shared-memory limit of a kernel once per device.
 template <typename Kern>
 int allow_smem(Kern kernel, size_t bytes, std::atomic<unsigned char>* done) {
@@ -140,6 +128,53 @@ int allow_smem(Kern kernel, size_t bytes, std::atomic<unsigned char>* done) {
   }
   done[dev].store(1, std::memory_order_release);
   return QL_OK;
+}
+
+ql::kvc::Divisor divisor(int64_t d) {
+  unsigned log = 0;
+  while ((1ll << log) < d) ++log;
+  return {(unsigned)cdiv(1ll << (31 + log), d), 31 + log};
+}
+
+// Threads over tokens and `per_thread` heads each; with few tokens a head
+// each, since then all is latency.
+ql::kvc::Grid make_grid(int64_t tokens, int64_t heads, int64_t chunks, int per_thread, int sms) {
+  ql::kvc::Grid g;
+  const int64_t wanted = tokens <= sms ? heads : cdiv(heads, per_thread);
+  g.chunks = (int)chunks;
+  g.beside = (int)std::max<int64_t>(1, std::min(wanted, 256 / chunks));
+  const int64_t threads = g.beside * chunks;
+  g.tokens = tokens <= sms ? 1 : (int)(256 / threads);
+  g.by_token = divisor(threads);
+  g.by_chunks = divisor(chunks);
+  return g;
+}
+unsigned threads_of(const ql::kvc::Grid& g) { return (unsigned)cdiv((int64_t)g.beside * g.chunks * g.tokens, 32) * 32; }
+
+template <typename T, int LANES>
+int run_append_bits(const ql::kvc::AppendParams& p, dim3 grid, dim3 block, void* stream, int64_t flags) {
+  return p.cache.bits == 8 ? launch(ql::kvc::append_kernel<T, LANES, 8>, grid, block, 0, stream, flags, p)
+                           : launch(ql::kvc::append_kernel<T, LANES, 4>, grid, block, 0, stream, flags, p);
+}
+
+template <typename T>
+int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, int64_t flags) {
+  p.grid = make_grid(p.tokens, p.cache.heads, chunks, 1, sms);
+  p.kv_ctas = (int)cdiv(p.tokens, p.grid.tokens);
+  unsigned threads = threads_of(p.grid);
+  int64_t ctas = p.kv_ctas;
+  if (p.q.heads > 0) {
+    p.q.grid = make_grid(p.tokens, p.q.heads, chunks, ql::kvc::kHeads, sms);
+    threads = std::max(threads, threads_of(p.q.grid));
+    ctas += cdiv(p.tokens, p.q.grid.tokens);
+  }
+  if (ctas > INT_MAX) return QL_ERR_BAD_SHAPE;
+  const dim3 grid((unsigned)ctas), block(threads);
+  switch (chunks) {
+    case 8: return run_append_bits<T, 8>(p, grid, block, stream, flags);
+    case 16: return run_append_bits<T, 16>(p, grid, block, stream, flags);
+    default: return run_append_bits<T, 32>(p, grid, block, stream, flags);
+  }
 }
 
 struct Attention {
@@ -199,7 +234,7 @@ extern "C" {
 int ql_rotary(const ql_rotary_args* a, void* stream) {
   if (!a) return QL_ERR_NULL_POINTER;
   if (a->tokens < 0 || a->heads < 0 || a->tokens > INT_MAX || a->head_dim <= 0 || a->head_dim % 8 != 0 ||
-      a->head_dim > 65536 || a->heads > 65536 || a->heads * a->head_dim > INT_MAX)
+      a->head_dim > 2048 || a->heads > 65536 || a->heads * a->head_dim > INT_MAX)
     return QL_ERR_BAD_SHAPE;
   if (!act_dtype(a->dtype)) return QL_ERR_UNSUPPORTED;
   if (a->tokens == 0 || a->heads == 0) return QL_OK;
@@ -212,15 +247,13 @@ int ql_rotary(const ql_rotary_args* a, void* stream) {
   if (st != QL_OK) return st;
   ql_host::Device dev;
   if ((st = ql_host::current(&dev)) != QL_OK) return st;
-  p.tokens = a->tokens;
+  p.tokens = (int)a->tokens;
   p.heads = (int)a->heads;
-  p.chunks = (int)(a->head_dim / 8);
+  p.grid = make_grid(a->tokens, a->heads, a->head_dim / 8, ql::kvc::kHeads, dev.sms);
   p.err = dev.err_word;
-  const int threads = (int)std::min<int64_t>(256, cdiv((int64_t)p.heads * p.chunks, 32) * 32);
-  const dim3 grid((unsigned)a->tokens), block((unsigned)threads);
-  return a->dtype == QL_DTYPE_F16
-             ? launch(ql::kvc::rotary_kernel<__half>, grid, block, 0, stream, a->flags, p)
-             : launch(ql::kvc::rotary_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p);
+  const dim3 grid((unsigned)cdiv(a->tokens, p.grid.tokens)), block(threads_of(p.grid));
+  return a->dtype == QL_DTYPE_F16 ? launch(ql::kvc::rotary_kernel<__half>, grid, block, 0, stream, a->flags, p)
+                                  : launch(ql::kvc::rotary_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p);
 }
 
 int ql_kv_append(const ql_kv_append_args* a, void* stream) {
@@ -237,11 +270,11 @@ int ql_kv_append(const ql_kv_append_args* a, void* stream) {
   if ((st = make_rows(&p.k, a->k, a->k_token_stride, a->k_head_stride, d)) != QL_OK) return st;
   if ((st = make_rows(&p.v, a->v, a->v_token_stride, a->v_head_stride, d)) != QL_OK) return st;
   if (a->q_heads > 0) {
-    if ((st = make_rows(&p.q, a->q, a->q_token_stride, a->q_head_stride, d)) != QL_OK) return st;
-    if ((st = make_rows(&p.q_out, a->q_out, a->q_out_token_stride, a->q_out_head_stride, d)) != QL_OK) return st;
+    if ((st = make_rows(&p.q.x, a->q, a->q_token_stride, a->q_head_stride, d)) != QL_OK) return st;
+    if ((st = make_rows(&p.q.out, a->q_out, a->q_out_token_stride, a->q_out_head_stride, d)) != QL_OK) return st;
   }
   if (a->rotary_dim != 0) {
-    st = make_turn(&p.turn, a->table, a->positions, a->position_bytes, a->max_positions, a->rotary_dim, d, a->layout,
+    st = make_turn(&p.q.turn, a->table, a->positions, a->position_bytes, a->max_positions, a->rotary_dim, d, a->layout,
                    0);
     if (st != QL_OK) return st;
   }
@@ -249,11 +282,11 @@ int ql_kv_append(const ql_kv_append_args* a, void* stream) {
   if ((st = ql_host::current(&dev)) != QL_OK) return st;
   p.slots = a->slots;
   p.wide_slots = a->slot_bytes == 8;
-  p.tokens = a->tokens;
-  p.q_heads = (int)a->q_heads;
-  p.err = dev.err_word;
-  return a->dtype == QL_DTYPE_F16 ? run_append<__half>(p, d, stream, a->flags)
-                                  : run_append<__nv_bfloat16>(p, d, stream, a->flags);
+  p.tokens = p.q.tokens = (int)a->tokens;
+  p.q.heads = (int)a->q_heads;
+  p.q.err = dev.err_word;
+  return a->dtype == QL_DTYPE_F16 ? run_append<__half>(p, d / 8, dev.sms, stream, a->flags)
+                                  : run_append<__nv_bfloat16>(p, d / 8, dev.sms, stream, a->flags);
 }
 
 int ql_kv_read(const ql_kv_read_args* a, void* stream) {
@@ -267,8 +300,11 @@ int ql_kv_read(const ql_kv_read_args* a, void* stream) {
   if (!a->slots || !a->k || !a->v) return QL_ERR_NULL_POINTER;
   if (!aligned(a->slots, (size_t)a->slot_bytes) || !aligned(a->k, 16) || !aligned(a->v, 16))
     return QL_ERR_UNSUPPORTED;
-  const int64_t chunks = a->cache.head_dim / 8, blocks = cdiv(a->tokens * a->cache.kv_heads * chunks, 256);
-  if (blocks > INT_MAX) return QL_ERR_BAD_SHAPE;
+  // tokens side by side in a CTA, or CTAs to a token
+  const int64_t per_token = a->cache.kv_heads * a->cache.head_dim / 8;
+  const int side = per_token <= 256 ? (int)(256 / per_token) : 1, split = (int)cdiv(per_token, 256);
+  const int64_t blocks = cdiv(a->tokens, (int64_t)side * ql::kvc::kTokens) * split;
+  const int log_chunks = __builtin_ctzll((unsigned long long)a->cache.head_dim / 8);
   ql_host::Device dev;
   if ((st = ql_host::current(&dev)) != QL_OK) return st;
   p.slots = a->slots;
@@ -277,10 +313,11 @@ int ql_kv_read(const ql_kv_read_args* a, void* stream) {
   p.k = a->k;
   p.v = a->v;
   p.err = dev.err_word;
-  const dim3 grid((unsigned)blocks, 2), block(256);
+  if (blocks > INT_MAX) return QL_ERR_BAD_SHAPE;
+  const dim3 grid((unsigned)blocks), block(256);
   return a->dtype == QL_DTYPE_F16
-             ? launch(ql::kvc::read_kernel<__half>, grid, block, 0, stream, a->flags, p, (int)chunks)
-             : launch(ql::kvc::read_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p, (int)chunks);
+             ? launch(ql::kvc::read_kernel<__half>, grid, block, 0, stream, a->flags, p, log_chunks, side, split)
+             : launch(ql::kvc::read_kernel<__nv_bfloat16>, grid, block, 0, stream, a->flags, p, log_chunks, side, split);
 }
 
 int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
@@ -317,9 +354,7 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   p.total_q = (int)a->total_q;
   p.q_heads = (int)a->q_heads;
   p.group = (int)(a->q_heads / a->cache.kv_heads);
-  unsigned log = 0;
-  while ((1ll << log) < p.group) ++log;
-  p.by_group = {(unsigned)cdiv(1ll << (31 + log), p.group), 31 + log};
+  p.by_group = divisor(p.group);
   p.mask_words = (int)a->mask_words;
   p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   p.err = dev.err_word;

@@ -45,63 +45,29 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
 }
 __device__ __forceinline__ float bf16_bits_to_f(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
 
+// Two neighbouring elements in a word.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ void unpack2(float& lo, float& hi, uint32_t v);
+template <> __device__ __forceinline__ void unpack2<__half>(float& lo, float& hi, uint32_t v) {
+  const float2 f = h2_to_f2(v);
+  lo = f.x;
+  hi = f.y;
+}
+template <> __device__ __forceinline__ void unpack2<__nv_bfloat16>(float& lo, float& hi, uint32_t v) {
+  lo = __uint_as_float(v << 16);
+  hi = __uint_as_float(v & 0xFFFF0000u);
+}
+
 template <typename T> struct alignas(8) Vec4 { T v[4]; };
 template <typename T> struct alignas(16) Vec8 { T v[8]; };
-
-// Four neighbouring elements, in one access where `vec` says that rows are
-// 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load4(float (&f)[4], const T* p, bool vec) {
-  if (vec) {
-    const Vec4<T> a = *reinterpret_cast<const Vec4<T>*>(p);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_f(a.v[i]);
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_f(p[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void load8(float (&a)[4], float (&b)[4], const T* p, bool vec) {
-  if (vec) {
-    const Vec8<T> x = *reinterpret_cast<const Vec8<T>*>(p);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = to_f(x.v[i]);
-      b[i] = to_f(x.v[4 + i]);
-    }
-  } else {
-    load4(a, p, false);
-    load4(b, p + 4, false);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&f)[4], bool vec) {
-  Vec4<T> a;
-  #pragma unroll
-  for (int i = 0; i < 4; ++i) a.v[i] = from_f<T>(f[i]);
-  if (vec) {
-    *reinterpret_cast<Vec4<T>*>(p) = a;
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = a.v[i];
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&a)[4], const float (&b)[4], bool vec) {
-  if (vec) {
-    Vec8<T> x;
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x.v[i] = from_f<T>(a[i]);
-      x.v[4 + i] = from_f<T>(b[i]);
-    }
-    *reinterpret_cast<Vec8<T>*>(p) = x;
-  } else {
-    store4(p, a, false);
-    store4(p + 4, b, false);
-  }
-}
 
 __device__ __forceinline__ long long load_index(const void* p, long long i, int wide) {
   return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
@@ -131,34 +97,45 @@ __device__ __forceinline__ Chunk chunk_of(int c, const Turn& t, bool rotate) {
   k.ob = split ? (t.rotary_dim >> 1) + 4 * c : 8 * c + 4;
   return k;
 }
+// A chunk as it lies in memory: the run at oa (x, y), then the one at ob.
+// `vec`: rows start on 16 bytes, so that runs are read and written at once.
 template <typename T>
-__device__ __forceinline__ void load_chunk(float (&a)[4], float (&b)[4], const T* row, const Chunk& k, bool vec) {
-  if (k.ob == k.oa + 4) {
-    load8(a, b, row + k.oa, vec);
-  } else {
-    load4(a, row + k.oa, vec);
-    load4(b, row + k.ob, vec);
+__device__ __forceinline__ uint4 load_chunk(const T* row, const Chunk& k, bool vec) {
+  if (vec) {
+    if (k.ob == k.oa + 4) return *reinterpret_cast<const uint4*>(row + k.oa);
+    const uint2 a = *reinterpret_cast<const uint2*>(row + k.oa), b = *reinterpret_cast<const uint2*>(row + k.ob);
+    return make_uint4(a.x, a.y, b.x, b.y);
   }
+  const unsigned short *a = reinterpret_cast<const unsigned short*>(row + k.oa),
+                       *b = reinterpret_cast<const unsigned short*>(row + k.ob);
+  return make_uint4(a[0] | (unsigned)a[1] << 16, a[2] | (unsigned)a[3] << 16, b[0] | (unsigned)b[1] << 16,
+                    b[2] | (unsigned)b[3] << 16);
 }
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* row, const float (&a)[4], const float (&b)[4], const Chunk& k,
                                             bool vec) {
-  if (k.ob == k.oa + 4) {
-    store8(row + k.oa, a, b, vec);
+  const uint4 v = make_uint4(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3]));
+  if (vec && k.ob == k.oa + 4) {
+    *reinterpret_cast<uint4*>(row + k.oa) = v;
+  } else if (vec) {
+    *reinterpret_cast<uint2*>(row + k.oa) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(row + k.ob) = make_uint2(v.z, v.w);
   } else {
-    store4(row + k.oa, a, vec);
-    store4(row + k.ob, b, vec);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      row[k.oa + i] = from_f<T>(a[i]);
+      row[k.ob + i] = from_f<T>(b[i]);
+    }
   }
 }
 
-// cos and sin of the chunk's four pairs.
-__device__ __forceinline__ void load_angles(float (&cs)[4], float (&sn)[4], const float2* angles, int c,
-                                            int inverse) {
+// cos and sin of a chunk's four pairs: cos, sin, cos, sin of pairs 0 and 1, of 2 and 3.
+struct Angles {
+  float4 u, w;
+};
+__device__ __forceinline__ Angles load_angles(const float2* angles, int c) {
   const float4* p = reinterpret_cast<const float4*>(angles + 4 * c);
-  const float4 u = __ldg(p), w = __ldg(p + 1);
-  const float m = inverse ? -1.f : 1.f;
-  cs[0] = u.x; sn[0] = m * u.y; cs[1] = u.z; sn[1] = m * u.w;
-  cs[2] = w.x; sn[2] = m * w.y; cs[3] = w.z; sn[3] = m * w.w;
+  return {__ldg(p), __ldg(p + 1)};
 }
 
 __device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s) {
@@ -167,23 +144,33 @@ __device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s
   x1 = y1;
   x2 = y2;
 }
-__device__ __forceinline__ void turn_chunk(float (&a)[4], float (&b)[4], const float (&cs)[4],
-                                           const float (&sn)[4], int interleaved) {
-  if (interleaved) {
-    turn_pair(a[0], a[1], cs[0], sn[0]);
-    turn_pair(a[2], a[3], cs[1], sn[1]);
-    turn_pair(b[0], b[1], cs[2], sn[2]);
-    turn_pair(b[2], b[3], cs[3], sn[3]);
+__device__ __forceinline__ void turn_chunk(float (&a)[4], float (&b)[4], const Angles& t, const Chunk& k,
+                                           const Turn& turn) {
+  if (!k.turns) return;
+  const float m = turn.inverse ? -1.f : 1.f;
+  if (turn.interleaved) {
+    turn_pair(a[0], a[1], t.u.x, m * t.u.y);
+    turn_pair(a[2], a[3], t.u.z, m * t.u.w);
+    turn_pair(b[0], b[1], t.w.x, m * t.w.y);
+    turn_pair(b[2], b[3], t.w.z, m * t.w.w);
   } else {
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) turn_pair(a[i], b[i], cs[i], sn[i]);
+    turn_pair(a[0], b[0], t.u.x, m * t.u.y);
+    turn_pair(a[1], b[1], t.u.z, m * t.u.w);
+    turn_pair(a[2], b[2], t.w.x, m * t.w.y);
+    turn_pair(a[3], b[3], t.w.z, m * t.w.w);
   }
 }
+template <typename T>
+__device__ __forceinline__ void widen(float (&a)[4], float (&b)[4], const uint4& r) {
+  unpack2<T>(a[0], a[1], r.x);
+  unpack2<T>(a[2], a[3], r.y);
+  unpack2<T>(b[0], b[1], r.z);
+  unpack2<T>(b[2], b[3], r.w);
+}
 
-// The token's row of the table; a position outside it is recorded in the
+// The row of the table of position p; one outside it is recorded in the
 // device error word and takes the nearest row.
-__device__ __forceinline__ const float2* angles_of(const Turn& t, long long token, unsigned* err) {
-  long long p = load_index(t.positions, token, t.wide);
+__device__ __forceinline__ const float2* angles_of(const Turn& t, long long p, unsigned* err) {
   if (p < 0 || p >= t.max_positions) {
     atomicCAS(err, 0u, (unsigned)kDevErrBadIndex);
     p = p < 0 ? 0 : t.max_positions - 1;
@@ -197,35 +184,74 @@ struct Rows {              // [tokens][heads][head_dim] with strides in elements
   int vec;                 // every row starts on 16 bytes
 };
 
+// Division of numbers below 2^31 by one known on the host: with s the
+// smallest power of two at least d and m = ceil(2^31 s / d), n m / (2^31 s)
+// exceeds n / d by less than 1 / d, so its whole part is n / d's.
+struct Divisor {
+  unsigned m, shift;
+  __device__ __forceinline__ int of(int n) const { return (int)(((unsigned long long)(unsigned)n * m) >> shift); }
+};
+
 // -------------------------------------------------------------------- rotary
+// How threads lie over (token, head, chunk): `beside` heads of a token side by
+// side, `tokens` tokens to a CTA.
+struct Grid {
+  int beside, tokens, chunks;      // chunks = head_dim / 8
+  Divisor by_token, by_chunks;     // by beside * chunks, by chunks
+};
+struct Place {
+  int token, head, c;              // token -1: none
+};
+__device__ __forceinline__ Place place_of(const Grid& g, int cta, int total) {
+  const int mine = g.by_token.of(threadIdx.x), rest = threadIdx.x - mine * g.beside * g.chunks;
+  const int token = cta * g.tokens + mine, head = g.by_chunks.of(rest);
+  return {mine < g.tokens && token < total ? token : -1, head, rest - head * g.chunks};
+}
+
+// Bound by memory, and by the chain behind a token: its position, then its
+// angles.  A thread keeps one chunk of 8 elements, and so its angles, over
+// kHeads heads whose loads are all in flight before the angles are waited for.
+constexpr int kHeads = 4;
 struct RotaryParams {
   Turn turn;
   Rows x, out;
-  long long tokens;
-  int heads, chunks;       // chunks = head_dim / 8
+  Grid grid;
+  int tokens, heads;
   unsigned* err;
 };
-
-// One CTA per token; a thread takes chunks of 8 elements across the heads.
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+__device__ __forceinline__ void rotate_heads(const RotaryParams& p, int cta) {
+  const Place at = place_of(p.grid, cta, p.tokens);
+  if (at.token < 0) return;
+  const Chunk k = chunk_of(at.c, p.turn, true);
+  const long long x_step = p.grid.beside * p.x.head_stride, out_step = p.grid.beside * p.out.head_stride;
+  const T* x = static_cast<const T*>(p.x.p) + at.token * p.x.token_stride + at.head * p.x.head_stride;
+  T* out = static_cast<T*>(const_cast<void*>(p.out.p)) + at.token * p.out.token_stride + at.head * p.out.head_stride;
+  const long long position = load_index(p.turn.positions, at.token, p.turn.wide);
+  Angles angles = {};
+  for (int h = at.head; h < p.heads; h += kHeads * p.grid.beside) {
+    uint4 raw[kHeads];
+    #pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (h + i * p.grid.beside < p.heads) raw[i] = load_chunk(x + i * x_step, k, p.x.vec);
+    if (h == at.head && k.turns) angles = load_angles(angles_of(p.turn, position, p.err), at.c);
+    #pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (h + i * p.grid.beside < p.heads) {
+        float a[4], b[4];
+        widen<T>(a, b, raw[i]);
+        turn_chunk(a, b, angles, k, p.turn);
+        store_chunk(out + i * out_step, a, b, k, p.out.vec);
+      }
+    x += kHeads * x_step;
+    out += kHeads * out_step;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256, 5) rotary_kernel(const RotaryParams p) {
   griddep_launch_dependents();
   griddep_wait();
-  const long long token = blockIdx.x;
-  const float2* angles = angles_of(p.turn, token, p.err);
-  const int n = p.heads * p.chunks;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int h = i / p.chunks, c = i - h * p.chunks;
-    const Chunk k = chunk_of(c, p.turn, true);
-    float a[4], b[4], cs[4], sn[4];
-    load_chunk(a, b, static_cast<const T*>(p.x.p) + token * p.x.token_stride + h * p.x.head_stride, k, p.x.vec);
-    if (k.turns) {
-      load_angles(cs, sn, angles, c, p.turn.inverse);
-      turn_chunk(a, b, cs, sn, p.turn.interleaved);
-    }
-    T* row = static_cast<T*>(const_cast<void*>(p.out.p)) + token * p.out.token_stride + h * p.out.head_stride;
-    store_chunk(row, a, b, k, p.out.vec);
-  }
+  rotate_heads<T>(p, blockIdx.x);
 }
 
 // --------------------------------------------------------------------- cache
@@ -251,101 +277,131 @@ __device__ __forceinline__ RowAt row_at(const Pool& c, long long slot, int head,
 }
 
 struct AppendParams {
-  Turn turn;
+  RotaryParams q;          // the queries, whose turn is the keys' too (rotary_dim 0: nothing turns)
   Pool cache;
-  Rows q, q_out, k, v;
+  Rows k, v;
+  Grid grid;               // of the keys and values
   const void* slots;
-  int wide_slots;
-  long long tokens;
-  int q_heads;             // 0: no queries
-  unsigned* err;
+  int wide_slots, tokens;
+  int kv_ctas;             // the CTAs before those of the queries
 };
 
-// Codes of four elements against a scale that is positive and finite.
-__device__ __forceinline__ unsigned quantise4(const float (&f)[4], float s, int bits) {
-  unsigned w = 0;
+// Codes of four elements against a scale that is positive and finite, and
+// inv = 1 / s: rne(x / s) without a division.  x inv is within 2^-22 of x / s
+// relatively, 2^-15 where codes can differ (below 128), so it rounds alike
+// unless it is that close to half way between two codes; those few elements
+// are divided.  Adding 1.5 * 2^23 leaves the rounded integer in the low bits.
+template <int BITS>
+__device__ __forceinline__ unsigned quantise4(const float (&f)[4], float s, float inv) {
+  constexpr float kRound = 12582912.f;
+  constexpr float top = BITS == 8 ? 127.f : 7.f;
+  unsigned q[4];
+  bool close = !(inv < INFINITY);
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float top = bits == 8 ? 127.f : 7.f;
-    const int q = (int)fminf(fmaxf(rintf(__fdiv_rn(f[i], s)), -top), top);
-    w |= bits == 8 ? (unsigned)(q & 0xFF) << (8 * i) : (unsigned)(q + 8) << (4 * i);
+    const float y = fminf(fmaxf(__fmul_rn(f[i], inv), -top), top);
+    const float r = __fadd_rn(y, kRound);
+    q[i] = __float_as_uint(r);
+    close |= fabsf(__fsub_rn(y, __fsub_rn(r, kRound))) > 0.5f - 0x1p-14f;
   }
-  return w;
+  if (close) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(f[i], s), -top), top), kRound));
+  }
+  if (BITS == 8) return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = (q[i] + 8u) & 15u;
+  return q[0] | q[1] << 4 | q[2] << 8 | q[3] << 12;
 }
 
-// One CTA per token; LANES = head_dim / 8 neighbouring lanes hold one row
-// (query, key or value head) and reduce its maxima by shuffles.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+// One row to its slot: LANES neighbouring lanes hold it and reduce its maxima
+// by shuffles, which all lanes of the warp take part in; `live` lanes write.
+template <int LANES, int BITS>
+__device__ __forceinline__ void store_row(const RowAt& dst, const float (&a)[4], const float (&b)[4], const Chunk& k,
+                                          int c, bool live) {
+  constexpr int kGroups = BITS == 8 ? 1 : LANES * 8 / kGroup4;
+  // |x| as ordered integers: an infinity or NaN ends up as the maximum
+  unsigned ma = 0, mb = 0;
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ma = max(ma, __float_as_uint(a[i]) & 0x7FFFFFFFu);
+    mb = max(mb, __float_as_uint(b[i]) & 0x7FFFFFFFu);
+  }
+  const int ga = kGroups > 1 ? k.oa / kGroup4 : 0, gb = kGroups > 1 ? k.ob / kGroup4 : 0;
+  float sa = 0.f, sb = 0.f;
+  #pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    unsigned m = kGroups == 1 ? max(ma, mb) : max(ga == g ? ma : 0u, gb == g ? mb : 0u);
+    #pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    constexpr float kInvTop = BITS == 8 ? (float)(1.0 / 127.0) : (float)(1.0 / 7.0);
+    const unsigned short s16 = __bfloat16_as_ushort(__float2bfloat16_rn(__fmul_rn(__uint_as_float(m), kInvTop)));
+    const float s = bf16_bits_to_f(s16);
+    if (ga == g) sa = s;
+    if (gb == g) sb = s;
+    if (live && c == 0) dst.scales[g] = s16;
+  }
+  if (!live) return;
+  // a scale below 2^-125 has no reciprocal in fp32's normal range: such rows are divided
+  constexpr unsigned kNone = BITS == 8 ? 0u : 0x8888u;
+  const bool fa = sa > 0.f && sa < INFINITY, fb = sb > 0.f && sb < INFINITY;
+  const float ia = sa >= 0x1p-125f ? __frcp_rn(sa) : INFINITY;
+  const float ib = kGroups == 1 || sb == sa ? ia : sb >= 0x1p-125f ? __frcp_rn(sb) : INFINITY;
+  const unsigned qa = fa ? quantise4<BITS>(a, sa, ia) : kNone, qb = fb ? quantise4<BITS>(b, sb, ib) : kNone;
+  if (BITS == 8) {
+    if (k.ob == k.oa + 4) {
+      *reinterpret_cast<uint2*>(dst.codes + k.oa) = make_uint2(qa, qb);
+    } else {
+      *reinterpret_cast<unsigned*>(dst.codes + k.oa) = qa;
+      *reinterpret_cast<unsigned*>(dst.codes + k.ob) = qb;
+    }
+  } else if (k.ob == k.oa + 4) {
+    *reinterpret_cast<unsigned*>(dst.codes + k.oa / 2) = qa | qb << 16;
+  } else {
+    *reinterpret_cast<unsigned short*>(dst.codes + k.oa / 2) = (unsigned short)qa;
+    *reinterpret_cast<unsigned short*>(dst.codes + k.ob / 2) = (unsigned short)qb;
+  }
+}
+
+// The first CTAs write keys and values, LANES = head_dim / 8 lanes taking the
+// key and the value row of a head; the others turn the queries.
+template <typename T, int LANES, int BITS>
+__global__ void __launch_bounds__(256, 5) append_kernel(const AppendParams p) {
   griddep_launch_dependents();
   griddep_wait();
-  const long long token = blockIdx.x;
-  const Pool& kv = p.cache;
-  const int lane = threadIdx.x % LANES, rows_per_pass = blockDim.x / LANES;
-  const int total = p.q_heads + 2 * kv.heads;
-  long long slot = load_index(p.slots, token, p.wide_slots);
-  if (slot >= kv.slots) {
-    if (threadIdx.x == 0) atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
-    slot = -1;
+  if ((int)blockIdx.x >= p.kv_ctas) {
+    rotate_heads<T>(p.q, blockIdx.x - p.kv_ctas);
+    return;
   }
-  const bool rotary = p.turn.rotary_dim > 0;
-  float cs[4], sn[4];
-  if (rotary && lane < (p.turn.rotary_dim >> 3))
-    load_angles(cs, sn, angles_of(p.turn, token, p.err), lane, p.turn.inverse);
-
-  // every lane takes every pass, so that the shuffles find all lanes
-  for (int first = 0; first < total; first += rows_per_pass) {
-    const int row = first + threadIdx.x / LANES;
-    const bool query = row < p.q_heads, value = row >= p.q_heads + kv.heads;
-    const bool live = row < total && (query || slot >= 0);
-    const int head = query ? row : row - p.q_heads - (value ? kv.heads : 0);
-    const Chunk k = chunk_of(lane, p.turn, rotary && !value);
-    float a[4] = {}, b[4] = {};
-    if (live) {
-      const Rows& src = query ? p.q : value ? p.v : p.k;
-      load_chunk(a, b, static_cast<const T*>(src.p) + token * src.token_stride + head * src.head_stride, k,
-                 src.vec);
-      if (k.turns) turn_chunk(a, b, cs, sn, p.turn.interleaved);
-    }
-    if (live && query) {
-      T* out = static_cast<T*>(const_cast<void*>(p.q_out.p)) + token * p.q_out.token_stride +
-               head * p.q_out.head_stride;
-      store_chunk(out, a, b, k, p.q_out.vec);
-    }
-    // |x| as ordered integers: an infinity or NaN ends up as the maximum
-    unsigned ma = 0, mb = 0;
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ma = max(ma, __float_as_uint(a[i]) & 0x7FFFFFFFu);
-      mb = max(mb, __float_as_uint(b[i]) & 0x7FFFFFFFu);
-    }
-    const int ga = kv.groups > 1 ? k.oa / kGroup4 : 0, gb = kv.groups > 1 ? k.ob / kGroup4 : 0;
-    float sa = 0.f, sb = 0.f;
-    #pragma unroll 1
-    for (int g = 0; g < kv.groups; ++g) {
-      unsigned m = max(ga == g ? ma : 0u, gb == g ? mb : 0u);
-      #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float inv_top = kv.bits == 8 ? (float)(1.0 / 127.0) : (float)(1.0 / 7.0);
-      const unsigned short s16 = __bfloat16_as_ushort(__float2bfloat16_rn(__fmul_rn(__uint_as_float(m), inv_top)));
-      const float s = bf16_bits_to_f(s16);
-      if (ga == g) sa = s;
-      if (gb == g) sb = s;
-      if (live && !query && lane == 0) row_at(kv, slot, head, value).scales[g] = s16;
-    }
-    if (live && !query) {
-      const bool fa = sa > 0.f && sa < INFINITY, fb = sb > 0.f && sb < INFINITY;
-      const unsigned none = kv.bits == 8 ? 0u : 0x8888u;
-      const unsigned qa = fa ? quantise4(a, sa, kv.bits) : none, qb = fb ? quantise4(b, sb, kv.bits) : none;
-      unsigned char* codes = row_at(kv, slot, head, value).codes;
-      if (kv.bits == 8) {
-        *reinterpret_cast<unsigned*>(codes + k.oa) = qa;
-        *reinterpret_cast<unsigned*>(codes + k.ob) = qb;
-      } else {
-        *reinterpret_cast<unsigned short*>(codes + k.oa / 2) = (unsigned short)qa;
-        *reinterpret_cast<unsigned short*>(codes + k.ob / 2) = (unsigned short)qb;
+  const Pool& kv = p.cache;
+  const Turn& turn = p.q.turn;
+  const Place at = place_of(p.grid, blockIdx.x, p.tokens);
+  const int token = max(at.token, 0);
+  const Chunk straight = chunk_of(at.c, turn, false), turned = chunk_of(at.c, turn, turn.rotary_dim > 0);
+  long long slot = load_index(p.slots, token, p.wide_slots);
+  const long long position = turned.turns ? load_index(turn.positions, token, turn.wide) : 0;
+  Angles angles = {};
+  for (int first = 0; first < kv.heads; first += p.grid.beside) {       // every lane: the shuffles want them all
+    const int h = min(first + at.head, kv.heads - 1);
+    const uint4 k_raw = load_chunk(static_cast<const T*>(p.k.p) + token * p.k.token_stride + h * p.k.head_stride, turned, p.k.vec);
+    const uint4 v_raw = load_chunk(static_cast<const T*>(p.v.p) + token * p.v.token_stride + h * p.v.head_stride, straight, p.v.vec);
+    if (first == 0) {
+      if (turned.turns) angles = load_angles(angles_of(turn, position, p.q.err), at.c);
+      if (at.token < 0) slot = -1;
+      if (slot >= kv.slots) {
+        atomicCAS(p.q.err, 0u, (unsigned)kDevErrBadIndex);
+        slot = -1;
       }
     }
+    const bool live = slot >= 0 && first + at.head < kv.heads;
+    const long long where = max(slot, 0ll);
+    float a[4], b[4];
+    widen<T>(a, b, k_raw);
+    turn_chunk(a, b, angles, turned, turn);
+    store_row<LANES, BITS>(row_at(kv, where, h, false), a, b, turned, at.c, live);
+    widen<T>(a, b, v_raw);
+    store_row<LANES, BITS>(row_at(kv, where, h, true), a, b, straight, at.c, live);
   }
 }
 
@@ -360,50 +416,78 @@ struct ReadParams {
 };
 
 // Codes of 8 elements as integers in fp32.
-__device__ __forceinline__ void codes8(float (&f)[8], const unsigned char* p, int bits) {
+__device__ __forceinline__ void codes8(float (&f)[8], uint2 w, int bits) {
   if (bits == 8) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[i] = (float)(int)(signed char)(w.x >> (8 * i));
       f[4 + i] = (float)(int)(signed char)(w.y >> (8 * i));
     }
   } else {
-    const unsigned w = *reinterpret_cast<const unsigned*>(p);
     #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)((int)((w >> (4 * i)) & 15u) - 8);
+    for (int i = 0; i < 8; ++i) f[i] = (float)((int)((w.x >> (4 * i)) & 15u) - 8);
   }
 }
 
-// A thread per 8 elements of a (token, head, key or value) row.
+// A thread takes 8 elements of the key and of the value row of kTokens tokens,
+// 256 / (heads * chunks) apart or more, so that twice as many loads are in
+// flight: CTA i has tokens i * span .., span = tokens side by side * kTokens.
+constexpr int kTokens = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(const ReadParams p, int chunks) {
+__global__ void __launch_bounds__(256) read_kernel(const ReadParams p, int log_chunks, int side, int split) {
   griddep_launch_dependents();
   griddep_wait();
   const Pool& kv = p.cache;
-  const long long n = p.tokens * kv.heads * chunks;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int c = (int)(i % chunks);
-  const long long row = i / chunks;
-  const long long token = row / kv.heads;
-  const int head = (int)(row - token * kv.heads);
-  const bool value = blockIdx.y != 0;
-  const long long slot = load_index(p.slots, token, p.wide_slots);
-  float f[8] = {};
-  if (slot >= kv.slots) {
-    atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
-  } else if (slot >= 0) {
-    const RowAt r = row_at(kv, slot, head, value);
-    codes8(f, r.codes + c * kv.bits, kv.bits);
-    const float s = bf16_bits_to_f(r.scales[kv.groups > 1 ? c * 8 / kGroup4 : 0]);
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= s;
-  }
-  Vec8<T> o;
+  // part of a token's heads * chunks that this CTA has (all of it where split is 1), and the token of the thread
+  const int per_token = kv.heads << log_chunks;
+  const int part = split > 1 ? blockIdx.x % split : 0;
+  const long long group = split > 1 ? blockIdx.x / split : blockIdx.x;
+  const int beside = split > 1 ? 0 : threadIdx.x / per_token;
+  const int at = split > 1 ? part * 256 + threadIdx.x : threadIdx.x - beside * per_token;
+  if (beside >= side || at >= per_token) return;
+  const int head = at >> log_chunks, c = at & ((1 << log_chunks) - 1);
+  const long long first = group * side * kTokens + beside;
+  long long slot[kTokens];
   #pragma unroll
-  for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(f[j]);
-  *reinterpret_cast<Vec8<T>*>(static_cast<T*>(value ? p.v : p.k) + i * 8) = o;
+  for (int i = 0; i < kTokens; ++i) {
+    const long long token = first + i * side;
+    slot[i] = token < p.tokens ? load_index(p.slots, token, p.wide_slots) : -1;
+    if (slot[i] >= kv.slots) {
+      atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+      slot[i] = -1;
+    }
+  }
+  uint2 w[kTokens][2];
+  unsigned short s[kTokens][2];
+  #pragma unroll
+  for (int i = 0; i < kTokens; ++i)
+    #pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      w[i][v] = make_uint2(0u, 0u);
+      s[i][v] = 0;
+      if (slot[i] >= 0) {
+        const RowAt r = row_at(kv, slot[i], head, v != 0);
+        if (kv.bits == 8)
+          w[i][v] = *reinterpret_cast<const uint2*>(r.codes + c * 8);
+        else
+          w[i][v].x = *reinterpret_cast<const unsigned*>(r.codes + c * 4);
+        s[i][v] = r.scales[kv.groups > 1 ? c * 8 / kGroup4 : 0];
+      }
+    }
+  #pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    const long long token = first + i * side;
+    if (token >= p.tokens) break;
+    #pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      float f[8];
+      codes8(f, w[i][v], kv.bits);
+      const float scale = bf16_bits_to_f(s[i][v]);
+      *reinterpret_cast<uint4*>(static_cast<T*>(v ? p.v : p.k) + ((token * per_token + at) << 3)) =
+          make_uint4(pack2<T>(f[0] * scale, f[1] * scale), pack2<T>(f[2] * scale, f[3] * scale),
+                     pack2<T>(f[4] * scale, f[5] * scale), pack2<T>(f[6] * scale, f[7] * scale));
+    }
+  }
 }
 
 }  // namespace kvc
