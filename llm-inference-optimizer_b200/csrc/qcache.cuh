@@ -309,10 +309,13 @@ __device__ __forceinline__ unsigned quantise4(const float (&f)[4], float s, floa
     for (int i = 0; i < 4; ++i)
       q[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(f[i], s), -top), top), kRound));
   }
-  if (BITS == 8) return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-  #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = (q[i] + 8u) & 15u;
-  return q[0] | q[1] << 4 | q[2] << 8 | q[3] << 12;
+  if constexpr (BITS == 8) {
+    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = (q[i] + 8u) & 15u;
+    return q[0] | q[1] << 4 | q[2] << 8 | q[3] << 12;
+  }
 }
 
 // One row to its slot: LANES neighbouring lanes hold it and reduce its maxima
@@ -367,7 +370,7 @@ __device__ __forceinline__ void store_row(const RowAt& dst, const float (&a)[4],
 // The first CTAs write keys and values, LANES = head_dim / 8 lanes taking the
 // key and the value row of a head; the others turn the queries.
 template <typename T, int LANES, int BITS>
-__global__ void __launch_bounds__(256, 5) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 4) append_kernel(const AppendParams p) {
   griddep_launch_dependents();
   griddep_wait();
   if ((int)blockIdx.x >= p.kv_ctas) {
