@@ -67,7 +67,7 @@ constexpr float kLow = -1e30f;             // the maximum of nothing: below ever
 constexpr int kUnitKeys = 128;
 constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMinUnits = 2;               // keys worth a CTA of their own: 256
+constexpr int kMinUnits = 2;               // units worth a CTA of their own: 256 keys
 constexpr int kJoin = 16;                  // parts of an item that are joined at once
 constexpr int kMaxCtas = 1024;
 constexpr int kHeaderBytes = 2 * 4 * kMaxCtas;   // counters of items and of groups of parts
@@ -83,22 +83,23 @@ struct Work {
   }
 };
 
+template <int MIN_UNITS>
 __device__ __forceinline__ int item_units(const Request& r) {
   const int n = (r.kv_len + kUnitKeys - 1) / kUnitKeys;
-  return max((n + kMinUnits - 1) / kMinUnits, 1) * kMinUnits;
+  return max((n + MIN_UNITS - 1) / MIN_UNITS, 1) * MIN_UNITS;
 }
-template <int ROWS>
+template <int ROWS, int MIN_UNITS>
 __device__ __forceinline__ long long request_units(const Params& p, const Request& r) {
   const unsigned tiles = (unsigned)(r.q_len * p.group + ROWS - 1) / ROWS;
-  return (long long)tiles * p.cache.heads * item_units(r);
+  return (long long)tiles * p.cache.heads * item_units<MIN_UNITS>(r);
 }
 
 // Sums the requests' units and finds the request that holds this CTA's first
 // unit: *b, the unit at which it begins, and its lengths.  All threads call
 // it; up to 32 requests each warp does so by itself.
-template <int ROWS>
+template <int ROWS, int MIN_UNITS, int THREADS>
 __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* base, Request* r) {
-  __shared__ long long warp_sum[kWarps];
+  __shared__ long long warp_sum[THREADS / 32];
   __shared__ long long found_base;
   __shared__ int found_b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -116,11 +117,11 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
     long long units = 0;
     if (lane < p.batch) {
       mine = request(p, lane);
-      units = request_units<ROWS>(p, mine);
+      units = request_units<ROWS, MIN_UNITS>(p, mine);
     }
     const long long incl = warp_scan(units);
     w.total = __shfl_sync(0xffffffffu, incl, 31);
-    w.ctas = (int)min((long long)gridDim.x, w.total / kMinUnits);
+    w.ctas = (int)min((long long)gridDim.x, w.total / MIN_UNITS);
     if ((int)blockIdx.x >= w.ctas) return w;
     const long long u = w.first_unit(blockIdx.x);
     const int at = __ffs(__ballot_sync(0xffffffffu, u < incl)) - 1;      // some lane: u < total
@@ -138,7 +139,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
     __syncthreads();
     long long before = 0, all = 0;
     #pragma unroll
-    for (int x = 0; x < kWarps; ++x) {
+    for (int x = 0; x < THREADS / 32; ++x) {
       if (x < warp) before += warp_sum[x];
       all += warp_sum[x];
     }
@@ -146,20 +147,20 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
     return v + before;
   };
   long long mine = 0, incl = 0, sum;
-  for (int i = 0; i < p.batch; i += kThreads) {
+  for (int i = 0; i < p.batch; i += THREADS) {
     const int at = i + threadIdx.x;
-    mine = at < p.batch ? request_units<ROWS>(p, request(p, at)) : 0;
+    mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request(p, at)) : 0;
     incl = scan(mine, &sum);
     w.total += sum;
   }
-  w.ctas = (int)min((long long)gridDim.x, w.total / kMinUnits);
+  w.ctas = (int)min((long long)gridDim.x, w.total / MIN_UNITS);
   if ((int)blockIdx.x >= w.ctas) return w;
   const long long u = w.first_unit(blockIdx.x);
   long long before = 0;
-  for (int i = 0; i < p.batch; i += kThreads) {
-    if (p.batch > kThreads) {                          // else mine, incl and sum are still these
+  for (int i = 0; i < p.batch; i += THREADS) {
+    if (p.batch > THREADS) {                          // else mine, incl and sum are still these
       const int at = i + threadIdx.x;
-      mine = at < p.batch ? request_units<ROWS>(p, request(p, at)) : 0;
+      mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request(p, at)) : 0;
       incl = scan(mine, &sum);
     }
     const long long from = before + incl - mine;
@@ -383,20 +384,20 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
   int b;
   long long base;
   Request r;
-  const Work work = find_work<S::kRows>(p, &b, &base, &r);
+  const Work work = find_work<S::kRows, kMinUnits, kThreads>(p, &b, &base, &r);
   if ((int)blockIdx.x >= work.ctas) return;
   long long u = work.first_unit(blockIdx.x);
   const long long u_end = work.first_unit(blockIdx.x + 1);
 
   while (u < u_end) {
     // ------------------------------------------------------ the next segment
-    long long mine = request_units<S::kRows>(p, r);
+    long long mine = request_units<S::kRows, kMinUnits>(p, r);
     while (u >= base + mine) {
       base += mine;
       r = request(p, ++b);
-      mine = request_units<S::kRows>(p, r);
+      mine = request_units<S::kRows, kMinUnits>(p, r);
     }
-    const int per_item = item_units(r);
+    const int per_item = item_units<kMinUnits>(r);
     const int tiles = (int)((unsigned)(r.q_len * p.group + S::kRows - 1) / S::kRows);
     const long long item = Work::quotient(u - base, per_item);
     const int k_begin = (int)((u - base) - item * per_item);

@@ -13,6 +13,7 @@
 #include "ql_host.h"
 #include "qattend.cuh"
 #include "qcache.cuh"
+#include "qtree.cuh"
 
 namespace {
 
@@ -177,6 +178,10 @@ int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, i
   }
 }
 
+// Rows of a request under one key/value head from which the tensor-core
+// kernel is taken.
+constexpr int64_t kTreeRows = 32;
+
 struct Attention {
   ql::att::Params p;
   int64_t max_q, max_kv, flags;
@@ -212,8 +217,34 @@ int run_stream(const Attention& a) {
                 reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes));
 }
 
+template <int D, int BITS>
+size_t tree_workspace(int sms) {
+  return ql::att::kHeaderBytes + 2 * (size_t)std::min(ql::att::kMaxCtas, sms) * ql::tree::Shape<D, BITS>::kPartial * sizeof(float);
+}
+
+template <typename T, int D, int BITS>
+int run_tree(const Attention& a) {
+  using S = ql::tree::Shape<D, BITS>;
+  if (a.workspace_bytes < tree_workspace<D, BITS>(a.sms)) return QL_ERR_WORKSPACE;
+  auto kernel = ql::tree::tree_kernel<T, D, BITS>;
+  static std::atomic<unsigned char> done[kMaxDevices];
+  const int st = allow_smem(kernel, S::kSmem, done);
+  if (st != QL_OK) return st;
+  const int64_t tiles = cdiv(std::max<int64_t>(a.max_q, 1) * a.p.group, ql::tree::kRows);
+  const int64_t runs = cdiv(std::max<int64_t>(a.max_kv, 1), ql::att::kUnitKeys * ql::tree::kMinUnits);
+  int64_t ctas = std::min<int64_t>(ql::att::kMaxCtas, a.sms);
+  const double bound = (double)a.p.batch * a.p.cache.heads * (double)tiles * (double)runs;
+  if (bound < (double)ctas) ctas = std::max<int64_t>((int64_t)bound, 1);
+  return launch(kernel, dim3((unsigned)ctas), dim3(ql::tree::kThreads), S::kSmem, a.stream, a.flags, a.p,
+                static_cast<unsigned*>(a.workspace),
+                reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes));
+}
+
 template <typename T, int D, int BITS>
 int run_rows(const Attention& a) {
+  if constexpr (D <= 128) {
+    if (a.max_q * a.p.group > kTreeRows) return run_tree<T, D, BITS>(a);
+  }
   return a.max_q * a.p.group <= 8 ? run_stream<T, D, BITS, 1>(a) : run_stream<T, D, BITS, 2>(a);
 }
 
@@ -368,8 +399,8 @@ size_t ql_tree_attention_workspace_size(int64_t head_dim) {
   ql_host::Device dev;
   if (ql_host::current(&dev) != QL_OK) return 0;
   switch (head_dim) {   // the largest of the variants' (equal for 8 and 4 bits)
-    case 64: return std::max(stream_workspace<64, 8, 1>(dev.sms), stream_workspace<64, 8, 2>(dev.sms));
-    case 128: return std::max(stream_workspace<128, 8, 1>(dev.sms), stream_workspace<128, 8, 2>(dev.sms));
+    case 64: return std::max({stream_workspace<64, 8, 1>(dev.sms), stream_workspace<64, 8, 2>(dev.sms), tree_workspace<64, 8>(dev.sms)});
+    case 128: return std::max({stream_workspace<128, 8, 1>(dev.sms), stream_workspace<128, 8, 2>(dev.sms), tree_workspace<128, 8>(dev.sms)});
     case 256: return std::max(stream_workspace<256, 8, 1>(dev.sms), stream_workspace<256, 8, 2>(dev.sms));
     default: return 0;
   }

@@ -1,0 +1,707 @@
+// qtree.cuh — attention of many new tokens per request (trees and chains of
+// drafted tokens) over the quantised paged cache, on the 5th-generation
+// tensor cores (tcgen05 / TMEM, sm_100a).  The mathematics and the division
+// of work are those of qattend.cuh; here an item has 256 rows.
+//
+// With t new tokens under g query heads per key/value head, a key serves t g
+// rows: at a few dozen rows the products, not the cache, set the time, and
+// mma.sync with one decode per 16 rows is an order of magnitude from the
+// tensor cores' rate.  So the codes are decoded once per 256 rows into shared
+// memory, as the B operands of
+//   S_w [128 rows, keys] = Q_w K^T        (Q_w and K in shared memory)
+//   O_w [128 rows, d]   += P_w V          (P_w in TMEM, V in shared memory)
+// for two tiles w of 128 rows, and the work is spread over warps:
+//   * 4 decode warps: read codes, a step ahead, into registers; decode them
+//     exactly to 16 bits and store them in the 128-byte-swizzled layout that
+//     both products read (K with d, V with the keys as the sum's direction);
+//     publish the step's scales.
+//   * 1 warp issues the products: S_0, S_1 of a step, then P_0 V and S_0 of
+//     the next, P_1 V and S_1 of the next, so that one tile's softmax runs
+//     under the other's products.
+//   * 8 softmax warps, a thread a row: S from TMEM twice, for the maximum and
+//     for the weights, which go back to TMEM in the place of S.  Key scales
+//     multiply the scores, value scales the weights; a row's reference
+//     exponent holds its maximum and the largest value scale seen, and moves
+//     (with its outputs in TMEM) when a score passes it by 2^4.
+// At 4 bits and head_dim 128, where a scale covers 64 elements, a step is 64
+// keys with a sum and a set of weights per group.
+//
+// fp16 calls multiply in fp16, the weights rounded once; bf16 calls in bf16,
+// the weights as a sum of two (16 bits, fp32's range).  Every wait is bounded;
+// after one runs out the others end at once, the loops run to their end
+// without meaning, and the device error word tells.
+#pragma once
+
+#include "qattend.cuh"
+#include "qgemm.cuh"
+
+namespace ql {
+namespace tree {
+
+using att::Params;
+using att::Request;
+using att::Work;
+
+constexpr int kTileRows = 128;
+constexpr int kRows = 2 * kTileRows;
+constexpr int kMinUnits = 4;             // of 128 keys: a part's outputs are worth 512 keys
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
+constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + kDecodeWarps);
+
+template <int D, int BITS>
+struct Shape {
+  static constexpr int kAtoms = D / 64;                             // of 64 elements
+  static constexpr int kGroups = BITS == 8 ? 1 : kAtoms;
+  static constexpr int kKeys = 128 / kGroups;                       // of a step
+  static constexpr int kRowBytes = D * BITS / 8;
+  static constexpr int kStages = 2 * kGroups;
+  static constexpr int kSlots = kStages + 2;                        // of scales: outlive their step's keys
+  static constexpr int kQBytes = 2 * kAtoms * kTileRows * 128;
+  static constexpr int kStepBytes = kAtoms * kKeys * 128;           // keys, or values, of a step
+  static constexpr int kPieces = kKeys * kRowBytes / 16 / (32 * kDecodeWarps);   // 16-byte runs of codes a thread
+  static constexpr int kPerPiece = 128 / BITS;                      // elements
+  static constexpr int kColumns = 256 + 2 * D;                      // S_0, S_1, O_0, O_1
+  // partial of an item: per row its reference and sum, then D outputs
+  static constexpr int kPartial = kRows * (D + 2);
+  struct Slot {
+    float k[128], v[128];                                           // [group][key]
+    unsigned v_top[4];                                              // largest finite value scales
+    unsigned bad;                                                   // bit i: keys 16 i .. are in no page
+    unsigned pad[3];
+  };
+  static constexpr size_t kSmem = 1024 + kQBytes + 2 * (size_t)kStages * kStepBytes + kSlots * sizeof(Slot) + 512;
+  static_assert(kPieces >= 1 && kPieces * kPerPiece * 32 * kDecodeWarps == kKeys * D, "");
+};
+
+// D[tmem] (+)= A[smem] B[smem], kind::f16.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: fp32 sums, M = 128, N; A and B fp16 or bf16; B's
+// rows along the sum (K-major) or along N.
+__device__ __forceinline__ uint32_t instruction(bool bf16, bool b_along_n, int n) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_along_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTileRows >> 4) << 24);
+}
+// Shared-memory descriptor of values [key][64 elements] (128-byte rows,
+// swizzled): runs of 64 elements lie `atom_bytes` apart, groups of 8 keys 1024.
+__device__ __forceinline__ uint64_t desc_values(uint32_t addr, uint32_t atom_bytes) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(atom_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+// Waits for this thread's TMEM loads; the values pass through, so that nothing uses them before.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                    "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                    "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// Which of 32 positions from j on row i of the request sees, as bits.
+__device__ __forceinline__ unsigned sees32(const Params& p, const Request& r, int i, int j) {
+  const int d0 = j - (r.kv_len - r.q_len), left = r.kv_len - j;        // which new token j is; positions left
+  const auto low = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
+  if (!p.mask) return low(min(left, i - d0 + 1));
+  unsigned see = 0xFFFFFFFFu;
+  if (d0 > -32) {
+    const unsigned long long* words = p.mask + (long long)(r.q0 + i) * p.mask_words;
+    const auto word = [&](int w) { return w < p.mask_words ? words[w] : 0ull; };
+    if (d0 < 0) {
+      see = low(-d0) | (unsigned)(word(0) << -d0);
+    } else {
+      const int sh = d0 & 63;
+      see = (unsigned)(word(d0 >> 6) >> sh);
+      if (sh > 32) see |= (unsigned)(word((d0 >> 6) + 1) << (64 - sh));
+    }
+  }
+  return see & low(left);
+}
+
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsigned* counters, float* partials) {
+  using S = Shape<D, BITS>;
+  using Slot = typename S::Slot;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  constexpr int kTerms = kBf16 ? 2 : 1;
+  griddep_launch_dependents();
+  griddep_wait();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sm_q = smem;
+  uint8_t* sm_k = sm_q + S::kQBytes;
+  uint8_t* sm_v = sm_k + S::kStages * S::kStepBytes;
+  Slot* slots = reinterpret_cast<Slot*>(sm_v + S::kStages * S::kStepBytes);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(slots + S::kSlots);
+  uint64_t* k_free = k_full + S::kStages;
+  uint64_t* v_full = k_free + S::kStages;
+  uint64_t* v_free = v_full + S::kStages;
+  uint64_t* s_full = v_free + S::kStages;                    // per tile
+  uint64_t* p_ready = s_full + 2;
+  uint64_t* q_ready = p_ready + 2;
+  uint64_t* o_done = q_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* last_one = reinterpret_cast<int*>(tmem_slot + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int b;
+  long long base;
+  Request r;
+  const Work work = att::find_work<kRows, kMinUnits, kThreads>(p, &b, &base, &r);
+  if ((int)blockIdx.x >= work.ctas) return;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(k_full + s, kDecodeWarps);
+      mbar_init(k_free + s, 1);
+      mbar_init(v_full + s, kDecodeWarps);
+      mbar_init(v_free + s, 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full + w, 1);
+      mbar_init(p_ready + w, 4);
+    }
+    mbar_init(q_ready, kSoftmaxWarps);
+    mbar_init(o_done, 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kSoftmaxWarps) gemm::tmem_alloc(smem_u32(tmem_slot), 512);
+  gemm::tc_fence_before();
+  __syncthreads();
+  gemm::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  static_assert(S::kColumns <= 512, "");
+
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned code) {
+    if (!mbar_wait(bar, parity & 1, p.err, code, abort)) *abort = 1;
+  };
+
+  // Every role goes through the same segments: runs of steps of one item.
+  long long u = work.first_unit(blockIdx.x);
+  const long long u_end = work.first_unit(blockIdx.x + 1);
+  int step = 0, segment = 0;                                 // over the whole launch
+  int tile_steps = 0;                                        // steps in which this softmax tile took part
+  int pair_steps = 0;                                        // steps with a second tile
+  for (; u < u_end; ++segment) {
+    long long mine = att::request_units<kRows, kMinUnits>(p, r);
+    while (u >= base + mine) {
+      base += mine;
+      r = att::request(p, ++b);
+      mine = att::request_units<kRows, kMinUnits>(p, r);
+    }
+    const int per_item = att::item_units<kMinUnits>(r);
+    const int tiles = (r.q_len * p.group + kRows - 1) / kRows;
+    const long long item = Work::quotient(u - base, per_item);
+    const int k_begin = (int)((u - base) - item * per_item);
+    const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
+    const int head = (int)Work::quotient(item, tiles), row0 = (int)(item - (long long)head * tiles) * kRows;
+    const int rows = min(kRows, r.q_len * p.group - row0);
+    const int j_begin = k_begin * att::kUnitKeys, j_end = min(k_end * att::kUnitKeys, r.kv_len);
+    const int steps = j_begin < j_end ? (j_end - j_begin + S::kKeys - 1) / S::kKeys : 0;
+    const bool pair = rows > kTileRows;
+
+    if (warp == kSoftmaxWarps) {
+      // ----------------------------------------------------------- products
+      if (lane == 0) wait(q_ready, segment, kDevErrMmaWait);
+      if (lane == 0 && steps > 0) {
+        const uint32_t q_at = smem_u32(sm_q), k_at = smem_u32(sm_k), v_at = smem_u32(sm_v);
+        const uint32_t scores = instruction(kBf16, false, S::kKeys);
+        const uint32_t outputs = instruction(kBf16, true, D / S::kGroups);
+        auto score = [&](int w, int n) {                     // S_w of step n
+          const uint32_t k_stage = k_at + (uint32_t)(n % S::kStages) * S::kStepBytes;
+          #pragma unroll
+          for (int a = 0; a < S::kAtoms; ++a)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_ss(tmem + (uint32_t)(w * 128 + (S::kGroups > 1 ? a * S::kKeys : 0)),
+                     gemm::desc_sw128(q_at + (uint32_t)((w * S::kAtoms + a) * kTileRows * 128 + i * 32)),
+                     gemm::desc_sw128(k_stage + (uint32_t)(a * S::kKeys * 128 + i * 32)), scores,
+                     i > 0 || (S::kGroups == 1 && a > 0) ? 1u : 0u);
+          gemm::tc_commit(s_full + w);
+        };
+        auto output = [&](int w, int n, bool begin) {        // O_w += P_w V of step n
+          const uint32_t v_stage = v_at + (uint32_t)(n % S::kStages) * S::kStepBytes;
+          #pragma unroll
+          for (int q = 0; q < S::kGroups; ++q)
+            #pragma unroll
+            for (int i = 0; i < S::kKeys / 16; ++i)
+              #pragma unroll
+              for (int e = 0; e < kTerms; ++e)
+                gemm::tc_mma_ts(tmem + (uint32_t)(256 + w * D + q * 64),
+                                tmem + (uint32_t)(w * 128 + q * S::kKeys + (i >> 1) * 32 + (i & 1) * 8 + e * 16),
+                                desc_values(v_stage + (uint32_t)(q * S::kKeys * 128 + i * 2048), S::kKeys * 128), outputs,
+                                begin && i == 0 && e == 0 ? 0u : 1u);
+        };
+        wait(k_full + step % S::kStages, step / S::kStages, kDevErrMmaWait);
+        gemm::tc_fence_after();
+        score(0, step);
+        if (pair) score(1, step);
+        gemm::tc_commit(k_free + step % S::kStages);
+        for (int i = 0; i < steps; ++i) {
+          const int n = step + i, next = n + 1;
+          wait(p_ready + 0, tile_steps + i, kDevErrMmaWait);
+          wait(v_full + n % S::kStages, n / S::kStages, kDevErrMmaWait);
+          gemm::tc_fence_after();
+          output(0, n, i == 0);
+          if (i + 1 < steps) {
+            wait(k_full + next % S::kStages, next / S::kStages, kDevErrMmaWait);
+            gemm::tc_fence_after();
+            score(0, next);
+          }
+          if (pair) {
+            wait(p_ready + 1, pair_steps + i, kDevErrMmaWait);
+            gemm::tc_fence_after();
+            output(1, n, i == 0);
+          }
+          gemm::tc_commit(v_free + n % S::kStages);
+          if (i + 1 < steps) {
+            if (pair) score(1, next);
+            gemm::tc_commit(k_free + next % S::kStages);
+          }
+        }
+        gemm::tc_commit(o_done);
+        // nothing of the products is in flight beyond this point, so TMEM can be let go
+        wait(o_done, segment, kDevErrMmaWait);
+      } else if (lane == 0) {
+        gemm::tc_commit(o_done);
+        wait(o_done, segment, kDevErrMmaWait);
+      }
+      __syncwarp();
+      tile_steps += steps;
+    } else if (warp > kSoftmaxWarps) {
+      // -------------------------------------------------------------- decode
+      const kvc::Pool& kv = p.cache;
+      const int t = threadIdx.x - 32 * (kSoftmaxWarps + 1);
+      constexpr int kRowPieces = S::kRowBytes / 16, kRowStep = 32 * kDecodeWarps / kRowPieces;
+      const int row = t / kRowPieces, piece = t % kRowPieces;          // of pieces row + i kRowStep
+      const int* pages = p.page_table + b * p.table_stride;
+      const int in_page = (1 << kv.page_shift) - 1;
+      auto page_at = [&](int j) { return pages[min(j, r.kv_len - 1) >> kv.page_shift]; };
+      auto usable = [&](int page) { return page >= 0 && page < p.num_pages; };
+      // pages of the next step's pieces and of the thread's scale; codes and scale of the next step
+      int page[S::kPieces], scale_page = 0, block_page = 0;
+      uint4 k_code[S::kPieces], v_code[S::kPieces];
+      unsigned short k_scale = 0, v_scale = 0;
+      bool scale_live = false;
+      unsigned bad = 0;
+      const int scale_key = t / S::kGroups, scale_group = t % S::kGroups;
+      auto fetch_pages = [&](int j0) {
+        #pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) page[i] = page_at(j0 + row + i * kRowStep);
+        scale_page = page_at(j0 + scale_key);
+        block_page = page_at(j0 + min(lane, S::kKeys / 16 - 1) * 16);
+      };
+      auto address = [&](int i, int j0, bool value) -> const uint4* {
+        const unsigned g = usable(page[i]) ? (unsigned)page[i] : 0u;
+        const unsigned at = (head << kv.page_shift) + ((j0 + row + i * kRowStep) & in_page);
+        return reinterpret_cast<const uint4*>((value ? kv.v_codes + (unsigned long long)g * kv.v_page
+                                                     : kv.k_codes + (unsigned long long)g * kv.k_page) +
+                                              (unsigned long long)at * S::kRowBytes + piece * 16);
+      };
+      auto fetch_keys = [&](int j0) {
+        #pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) k_code[i] = *address(i, j0, false);
+        const unsigned g = usable(scale_page) ? (unsigned)scale_page : 0u;
+        const unsigned at = (head << kv.page_shift) + ((j0 + scale_key) & in_page);
+        const unsigned long long sc = (unsigned long long)at * S::kGroups + scale_group;
+        k_scale = kv.k_scales[(unsigned long long)g * kv.ks_page + sc];
+        v_scale = kv.v_scales[(unsigned long long)g * kv.vs_page + sc];
+        scale_live = usable(scale_page) && j0 + scale_key < r.kv_len;
+        const bool block_bad = lane < S::kKeys / 16 && !usable(block_page);
+        bad = __ballot_sync(0xffffffffu, block_bad);
+        if (block_bad && j0 + lane * 16 < r.kv_len) atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+      };
+      auto fetch_values = [&](int j0) {
+        #pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) v_code[i] = *address(i, j0, true);
+      };
+      // a piece's elements, 8 to 16 bytes, to their places in a swizzled stage
+      auto store = [&](uint8_t* stage, int i, const uint4& code) {
+        const int key = row + i * kRowStep;
+        const uint32_t words[4] = {code.x, code.y, code.z, code.w};
+        constexpr int kChunks = S::kPerPiece / 8;                      // 16-byte runs of results
+        #pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          uint4 v;
+          // lanes of the odd atoms begin with the second run: eight lanes then write eight different banks
+          const int cc = BITS == 8 ? c ^ (piece >> 2 & 1) : c;
+          if constexpr (BITS == 8) {
+            const uint32_t x = cc ? words[2] : words[0], y = cc ? words[3] : words[1];
+            if constexpr (kBf16) {
+              att::dec8_b(x, v.x, v.y);
+              att::dec8_b(y, v.z, v.w);
+            } else {
+              dec_w8(x, v.x, v.y);
+              dec_w8(y, v.z, v.w);
+            }
+          } else {
+            const uint32_t x = words[c];
+            if constexpr (kBf16) {
+              // 16-bit lanes with nibbles 2 i and 2 i + 1 at the bottom; 0x430n is 128 + n
+              const uint32_t y = x >> 4;
+              const uint32_t w0 = __byte_perm(x, y, 0x4400), w1 = __byte_perm(x, y, 0x5511), w2 = __byte_perm(x, y, 0x6622),
+                             w3 = __byte_perm(x, y, 0x7733);
+              v.x = att::b2_sub(lop3_and_or(w0, 0x000F000Fu, 0x43004300u), 0x43084308u);
+              v.y = att::b2_sub(lop3_and_or(w1, 0x000F000Fu, 0x43004300u), 0x43084308u);
+              v.z = att::b2_sub(lop3_and_or(w2, 0x000F000Fu, 0x43004300u), 0x43084308u);
+              v.w = att::b2_sub(lop3_and_or(w3, 0x000F000Fu, 0x43004300u), 0x43084308u);
+            } else {
+              dec_w4_adjacent(x, v.x, v.y, v.z, v.w);
+            }
+          }
+          const int d = piece * S::kPerPiece + cc * 8;                 // first element
+          const int chunk = (d & 63) >> 3;
+          *reinterpret_cast<uint4*>(stage + (d >> 6) * S::kKeys * 128 + key * 128 + ((chunk ^ (key & 7)) << 4)) = v;
+        }
+      };
+      if (steps > 0) {
+        fetch_pages(j_begin);
+        fetch_keys(j_begin);
+        fetch_values(j_begin);
+      }
+      for (int i = 0; i < steps; ++i) {
+        const int n = step + i, st = n % S::kStages, j0 = j_begin + i * S::kKeys;
+        const uint32_t before = (uint32_t)(n / S::kStages - 1);        // parity of the stage's last use
+        if (i + 1 < steps) fetch_pages(j0 + S::kKeys);
+        if (n >= S::kStages) wait(k_free + st, before, kDevErrEmptyWait);
+        #pragma unroll
+        for (int q = 0; q < S::kPieces; ++q) store(sm_k + st * S::kStepBytes, q, k_code[q]);
+        Slot& slot = slots[n % S::kSlots];
+        const float v_sc = scale_live ? kvc::bf16_bits_to_f(v_scale) : 0.f;
+        slot.k[scale_group * S::kKeys + scale_key] = scale_live ? kvc::bf16_bits_to_f(k_scale) * p.scale_log2 : 0.f;
+        slot.v[scale_group * S::kKeys + scale_key] = v_sc;
+        const unsigned bits = __float_as_uint(v_sc);
+        const unsigned top = __reduce_max_sync(0xffffffffu, bits < 0x7F800000u ? bits : 0u);
+        if (lane == 0) slot.v_top[t >> 5] = top;
+        if (t == 0) slot.bad = bad;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full + st);
+        if (i + 1 < steps) fetch_keys(j0 + S::kKeys);
+        if (n >= S::kStages) wait(v_free + st, before, kDevErrEmptyWait);
+        #pragma unroll
+        for (int q = 0; q < S::kPieces; ++q) store(sm_v + st * S::kStepBytes, q, v_code[q]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full + st);
+        if (i + 1 < steps) fetch_values(j0 + S::kKeys);
+      }
+    } else {
+      // ------------------------------------------------------------- softmax
+      const int w = warp >> 2, quarter = warp & 3;
+      const int local = w * kTileRows + quarter * 32 + lane;           // row of the item
+      const bool live = local < rows;
+      const int token = live ? p.by_group.of(row0 + local) : 0;
+      const int qh = head * p.group + (live ? row0 + local - token * p.group : 0);
+      const bool active = w == 0 || pair;
+      // the row's query into shared memory
+      if (active && steps > 0) {
+        const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
+        #pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (live) {
+            const kvc::Chunk k = {c * 8, c * 8 + 4, false};
+            v = kvc::load_chunk(src, k, p.q.vec);
+          }
+          *reinterpret_cast<uint4*>(sm_q + ((w * S::kAtoms + (c >> 3)) * kTileRows + (local & 127)) * 128 +
+                                    (((c & 7) ^ (local & 7)) << 4)) = v;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gemm::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const uint32_t s_at = tmem + lanes + (uint32_t)(w * 128), o_at = tmem + lanes + (uint32_t)(256 + w * D);
+      float ref = 0.f, sum = 0.f;          // weights are 2^(score - ref); the maximum is ref + shift
+      int shift = 0;                       // log2 of what the weights are raised by, by the largest value scale
+      float v_ref = 0.f;
+      for (int i = 0; i < steps && active; ++i) {
+        const int n = step + i, j0 = j_begin + i * S::kKeys;
+        const Slot& slot = slots[n % S::kSlots];
+        wait(s_full + w, tile_steps + i, kDevErrFullWait);
+        gemm::tc_fence_after();
+        const unsigned bad = slot.bad;
+        const bool some_hidden = bad != 0 || j0 + S::kKeys > r.kv_len - r.q_len;
+        // 32 scores of the row, in units of log2
+        auto scores = [&](int c, float (&f)[32], unsigned& see) {
+          uint32_t x[32];
+          tmem_ld32(s_at + (uint32_t)(c * 32), x);
+          see = 0xFFFFFFFFu;
+          if (some_hidden) {
+            see = live ? sees32(p, r, token, j0 + c * 32) : 0u;
+            if (bad >> (2 * c) & 1) see &= 0xFFFF0000u;
+            if (bad >> (2 * c + 1) & 1) see &= 0x0000FFFFu;
+          }
+          tmem_wait(x);
+          if constexpr (S::kGroups == 1) {
+            #pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * 32 + e]);
+              f[e] = __uint_as_float(x[e]) * k.x;
+              f[e + 1] = __uint_as_float(x[e + 1]) * k.y;
+              f[e + 2] = __uint_as_float(x[e + 2]) * k.z;
+              f[e + 3] = __uint_as_float(x[e + 3]) * k.w;
+            }
+          } else {
+            uint32_t y[32];
+            tmem_ld32(s_at + (uint32_t)(S::kKeys + c * 32), y);
+            tmem_wait(y);
+            #pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * 32 + e]);
+              const float4 l = *reinterpret_cast<const float4*>(&slot.k[S::kKeys + c * 32 + e]);
+              f[e] = fmaf(__uint_as_float(y[e]), l.x, __uint_as_float(x[e]) * k.x);
+              f[e + 1] = fmaf(__uint_as_float(y[e + 1]), l.y, __uint_as_float(x[e + 1]) * k.y);
+              f[e + 2] = fmaf(__uint_as_float(y[e + 2]), l.z, __uint_as_float(x[e + 2]) * k.z);
+              f[e + 3] = fmaf(__uint_as_float(y[e + 3]), l.w, __uint_as_float(x[e + 3]) * k.w);
+            }
+          }
+          if (some_hidden) {
+            #pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(see >> e & 1)) f[e] = -INFINITY;
+          }
+        };
+        // the maximum, and the row's reference
+        float top = -INFINITY;
+        #pragma unroll 1
+        for (int c = 0; c < S::kKeys / 32; ++c) {
+          float f[32];
+          unsigned see;
+          scores(c, f, see);
+          float t0 = f[0], t1 = f[1];
+          #pragma unroll
+          for (int e = 2; e < 32; e += 2) {
+            t0 = fmaxf(t0, f[e]);
+            t1 = fmaxf(t1, f[e + 1]);
+          }
+          top = fmaxf(top, fmaxf(t0, t1));
+        }
+        const float v_top = __uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3])));
+        float next = ref;
+        if (v_top > v_ref) {                                           // the same in all rows
+          const int e = max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -60);    // 2^e >= v_top
+          v_ref = e > 127 ? INFINITY : att::pow2(e);
+          next += (float)shift - (float)(11 - e);
+          shift = 11 - e;
+        }
+        const bool fresh = !(sum > 0.f);                               // it has seen nothing yet
+        if (top > next + (float)shift + 4.f || (fresh && top > -INFINITY)) next = top - (float)shift;
+        const float keep = fresh ? 1.f : att::ex2<true>(ref - next);
+        if (__any_sync(0xffffffffu, keep != 1.f)) {
+          sum *= keep;
+          if (i > 0) {
+            #pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t x[32];
+              tmem_ld32(o_at + (uint32_t)(c * 32), x);
+              tmem_wait(x);
+              uint32_t y[16];
+              #pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                #pragma unroll
+                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * keep);
+                tmem_st16(o_at + (uint32_t)(c * 32 + 16 * h), y);
+              }
+            }
+          }
+        }
+        ref = next;
+        // the weights, in the place of the scores
+        #pragma unroll 1
+        for (int c = 0; c < S::kKeys / 32; ++c) {
+          float f[32];
+          unsigned see;
+          scores(c, f, see);
+          float part = 0.f;
+          #pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            f[e] = att::ex2<kBf16>(f[e] - ref);
+            part += f[e];
+          }
+          sum += part;
+          #pragma unroll
+          for (int q = 0; q < S::kGroups; ++q) {
+            uint32_t hi[16], lo[16];
+            #pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(&slot.v[q * S::kKeys + c * 32 + e]);
+              float a[4] = {f[e] * v.x, f[e + 1] * v.y, f[e + 2] * v.z, f[e + 3] * v.w};
+              if (some_hidden) {
+                #pragma unroll
+                for (int h = 0; h < 4; ++h)
+                  if (!(see >> (e + h) & 1)) a[h] = 0.f;               // whatever a hidden value's scale is
+              }
+              #pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if constexpr (kBf16) {
+                  const uint32_t u2 = att::pack_b2(a[2 * h], a[2 * h + 1]);
+                  hi[e / 2 + h] = u2;
+                  lo[e / 2 + h] = att::pack_b2(a[2 * h] - __uint_as_float(u2 << 16),
+                                               a[2 * h + 1] - __uint_as_float(u2 & 0xFFFF0000u));
+                } else {
+                  hi[e / 2 + h] = att::pack_h2(a[2 * h], a[2 * h + 1]);
+                }
+              }
+            }
+            tmem_st16(s_at + (uint32_t)(q * S::kKeys + c * 32), hi);
+            if constexpr (kBf16) tmem_st16(s_at + (uint32_t)(q * S::kKeys + c * 32 + 16), lo);
+          }
+        }
+        gemm::tmem_st_wait();
+        gemm::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + w);
+      }
+      wait(o_done, segment, kDevErrFullWait);
+      gemm::tc_fence_after();
+      if (!(sum != 0.f)) ref = att::kLow;                              // nothing seen (a NaN sum stays one)
+
+      // ------------------------------------------------- outputs, or a part
+      const long long item_begin = base + item * per_item;
+      const bool whole = k_begin == 0 && k_end == per_item;
+      const long long out_at = (long long)(r.q0 + token) * p.q_heads + qh;
+      auto finish = [&](int c, const float (&o)[32], float top, float l) {     // 32 outputs of the row
+        if (!live) return;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_at * D + c * 32);
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float* f = o + 8 * e;
+          dst[e] = make_uint4(kvc::pack2<T>(f[0] * inv, f[1] * inv), kvc::pack2<T>(f[2] * inv, f[3] * inv),
+                              kvc::pack2<T>(f[4] * inv, f[5] * inv), kvc::pack2<T>(f[6] * inv, f[7] * inv));
+        }
+        if (p.lse && c == 0) p.lse[out_at] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.69314718056f;
+      };
+      // a part: [reference][sum] of the rows, then runs of 4 outputs of all rows one behind another
+      auto park = [&](float* dst, int c, const float (&o)[32], float top, float l) {
+        #pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<float4*>(dst + 2 * kRows + ((c * 8 + e) * kRows + local) * 4) =
+              make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        if (c == 0) {
+          dst[local] = top;
+          dst[kRows + local] = l;
+        }
+      };
+      float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
+      if (active) {
+        #pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32] = {};
+          float o[32];
+          if (steps > 0) {
+            tmem_ld32(o_at + (uint32_t)(c * 32), x);
+            tmem_wait(x);
+          }
+          #pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(x[e]);
+          if (whole)
+            finish(c, o, ref, sum);
+          else
+            park(mine_out, c, o, ref, sum);
+        }
+      }
+      if (!whole) {
+        const int c_first = work.cta_of(item_begin), parts = work.cta_of(item_begin + per_item - 1) - c_first + 1;
+        const int groups = (parts + att::kJoin - 1) / att::kJoin, me = (int)blockIdx.x - c_first, group = me / att::kJoin;
+        auto part = [&](int q) {                            // the first begins the item: its CTA's second slot
+          return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
+        };
+        auto arrive = [&](unsigned* counter, int n) {       // true in the last of n CTAs, which sees the others' parts
+          __threadfence();
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          if (threadIdx.x == 0) {
+            *last_one = atomic_add_acq_rel_gpu(counter, 1u) == (unsigned)n - 1;
+            if (*last_one) *counter = 0;
+          }
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          return *last_one != 0;
+        };
+        // a thread joins its own row, and no other reads the row's parts
+        auto join = [&](int first, int stride, int count, auto out) {
+          float top = att::kLow, l = 0.f;
+          for (int q = 0; q < count; ++q) top = fmaxf(top, __ldcg(part(first + q * stride) + local));
+          for (int q = 0; q < count; ++q) {
+            const float* src = part(first + q * stride);
+            l += __ldcg(src + kRows + local) * att::ex2<true>(__ldcg(src + local) - top);
+          }
+          float f0 = 0.f;                                   // of the part that `out` may write over: read before
+          f0 = att::ex2<true>(__ldcg(part(first) + local) - top);
+          #pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32] = {};
+            for (int q = 0; q < count; ++q) {
+              const float* src = part(first + q * stride);
+              const float f = q == 0 ? f0 : att::ex2<true>(__ldcg(src + local) - top);
+              #pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src + 2 * kRows + ((c * 8 + e) * kRows + local) * 4));
+                o[4 * e] = fmaf(v.x, f, o[4 * e]);
+                o[4 * e + 1] = fmaf(v.y, f, o[4 * e + 1]);
+                o[4 * e + 2] = fmaf(v.z, f, o[4 * e + 2]);
+                o[4 * e + 3] = fmaf(v.w, f, o[4 * e + 3]);
+              }
+            }
+            out(c, o, top, l);
+          }
+        };
+        bool last = true;
+        if (groups > 1) {
+          const int n = min(att::kJoin, parts - group * att::kJoin);
+          last = arrive(counters + att::kMaxCtas + c_first + group * att::kJoin, n);
+          if (last && active)
+            join(group * att::kJoin, 1, n, [&](int c, const float (&o)[32], float top, float l) {
+              park(part(group * att::kJoin), c, o, top, l);
+            });
+        }
+        if (last && arrive(counters + c_first, groups > 1 ? groups : parts) && active)
+          join(0, groups > 1 ? att::kJoin : 1, groups > 1 ? groups : parts, finish);
+      }
+      if (active) tile_steps += steps;
+    }
+    if (pair) pair_steps += steps;
+    step += steps;
+    u += k_end - k_begin;
+  }
+
+  gemm::tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps) {
+    gemm::tc_fence_after();
+    gemm::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace tree
+}  // namespace ql
