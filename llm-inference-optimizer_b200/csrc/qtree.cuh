@@ -18,11 +18,8 @@
 //   * 1 warp issues the products: S_0, S_1 of a step, then P_0 V and S_0 of
 //     the next, P_1 V and S_1 of the next, so that one tile's softmax runs
 //     under the other's products.
-//   * 8 softmax warps, a thread a row: S from TMEM twice, for the maximum and
-//     for the weights, which go back to TMEM in the place of S.  Key scales
-//     multiply the scores, value scales the weights; a row's reference
-//     exponent holds its maximum and the largest value scale seen, and moves
-//     (with its outputs in TMEM) when a score passes it by 2^4.
+//   * 8 softmax warps, a thread a row: S from TMEM, the weights back to TMEM
+//     in its place.  Key scales multiply the scores, value scales the weights.
 // At 4 bits and head_dim 128, where a scale covers 64 elements, a step is 64
 // keys with a sum and a set of weights per group.
 //
@@ -124,6 +121,36 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
       : "memory");
 }
 
+// Two fp32 operations an instruction.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ unsigned long long bits2(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ F2 floats2(unsigned long long v) {
+  F2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)), "l"(bits2(c.x, c.y)));
+  return floats2(r);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)));
+  return floats2(r);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)));
+  return floats2(r);
+}
+
 // Which of 32 positions from j on row i of the request sees, as bits.
 __device__ __forceinline__ unsigned sees32(const Params& p, const Request& r, int i, int j) {
   const int d0 = j - (r.kv_len - r.q_len), left = r.kv_len - j;        // which new token j is; positions left
@@ -150,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   using Slot = typename S::Slot;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   constexpr int kTerms = kBf16 ? 2 : 1;
+  constexpr int kRun = S::kGroups == 1 ? 64 : 32;            // scores that a softmax thread takes at once
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ uint8_t smem_raw[];
@@ -442,9 +470,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
 
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const uint32_t s_at = tmem + lanes + (uint32_t)(w * 128), o_at = tmem + lanes + (uint32_t)(256 + w * D);
-      float ref = 0.f, sum = 0.f;          // weights are 2^(score - ref); the maximum is ref + shift
-      int shift = 0;                       // log2 of what the weights are raised by, by the largest value scale
-      float v_ref = 0.f;
+      // Weights are 2^(score - ref), and ref + shift is about the row's maximum: a step's weights are taken with the
+      // reference as it is, and only where a run of them adds up to more than 2^9 of it (an overflow too) does it move,
+      // by a whole number, so that the weights written and the outputs follow exactly.  shift raises them to the
+      // largest value scale seen, weight * scale to at most 2^15.
+      float ref = 0.f, sum = 0.f, v_ref = 0.f;
+      int shift = 0;
       for (int i = 0; i < steps && active; ++i) {
         const int n = step + i, j0 = j_begin + i * S::kKeys;
         const Slot& slot = slots[n % S::kSlots];
@@ -452,131 +483,195 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         gemm::tc_fence_after();
         const unsigned bad = slot.bad;
         const bool some_hidden = bad != 0 || j0 + S::kKeys > r.kv_len - r.q_len;
-        // 32 scores of the row, in units of log2
-        auto scores = [&](int c, float (&f)[32], unsigned& see) {
-          uint32_t x[32];
-          tmem_ld32(s_at + (uint32_t)(c * 32), x);
-          see = 0xFFFFFFFFu;
+        const float v_top = __uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3])));
+        // the positions of run c that the row sees, as bits
+        auto seen = [&](int c) {
+          unsigned long long see = ~0ull;
           if (some_hidden) {
-            see = live ? sees32(p, r, token, j0 + c * 32) : 0u;
-            if (bad >> (2 * c) & 1) see &= 0xFFFF0000u;
-            if (bad >> (2 * c + 1) & 1) see &= 0x0000FFFFu;
-          }
-          tmem_wait(x);
-          if constexpr (S::kGroups == 1) {
+            see = 0;
             #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * 32 + e]);
-              f[e] = __uint_as_float(x[e]) * k.x;
-              f[e + 1] = __uint_as_float(x[e + 1]) * k.y;
-              f[e + 2] = __uint_as_float(x[e + 2]) * k.z;
-              f[e + 3] = __uint_as_float(x[e + 3]) * k.w;
-            }
-          } else {
-            uint32_t y[32];
-            tmem_ld32(s_at + (uint32_t)(S::kKeys + c * 32), y);
-            tmem_wait(y);
-            #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * 32 + e]);
-              const float4 l = *reinterpret_cast<const float4*>(&slot.k[S::kKeys + c * 32 + e]);
-              f[e] = fmaf(__uint_as_float(y[e]), l.x, __uint_as_float(x[e]) * k.x);
-              f[e + 1] = fmaf(__uint_as_float(y[e + 1]), l.y, __uint_as_float(x[e + 1]) * k.y);
-              f[e + 2] = fmaf(__uint_as_float(y[e + 2]), l.z, __uint_as_float(x[e + 2]) * k.z);
-              f[e + 3] = fmaf(__uint_as_float(y[e + 3]), l.w, __uint_as_float(x[e + 3]) * k.w);
+            for (int h = 0; h < kRun / 32; ++h) {
+              unsigned s32 = live ? sees32(p, r, token, j0 + c * kRun + h * 32) : 0u;
+              if (bad >> (c * (kRun / 16) + 2 * h) & 1) s32 &= 0xFFFF0000u;
+              if (bad >> (c * (kRun / 16) + 2 * h + 1) & 1) s32 &= 0x0000FFFFu;
+              see |= (unsigned long long)s32 << (32 * h);
             }
           }
+          return see;
+        };
+        // f = scores of run c less `less`, in units of log2, from sums x (and y of the second group)
+        auto scores = [&](float (&f)[kRun], const uint32_t (&x)[kRun], const uint32_t (&y)[kRun], int c, float less,
+                          unsigned long long see) {
+          #pragma unroll
+          for (int e = 0; e < kRun; e += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * kRun + e]);
+            F2 a = fma2({__uint_as_float(x[e]), __uint_as_float(x[e + 1])}, {k.x, k.y}, {-less, -less});
+            F2 b = fma2({__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])}, {k.z, k.w}, {-less, -less});
+            if constexpr (S::kGroups > 1) {
+              const float4 l = *reinterpret_cast<const float4*>(&slot.k[S::kKeys + c * kRun + e]);
+              a = fma2({__uint_as_float(y[e]), __uint_as_float(y[e + 1])}, {l.x, l.y}, a);
+              b = fma2({__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])}, {l.z, l.w}, b);
+            }
+            f[e] = a.x;
+            f[e + 1] = a.y;
+            f[e + 2] = b.x;
+            f[e + 3] = b.y;
+          }
           if (some_hidden) {
             #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < kRun; ++e)
               if (!(see >> e & 1)) f[e] = -INFINITY;
           }
         };
-        // the maximum, and the row's reference
-        float top = -INFINITY;
-        #pragma unroll 1
-        for (int c = 0; c < S::kKeys / 32; ++c) {
-          float f[32];
-          unsigned see;
-          scores(c, f, see);
-          float t0 = f[0], t1 = f[1];
+        auto load = [&](uint32_t (&x)[kRun], uint32_t (&y)[kRun], int c) {
           #pragma unroll
-          for (int e = 2; e < 32; e += 2) {
-            t0 = fmaxf(t0, f[e]);
-            t1 = fmaxf(t1, f[e + 1]);
+          for (int h = 0; h < kRun / 32; ++h)
+            tmem_ld32(s_at + (uint32_t)(c * kRun + h * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[32 * h]));
+          if constexpr (S::kGroups > 1) tmem_ld32(s_at + (uint32_t)(S::kKeys + c * kRun), *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
+          #pragma unroll
+          for (int h = 0; h < kRun / 32; ++h) tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&x[32 * h]));
+          if constexpr (S::kGroups > 1) tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&y[0]));
+        };
+        auto most = [](const float (&f)[kRun]) {
+          float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
+          #pragma unroll
+          for (int e = 4; e < kRun; e += 4) {
+            a = fmaxf(a, fmaxf(f[e], f[e + 1]));
+            b = fmaxf(b, fmaxf(f[e + 2], f[e + 3]));
           }
-          top = fmaxf(top, fmaxf(t0, t1));
-        }
-        const float v_top = __uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3])));
-        float next = ref;
-        if (v_top > v_ref) {                                           // the same in all rows
-          const int e = max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -60);    // 2^e >= v_top
-          v_ref = e > 127 ? INFINITY : att::pow2(e);
-          next += (float)shift - (float)(11 - e);
-          shift = 11 - e;
-        }
-        const bool fresh = !(sum > 0.f);                               // it has seen nothing yet
-        if (top > next + (float)shift + 4.f || (fresh && top > -INFINITY)) next = top - (float)shift;
-        const float keep = fresh ? 1.f : att::ex2<true>(ref - next);
-        if (__any_sync(0xffffffffu, keep != 1.f)) {
-          sum *= keep;
+          return fmaxf(a, b);
+        };
+        // sum and outputs times 2^by, and the first `runs` runs of this step's weights
+        auto raise = [&](int by, int runs) {
+          const float factor = by <= -126 ? 0.f : att::pow2(min(by, 127));
+          sum *= factor;
+          gemm::tmem_st_wait();
           if (i > 0) {
             #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t x[32];
+              uint32_t x[32], y[16];
               tmem_ld32(o_at + (uint32_t)(c * 32), x);
               tmem_wait(x);
-              uint32_t y[16];
               #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * keep);
+                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * factor);
                 tmem_st16(o_at + (uint32_t)(c * 32 + 16 * h), y);
               }
             }
           }
+          const uint32_t f2 = kBf16 ? att::pack_b2(factor, factor) : att::pack_h2(factor, factor);
+          #pragma unroll 1
+          for (int c = 0; c < runs * (kRun / 32) * S::kGroups; ++c) {     // 32 keys of a group at a time
+            const int in_group = runs * (kRun / 32);
+            const uint32_t at = s_at + (uint32_t)((c / in_group) * S::kKeys + (c % in_group) * 32);
+            uint32_t x[32], y[16];
+            tmem_ld32(at, x);
+            tmem_wait(x);
+            #pragma unroll
+            for (int h = 0; h < kTerms; ++h) {
+              #pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                if constexpr (kBf16) {
+                  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[16 * h + e]),
+                                                   *reinterpret_cast<const __nv_bfloat162*>(&f2));
+                  y[e] = *reinterpret_cast<const uint32_t*>(&v);
+                } else {
+                  y[e] = gemm::h2_mul(x[16 * h + e], f2);
+                }
+              }
+              tmem_st16(at + (uint32_t)(16 * h), y);
+            }
+          }
+        };
+        if (v_top > v_ref) {                                           // the same in all rows
+          const int e = max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -60);    // 2^e >= v_top
+          const int by = 6 - e - shift;
+          v_ref = e > 127 ? INFINITY : att::pow2(e);
+          shift += by;
+          ref -= (float)by;
+          raise(by, 0);
         }
-        ref = next;
+        if (__any_sync(0xffffffffu, !(sum > 0.f))) {                    // rows that have seen nothing yet
+          float top = -INFINITY;
+          #pragma unroll 1
+          for (int c = 0; c < S::kKeys / kRun; ++c) {
+            uint32_t x[kRun], y[kRun];
+            float f[kRun];
+            load(x, y, c);
+            scores(f, x, y, c, 0.f, seen(c));
+            top = fmaxf(top, most(f));
+          }
+          if (!(sum > 0.f) && top > -INFINITY) ref = top - (float)shift;
+        }
         // the weights, in the place of the scores
         #pragma unroll 1
-        for (int c = 0; c < S::kKeys / 32; ++c) {
-          float f[32];
-          unsigned see;
-          scores(c, f, see);
-          float part = 0.f;
-          #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            f[e] = att::ex2<kBf16>(f[e] - ref);
-            part += f[e];
+        for (int c = 0; c < S::kKeys / kRun; ++c) {
+          const unsigned long long see = seen(c);
+          float f[kRun], part;
+          uint32_t hi[S::kGroups][kRun / 2], lo[S::kGroups][kRun / 2];
+          auto weigh = [&] {
+            {
+              uint32_t x[kRun], y[kRun];
+              load(x, y, c);
+              scores(f, x, y, c, ref, see);
+            }
+            #pragma unroll
+            for (int e = 0; e < kRun; ++e) f[e] = att::ex2<kBf16>(f[e]);
+            F2 sums[2] = {{f[0], f[1]}, {f[2], f[3]}};
+            #pragma unroll
+            for (int e = 4; e < kRun; e += 4) {
+              sums[0] = add2(sums[0], {f[e], f[e + 1]});
+              sums[1] = add2(sums[1], {f[e + 2], f[e + 3]});
+            }
+            part = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+            #pragma unroll
+            for (int q = 0; q < S::kGroups; ++q)
+              #pragma unroll
+              for (int e = 0; e < kRun; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(&slot.v[q * S::kKeys + c * kRun + e]);
+                F2 a[2] = {mul2({f[e], f[e + 1]}, {v.x, v.y}), mul2({f[e + 2], f[e + 3]}, {v.z, v.w})};
+                if (some_hidden) {                                     // whatever a hidden value's scale is
+                  if (!(see >> e & 1)) a[0].x = 0.f;
+                  if (!(see >> (e + 1) & 1)) a[0].y = 0.f;
+                  if (!(see >> (e + 2) & 1)) a[1].x = 0.f;
+                  if (!(see >> (e + 3) & 1)) a[1].y = 0.f;
+                }
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  if constexpr (kBf16) {
+                    const uint32_t u2 = att::pack_b2(a[h].x, a[h].y);
+                    hi[q][e / 2 + h] = u2;
+                    lo[q][e / 2 + h] = att::pack_b2(a[h].x - __uint_as_float(u2 << 16), a[h].y - __uint_as_float(u2 & 0xFFFF0000u));
+                  } else {
+                    hi[q][e / 2 + h] = att::pack_h2(a[h].x, a[h].y);
+                  }
+                }
+              }
+          };
+          weigh();
+          const bool over = part > att::pow2(min(9 + shift, 126));
+          if (__any_sync(0xffffffffu, over)) {
+            {
+              uint32_t x[kRun], y[kRun];                               // the scores are still there
+              load(x, y, c);
+              scores(f, x, y, c, ref + (float)shift, see);
+            }
+            const float top = most(f);
+            const int by = over && top < 1e6f ? (int)ceilf(top) : 0;
+            raise(-by, c);
+            ref += (float)by;
+            weigh();
           }
           sum += part;
           #pragma unroll
-          for (int q = 0; q < S::kGroups; ++q) {
-            uint32_t hi[16], lo[16];
+          for (int q = 0; q < S::kGroups; ++q)
             #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 v = *reinterpret_cast<const float4*>(&slot.v[q * S::kKeys + c * 32 + e]);
-              float a[4] = {f[e] * v.x, f[e + 1] * v.y, f[e + 2] * v.z, f[e + 3] * v.w};
-              if (some_hidden) {
-                #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                  if (!(see >> (e + h) & 1)) a[h] = 0.f;               // whatever a hidden value's scale is
-              }
-              #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if constexpr (kBf16) {
-                  const uint32_t u2 = att::pack_b2(a[2 * h], a[2 * h + 1]);
-                  hi[e / 2 + h] = u2;
-                  lo[e / 2 + h] = att::pack_b2(a[2 * h] - __uint_as_float(u2 << 16),
-                                               a[2 * h + 1] - __uint_as_float(u2 & 0xFFFF0000u));
-                } else {
-                  hi[e / 2 + h] = att::pack_h2(a[2 * h], a[2 * h + 1]);
-                }
-              }
+            for (int h = 0; h < kRun / 32; ++h) {
+              const uint32_t at = s_at + (uint32_t)(q * S::kKeys + c * kRun + h * 32);
+              tmem_st16(at, *reinterpret_cast<const uint32_t(*)[16]>(&hi[q][16 * h]));
+              if constexpr (kBf16) tmem_st16(at + 16u, *reinterpret_cast<const uint32_t(*)[16]>(&lo[q][16 * h]));
             }
-            tmem_st16(s_at + (uint32_t)(q * S::kKeys + c * 32), hi);
-            if constexpr (kBf16) tmem_st16(s_at + (uint32_t)(q * S::kKeys + c * 32 + 16), lo);
-          }
         }
         gemm::tmem_st_wait();
         gemm::tc_fence_before();
