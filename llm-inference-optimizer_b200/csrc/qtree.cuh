@@ -42,8 +42,10 @@ using att::Work;
 constexpr int kTileRows = 128;
 constexpr int kRows = 2 * kTileRows;
 constexpr int kMinUnits = 4;             // of 128 keys: a part's outputs are worth 512 keys
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
-constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + kDecodeWarps);
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kMmaWarp = kSoftmaxWarps + kDecodeWarps;
+constexpr int kThreads = 512;            // the last three warps idle: warpgroups trade registers as a whole
+// Registers a thread, of the 128 that the launch gives each: 8 x 160 + 4 x 112 + 4 x 80 = 16 x 128.
+constexpr int kSoftmaxRegisters = 160, kDecodeRegisters = 112, kMmaRegisters = 80;
 
 template <int D, int BITS>
 struct Shape {
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     *abort = 0;
     fence_barrier_init();
   }
-  if (warp == kSoftmaxWarps) gemm::tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == kMmaWarp) gemm::tmem_alloc(smem_u32(tmem_slot), 512);
   gemm::tc_fence_before();
   __syncthreads();
   gemm::tc_fence_after();
@@ -234,58 +236,89 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   // Every role goes through the same segments: runs of steps of one item.
   long long u = work.first_unit(blockIdx.x);
   const long long u_end = work.first_unit(blockIdx.x + 1);
+  struct Segment {
+    long long item_begin;                                    // the item's first unit
+    int per_item, k_begin, k_end;                            // its units, and those of the segment
+    int head, row0, rows, j_begin, steps;
+    bool pair;                                               // more than one tile of rows
+  };
   int step = 0, segment = 0;                                 // over the whole launch
-  int tile_steps = 0;                                        // steps in which this softmax tile took part
+  int tile_steps = 0;                                        // steps in which this role's first tile took part
   int pair_steps = 0;                                        // steps with a second tile
-  for (; u < u_end; ++segment) {
+  auto next_segment = [&] {
+    Segment g;
     long long mine = att::request_units<kRows, kMinUnits>(p, r);
     while (u >= base + mine) {
       base += mine;
       r = att::request(p, ++b);
       mine = att::request_units<kRows, kMinUnits>(p, r);
     }
-    const int per_item = att::item_units<kMinUnits>(r);
+    g.per_item = att::item_units<kMinUnits>(r);
     const int tiles = (r.q_len * p.group + kRows - 1) / kRows;
-    const long long item = Work::quotient(u - base, per_item);
-    const int k_begin = (int)((u - base) - item * per_item);
-    const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
-    const int head = (int)Work::quotient(item, tiles), row0 = (int)(item - (long long)head * tiles) * kRows;
-    const int rows = min(kRows, r.q_len * p.group - row0);
-    const int j_begin = k_begin * att::kUnitKeys, j_end = min(k_end * att::kUnitKeys, r.kv_len);
-    const int steps = j_begin < j_end ? (j_end - j_begin + S::kKeys - 1) / S::kKeys : 0;
-    const bool pair = rows > kTileRows;
+    const long long item = Work::quotient(u - base, g.per_item);
+    g.item_begin = base + item * g.per_item;
+    g.k_begin = (int)(u - g.item_begin);
+    g.k_end = (int)min((long long)g.per_item, g.k_begin + (u_end - u));
+    g.head = (int)Work::quotient(item, tiles);
+    g.row0 = (int)(item - (long long)g.head * tiles) * kRows;
+    g.rows = min(kRows, r.q_len * p.group - g.row0);
+    g.j_begin = g.k_begin * att::kUnitKeys;
+    const int j_end = min(g.k_end * att::kUnitKeys, r.kv_len);
+    g.steps = g.j_begin < j_end ? (j_end - g.j_begin + S::kKeys - 1) / S::kKeys : 0;
+    g.pair = g.rows > kTileRows;
+    return g;
+  };
+  auto end_segment = [&](const Segment& g) {
+    if (g.pair) pair_steps += g.steps;
+    step += g.steps;
+    u += g.k_end - g.k_begin;
+    ++segment;
+  };
 
-    if (warp == kSoftmaxWarps) {
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
+    while (warp == kMmaWarp && u < u_end) {
       // ----------------------------------------------------------- products
+      const Segment g = next_segment();
+      const int steps = g.steps;
+      const bool pair = g.pair;
       if (lane == 0) wait(q_ready, segment, kDevErrMmaWait);
       if (lane == 0 && steps > 0) {
         const uint32_t q_at = smem_u32(sm_q), k_at = smem_u32(sm_k), v_at = smem_u32(sm_v);
         const uint32_t scores = instruction(kBf16, false, S::kKeys);
         const uint32_t outputs = instruction(kBf16, true, D / S::kGroups);
         auto score = [&](int w, int n) {                     // S_w of step n
-          const uint32_t k_stage = k_at + (uint32_t)(n % S::kStages) * S::kStepBytes;
-          #pragma unroll
-          for (int a = 0; a < S::kAtoms; ++a)
+          uint64_t qd = gemm::desc_sw128(q_at + (uint32_t)(w * S::kAtoms * kTileRows * 128));
+          uint64_t kd = gemm::desc_sw128(k_at + (uint32_t)(n % S::kStages) * S::kStepBytes);
+          uint32_t d = tmem + (uint32_t)(w * 128);
+          #pragma unroll 1
+          for (int a = 0; a < S::kAtoms; ++a) {
             #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma_ss(tmem + (uint32_t)(w * 128 + (S::kGroups > 1 ? a * S::kKeys : 0)),
-                     gemm::desc_sw128(q_at + (uint32_t)((w * S::kAtoms + a) * kTileRows * 128 + i * 32)),
-                     gemm::desc_sw128(k_stage + (uint32_t)(a * S::kKeys * 128 + i * 32)), scores,
-                     i > 0 || (S::kGroups == 1 && a > 0) ? 1u : 0u);
+            for (int i = 0; i < 4; ++i)                      // 32 bytes, 16 elements, along the swizzled rows
+              mma_ss(d, qd + 2 * i, kd + 2 * i, scores, i > 0 || (S::kGroups == 1 && a > 0) ? 1u : 0u);
+            qd += kTileRows * 128 / 16;
+            kd += S::kKeys * 128 / 16;
+            if (S::kGroups > 1) d += S::kKeys;
+          }
           gemm::tc_commit(s_full + w);
         };
         auto output = [&](int w, int n, bool begin) {        // O_w += P_w V of step n
-          const uint32_t v_stage = v_at + (uint32_t)(n % S::kStages) * S::kStepBytes;
-          #pragma unroll
-          for (int q = 0; q < S::kGroups; ++q)
-            #pragma unroll
-            for (int i = 0; i < S::kKeys / 16; ++i)
+          uint64_t vd = desc_values(v_at + (uint32_t)(n % S::kStages) * S::kStepBytes, S::kKeys * 128);
+          uint32_t a = tmem + (uint32_t)(w * 128);
+          #pragma unroll 1
+          for (int q = 0; q < S::kGroups; ++q) {
+            #pragma unroll 1
+            for (int i = 0; i < S::kKeys / 32; ++i) {        // 32 keys: 16 columns of weights and, with two terms, 16 more
               #pragma unroll
-              for (int e = 0; e < kTerms; ++e)
-                gemm::tc_mma_ts(tmem + (uint32_t)(256 + w * D + q * 64),
-                                tmem + (uint32_t)(w * 128 + q * S::kKeys + (i >> 1) * 32 + (i & 1) * 8 + e * 16),
-                                desc_values(v_stage + (uint32_t)(q * S::kKeys * 128 + i * 2048), S::kKeys * 128), outputs,
-                                begin && i == 0 && e == 0 ? 0u : 1u);
+              for (int h = 0; h < 2; ++h)
+                #pragma unroll
+                for (int e = 0; e < kTerms; ++e)
+                  gemm::tc_mma_ts(tmem + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
+                                  vd + (uint64_t)(h * 2048 / 16), outputs, begin && i == 0 && h == 0 && e == 0 ? 0u : 1u);
+              a += 32;
+              vd += 2 * 2048 / 16;
+            }
+          }
         };
         wait(k_full + step % S::kStages, step / S::kStages, kDevErrMmaWait);
         gemm::tc_fence_after();
@@ -323,10 +356,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       }
       __syncwarp();
       tile_steps += steps;
-    } else if (warp > kSoftmaxWarps) {
+      end_segment(g);
+    }
+  } else if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegisters));
+    while (u < u_end) {
       // -------------------------------------------------------------- decode
+      const Segment g = next_segment();
+      const int steps = g.steps, head = g.head, j_begin = g.j_begin;
       const kvc::Pool& kv = p.cache;
-      const int t = threadIdx.x - 32 * (kSoftmaxWarps + 1);
+      const int t = threadIdx.x - 32 * kSoftmaxWarps;
       constexpr int kRowPieces = S::kRowBytes / 16, kRowStep = 32 * kDecodeWarps / kRowPieces;
       const int row = t / kRowPieces, piece = t % kRowPieces;          // of pieces row + i kRowStep
       const int* pages = p.page_table + b * p.table_stride;
@@ -441,14 +480,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         if (lane == 0) mbar_arrive(v_full + st);
         if (i + 1 < steps) fetch_values(j0 + S::kKeys);
       }
-    } else {
+      end_segment(g);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    while (u < u_end) {
       // ------------------------------------------------------------- softmax
+      const Segment g = next_segment();
+      const int steps = g.steps, head = g.head, j_begin = g.j_begin, row0 = g.row0, rows = g.rows;
+      const int k_begin = g.k_begin, per_item = g.per_item;
       const int w = warp >> 2, quarter = warp & 3;
       const int local = w * kTileRows + quarter * 32 + lane;           // row of the item
       const bool live = local < rows;
       const int token = live ? p.by_group.of(row0 + local) : 0;
       const int qh = head * p.group + (live ? row0 + local - token * p.group : 0);
-      const bool active = w == 0 || pair;
+      const bool active = w == 0 || g.pair;
       // the row's query into shared memory
       if (active && steps > 0) {
         const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
@@ -683,8 +729,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       if (!(sum != 0.f)) ref = att::kLow;                              // nothing seen (a NaN sum stays one)
 
       // ------------------------------------------------- outputs, or a part
-      const long long item_begin = base + item * per_item;
-      const bool whole = k_begin == 0 && k_end == per_item;
+      const long long item_begin = g.item_begin;
+      const bool whole = k_begin == 0 && g.k_end == per_item;
       const long long out_at = (long long)(r.q0 + token) * p.q_heads + qh;
       auto finish = [&](int c, const float (&o)[32], float top, float l) {     // 32 outputs of the row
         if (!live) return;
@@ -784,15 +830,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           join(0, groups > 1 ? att::kJoin : 1, groups > 1 ? groups : parts, finish);
       }
       if (active) tile_steps += steps;
+      end_segment(g);
     }
-    if (pair) pair_steps += steps;
-    step += steps;
-    u += k_end - k_begin;
   }
 
   gemm::tc_fence_before();
   __syncthreads();
-  if (warp == kSoftmaxWarps) {
+  if (warp == kMmaWarp) {
     gemm::tc_fence_after();
     gemm::tmem_dealloc(tmem, 512);
   }
