@@ -72,12 +72,31 @@ struct Shape {
   static_assert(kPieces >= 1 && kPieces * kPerPiece * 32 * kDecodeWarps == kKeys * D, "");
 };
 
+// The products and their commits, by one elected lane of a whole warp in
+// uniform control flow: the operands then stay in uniform registers, where a
+// branch to one lane would move each of them there anew (140 cycles a product
+// under load against 64 of the product itself).
 // D[tmem] (+)= A[smem] B[smem], kind::f16.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem].
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrival on `bar` once the products issued so far are done.
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 // Instruction descriptor: fp32 sums, M = 128, N; A and B fp16 or bf16; B's
@@ -282,8 +301,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const Segment g = next_segment();
       const int steps = g.steps;
       const bool pair = g.pair;
-      if (lane == 0) wait(q_ready, segment, kDevErrMmaWait);
-      if (lane == 0 && steps > 0) {
+      wait(q_ready, segment, kDevErrMmaWait);
+      gemm::tc_fence_after();
+      if (steps > 0) {
         const uint32_t q_at = smem_u32(sm_q), k_at = smem_u32(sm_k), v_at = smem_u32(sm_v);
         const uint32_t scores = instruction(kBf16, false, S::kKeys);
         const uint32_t outputs = instruction(kBf16, true, D / S::kGroups);
@@ -300,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             kd += S::kKeys * 128 / 16;
             if (S::kGroups > 1) d += S::kKeys;
           }
-          gemm::tc_commit(s_full + w);
+          commit(s_full + w);
         };
         auto output = [&](int w, int n, bool begin) {        // O_w += P_w V of step n
           uint64_t vd = desc_values(v_at + (uint32_t)(n % S::kStages) * S::kStepBytes, S::kKeys * 128);
@@ -313,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               for (int h = 0; h < 2; ++h)
                 #pragma unroll
                 for (int e = 0; e < kTerms; ++e)
-                  gemm::tc_mma_ts(tmem + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
+                  mma_ts(tmem + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
                                   vd + (uint64_t)(h * 2048 / 16), outputs, begin && i == 0 && h == 0 && e == 0 ? 0u : 1u);
               a += 32;
               vd += 2 * 2048 / 16;
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         gemm::tc_fence_after();
         score(0, step);
         if (pair) score(1, step);
-        gemm::tc_commit(k_free + step % S::kStages);
+        commit(k_free + step % S::kStages);
         for (int i = 0; i < steps; ++i) {
           const int n = step + i, next = n + 1;
           wait(p_ready + 0, tile_steps + i, kDevErrMmaWait);
@@ -341,20 +361,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             gemm::tc_fence_after();
             output(1, n, i == 0);
           }
-          gemm::tc_commit(v_free + n % S::kStages);
+          commit(v_free + n % S::kStages);
           if (i + 1 < steps) {
             if (pair) score(1, next);
-            gemm::tc_commit(k_free + next % S::kStages);
+            commit(k_free + next % S::kStages);
           }
         }
-        gemm::tc_commit(o_done);
-        // nothing of the products is in flight beyond this point, so TMEM can be let go
-        wait(o_done, segment, kDevErrMmaWait);
-      } else if (lane == 0) {
-        gemm::tc_commit(o_done);
-        wait(o_done, segment, kDevErrMmaWait);
       }
-      __syncwarp();
+      commit(o_done);
+      // nothing of the products is in flight beyond this point, so TMEM can be let go
+      wait(o_done, segment, kDevErrMmaWait);
       tile_steps += steps;
       end_segment(g);
     }
