@@ -69,7 +69,7 @@ struct Shape {
     unsigned pad[3];
   };
   static constexpr size_t kSmem = 1024 + kQBytes + 2 * (size_t)kStages * kStepBytes + kSlots * sizeof(Slot) + 512;
-  static_assert(kPieces >= 1 && kPieces * kPerPiece * 32 * kDecodeWarps == kKeys * D, "");
+  static_assert(kKeys % 64 == 0 && kPieces >= 1 && kPieces * kPerPiece * 32 * kDecodeWarps == kKeys * D, "");
 };
 
 // The products and their commits, by one elected lane of a whole warp in
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   using Slot = typename S::Slot;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   constexpr int kTerms = kBf16 ? 2 : 1;
-  constexpr int kRun = S::kGroups == 1 ? 64 : 32;            // scores that a softmax thread takes at once
+  constexpr int kRun = S::kKeys / 2;                         // scores that a softmax thread takes at once
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ uint8_t smem_raw[];
@@ -212,8 +212,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   uint64_t* v_full = k_free + S::kStages;
   uint64_t* v_free = v_full + S::kStages;
   uint64_t* s_full = v_free + S::kStages;                    // per tile
-  uint64_t* p_ready = s_full + 2;
-  uint64_t* q_ready = p_ready + 2;
+  uint64_t* p_ready = s_full + 2;                            // per tile and half of a step
+  uint64_t* half_done = p_ready + 4;                         // the products of a step's first weights
+  uint64_t* q_ready = half_done + 2;
   uint64_t* o_done = q_ready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -234,7 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full + w, 1);
-      mbar_init(p_ready + w, 4);
+      mbar_init(p_ready + 2 * w, 4);
+      mbar_init(p_ready + 2 * w + 1, 4);
+      mbar_init(half_done + w, 1);
     }
     mbar_init(q_ready, kSoftmaxWarps);
     mbar_init(o_done, 1);
@@ -262,8 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     bool pair;                                               // more than one tile of rows
   };
   int step = 0, segment = 0;                                 // over the whole launch
-  int tile_steps = 0;                                        // steps in which this role's first tile took part
-  int pair_steps = 0;                                        // steps with a second tile
+  int tile_steps = 0;                                        // a softmax tile's: those in which it took part
+  int pair_steps = 0;                                        // the products': those with a second tile
   auto next_segment = [&] {
     Segment g;
     long long mine = att::request_units<kRows, kMinUnits>(p, r);
@@ -288,7 +291,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     return g;
   };
   auto end_segment = [&](const Segment& g) {
-    if (g.pair) pair_steps += g.steps;
     step += g.steps;
     u += g.k_end - g.k_begin;
     ++segment;
@@ -322,56 +324,62 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           }
           commit(s_full + w);
         };
-        auto output = [&](int w, int n, bool begin) {        // O_w += P_w V of step n
+        auto output = [&](int w, int n, int half, bool begin) {   // O_w += P_w V over half the keys of step n
           uint64_t vd = desc_values(v_at + (uint32_t)(n % S::kStages) * S::kStepBytes, S::kKeys * 128);
-          uint32_t a = tmem + (uint32_t)(w * 128);
+          vd += (uint64_t)(half * S::kKeys * 64 / 16);
           #pragma unroll 1
           for (int q = 0; q < S::kGroups; ++q) {
+            uint32_t a = tmem + (uint32_t)(w * 128 + q * S::kKeys + half * S::kKeys / 2);
+            uint64_t v = vd + (uint64_t)(q * S::kKeys * 128 / 16);
             #pragma unroll 1
-            for (int i = 0; i < S::kKeys / 32; ++i) {        // 32 keys: 16 columns of weights and, with two terms, 16 more
+            for (int i = 0; i < S::kKeys / 64; ++i) {        // 32 keys: 16 columns of weights and, with two terms, 16 more
               #pragma unroll
               for (int h = 0; h < 2; ++h)
                 #pragma unroll
                 for (int e = 0; e < kTerms; ++e)
                   mma_ts(tmem + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
-                                  vd + (uint64_t)(h * 2048 / 16), outputs, begin && i == 0 && h == 0 && e == 0 ? 0u : 1u);
+                         v + (uint64_t)(h * 2048 / 16), outputs, begin && i == 0 && h == 0 && e == 0 ? 0u : 1u);
               a += 32;
-              vd += 2 * 2048 / 16;
+              v += 2 * 2048 / 16;
             }
+          }
+        };
+        // A tile's turn: its weights come in two halves.  The second tile begins when the first has half of its
+        // first weights, so that the two stay half a step apart and neither waits for the other's products.
+        auto turn = [&](int w, int i, int done) {
+          const int n = step + i, next = n + 1;
+          wait(p_ready + 2 * w, done, kDevErrMmaWait);
+          if (w == 0) wait(v_full + n % S::kStages, n / S::kStages, kDevErrMmaWait);
+          gemm::tc_fence_after();
+          output(w, n, 0, i == 0);
+          commit(half_done + w);
+          if (w == 0 && i == 0 && pair) score(1, step);
+          if (i == 0 && w == (pair ? 1 : 0)) commit(k_free + step % S::kStages);
+          wait(p_ready + 2 * w + 1, done, kDevErrMmaWait);
+          gemm::tc_fence_after();
+          output(w, n, 1, false);
+          if (w == (pair ? 1 : 0)) commit(v_free + n % S::kStages);
+          if (i + 1 < steps) {
+            if (w == 0) {
+              wait(k_full + next % S::kStages, next / S::kStages, kDevErrMmaWait);
+              gemm::tc_fence_after();
+            }
+            score(w, next);
+            if (w == (pair ? 1 : 0)) commit(k_free + next % S::kStages);
           }
         };
         wait(k_full + step % S::kStages, step / S::kStages, kDevErrMmaWait);
         gemm::tc_fence_after();
         score(0, step);
-        if (pair) score(1, step);
-        commit(k_free + step % S::kStages);
         for (int i = 0; i < steps; ++i) {
-          const int n = step + i, next = n + 1;
-          wait(p_ready + 0, tile_steps + i, kDevErrMmaWait);
-          wait(v_full + n % S::kStages, n / S::kStages, kDevErrMmaWait);
-          gemm::tc_fence_after();
-          output(0, n, i == 0);
-          if (i + 1 < steps) {
-            wait(k_full + next % S::kStages, next / S::kStages, kDevErrMmaWait);
-            gemm::tc_fence_after();
-            score(0, next);
-          }
-          if (pair) {
-            wait(p_ready + 1, pair_steps + i, kDevErrMmaWait);
-            gemm::tc_fence_after();
-            output(1, n, i == 0);
-          }
-          commit(v_free + n % S::kStages);
-          if (i + 1 < steps) {
-            if (pair) score(1, next);
-            commit(k_free + next % S::kStages);
-          }
+          turn(0, i, step + i);
+          if (pair) turn(1, i, pair_steps + i);
         }
       }
       commit(o_done);
       // nothing of the products is in flight beyond this point, so TMEM can be let go
       wait(o_done, segment, kDevErrMmaWait);
-      tile_steps += steps;
+      if (pair) pair_steps += steps;
       end_segment(g);
     }
   } else if (warp >= kSoftmaxWarps) {
@@ -511,18 +519,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const int token = live ? p.by_group.of(row0 + local) : 0;
       const int qh = head * p.group + (live ? row0 + local - token * p.group : 0);
       const bool active = w == 0 || g.pair;
-      // the row's query into shared memory
+      // the warp's 32 rows of queries into shared memory, neighbouring lanes at neighbouring addresses
       if (active && steps > 0) {
-        const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
-        #pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
+        constexpr int kChunks = D / 8;
+        #pragma unroll 8
+        for (int i = 0; i < kChunks; ++i) {
+          const int at = w * kTileRows + quarter * 32 + (i * 32 + lane) / kChunks, c = lane % kChunks;
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live) {
+          if (at < rows) {
+            const int tok = p.by_group.of(row0 + at), h = head * p.group + row0 + at - tok * p.group;
             const kvc::Chunk k = {c * 8, c * 8 + 4, false};
-            v = kvc::load_chunk(src, k, p.q.vec);
+            v = kvc::load_chunk(static_cast<const T*>(p.q.p) + (long long)(r.q0 + tok) * p.q.token_stride + h * p.q.head_stride,
+                                k, p.q.vec);
           }
-          *reinterpret_cast<uint4*>(sm_q + ((w * S::kAtoms + (c >> 3)) * kTileRows + (local & 127)) * 128 +
-                                    (((c & 7) ^ (local & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(sm_q + ((w * S::kAtoms + (c >> 3)) * kTileRows + (at & 127)) * 128 +
+                                    (((c & 7) ^ (at & 7)) << 4)) = v;
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -533,8 +544,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const uint32_t s_at = tmem + lanes + (uint32_t)(w * 128), o_at = tmem + lanes + (uint32_t)(256 + w * D);
       // Weights are 2^(score - ref), and ref + shift is about the row's maximum: a step's weights are taken with the
-      // reference as it is, and only where a run of them adds up to more than 2^9 of it (an overflow too) does it move,
-      // by a whole number, so that the weights written and the outputs follow exactly.  shift raises them to the
+      // reference as it is, half a step at a time, and only where a half adds up to more than 2^9 of it (an overflow
+      // too) does it move, by a whole number, so that the outputs follow exactly.  shift raises them to the
       // largest value scale seen, weight * scale to at most 2^15.
       float ref = 0.f, sum = 0.f, v_ref = 0.f;
       int shift = 0;
@@ -603,46 +614,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           }
           return fmaxf(a, b);
         };
-        // sum and outputs times 2^by, and the first `runs` runs of this step's weights
-        auto raise = [&](int by, int runs) {
+        // sum and outputs times 2^by
+        auto raise = [&](int by, bool outputs) {
           const float factor = by <= -126 ? 0.f : att::pow2(min(by, 127));
           sum *= factor;
-          gemm::tmem_st_wait();
-          if (i > 0) {
-            #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t x[32], y[16];
-              tmem_ld32(o_at + (uint32_t)(c * 32), x);
-              tmem_wait(x);
-              #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * factor);
-                tmem_st16(o_at + (uint32_t)(c * 32 + 16 * h), y);
-              }
-            }
-          }
-          const uint32_t f2 = kBf16 ? att::pack_b2(factor, factor) : att::pack_h2(factor, factor);
+          if (!outputs) return;
           #pragma unroll 1
-          for (int c = 0; c < runs * (kRun / 32) * S::kGroups; ++c) {     // 32 keys of a group at a time
-            const int in_group = runs * (kRun / 32);
-            const uint32_t at = s_at + (uint32_t)((c / in_group) * S::kKeys + (c % in_group) * 32);
+          for (int c = 0; c < D / 32; ++c) {
             uint32_t x[32], y[16];
-            tmem_ld32(at, x);
+            tmem_ld32(o_at + (uint32_t)(c * 32), x);
             tmem_wait(x);
             #pragma unroll
-            for (int h = 0; h < kTerms; ++h) {
+            for (int h = 0; h < 2; ++h) {
               #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if constexpr (kBf16) {
-                  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[16 * h + e]),
-                                                   *reinterpret_cast<const __nv_bfloat162*>(&f2));
-                  y[e] = *reinterpret_cast<const uint32_t*>(&v);
-                } else {
-                  y[e] = gemm::h2_mul(x[16 * h + e], f2);
-                }
-              }
-              tmem_st16(at + (uint32_t)(16 * h), y);
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * factor);
+              tmem_st16(o_at + (uint32_t)(c * 32 + 16 * h), y);
             }
           }
         };
@@ -652,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           v_ref = e > 127 ? INFINITY : att::pow2(e);
           shift += by;
           ref -= (float)by;
-          raise(by, 0);
+          raise(by, i > 0);
         }
         if (__any_sync(0xffffffffu, !(sum > 0.f))) {                    // rows that have seen nothing yet
           float top = -INFINITY;
@@ -721,7 +707,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             }
             const float top = most(f);
             const int by = over && top < 1e6f ? (int)ceilf(top) : 0;
-            raise(-by, c);
+            if (c > 0) wait(half_done + w, tile_steps + i, kDevErrFullWait);   // the first half is in the outputs
+            gemm::tc_fence_after();
+            raise(-by, i > 0 || c > 0);
             ref += (float)by;
             weigh();
           }
@@ -734,11 +722,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               tmem_st16(at, *reinterpret_cast<const uint32_t(*)[16]>(&hi[q][16 * h]));
               if constexpr (kBf16) tmem_st16(at + 16u, *reinterpret_cast<const uint32_t(*)[16]>(&lo[q][16 * h]));
             }
+          gemm::tmem_st_wait();
+          gemm::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready + 2 * w + c);
         }
-        gemm::tmem_st_wait();
-        gemm::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + w);
       }
       wait(o_done, segment, kDevErrFullWait);
       gemm::tc_fence_after();
@@ -762,6 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       };
       // a part: [reference][sum] of the rows, then runs of 4 outputs of all rows one behind another
       auto park = [&](float* dst, int c, const float (&o)[32], float top, float l) {
+        if (!live) return;
         #pragma unroll
         for (int e = 0; e < 8; ++e)
           *reinterpret_cast<float4*>(dst + 2 * kRows + ((c * 8 + e) * kRows + local) * 4) =
@@ -837,12 +826,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         if (groups > 1) {
           const int n = min(att::kJoin, parts - group * att::kJoin);
           last = arrive(counters + att::kMaxCtas + c_first + group * att::kJoin, n);
-          if (last && active)
+          if (last && live)
             join(group * att::kJoin, 1, n, [&](int c, const float (&o)[32], float top, float l) {
               park(part(group * att::kJoin), c, o, top, l);
             });
         }
-        if (last && arrive(counters + c_first, groups > 1 ? groups : parts) && active)
+        if (last && arrive(counters + c_first, groups > 1 ? groups : parts) && live)
           join(0, groups > 1 ? att::kJoin : 1, groups > 1 ? groups : parts, finish);
       }
       if (active) tile_steps += steps;
