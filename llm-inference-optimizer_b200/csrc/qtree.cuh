@@ -198,7 +198,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   using Slot = typename S::Slot;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   constexpr int kTerms = kBf16 ? 2 : 1;
-  constexpr int kRun = S::kKeys / 2;                         // scores that a softmax thread takes at once
   griddep_launch_dependents();
   griddep_wait();
   extern __shared__ uint8_t smem_raw[];
@@ -394,57 +393,60 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const int row = t / kRowPieces, piece = t % kRowPieces;          // of pieces row + i kRowStep
       const int* pages = p.page_table + b * p.table_stride;
       const int in_page = (1 << kv.page_shift) - 1;
-      auto page_at = [&](int j) { return pages[min(j, r.kv_len - 1) >> kv.page_shift]; };
-      auto usable = [&](int page) { return page >= 0 && page < p.num_pages; };
-      // pages of the next step's pieces and of the thread's scale; codes and scale of the next step
-      int page[S::kPieces], scale_page = 0, block_page = 0;
+      // Lane x looks up the page of keys 16 x .. of a step (one of a page outside the pool becomes 0 and a bit of
+      // `bad`); a piece's page then comes from the lane of its block.
+      constexpr int kBlocks = S::kKeys / 16;
+      int page = 0;
+      unsigned bad = 0, bad_next = 0;
+      auto fetch_pages = [&](int j0) {
+        const int j = j0 + (lane & (kBlocks - 1)) * 16;
+        page = pages[min(j, r.kv_len - 1) >> kv.page_shift];
+        const bool block_bad = page < 0 || page >= p.num_pages;
+        bad_next = __ballot_sync(0xffffffffu, block_bad) & ((1u << kBlocks) - 1u);
+        if (block_bad) {
+          if (j < r.kv_len) atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+          page = 0;
+        }
+      };
       uint4 k_code[S::kPieces], v_code[S::kPieces];
       unsigned short k_scale = 0, v_scale = 0;
-      bool scale_live = false;
-      unsigned bad = 0;
       const int scale_key = t / S::kGroups, scale_group = t % S::kGroups;
-      auto fetch_pages = [&](int j0) {
+      const unsigned char *k_base = kv.k_codes + piece * 16, *v_base = kv.v_codes + piece * 16;
+      const unsigned head_at = (unsigned)head << kv.page_shift;
+      auto fetch = [&](uint4 (&code)[S::kPieces], const unsigned char* from, unsigned stride, int j0) {
         #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) page[i] = page_at(j0 + row + i * kRowStep);
-        scale_page = page_at(j0 + scale_key);
-        block_page = page_at(j0 + min(lane, S::kKeys / 16 - 1) * 16);
-      };
-      auto address = [&](int i, int j0, bool value) -> const uint4* {
-        const unsigned g = usable(page[i]) ? (unsigned)page[i] : 0u;
-        const unsigned at = (head << kv.page_shift) + ((j0 + row + i * kRowStep) & in_page);
-        return reinterpret_cast<const uint4*>((value ? kv.v_codes + (unsigned long long)g * kv.v_page
-                                                     : kv.k_codes + (unsigned long long)g * kv.k_page) +
-                                              (unsigned long long)at * S::kRowBytes + piece * 16);
+        for (int i = 0; i < S::kPieces; ++i) {
+          const unsigned g = (unsigned)__shfl_sync(0xffffffffu, page, i * (kRowStep / 16) + (row >> 4));
+          const unsigned at = head_at + ((j0 + row + i * kRowStep) & in_page);
+          code[i] = *reinterpret_cast<const uint4*>(from + (unsigned long long)g * stride + (unsigned long long)at * S::kRowBytes);
+        }
       };
       auto fetch_keys = [&](int j0) {
-        #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) k_code[i] = *address(i, j0, false);
-        const unsigned g = usable(scale_page) ? (unsigned)scale_page : 0u;
-        const unsigned at = (head << kv.page_shift) + ((j0 + scale_key) & in_page);
-        const unsigned long long sc = (unsigned long long)at * S::kGroups + scale_group;
-        k_scale = kv.k_scales[(unsigned long long)g * kv.ks_page + sc];
-        v_scale = kv.v_scales[(unsigned long long)g * kv.vs_page + sc];
-        scale_live = usable(scale_page) && j0 + scale_key < r.kv_len;
-        const bool block_bad = lane < S::kKeys / 16 && !usable(block_page);
-        bad = __ballot_sync(0xffffffffu, block_bad);
-        if (block_bad && j0 + lane * 16 < r.kv_len) atomicCAS(p.err, 0u, (unsigned)kDevErrBadIndex);
+        bad = bad_next;
+        fetch(k_code, k_base, kv.k_page, j0);
+        const unsigned g = (unsigned)__shfl_sync(0xffffffffu, page, scale_key >> 4);
+        const unsigned at = (head_at + ((j0 + scale_key) & in_page)) * S::kGroups + scale_group;
+        k_scale = kv.k_scales[(unsigned long long)g * kv.ks_page + at];
+        v_scale = kv.v_scales[(unsigned long long)g * kv.vs_page + at];
       };
-      auto fetch_values = [&](int j0) {
-        #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) v_code[i] = *address(i, j0, true);
-      };
+      auto fetch_values = [&](int j0) { fetch(v_code, v_base, kv.v_page, j0); };
+      // Where the thread's first piece goes in a stage: a later one lies kRowStep rows, the same swizzle, further on.
+      // Lanes of the odd atoms begin with the second run of results: eight lanes then write eight different banks.
+      const int flip = BITS == 8 ? piece >> 2 & 1 : 0;
+      uint32_t place[S::kPerPiece / 8];
+      #pragma unroll
+      for (int c = 0; c < S::kPerPiece / 8; ++c) {
+        const int d = piece * S::kPerPiece + (c ^ flip) * 8;
+        place[c] = (uint32_t)((d >> 6) * S::kKeys * 128 + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4));
+      }
       // a piece's elements, 8 to 16 bytes, to their places in a swizzled stage
       auto store = [&](uint8_t* stage, int i, const uint4& code) {
-        const int key = row + i * kRowStep;
         const uint32_t words[4] = {code.x, code.y, code.z, code.w};
-        constexpr int kChunks = S::kPerPiece / 8;                      // 16-byte runs of results
         #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < S::kPerPiece / 8; ++c) {                   // 16-byte runs of results
           uint4 v;
-          // lanes of the odd atoms begin with the second run: eight lanes then write eight different banks
-          const int cc = BITS == 8 ? c ^ (piece >> 2 & 1) : c;
           if constexpr (BITS == 8) {
-            const uint32_t x = cc ? words[2] : words[0], y = cc ? words[3] : words[1];
+            const uint32_t x = c ^ flip ? words[2] : words[0], y = c ^ flip ? words[3] : words[1];
             if constexpr (kBf16) {
               att::dec8_b(x, v.x, v.y);
               att::dec8_b(y, v.z, v.w);
@@ -467,9 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               dec_w4_adjacent(x, v.x, v.y, v.z, v.w);
             }
           }
-          const int d = piece * S::kPerPiece + cc * 8;                 // first element
-          const int chunk = (d & 63) >> 3;
-          *reinterpret_cast<uint4*>(stage + (d >> 6) * S::kKeys * 128 + key * 128 + ((chunk ^ (key & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(stage + place[c] + i * kRowStep * 128) = v;
         }
       };
       if (steps > 0) {
@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         #pragma unroll
         for (int q = 0; q < S::kPieces; ++q) store(sm_k + st * S::kStepBytes, q, k_code[q]);
         Slot& slot = slots[n % S::kSlots];
+        const bool scale_live = j0 + scale_key < r.kv_len && !(bad >> (scale_key >> 4) & 1);
         const float v_sc = scale_live ? kvc::bf16_bits_to_f(v_scale) : 0.f;
         slot.k[scale_group * S::kKeys + scale_key] = scale_live ? kvc::bf16_bits_to_f(k_scale) * p.scale_log2 : 0.f;
         slot.v[scale_group * S::kKeys + scale_key] = v_sc;
@@ -557,31 +558,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         const unsigned bad = slot.bad;
         const bool some_hidden = bad != 0 || j0 + S::kKeys > r.kv_len - r.q_len;
         const float v_top = __uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3])));
-        // the positions of run c that the row sees, as bits
+        // the 32 positions of run c that the row sees, as bits
         auto seen = [&](int c) {
-          unsigned long long see = ~0ull;
-          if (some_hidden) {
-            see = 0;
-            #pragma unroll
-            for (int h = 0; h < kRun / 32; ++h) {
-              unsigned s32 = live ? sees32(p, r, token, j0 + c * kRun + h * 32) : 0u;
-              if (bad >> (c * (kRun / 16) + 2 * h) & 1) s32 &= 0xFFFF0000u;
-              if (bad >> (c * (kRun / 16) + 2 * h + 1) & 1) s32 &= 0x0000FFFFu;
-              see |= (unsigned long long)s32 << (32 * h);
-            }
-          }
+          unsigned see = live ? sees32(p, r, token, j0 + c * 32) : 0u;
+          if (bad >> (2 * c) & 1) see &= 0xFFFF0000u;
+          if (bad >> (2 * c + 1) & 1) see &= 0x0000FFFFu;
           return see;
         };
-        // f = scores of run c less `less`, in units of log2, from sums x (and y of the second group)
-        auto scores = [&](float (&f)[kRun], const uint32_t (&x)[kRun], const uint32_t (&y)[kRun], int c, float less,
-                          unsigned long long see) {
+        // f = the 32 scores of run c less `less`, in units of log2.  (hidden: some of the step's positions are hidden
+        // from some row; always a constant.  Two bodies: a branch around the selections within one becomes as many
+        // predicated ones that every step executes, 30 of 176 us.)
+        auto scores = [&](bool hidden, float (&f)[32], int c, float less, unsigned see) __attribute__((always_inline)) {
+          uint32_t x[32], y[32];
+          tmem_ld32(s_at + (uint32_t)(c * 32), x);
+          if constexpr (S::kGroups > 1) tmem_ld32(s_at + (uint32_t)(S::kKeys + c * 32), y);
+          tmem_wait(x);
+          if constexpr (S::kGroups > 1) tmem_wait(y);
           #pragma unroll
-          for (int e = 0; e < kRun; e += 4) {
-            const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * kRun + e]);
+          for (int e = 0; e < 32; e += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(&slot.k[c * 32 + e]);
             F2 a = fma2({__uint_as_float(x[e]), __uint_as_float(x[e + 1])}, {k.x, k.y}, {-less, -less});
             F2 b = fma2({__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])}, {k.z, k.w}, {-less, -less});
             if constexpr (S::kGroups > 1) {
-              const float4 l = *reinterpret_cast<const float4*>(&slot.k[S::kKeys + c * kRun + e]);
+              const float4 l = *reinterpret_cast<const float4*>(&slot.k[S::kKeys + c * 32 + e]);
               a = fma2({__uint_as_float(y[e]), __uint_as_float(y[e + 1])}, {l.x, l.y}, a);
               b = fma2({__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])}, {l.z, l.w}, b);
             }
@@ -590,29 +589,28 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             f[e + 2] = b.x;
             f[e + 3] = b.y;
           }
-          if (some_hidden) {
+          if (hidden) {
             #pragma unroll
-            for (int e = 0; e < kRun; ++e)
+            for (int e = 0; e < 32; ++e)
               if (!(see >> e & 1)) f[e] = -INFINITY;
           }
         };
-        auto load = [&](uint32_t (&x)[kRun], uint32_t (&y)[kRun], int c) {
-          #pragma unroll
-          for (int h = 0; h < kRun / 32; ++h)
-            tmem_ld32(s_at + (uint32_t)(c * kRun + h * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[32 * h]));
-          if constexpr (S::kGroups > 1) tmem_ld32(s_at + (uint32_t)(S::kKeys + c * kRun), *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
-          #pragma unroll
-          for (int h = 0; h < kRun / 32; ++h) tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&x[32 * h]));
-          if constexpr (S::kGroups > 1) tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&y[0]));
-        };
-        auto most = [](const float (&f)[kRun]) {
-          float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
-          #pragma unroll
-          for (int e = 4; e < kRun; e += 4) {
-            a = fmaxf(a, fmaxf(f[e], f[e + 1]));
-            b = fmaxf(b, fmaxf(f[e + 2], f[e + 3]));
+        // the largest of runs c .. c + n - 1, less `less`
+        auto most = [&](int c, int n, float less) {
+          float top = -INFINITY;
+          #pragma unroll 1
+          for (; n > 0; --n, ++c) {
+            float f[32];
+            scores(true, f, c, less, seen(c));
+            float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
+            #pragma unroll
+            for (int e = 4; e < 32; e += 4) {
+              a = fmaxf(a, fmaxf(f[e], f[e + 1]));
+              b = fmaxf(b, fmaxf(f[e + 2], f[e + 3]));
+            }
+            top = fmaxf(top, fmaxf(a, b));
           }
-          return fmaxf(a, b);
+          return top;
         };
         // sum and outputs times 2^by
         auto raise = [&](int by, bool outputs) {
@@ -641,91 +639,87 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           raise(by, i > 0);
         }
         if (__any_sync(0xffffffffu, !(sum > 0.f))) {                    // rows that have seen nothing yet
-          float top = -INFINITY;
-          #pragma unroll 1
-          for (int c = 0; c < S::kKeys / kRun; ++c) {
-            uint32_t x[kRun], y[kRun];
-            float f[kRun];
-            load(x, y, c);
-            scores(f, x, y, c, 0.f, seen(c));
-            top = fmaxf(top, most(f));
-          }
+          const float top = most(0, S::kKeys / 32, 0.f);
           if (!(sum > 0.f) && top > -INFINITY) ref = top - (float)shift;
         }
-        // the weights, in the place of the scores
-        #pragma unroll 1
-        for (int c = 0; c < S::kKeys / kRun; ++c) {
-          const unsigned long long see = seen(c);
-          float f[kRun], part;
-          uint32_t hi[S::kGroups][kRun / 2], lo[S::kGroups][kRun / 2];
-          auto weigh = [&] {
-            {
-              uint32_t x[kRun], y[kRun];
-              load(x, y, c);
-              scores(f, x, y, c, ref, see);
-            }
+        // the weights of half h, in the place of its scores
+        constexpr int kRuns = S::kKeys / 64;                           // of 32 scores
+        auto weigh_half = [&](bool hidden, int h) __attribute__((always_inline)) {
+          float part;
+          uint32_t hi[kRuns][S::kGroups][16], lo[kRuns][S::kGroups][16];
+          auto weigh = [&]() __attribute__((always_inline)) {
+            F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             #pragma unroll
-            for (int e = 0; e < kRun; ++e) f[e] = att::ex2<kBf16>(f[e]);
-            F2 sums[2] = {{f[0], f[1]}, {f[2], f[3]}};
-            #pragma unroll
-            for (int e = 4; e < kRun; e += 4) {
-              sums[0] = add2(sums[0], {f[e], f[e + 1]});
-              sums[1] = add2(sums[1], {f[e + 2], f[e + 3]});
-            }
-            part = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-            #pragma unroll
-            for (int q = 0; q < S::kGroups; ++q)
+            for (int i32 = 0; i32 < kRuns; ++i32) {
+              const int c = h * kRuns + i32;
+              const unsigned see = hidden ? seen(c) : 0xFFFFFFFFu;
+              float f[32];
+              scores(hidden, f, c, ref, see);
               #pragma unroll
-              for (int e = 0; e < kRun; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(&slot.v[q * S::kKeys + c * kRun + e]);
-                F2 a[2] = {mul2({f[e], f[e + 1]}, {v.x, v.y}), mul2({f[e + 2], f[e + 3]}, {v.z, v.w})};
-                if (some_hidden) {                                     // whatever a hidden value's scale is
-                  if (!(see >> e & 1)) a[0].x = 0.f;
-                  if (!(see >> (e + 1) & 1)) a[0].y = 0.f;
-                  if (!(see >> (e + 2) & 1)) a[1].x = 0.f;
-                  if (!(see >> (e + 3) & 1)) a[1].y = 0.f;
-                }
+              for (int e = 0; e < 32; ++e) f[e] = att::ex2<kBf16>(f[e]);
+              #pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                sums[0] = add2(sums[0], {f[e], f[e + 1]});
+                sums[1] = add2(sums[1], {f[e + 2], f[e + 3]});
+              }
+              #pragma unroll
+              for (int q = 0; q < S::kGroups; ++q)
                 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  if constexpr (kBf16) {
-                    const uint32_t u2 = att::pack_b2(a[h].x, a[h].y);
-                    hi[q][e / 2 + h] = u2;
-                    lo[q][e / 2 + h] = att::pack_b2(a[h].x - __uint_as_float(u2 << 16), a[h].y - __uint_as_float(u2 & 0xFFFF0000u));
-                  } else {
-                    hi[q][e / 2 + h] = att::pack_h2(a[h].x, a[h].y);
+                for (int e = 0; e < 32; e += 4) {
+                  const float4 v = *reinterpret_cast<const float4*>(&slot.v[q * S::kKeys + c * 32 + e]);
+                  F2 a[2] = {mul2({f[e], f[e + 1]}, {v.x, v.y}), mul2({f[e + 2], f[e + 3]}, {v.z, v.w})};
+                  if (hidden) {                                        // whatever a hidden value's scale is
+                    if (!(see >> e & 1)) a[0].x = 0.f;
+                    if (!(see >> (e + 1) & 1)) a[0].y = 0.f;
+                    if (!(see >> (e + 2) & 1)) a[1].x = 0.f;
+                    if (!(see >> (e + 3) & 1)) a[1].y = 0.f;
+                  }
+                  #pragma unroll
+                  for (int g2 = 0; g2 < 2; ++g2) {
+                    if constexpr (kBf16) {
+                      const uint32_t u2 = att::pack_b2(a[g2].x, a[g2].y);
+                      hi[i32][q][e / 2 + g2] = u2;
+                      lo[i32][q][e / 2 + g2] =
+                          att::pack_b2(a[g2].x - __uint_as_float(u2 << 16), a[g2].y - __uint_as_float(u2 & 0xFFFF0000u));
+                    } else {
+                      hi[i32][q][e / 2 + g2] = att::pack_h2(a[g2].x, a[g2].y);
+                    }
                   }
                 }
-              }
+            }
+            part = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
           };
           weigh();
           const bool over = part > att::pow2(min(9 + shift, 126));
-          if (__any_sync(0xffffffffu, over)) {
-            {
-              uint32_t x[kRun], y[kRun];                               // the scores are still there
-              load(x, y, c);
-              scores(f, x, y, c, ref + (float)shift, see);
-            }
-            const float top = most(f);
+          if (__any_sync(0xffffffffu, over)) {                         // the scores are still there
+            const float top = most(h * kRuns, kRuns, ref + (float)shift);
             const int by = over && top < 1e6f ? (int)ceilf(top) : 0;
-            if (c > 0) wait(half_done + w, tile_steps + i, kDevErrFullWait);   // the first half is in the outputs
+            if (h > 0) wait(half_done + w, tile_steps + i, kDevErrFullWait);   // the first half is in the outputs
             gemm::tc_fence_after();
-            raise(-by, i > 0 || c > 0);
+            raise(-by, i > 0 || h > 0);
             ref += (float)by;
             weigh();
           }
           sum += part;
           #pragma unroll
-          for (int q = 0; q < S::kGroups; ++q)
+          for (int i32 = 0; i32 < kRuns; ++i32)
             #pragma unroll
-            for (int h = 0; h < kRun / 32; ++h) {
-              const uint32_t at = s_at + (uint32_t)(q * S::kKeys + c * kRun + h * 32);
-              tmem_st16(at, *reinterpret_cast<const uint32_t(*)[16]>(&hi[q][16 * h]));
-              if constexpr (kBf16) tmem_st16(at + 16u, *reinterpret_cast<const uint32_t(*)[16]>(&lo[q][16 * h]));
+            for (int q = 0; q < S::kGroups; ++q) {
+              const uint32_t at = s_at + (uint32_t)(q * S::kKeys + (h * kRuns + i32) * 32);
+              tmem_st16(at, hi[i32][q]);
+              if constexpr (kBf16) tmem_st16(at + 16u, lo[i32][q]);
             }
           gemm::tmem_st_wait();
           gemm::tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_ready + 2 * w + c);
+          if (lane == 0) mbar_arrive(p_ready + 2 * w + h);
+        };
+        #pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (some_hidden)
+            weigh_half(true, h);
+          else
+            weigh_half(false, h);
         }
       }
       wait(o_done, segment, kDevErrFullWait);
