@@ -178,9 +178,12 @@ int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, i
   }
 }
 
-// Rows of a request under one key/value head from which the tensor-core
-// kernel is taken.
-constexpr int64_t kTreeRows = 32;
+// Rows of a request under one key/value head above which the tensor-core
+// kernel is taken (head_dim 64 and 128; 256 does not fit its memories).
+// 8 requests of up to 6001 positions, 28 heads over 4: with 56 rows the
+// streaming kernel takes 45 us (fp16) and 47 us (bf16), the tensor-core
+// kernel 46 and 57; with 112 rows 66 and 69 against 47 and 59.
+constexpr int64_t kTreeRows = 64;
 
 struct Attention {
   ql::att::Params p;

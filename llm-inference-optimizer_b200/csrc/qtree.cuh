@@ -44,8 +44,6 @@ constexpr int kRows = 2 * kTileRows;
 constexpr int kMinUnits = 4;             // of 128 keys: a part's outputs are worth 512 keys
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kMmaWarp = kSoftmaxWarps + kDecodeWarps;
 constexpr int kThreads = 512;            // the last three warps idle: warpgroups trade registers as a whole
-// Registers a thread, of the 128 that the launch gives each: 8 x 160 + 4 x 112 + 4 x 80 = 16 x 128.
-constexpr int kSoftmaxRegisters = 160, kDecodeRegisters = 112, kMmaRegisters = 80;
 
 template <int D, int BITS>
 struct Shape {
@@ -60,6 +58,11 @@ struct Shape {
   static constexpr int kPieces = kKeys * kRowBytes / 16 / (32 * kDecodeWarps);   // 16-byte runs of codes a thread
   static constexpr int kPerPiece = 128 / BITS;                      // elements
   static constexpr int kColumns = 256 + 2 * D;                      // S_0, S_1, O_0, O_1
+  // Registers a thread, of the 128 that the launch gives each of 16 warps (8 softmax, 4 decode, 4 with the products'):
+  // a softmax thread of one group holds 64 scores, one of two groups 32.
+  static constexpr int kSoftmaxRegisters = kGroups > 1 ? 160 : 176, kDecodeRegisters = kGroups > 1 ? 112 : 96,
+                       kMmaRegisters = kGroups > 1 ? 80 : 64;
+  static_assert(8 * kSoftmaxRegisters + 4 * kDecodeRegisters + 4 * kMmaRegisters <= 16 * 128, "");
   // partial of an item: per row its reference and sum, then D outputs
   static constexpr int kPartial = kRows * (D + 2);
   struct Slot {
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   };
 
   if (warp >= kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kMmaRegisters));
     while (warp == kMmaWarp && u < u_end) {
       // ----------------------------------------------------------- products
       const Segment g = next_segment();
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       end_segment(g);
     }
   } else if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kDecodeRegisters));
     while (u < u_end) {
       // -------------------------------------------------------------- decode
       const Segment g = next_segment();
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       end_segment(g);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegisters));
     while (u < u_end) {
       // ------------------------------------------------------------- softmax
       const Segment g = next_segment();
