@@ -300,11 +300,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
 
   if (warp >= kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kMmaRegisters));
-    while (warp == kMmaWarp && u < u_end) {
+    // what the products' operands depend on, as values that the compiler knows to be the whole warp's
+    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const uint32_t tmem_u = (uint32_t)uniform((int)tmem);
+    int done = 0;                                            // steps before the segment
+    while (warp == kMmaWarp && uniform(u < u_end)) {
       // ----------------------------------------------------------- products
       const Segment g = next_segment();
-      const int steps = g.steps;
-      const bool pair = g.pair;
+      const int steps = uniform(g.steps);
+      const bool pair = uniform(g.pair) != 0;
       wait(q_ready, segment, kDevErrMmaWait);
       gemm::tc_fence_after();
       if (steps > 0) {
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         auto score = [&](int w, int n) {                     // S_w of step n
           uint64_t qd = gemm::desc_sw128(q_at + (uint32_t)(w * S::kAtoms * kTileRows * 128));
           uint64_t kd = gemm::desc_sw128(k_at + (uint32_t)(n % S::kStages) * S::kStepBytes);
-          uint32_t d = tmem + (uint32_t)(w * 128);
+          uint32_t d = tmem_u + (uint32_t)(w * 128);
           #pragma unroll 1
           for (int a = 0; a < S::kAtoms; ++a) {
             #pragma unroll
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           vd += (uint64_t)(half * S::kKeys * 64 / 16);
           #pragma unroll 1
           for (int q = 0; q < S::kGroups; ++q) {
-            uint32_t a = tmem + (uint32_t)(w * 128 + q * S::kKeys + half * S::kKeys / 2);
+            uint32_t a = tmem_u + (uint32_t)(w * 128 + q * S::kKeys + half * S::kKeys / 2);
             uint64_t v = vd + (uint64_t)(q * S::kKeys * 128 / 16);
             #pragma unroll 1
             for (int i = 0; i < S::kKeys / 64; ++i) {        // 32 keys: 16 columns of weights and, with two terms, 16 more
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               for (int h = 0; h < 2; ++h)
                 #pragma unroll
                 for (int e = 0; e < kTerms; ++e)
-                  mma_ts(tmem + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
+                  mma_ts(tmem_u + (uint32_t)(256 + w * D + q * 64), a + (uint32_t)(h * 8 + e * 16),
                          v + (uint64_t)(h * 2048 / 16), outputs, begin && i == 0 && h == 0 && e == 0 ? 0u : 1u);
               a += 32;
               v += 2 * 2048 / 16;
@@ -348,16 +352,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         };
         // A tile's turn: its weights come in two halves.  The second tile begins when the first has half of its
         // first weights, so that the two stay half a step apart and neither waits for the other's products.
-        auto turn = [&](int w, int i, int done) {
-          const int n = step + i, next = n + 1;
-          wait(p_ready + 2 * w, done, kDevErrMmaWait);
+        auto turn = [&](int w, int i, int uses) {
+          const int n = done + i, next = n + 1;
+          wait(p_ready + 2 * w, uses, kDevErrMmaWait);
           if (w == 0) wait(v_full + n % S::kStages, n / S::kStages, kDevErrMmaWait);
           gemm::tc_fence_after();
           output(w, n, 0, i == 0);
           commit(half_done + w);
-          if (w == 0 && i == 0 && pair) score(1, step);
-          if (i == 0 && w == (pair ? 1 : 0)) commit(k_free + step % S::kStages);
-          wait(p_ready + 2 * w + 1, done, kDevErrMmaWait);
+          if (w == 0 && i == 0 && pair) score(1, done);
+          if (i == 0 && w == (pair ? 1 : 0)) commit(k_free + done % S::kStages);
+          wait(p_ready + 2 * w + 1, uses, kDevErrMmaWait);
           gemm::tc_fence_after();
           output(w, n, 1, false);
           if (w == (pair ? 1 : 0)) commit(v_free + n % S::kStages);
@@ -370,11 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             if (w == (pair ? 1 : 0)) commit(k_free + next % S::kStages);
           }
         };
-        wait(k_full + step % S::kStages, step / S::kStages, kDevErrMmaWait);
+        wait(k_full + done % S::kStages, done / S::kStages, kDevErrMmaWait);
         gemm::tc_fence_after();
-        score(0, step);
+        score(0, done);
         for (int i = 0; i < steps; ++i) {
-          turn(0, i, step + i);
+          turn(0, i, done + i);
           if (pair) turn(1, i, pair_steps + i);
         }
       }
@@ -382,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       // nothing of the products is in flight beyond this point, so TMEM can be let go
       wait(o_done, segment, kDevErrMmaWait);
       if (pair) pair_steps += steps;
+      done += steps;
       end_segment(g);
     }
   } else if (warp >= kSoftmaxWarps) {
