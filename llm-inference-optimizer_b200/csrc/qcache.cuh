@@ -290,7 +290,11 @@ struct AppendParams {
 // inv = 1 / s: rne(x / s) without a division.  x inv is within 2^-22 of x / s
 // relatively, 2^-15 where codes can differ (below 128), so it rounds alike
 // unless it is that close to half way between two codes; those few elements
-// are divided.  Adding 1.5 * 2^23 leaves the rounded integer in the low bits.
+// are divided.  A row whose scale is below 2^-125 comes with inv = infinity and
+// is divided whole: there bf16 can round the scale far down, and only the clamp
+// keeps its codes in range.  A larger scale is a normal number, rounded to 8
+// bits: at least max|x| / top * (1 - 2^-8), so x / s is below top + 1/2 and
+// needs no clamp.  Adding 1.5 * 2^23 leaves the rounded integer in the low bits.
 template <int BITS>
 __device__ __forceinline__ unsigned quantise4(const float (&f)[4], float s, float inv) {
   constexpr float kRound = 12582912.f;
@@ -299,7 +303,7 @@ __device__ __forceinline__ unsigned quantise4(const float (&f)[4], float s, floa
   bool close = !(inv < INFINITY);
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float y = fminf(fmaxf(__fmul_rn(f[i], inv), -top), top);
+    const float y = __fmul_rn(f[i], inv);
     const float r = __fadd_rn(y, kRound);
     q[i] = __float_as_uint(r);
     close |= fabsf(__fsub_rn(y, __fsub_rn(r, kRound))) > 0.5f - 0x1p-14f;

@@ -131,6 +131,17 @@ def activation_code(dtype: torch.dtype, what: str) -> int:
 current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_call_flags: int | None = None
+
+
+def call_flags() -> int:
+    """default_flags, read once: looking at the environment costs as much as an eighth of a launch."""
+    global _call_flags
+    if _call_flags is None:
+        _call_flags = default_flags()
+    return _call_flags
+
+
 def call(entry, packed: bytes, device: torch.device) -> None:
     """entry(packed arguments, current stream) with `device` current (the ABI uses the current device)."""
     index = device.index

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._launch import activation_code, call, default_flags, index_bytes
+from ._launch import activation_code, call, call_flags, index_bytes
 from .rotary import RotaryTable
 
 GROUP4 = 64                     # elements that share a scale at 4 bits
@@ -149,7 +149,7 @@ def append_kv(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: 
     packed = _lib.KV_APPEND_ARGS.pack(
         *cache.fields, k.data_ptr(), v.data_ptr(), q_ptr, q_out_ptr, slots.data_ptr(), table, position_ptr, tokens,
         q_heads, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], code, index_bytes(slots, "slots"),
-        *turn, default_flags())
+        *turn, call_flags())
     call(_lib.load().ql_kv_append, packed, dev)
     return q_out
 
@@ -168,7 +168,7 @@ def read_kv(cache: QuantizedKVCache, slots: torch.Tensor,
     if not slots.is_contiguous():
         slots = slots.contiguous()
     packed = _lib.KV_READ_ARGS.pack(*cache.fields, slots.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, code,
-                                    index_bytes(slots, "slots"), default_flags())
+                                    index_bytes(slots, "slots"), call_flags())
     call(_lib.load().ql_kv_read, packed, dev)
     return k, v
 

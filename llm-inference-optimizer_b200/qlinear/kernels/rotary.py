@@ -14,7 +14,7 @@ import math
 import torch
 
 from .. import _lib
-from ._launch import activation_code, call, default_flags, index_bytes
+from ._launch import activation_code, call, call_flags, index_bytes
 
 LAYOUTS = {"half": _lib.QL_ROTARY_HALF, "interleaved": _lib.QL_ROTARY_INTERLEAVED}
 
@@ -151,7 +151,7 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     packed = _lib.ROTARY_ARGS.pack(
         x.data_ptr(), out.data_ptr(), rotary.ptr, positions.data_ptr(), tokens, heads, head_dim, rotary.rotary_dim,
         rotary.max_positions, xs[0], xs[1], os_[0], os_[1], dtype, rotary.layout_code,
-        index_bytes(positions, "positions"), 1 if inverse else 0, default_flags())
+        index_bytes(positions, "positions"), 1 if inverse else 0, call_flags())
     call(_lib.load().ql_rotary, packed, dev)
     return out
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._launch import activation_code, call, current_raw_stream, default_flags, on_device, scratch
+from ._launch import activation_code, call, current_raw_stream, call_flags, on_device, scratch
 from .kv_cache import QuantizedKVCache
 
 
@@ -132,7 +132,7 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
             *cache.fields, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(),
             kv_lens.data_ptr(), cu_ptr, mask_ptr, batch, total_q, q_heads, qs[0], qs[1], width,
             ts[0] if batch > 1 else width, words, max_q, max_kv, code,
-            head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), default_flags())
+            head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), call_flags())
         call(_lib.load().ql_tree_attention, packed, dev)
     return (out, lse) if return_lse else out
 
