@@ -432,7 +432,9 @@ int ql_kv_read(const ql_kv_read_args* args, void* stream);
  * Rows that cu_q does not cover are not written.  kv_lens is clamped to the
  * table; a page outside the pool hides its keys and records
  * QL_DEVICE_ERROR_BAD_INDEX.  max_q and max_kv bound the requests' tokens and
- * lengths and only choose the launch.
+ * lengths and only choose the launch.  flags: QL_FLAG_FORCE_GEMM (the
+ * tensor-core kernel for any number of rows, where head_dim is 64 or 128) and
+ * QL_FLAG_FORCE_GEMV (the streaming kernel) are test hooks.
  * q_heads is a multiple of kv_heads; query head h reads key/value head
  * h / (q_heads / kv_heads).
  *   workspace: ql_tree_attention_workspace_size(head_dim) bytes of the current

@@ -338,6 +338,12 @@ __host__ __device__ constexpr int step_add(int drow, int dchunk) {
 // A key's scale is read by its own lanes; hidden keys are removed by
 // selection, never by multiplication, so what unused rows of a page hold
 // does not matter.
+//
+// 64 requests of 4100 to 8192 positions, one token, 32 heads over 8 of 128, 8
+// bits: 129 us, 5.8 TB/s, 89 % of a plain copy.  At 4 bits half the bytes want
+// as many instructions (about 400 per warp and tile of 16 keys), which bound
+// it: one token over 130001 positions, 28 heads over 4: 30 us, of which the
+// tiles take 18, the rest being a CTA's start and the joining of parts.
 template <int D, int BITS, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;

@@ -178,12 +178,20 @@ int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, i
   }
 }
 
-// Rows of a request under one key/value head above which the tensor-core
-// kernel is taken (head_dim 64 and 128; 256 does not fit its memories).
-// 8 requests of up to 6001 positions, 28 heads over 4: with 56 rows the
-// streaming kernel takes 45 us (fp16) and 47 us (bf16), the tensor-core
-// kernel 46 and 57; with 112 rows 66 and 69 against 47 and 59.
-constexpr int64_t kTreeRows = 64;
+// The tensor-core kernel (head_dim 64 and 128; 256 does not fit its memories)
+// is taken above kTreeRows rows of a request under one key/value head, where
+// the streaming kernel would have kTreeWork units of work a CTA and more: units
+// of 128 keys by 16 rows, an item's start and end counted as kItemWork of them.
+// Below, the tensor-core kernel's start and end (22 us) outweigh its rate.
+// 32 heads over 4 of 128, 8 bits, fp16 / bf16, us, streaming | tensor-core:
+//   8 requests of up to 6001, 64 rows:    45 / 47 | 46 / 56
+//                            128 rows:    75 / 78 | 47 / 58
+//   16 requests of up to 600, 72 rows:    34 / 36 | 24 / 29    (28 units)
+//   1 request of 16001,      128 rows:    46 / 48 | 45 / 50    (29 units)
+//   2 requests of up to 3001, 256 rows:   34 / 36 | 38 / 45    (27.7 units)
+//   4 requests of up to 1500, 128 rows:   25 / 27 | 26 / 32    (17 units)
+//   1 request of 600,        512 rows:    22 / 23 | 30 / 36    (11 units)
+constexpr int64_t kTreeRows = 64, kTreeWork = 28, kItemWork = 8;
 
 struct Attention {
   ql::att::Params p;
@@ -246,7 +254,10 @@ int run_tree(const Attention& a) {
 template <typename T, int D, int BITS>
 int run_rows(const Attention& a) {
   if constexpr (D <= 128) {
-    if (a.max_q * a.p.group > kTreeRows) return run_tree<T, D, BITS>(a);
+    const int64_t rows = a.max_q * a.p.group, units = cdiv(a.max_kv, ql::att::kUnitKeys) + kItemWork;
+    const double work = (double)a.p.batch * a.p.cache.heads * (double)cdiv(rows, 16) * (double)units;
+    const bool tree = rows > kTreeRows && work >= (double)(kTreeWork * a.sms);
+    if (!(a.flags & QL_FLAG_FORCE_GEMV) && (tree || (a.flags & QL_FLAG_FORCE_GEMM))) return run_tree<T, D, BITS>(a);
   }
   return a.max_q * a.p.group <= 8 ? run_stream<T, D, BITS, 1>(a) : run_stream<T, D, BITS, 2>(a);
 }
