@@ -8,6 +8,7 @@
 // A row that sees nothing gives zeros and a log-sum of minus infinity.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "qcache.cuh"
@@ -339,11 +340,13 @@ __host__ __device__ constexpr int step_add(int drow, int dchunk) {
 // selection, never by multiplication, so what unused rows of a page hold
 // does not matter.
 //
-// 64 requests of 4100 to 8192 positions, one token, 32 heads over 8 of 128, 8
-// bits: 129 us, 5.8 TB/s, 89 % of a plain copy.  At 4 bits half the bytes want
-// as many instructions (about 400 per warp and tile of 16 keys), which bound
-// it: one token over 130001 positions, 28 heads over 4: 30 us, of which the
-// tiles take 18, the rest being a CTA's start and the joining of parts.
+// 64 requests of 3152 to 8192 positions, one token, 32 heads over 8 of 128, 8
+// bits: 129 us, 5.9 TB/s, 90 % of a plain copy's rate.  Repeated for seconds,
+// that draws the GPU's 1000 W; the SM clock falls from 1965 to about 1700 MHz
+// and the time rises to 147.  At 4 bits half the bytes want as many
+// instructions (about 400 per warp and tile of 16 keys), which bound it: one
+// token over 130001 positions, 28 heads over 4: 31 us, of which the tiles take
+// 18, the rest being a CTA's start and the joining of parts.
 template <int D, int BITS, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
@@ -360,7 +363,12 @@ struct Shape {
   static constexpr int kTileBytes = 16 * kRowBytes, kScaleBytes = 16 * kGroups * 2;
   static constexpr int kStageBytes = (2 * (kTileBytes + kScaleBytes) + 127) / 128 * 128;
   static constexpr int kBudget = (kCtas == 2 ? 108 : 216) * 1024;
-  static constexpr int kStages = kBudget / (kWarps * kStageBytes) < 6 ? kBudget / (kWarps * kStageBytes) : 6;
+  // Stages: as many as keep 64 KB on the way to an SM while one is worked on, no more than fit or than 6.  Deeper
+  // rings only lengthen the queues (8 bits and head_dim 128, 3 stages: 130.4 us against 128.6 with 2); at 4 bits and
+  // head_dim 64, 2 stages are too few (30.6 against 30.2).
+  static constexpr int kAll = kCtas * kWarps * kStageBytes, kFit = kBudget / (kWarps * kStageBytes);
+  static constexpr int kWant = std::min(1 + (64 * 1024 + kAll - 1) / kAll, 6);
+  static constexpr int kStages = std::min(kFit, kWant);
   static_assert(kStages >= 2 && 4 * kGroups <= 32, "");
   static constexpr size_t kRing = (size_t)kWarps * kStages * kStageBytes;
   // rows of the warps to be joined take the ring's place; their stride puts the rows that a quarter warp writes
