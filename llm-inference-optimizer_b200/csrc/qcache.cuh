@@ -133,9 +133,12 @@ __device__ __forceinline__ void store_chunk(T* row, const float (&a)[4], const f
 struct Angles {
   float4 u, w;
 };
-__device__ __forceinline__ Angles load_angles(const float2* angles, int c) {
+// The inverse's sines are negative: exact, so that the products need not know.
+__device__ __forceinline__ Angles load_angles(const float2* angles, int c, int inverse) {
   const float4* p = reinterpret_cast<const float4*>(angles + 4 * c);
-  return {__ldg(p), __ldg(p + 1)};
+  Angles t = {__ldg(p), __ldg(p + 1)};
+  if (inverse) t = {{t.u.x, -t.u.y, t.u.z, -t.u.w}, {t.w.x, -t.w.y, t.w.z, -t.w.w}};
+  return t;
 }
 
 __device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s) {
@@ -144,21 +147,27 @@ __device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s
   x1 = y1;
   x2 = y2;
 }
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn_chunk(float (&a)[4], float (&b)[4], const Angles& t) {
+  if (INTERLEAVED) {
+    turn_pair(a[0], a[1], t.u.x, t.u.y);
+    turn_pair(a[2], a[3], t.u.z, t.u.w);
+    turn_pair(b[0], b[1], t.w.x, t.w.y);
+    turn_pair(b[2], b[3], t.w.z, t.w.w);
+  } else {
+    turn_pair(a[0], b[0], t.u.x, t.u.y);
+    turn_pair(a[1], b[1], t.u.z, t.u.w);
+    turn_pair(a[2], b[2], t.w.x, t.w.y);
+    turn_pair(a[3], b[3], t.w.z, t.w.w);
+  }
+}
 __device__ __forceinline__ void turn_chunk(float (&a)[4], float (&b)[4], const Angles& t, const Chunk& k,
                                            const Turn& turn) {
   if (!k.turns) return;
-  const float m = turn.inverse ? -1.f : 1.f;
-  if (turn.interleaved) {
-    turn_pair(a[0], a[1], t.u.x, m * t.u.y);
-    turn_pair(a[2], a[3], t.u.z, m * t.u.w);
-    turn_pair(b[0], b[1], t.w.x, m * t.w.y);
-    turn_pair(b[2], b[3], t.w.z, m * t.w.w);
-  } else {
-    turn_pair(a[0], b[0], t.u.x, m * t.u.y);
-    turn_pair(a[1], b[1], t.u.z, m * t.u.w);
-    turn_pair(a[2], b[2], t.w.x, m * t.w.y);
-    turn_pair(a[3], b[3], t.w.z, m * t.w.w);
-  }
+  if (turn.interleaved)
+    turn_chunk<true>(a, b, t);
+  else
+    turn_chunk<false>(a, b, t);
 }
 template <typename T>
 __device__ __forceinline__ void widen(float (&a)[4], float (&b)[4], const uint4& r) {
@@ -219,37 +228,76 @@ struct RotaryParams {
   int tokens, heads;
   unsigned* err;
 };
-template <typename T>
-__device__ __forceinline__ void rotate_heads(const RotaryParams& p, int cta) {
-  const Place at = place_of(p.grid, cta, p.tokens);
-  if (at.token < 0) return;
-  const Chunk k = chunk_of(at.c, p.turn, true);
+// WHOLE_HALF: half layout, whole heads, 16-byte aligned rows; the questions
+// that each head of the general body asks are then settled.  By this body and
+// by the general one, 16384 tokens of 32 heads of 128: 45.7 us, 49.3; of 64
+// heads of 64: 47.8, 48.9; 4096 of 40 heads of 256: 35.3, 34.4; an append of
+// 8192 x (32 + 8 + 8) x 128: 44.1, 46.5.  For what else there is, bodies of
+// their own lost: interleaved 50.9 against 49.8, a part of the heads (where a
+// warp's chunks differ) 5.5 against 4.5.
+template <typename T, bool WHOLE_HALF>
+__device__ __forceinline__ void rotate_rows(const RotaryParams& p, const Place& at) {
+  const Chunk k = WHOLE_HALF ? Chunk{4 * at.c, 4 * (p.grid.chunks + at.c), true} : chunk_of(at.c, p.turn, true);
   const long long x_step = p.grid.beside * p.x.head_stride, out_step = p.grid.beside * p.out.head_stride;
   const T* x = static_cast<const T*>(p.x.p) + at.token * p.x.token_stride + at.head * p.x.head_stride;
   T* out = static_cast<T*>(const_cast<void*>(p.out.p)) + at.token * p.out.token_stride + at.head * p.out.head_stride;
   const long long position = load_index(p.turn.positions, at.token, p.turn.wide);
   Angles angles = {};
+  auto load = [&](const T* row) {
+    if (!WHOLE_HALF) return load_chunk(row, k, p.x.vec);
+    const uint2 a = *reinterpret_cast<const uint2*>(row + k.oa), b = *reinterpret_cast<const uint2*>(row + k.ob);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  };
+  auto turn_and_store = [&](T* row, const uint4& raw) {
+    float a[4], b[4];
+    widen<T>(a, b, raw);
+    if (WHOLE_HALF)
+      turn_chunk<false>(a, b, angles);
+    else
+      turn_chunk(a, b, angles, k, p.turn);
+    if (WHOLE_HALF) {
+      *reinterpret_cast<uint2*>(row + k.oa) = make_uint2(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]));
+      *reinterpret_cast<uint2*>(row + k.ob) = make_uint2(pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3]));
+    } else {
+      store_chunk(row, a, b, k, p.out.vec);
+    }
+  };
   for (int h = at.head; h < p.heads; h += kHeads * p.grid.beside) {
+    const bool all = WHOLE_HALF && h + (kHeads - 1) * p.grid.beside < p.heads;
     uint4 raw[kHeads];
-    #pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (h + i * p.grid.beside < p.heads) raw[i] = load_chunk(x + i * x_step, k, p.x.vec);
-    if (h == at.head && k.turns) angles = load_angles(angles_of(p.turn, position, p.err), at.c);
-    #pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (h + i * p.grid.beside < p.heads) {
-        float a[4], b[4];
-        widen<T>(a, b, raw[i]);
-        turn_chunk(a, b, angles, k, p.turn);
-        store_chunk(out + i * out_step, a, b, k, p.out.vec);
-      }
+    if (all) {
+      #pragma unroll
+      for (int i = 0; i < kHeads; ++i) raw[i] = load(x + i * x_step);
+    } else {
+      #pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (h + i * p.grid.beside < p.heads) raw[i] = load(x + i * x_step);
+    }
+    if (h == at.head && k.turns) angles = load_angles(angles_of(p.turn, position, p.err), at.c, p.turn.inverse);
+    if (all) {
+      #pragma unroll
+      for (int i = 0; i < kHeads; ++i) turn_and_store(out + i * out_step, raw[i]);
+    } else {
+      #pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (h + i * p.grid.beside < p.heads) turn_and_store(out + i * out_step, raw[i]);
+    }
     x += kHeads * x_step;
     out += kHeads * out_step;
   }
 }
+template <typename T>
+__device__ __forceinline__ void rotate_heads(const RotaryParams& p, int cta) {
+  const Place at = place_of(p.grid, cta, p.tokens);
+  if (at.token < 0) return;
+  if (p.x.vec && p.out.vec && !p.turn.interleaved && p.turn.rotary_dim == 8 * p.grid.chunks)
+    rotate_rows<T, true>(p, at);
+  else
+    rotate_rows<T, false>(p, at);
+}
 // Bound by reading and writing the heads once.  16384 tokens of 32 heads of
-// 128 (277 MB with the angles): 51 us in the half layout, 50 interleaved, 5.4
-// and 5.6 TB/s, where a plain copy reaches 6.5; one token: 1.8 us, a launch.
+// 128 (277 MB with the angles): 46 us in the half layout, 48 interleaved, 6.1
+// and 5.8 TB/s, where a plain copy reaches 6.5; one token: 1.8 us, a launch.
 template <typename T>
 __global__ void __launch_bounds__(256, 5) rotary_kernel(const RotaryParams p) {
   griddep_launch_dependents();
@@ -379,7 +427,7 @@ __device__ __forceinline__ void store_row(const RowAt& dst, const float (&a)[4],
 // the queries' CTAs instead, those of keys and values gain 1 % at 8192 tokens
 // and lose 3 % at 2501.  Queries are bound by memory; keys and values by the
 // instructions that a code takes.  8192 tokens, 32 + 8 + 8 heads of 128, fp16:
-// 47 us at 8 bits (4.0 TB/s) and 50 at 4; without queries 22 us (2.5 TB/s).
+// 44 us at 8 bits (4.3 TB/s) and 47 at 4; without queries 21.5 us (2.6 TB/s).
 template <typename T, int LANES, int BITS>
 __global__ void __launch_bounds__(256, 4) append_kernel(const AppendParams p) {
   griddep_launch_dependents();
@@ -401,7 +449,7 @@ __global__ void __launch_bounds__(256, 4) append_kernel(const AppendParams p) {
     const uint4 k_raw = load_chunk(static_cast<const T*>(p.k.p) + token * p.k.token_stride + h * p.k.head_stride, turned, p.k.vec);
     const uint4 v_raw = load_chunk(static_cast<const T*>(p.v.p) + token * p.v.token_stride + h * p.v.head_stride, straight, p.v.vec);
     if (first == 0) {
-      if (turned.turns) angles = load_angles(angles_of(turn, position, p.q.err), at.c);
+      if (turned.turns) angles = load_angles(angles_of(turn, position, p.q.err), at.c, turn.inverse);
       if (at.token < 0) slot = -1;
       if (slot >= kv.slots) {
         atomicCAS(p.q.err, 0u, (unsigned)kDevErrBadIndex);
