@@ -42,6 +42,7 @@ def workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> t
 
 
 _scratches: dict[tuple[int, int], torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []   # captured graphs may hold their addresses; at most one a head_dim and stream
 _SCRATCH_HEADER = 8192           # ql_tree_attention's counters
 
 
@@ -59,6 +60,8 @@ def scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
         with _ws_lock:
             buf = _scratches.get(key)
             if buf is None or buf.numel() < nbytes:
+                if buf is not None:
+                    _outgrown.append(buf)
                 buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
                 _scratches[key] = buf
     return buf
