@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "qcache.cuh"
+#include "qwork.h"
 
 namespace ql {
 namespace att {
@@ -57,32 +58,11 @@ __device__ __forceinline__ bool sees(const Params& p, const Request& r, int i, i
 }
 
 // ------------------------------------------------------------ work of a launch
-// Work is counted in units of 128 keys of one item: one request, one
-// key/value head, one tile of ROWS = 8 NT rows (row r of a request is new
-// token r / group under query head r % group of the key/value head).  Items
-// lie one behind another, each rounded up to a multiple of kMinUnits, and
-// the CTAs take equal runs of units, whatever the requests' lengths are: a
-// CTA may end one item, do some whole and begin another.  Lengths are read
-// on the device, so a captured launch serves other lengths later.
+// qwork.h says how it is divided; a tile has ROWS = 8 NT rows here.
 constexpr float kLow = -1e30f;             // the maximum of nothing: below every score, and finite
-constexpr int kUnitKeys = 128;
 constexpr int kWarps = kUnitKeys / 16;     // a warp takes 16 keys of every unit
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMinUnits = 2;               // units worth a CTA of their own: 256 keys
-constexpr int kJoin = 16;                  // parts of an item that are joined at once
-constexpr int kMaxCtas = 1024;
-constexpr int kHeaderBytes = 2 * 4 * kMaxCtas;   // counters of items and of groups of parts
-
-struct Work {
-  long long total;     // units of the launch
-  int ctas;            // CTAs that take part
-  __device__ long long first_unit(int cta) const { return quotient(total * cta, ctas); }
-  __device__ int cta_of(long long u) const { return (int)quotient((u + 1) * ctas - 1, total); }
-  // of non-negative numbers, by the short division where it does (nearly always)
-  static __device__ long long quotient(long long a, long long b) {
-    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
-  }
-};
 
 template <int MIN_UNITS>
 __device__ __forceinline__ int item_units(const Request& r) {
@@ -902,14 +882,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     }
 
     if (!whole) {
-      // The item's parts, one a CTA, are joined by its last CTA.  Many parts
-      // are joined in groups of kJoin first, each by its last CTA, so that no
-      // CTA reads more than a few dozen: with 74 parts a single one took
-      // longer than the keys had.
-      const int c_first = work.cta_of(item_begin), parts = work.cta_of(item_begin + per_item - 1) - c_first + 1;
-      const int groups = (parts + kJoin - 1) / kJoin, me = (int)blockIdx.x - c_first, group = me / kJoin;
+      const Join j = join_of(work, item_begin, per_item, (int)blockIdx.x);
       auto part = [&](int q) {                          // the first begins the item: its CTA's second slot
-        return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
+        return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * S::kPartial;
       };
       auto arrive = [&](unsigned* counter, int n) {     // true in the last of n CTAs, which sees the others' parts
         __threadfence();
@@ -951,16 +926,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         }
       };
       bool last = true;
-      if (groups > 1) {
-        const int n = min(kJoin, parts - group * kJoin);
-        last = arrive(counters + kMaxCtas + c_first + group * kJoin, n);
+      if (j.grouped()) {
+        last = arrive(counters + j.group_counter(), j.group_parts);
         if (last)
-          join(group * kJoin, 1, n, [&](int row, int d, const float4& o, float top, float sum) {
-            park(part(group * kJoin), row, d, o, top, sum);   // read by this thread alone; the row's m and l are in shared memory
+          join(j.group * kJoin, 1, j.group_parts, [&](int row, int d, const float4& o, float top, float sum) {
+            park(part(j.group * kJoin), row, d, o, top, sum);   // read by this thread alone; the row's m and l are in shared memory
           });
       }
-      if (last && arrive(counters + c_first, groups > 1 ? groups : parts))
-        join(0, groups > 1 ? kJoin : 1, groups > 1 ? groups : parts, finish);
+      if (last && arrive(counters + j.item_counter(), j.item_arrivals()))
+        join(0, j.groups > 1 ? kJoin : 1, j.item_arrivals(), finish);
     }
     __syncthreads();                                    // before the next segment reuses shared memory
     u += k_end - k_begin;

@@ -789,10 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         }
       }
       if (!whole) {
-        const int c_first = work.cta_of(item_begin), parts = work.cta_of(item_begin + per_item - 1) - c_first + 1;
-        const int groups = (parts + att::kJoin - 1) / att::kJoin, me = (int)blockIdx.x - c_first, group = me / att::kJoin;
+        const att::Join j = att::join_of(work, item_begin, per_item, (int)blockIdx.x);
         auto part = [&](int q) {                            // the first begins the item: its CTA's second slot
-          return partials + (long long)(2 * (c_first + q) + (q == 0)) * S::kPartial;
+          return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * S::kPartial;
         };
         auto arrive = [&](unsigned* counter, int n) {       // true in the last of n CTAs, which sees the others' parts
           __threadfence();
@@ -833,16 +832,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           }
         };
         bool last = true;
-        if (groups > 1) {
-          const int n = min(att::kJoin, parts - group * att::kJoin);
-          last = arrive(counters + att::kMaxCtas + c_first + group * att::kJoin, n);
+        if (j.grouped()) {
+          last = arrive(counters + j.group_counter(), j.group_parts);
           if (last && live)
-            join(group * att::kJoin, 1, n, [&](int c, const float (&o)[32], float top, float l) {
-              park(part(group * att::kJoin), c, o, top, l);
+            join(j.group * att::kJoin, 1, j.group_parts, [&](int c, const float (&o)[32], float top, float l) {
+              park(part(j.group * att::kJoin), c, o, top, l);
             });
         }
-        if (last && arrive(counters + c_first, groups > 1 ? groups : parts) && live)
-          join(0, groups > 1 ? att::kJoin : 1, groups > 1 ? groups : parts, finish);
+        if (last && arrive(counters + j.item_counter(), j.item_arrivals()) && live)
+          join(0, j.groups > 1 ? att::kJoin : 1, j.item_arrivals(), finish);
       }
       if (active) tile_steps += steps;
       end_segment(g);
