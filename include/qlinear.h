@@ -386,7 +386,8 @@ typedef struct {
 /*
  * Writes k[t, h] and v[t, h] to slot slots[t] of every head.  With rotary_dim
  * > 0, k is turned first (in fp32, unrounded) and, with q_heads > 0, q is
- * turned into q_out (which may be q).  A slot of -1 (any negative) writes
+ * turned into q_out (which may be q); q_heads > 0 without rotary_dim is
+ * QL_ERR_BAD_SHAPE.  A slot of -1 (any negative) writes
  * nothing, but its q is turned; one past the pool writes nothing and records
  * QL_DEVICE_ERROR_BAD_INDEX.  Two tokens with one slot leave either's row or
  * a mixture of both.

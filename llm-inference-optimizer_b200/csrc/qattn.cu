@@ -317,6 +317,7 @@ int ql_kv_append(const ql_kv_append_args* a, void* stream) {
   if (a->q_heads > 0) {
     if ((st = make_rows(&p.q.x, a->q, a->q_token_stride, a->q_head_stride, d)) != QL_OK) return st;
     if ((st = make_rows(&p.q.out, a->q_out, a->q_out_token_stride, a->q_out_head_stride, d)) != QL_OK) return st;
+    if (a->rotary_dim == 0) return QL_ERR_BAD_SHAPE;   // q is there to be turned: no angles, no positions
   }
   if (a->rotary_dim != 0) {
     st = make_turn(&p.q.turn, a->table, a->positions, a->position_bytes, a->max_positions, a->rotary_dim, d, a->layout,

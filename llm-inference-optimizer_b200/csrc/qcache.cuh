@@ -241,7 +241,7 @@ __device__ __forceinline__ void rotate_rows(const RotaryParams& p, const Place& 
   const long long x_step = p.grid.beside * p.x.head_stride, out_step = p.grid.beside * p.out.head_stride;
   const T* x = static_cast<const T*>(p.x.p) + at.token * p.x.token_stride + at.head * p.x.head_stride;
   T* out = static_cast<T*>(const_cast<void*>(p.out.p)) + at.token * p.out.token_stride + at.head * p.out.head_stride;
-  const long long position = load_index(p.turn.positions, at.token, p.turn.wide);
+  const long long position = k.turns ? load_index(p.turn.positions, at.token, p.turn.wide) : 0;
   Angles angles = {};
   auto load = [&](const T* row) {
     if (!WHOLE_HALF) return load_chunk(row, k, p.x.vec);
@@ -328,7 +328,7 @@ __device__ __forceinline__ RowAt row_at(const Pool& c, long long slot, int head,
 }
 
 struct AppendParams {
-  RotaryParams q;          // the queries, whose turn is the keys' too (rotary_dim 0: nothing turns)
+  RotaryParams q;          // the queries, whose turn is the keys' too (rotary_dim 0: no key turns, and there are no queries)
   Pool cache;
   Rows k, v;
   Grid grid;               // of the keys and values

@@ -101,6 +101,15 @@ def test_host_checks_without_gpu():
     assert lib.ql_kv_read(None, None) == _lib.QL_ERR_NULL_POINTER
 
 
+def test_queries_without_a_rotation_are_refused():
+    """q_heads > 0 with rotary_dim 0 has neither angles nor positions: refused before any launch."""
+    c, _ = cache_fields()
+    args = dict(k=64, v=64, q=64, q_out=64, slots=64, table=0, positions=0, tokens=2, q_heads=2, kt=128, kh=64, vt=128,
+                vh=64, qt=128, qh=64, ot=128, oh=64, dtype=_lib.QL_DTYPE_F16, slot_bytes=8, rotary_dim=0,
+                max_positions=0, layout=0, position_bytes=8, flags=0)
+    assert _lib.load().ql_kv_append(_lib.KV_APPEND_ARGS.pack(*c, *args.values()), None) == _lib.QL_ERR_BAD_SHAPE
+
+
 # ----------------------------------------------------------------------- GPU
 def stored(cache, slots):
     page, at = slots // cache.page_size, slots % cache.page_size
