@@ -440,7 +440,8 @@ int ql_kv_read(const ql_kv_read_args* args, void* stream);
  * h / (q_heads / kv_heads).
  *   workspace: ql_tree_attention_workspace_size(head_dim) bytes of the current
  *   device, 16-byte aligned, zeroed before its first use (a call leaves what
- *   the next one needs zero); calls that share one must not overlap.
+ *   the next one needs zero); calls that share one must not overlap, nor a
+ *   captured graph's replays with either.
  */
 typedef struct {
   ql_kv_cache cache;
@@ -454,6 +455,10 @@ typedef struct {
   int64_t workspace_bytes, flags;
 } ql_tree_attention_args;
 size_t ql_tree_attention_workspace_size(int64_t head_dim);
+/* The capture that records what is launched on `stream`, a number of its own
+ * for each; 0 while none does.  A graph's workspace has to be the graph's own
+ * (cleared in the graph): a replay may overlap later calls on the stream. */
+uint64_t ql_capture_id(void* stream);
 int ql_tree_attention(const ql_tree_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------- diagnostics */

@@ -410,6 +410,16 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
                                   : run_attention<__nv_bfloat16>(work, a->cache.head_dim);
 }
 
+uint64_t ql_capture_id(void* stream) {
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 size_t ql_tree_attention_workspace_size(int64_t head_dim) {
   ql_host::Device dev;
   if (ql_host::current(&dev) != QL_OK) return 0;

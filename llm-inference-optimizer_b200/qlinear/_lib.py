@@ -104,6 +104,7 @@ SIGNATURES = {
     "ql_kv_append": (_int, [ctypes.c_char_p, _vp]),
     "ql_kv_read": (_int, [ctypes.c_char_p, _vp]),
     "ql_tree_attention_workspace_size": (_sz, [_i64]),
+    "ql_capture_id": (ctypes.c_uint64, [_vp]),
     "ql_tree_attention": (_int, [ctypes.c_char_p, _vp]),
     "ql_strerror": (ctypes.c_char_p, [_int]),
     "ql_version": (_int, []),

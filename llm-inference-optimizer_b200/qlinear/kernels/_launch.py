@@ -42,28 +42,45 @@ def workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> t
 
 
 _scratches: dict[tuple[int, int], torch.Tensor] = {}
-_outgrown: list[torch.Tensor] = []   # captured graphs may hold their addresses; at most one a head_dim and stream
+_graph_scratches: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 _SCRATCH_HEADER = 8192           # ql_tree_attention's counters
+
+
+# Without the checks of torch.cuda's own: there are CUDA tensors by then.
+current_device = torch._C._cuda_getDevice
+is_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
+def capture_id(device: torch.device, stream: int) -> int:
+    """The capture that records what is launched on `stream` of `device`, or 0."""
+    if current_device() == device.index:
+        return _lib.load().ql_capture_id(stream) if is_capturing() else 0    # eager calls end here
+    with on_device(device):
+        return _lib.load().ql_capture_id(stream)
 
 
 def scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch whose head alone is kept zero by the kernels, one per (device,
-    stream handle) as `workspace`.  A stream that has none while it is being
-    captured gets one of the graph's own, whose head the graph clears."""
+    stream handle) as `workspace`, and one for each capture on it: a graph is
+    replayed on any stream, beside other graphs and later calls, so it shares
+    none.  Its first call clears the head at every replay.  `nbytes` is the
+    same on every call."""
     key = (device.index, stream)
-    buf = _scratches.get(key)
-    if buf is None or buf.numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    capture = capture_id(device, stream)
+    if capture:
+        held = _graph_scratches.get(key)
+        if held is None or held[0] != capture:
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)     # of the graph's memory pool
             buf[:_SCRATCH_HEADER].zero_()
-            return buf
+            # held so that nothing else that is captured gets this memory; the last capture's goes back to its pool
+            held = _graph_scratches[key] = (capture, buf)
+        return held[1]
+    buf = _scratches.get(key)
+    if buf is None:
         with _ws_lock:
             buf = _scratches.get(key)
-            if buf is None or buf.numel() < nbytes:
-                if buf is not None:
-                    _outgrown.append(buf)
-                buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-                _scratches[key] = buf
+            if buf is None:
+                buf = _scratches[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return buf
 
 
@@ -148,7 +165,7 @@ def call_flags() -> int:
 def call(entry, packed: bytes, device: torch.device) -> None:
     """entry(packed arguments, current stream) with `device` current (the ABI uses the current device)."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if current_device() == index:
         status = entry(packed, current_raw_stream(index))
     else:
         with on_device(device):

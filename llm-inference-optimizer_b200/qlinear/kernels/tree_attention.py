@@ -14,15 +14,15 @@ from ._launch import activation_code, call, current_raw_stream, call_flags, on_d
 from .kv_cache import QuantizedKVCache
 
 
-_workspace_bytes: dict[tuple[int, int], int] = {}
+_workspace_bytes: dict[int, int] = {}
 
 
-def _workspace(device: torch.device, head_dim: int) -> torch.Tensor:
-    nbytes = _workspace_bytes.get((device.index, head_dim))
+def _workspace(device: torch.device) -> torch.Tensor:
+    nbytes = _workspace_bytes.get(device.index)
     if nbytes is None:
-        with on_device(device):
-            nbytes = _lib.load().ql_tree_attention_workspace_size(head_dim)
-        _workspace_bytes[device.index, head_dim] = nbytes
+        with on_device(device):                      # what the largest head needs, so that no call outgrows it
+            nbytes = max(_lib.load().ql_tree_attention_workspace_size(d) for d in (64, 128, 256))
+        _workspace_bytes[device.index] = nbytes
     return scratch(device, current_raw_stream(device.index), nbytes)
 
 
@@ -127,7 +127,7 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
             ts = page_table.stride()
         if max_kv is None:
             max_kv = width * cache.page_size
-        ws = _workspace(dev, head_dim)
+        ws = _workspace(dev)
         packed = _lib.TREE_ATTENTION_ARGS.pack(
             *cache.fields, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(),
             kv_lens.data_ptr(), cu_ptr, mask_ptr, batch, total_q, q_heads, qs[0], qs[1], width,

@@ -45,3 +45,36 @@ def test_small_scratch_is_refused(monkeypatch):
         tree_attention(heads(1, 4, 64, torch.float16, 4), QuantizedKVCache(*random_cache(2, 16, 2, 64, 8, 5)),
                        torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"),
                        torch.tensor([20], dtype=torch.int32, device="cuda"))
+
+
+def test_graphs_have_scratch_of_their_own():
+    """A graph captured on a stream that has scratch, another captured after it there, and eager calls on that stream,
+    all at once: their scratch is apart, and each gives the bits that it gives alone."""
+    stream, aside = torch.cuda.Stream(), torch.cuda.Stream()
+    cache = QuantizedKVCache(*random_cache(626, 64, 2, 128, 8, 6))
+    lens = torch.tensor([40000], dtype=torch.int32, device="cuda")
+    table = torch.arange(626, dtype=torch.int32, device="cuda")[None]
+    qs = [heads(3, 4, 128, torch.float16, s) for s in (7, 8, 9)]
+    key = (torch.cuda.current_device(), stream.cuda_stream)
+    torch.cuda.synchronize()
+    graphs, outs, buffers = [], [], []
+    with torch.cuda.stream(stream):
+        want = [tree_attention(q, cache, table, lens) for q in qs]
+        buffers.append(_launch._scratches[key].data_ptr())
+        for q in qs[1:]:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                outs.append([tree_attention(q, cache, table, lens) for _ in range(3)])
+                buffers.append(_launch._graph_scratches[key][1].data_ptr())
+    torch.cuda.synchronize()
+    assert len(set(buffers)) == 3
+    for _ in range(20):
+        with torch.cuda.stream(aside):
+            graphs[0].replay()
+        graphs[1].replay()
+        with torch.cuda.stream(stream):
+            got = [tree_attention(qs[0], cache, table, lens) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[0]) for g in got)
+    for out, w in zip(outs, want[1:]):
+        assert all(torch.equal(o, w) for o in out)
