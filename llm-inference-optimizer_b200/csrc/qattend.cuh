@@ -692,10 +692,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             const bool fresh = !(__ballot_sync(0xffffffffu, l[n][x] > 0.f) & lanes);   // it has seen nothing yet
             float keep = 1.f;
             if (top > 4.f || (fresh && top > -INFINITY)) {
-              const float moved = m[n][x] + top, by = moved - m[n][x];
+              // rounded down, so that the row's largest weight is 1 at least; scores of 2^25 and more, which m follows
+              // in steps of more than 4, are then held to 4
+              const float moved = __fadd_rd(m[n][x], top), by = __fsub_rd(moved, m[n][x]);
               m[n][x] = moved;
-              d[n][x] -= by;
-              d[n][2 + x] -= by;
+              #pragma unroll
+              for (int e = x; e < 4; e += 2) {
+                const float less = d[n][e] - by;
+                d[n][e] = less > 4.f ? 4.f : less;
+              }
               keep = fresh ? 1.f : ex2<kBf16>(-by);
             } else if (fresh) {
               open = true;

@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const uint32_t s_at = tmem + lanes + (uint32_t)(w * 128), o_at = tmem + lanes + (uint32_t)(256 + w * D);
       // Weights are 2^(score - ref), and ref + shift is about the row's maximum: a step's weights are taken with the
       // reference as it is, half a step at a time, and only where a half adds up to more than 2^9 of it (an overflow
-      // too) does it move, by a whole number, so that the outputs follow exactly.  shift raises them to the
+      // too) does it move, by a whole number where it can, so that the outputs follow exactly.  shift raises them to the
       // largest value scale seen, weight * scale to at most 2^15.
       float ref = 0.f, sum = 0.f, v_ref = 0.f;
       int shift = 0;
@@ -629,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           return top;
         };
         // sum and outputs times 2^by
-        auto raise = [&](int by, bool outputs) {
-          const float factor = by <= -126 ? 0.f : att::pow2(min(by, 127));
+        auto raise = [&](float by, bool outputs) {
+          const float factor = by <= -126.f ? 0.f : att::ex2<false>(by);
           sum *= factor;
           if (!outputs) return;
           #pragma unroll 1
@@ -652,18 +652,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           v_ref = e > 127 ? INFINITY : att::pow2(e);
           shift += by;
           ref -= (float)by;
-          raise(by, i > 0);
+          raise((float)by, i > 0);
         }
         if (__any_sync(0xffffffffu, !(sum > 0.f))) {                    // rows that have seen nothing yet
           const float top = most(0, S::kKeys / 32, 0.f);
-          if (!(sum > 0.f) && top > -INFINITY) ref = top - (float)shift;
+          // (rounded down: a score of 2^23 and more that came out too high would leave its row without weight)
+          if (!(sum > 0.f) && top > -INFINITY) ref = top - (float)shift - fabsf(top) * 0x1p-22f;
         }
         // the weights of half h, in the place of its scores
         constexpr int kRuns = S::kKeys / 64;                           // of 32 scores
         auto weigh_half = [&](bool hidden, int h) __attribute__((always_inline)) {
           float part;
           uint32_t hi[kRuns][S::kGroups][16], lo[kRuns][S::kGroups][16];
-          auto weigh = [&]() __attribute__((always_inline)) {
+          auto weigh = [&](bool moved) __attribute__((always_inline)) {
+            const float cap = (float)(9 + shift);
             F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             #pragma unroll
             for (int i32 = 0; i32 < kRuns; ++i32) {
@@ -671,6 +673,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               const unsigned see = hidden ? seen(c) : 0xFFFFFFFFu;
               float f[32];
               scores(hidden, f, c, ref, see);
+              if (moved) {                                             // what the reference cannot follow (below)
+                #pragma unroll
+                for (int e = 0; e < 32; ++e) f[e] = f[e] > cap ? cap : f[e];
+              }
               #pragma unroll
               for (int e = 0; e < 32; ++e) f[e] = att::ex2<kBf16>(f[e]);
               #pragma unroll
@@ -705,16 +711,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             }
             part = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
           };
-          weigh();
+          weigh(false);
           const bool over = part > att::pow2(min(9 + shift, 126));
           if (__any_sync(0xffffffffu, over)) {                         // the scores are still there
             const float top = most(h * kRuns, kRuns, ref + (float)shift);
-            const int by = over && top < 1e6f ? (int)ceilf(top) : 0;
+            // A reference of 2^23 and more has no room for whole numbers.  It then stays below the largest score by
+            // what the two may be off, and weights beyond the cap, of scores equal to the last bits, become the cap's.
+            const float by_most = over && top < INFINITY ? ceilf(top - (fabsf(ref) + top) * 0x1p-22f) : 0.f;
+            const float moved = __fadd_rd(ref, fmaxf(by_most, 0.f)), by = moved - ref;
             if (h > 0) wait(half_done + w, tile_steps + i, kDevErrFullWait);   // the first half is in the outputs
             gemm::tc_fence_after();
             raise(-by, i > 0 || h > 0);
-            ref += (float)by;
-            weigh();
+            ref = moved;
+            weigh(true);
           }
           sum += part;
           #pragma unroll

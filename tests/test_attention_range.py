@@ -1,0 +1,57 @@
+"""Attention at the ends of the range: scores very far apart, value scales of
+very different sizes, queries with a few large elements; each kernel forced."""
+import sys
+
+import pytest
+import torch
+
+from qlinear import _lib
+from qlinear.kernels.tree_attention import tree_attention
+
+from attn_helpers import HALF_ULP, values
+from test_tree_attention import Problem
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="requires a CUDA GPU")]
+
+
+@pytest.fixture(autouse=True, params=["tensor cores", "streaming"])
+def family(request, monkeypatch):
+    force = _lib.QL_FLAG_FORCE_GEMM if request.param == "tensor cores" else _lib.QL_FLAG_FORCE_GEMV
+    monkeypatch.setattr(sys.modules[tree_attention.__module__], "call_flags", lambda: _lib.QL_FLAG_PDL | force)
+    return request.param
+
+
+def cached(p, b):
+    """Keys and values of request b in float64, [positions, heads, head_dim]."""
+    c, n = p.cache, p.lens[b]
+    pages = p.table[b, :-(-n // c.page_size)].long()
+    return [values(x[pages], s[pages], p.bits).transpose(1, 2).flatten(0, 1)[:n]
+            for x, s in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales))]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("scale", [1.0e5, -3.0e7])
+def test_scores_that_pass_one_another_by_millions(scale, bits, dtype):
+    """The softmax picks one position: its value, rounded once.  A score is off by 2^-20 of the sum of its products'
+    sizes at most (attention_bounds), so a winner that leads by 8 times that and 20 more is the kernel's too, and what
+    the others weigh, e^-20 each of 1500, is under 2^-18 of the value scales' largest."""
+    p = Problem([5, 40], [700, 1500], 12, 2, 128, bits, 16, dtype, seed=31)
+    out, _ = p.run(scale=scale)
+    assert bool(torch.isfinite(out).all())
+    at = checked = 0
+    for b, (t, n) in enumerate(zip(p.q_lens, p.lens)):
+        k, v = cached(p, b)
+        q = p.q[at:at + t].double().unflatten(1, (2, 6))
+        s = torch.einsum("thgd,nhd->thgn", q, k) * scale
+        size = torch.einsum("thgd,nhd->thgn", q.abs(), k.abs()).amax(-1) * abs(scale)
+        see = torch.arange(n, device="cuda")[None] <= torch.arange(n - t, n, device="cuda")[:, None]
+        two, who = s.masked_fill(~see[:, None, None], -torch.inf).topk(2, dim=-1)
+        sure = two[..., 0] - two[..., 1] > 8 * 2.0 ** -20 * size + 20
+        want = v[who[..., 0], torch.arange(2, device="cuda")[None, :, None]]
+        tol = HALF_ULP[dtype] * want.abs() + 2.0 ** -18 * v.abs().max() + 2.0 ** -11 * want.abs()
+        off = (out[at:at + t].double().unflatten(1, (2, 6)) - want).abs()
+        assert bool((off <= tol).all(-1)[sure].all())
+        checked += int(sure.sum())
+        at += t
+    assert checked > 0.9 * sum(p.q_lens) * 12
