@@ -647,9 +647,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           }
         };
         if (v_top > v_ref) {                                           // the same in all rows
-          const int e = max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -60);    // 2^e >= v_top
+          // 2^e >= v_top, but e no further from the rest than fp32 can follow: shift moves by 2^122 at most.  Scales
+          // beyond have room all the same: under 2^-32 no fp16 output shows them, and in bf16 weights have fp32's range.
+          const int e = min(max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -32), 90);
           const int by = 6 - e - shift;
-          v_ref = e > 127 ? INFINITY : att::pow2(e);
+          v_ref = e == 90 ? INFINITY : att::pow2(e);
           shift += by;
           ref -= (float)by;
           raise((float)by, i > 0);

@@ -55,3 +55,15 @@ def test_scores_that_pass_one_another_by_millions(scale, bits, dtype):
         checked += int(sure.sum())
         at += t
     assert checked > 0.9 * sum(p.q_lens) * 12
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("low,high", [(-70, 100), (-20, 110), (-100, 10)])
+def test_value_scales_from_one_end_to_the_other(low, high, q_len, bits):
+    """bf16 values near the least and then near the greatest: all positions count in the softmax's sum."""
+    p = Problem([q_len], [900], 4, 2, 128, bits, 16, torch.bfloat16, seed=32)
+    c = p.cache
+    for j in range(900):
+        c.v_scales[p.table[0, j // 16].long(), :, j % 16] *= 2.0 ** (low if j < 500 else high)
+    p.check(p.run())
