@@ -75,6 +75,7 @@ struct Shape {
   static constexpr int kPartial = kRows * (D + 2);
   struct Slot {
     float k[128], v[128];                                           // [group][key]
+    float v_log[kKeys];                                             // log2 of a key's largest value scale (kLeast .. kMost)
     unsigned v_top[4];                                              // largest finite value scales
     unsigned bad;                                                   // bit i: keys 16 i .. are in no page
     unsigned pad[3];
@@ -82,6 +83,13 @@ struct Shape {
   static constexpr size_t kSmem = 1024 + kQBytes + 2 * (size_t)kStages * kStepBytes + kSlots * sizeof(Slot) + 512;
   static_assert(kKeys % 64 == 0 && kPieces >= 1 && kPieces * kPerPiece * 32 * kDecodeWarps == kKeys * D, "");
 };
+
+// Where log2 of a value scale ends, so that fp32 follows a row from one end to
+// the other.  No fp16 output shows what is below; above, the products have
+// room in bf16 (2^(kAim + 61) at most, and sums of 2^21 times 127 of them).
+constexpr float kLeast = -32.f, kMost = 60.f;
+// log2 of the weight times scale that a row's reference is put at, and of the most that it may come to.
+constexpr float kAim = 6.f, kCap = 15.f;
 
 // The products and their commits, by one elected lane of a whole warp in
 // uniform control flow: the operands then stay in uniform registers, where a
@@ -505,6 +513,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         const float v_sc = scale_live ? kvc::bf16_bits_to_f(v_scale) : 0.f;
         slot.k[scale_group * S::kKeys + scale_key] = scale_live ? kvc::bf16_bits_to_f(k_scale) * p.scale_log2 : 0.f;
         slot.v[scale_group * S::kKeys + scale_key] = v_sc;
+        // zero, negative or not finite: as the least
+        float v_log = v_sc > 0.f && v_sc < INFINITY ? fminf(fmaxf(log2f(v_sc), kLeast), kMost) : kLeast;
+        #pragma unroll
+        for (int o = 1; o < S::kGroups; o <<= 1) v_log = fmaxf(v_log, __shfl_xor_sync(0xffffffffu, v_log, o));
+        if (scale_group == 0) slot.v_log[scale_key] = v_log;
         const unsigned bits = __float_as_uint(v_sc);
         const unsigned top = __reduce_max_sync(0xffffffffu, bits < 0x7F800000u ? bits : 0u);
         if (lane == 0) slot.v_top[t >> 5] = top;
@@ -560,12 +573,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
 
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const uint32_t s_at = tmem + lanes + (uint32_t)(w * 128), o_at = tmem + lanes + (uint32_t)(256 + w * D);
-      // Weights are 2^(score - ref), and ref + shift is about the row's maximum: a step's weights are taken with the
-      // reference as it is, half a step at a time, and only where a half adds up to more than 2^9 of it (an overflow
-      // too) does it move, by a whole number where it can, so that the outputs follow exactly.  shift raises them to the
-      // largest value scale seen, weight * scale to at most 2^15.
-      float ref = 0.f, sum = 0.f, v_ref = 0.f;
-      int shift = 0;
+      // Weights are 2^(score - ref).  What is multiplied is a weight times its value's scale, and ref is put where the
+      // row's largest such product is 2^kAim, so that in fp16 it is the small ones beside it that lose bits, whatever the
+      // scales are.  A step's weights are taken with the reference as it is, half a step at a time, and only where a
+      // product could pass 2^kCap (an overflow too) does it move, by a whole number where it can, so that the outputs
+      // follow exactly.  (At 4 bits a key's groups share its weight: one whose scales are all 2^-20 of the other's and
+      // less loses bits in fp16.)
+      float ref = 0.f, sum = 0.f;
       for (int i = 0; i < steps && active; ++i) {
         const int n = step + i, j0 = j_begin + i * S::kKeys;
         const Slot& slot = slots[n % S::kSlots];
@@ -573,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         gemm::tc_fence_after();
         const unsigned bad = slot.bad;
         const bool some_hidden = bad != 0 || j0 + S::kKeys > r.kv_len - r.q_len;
-        const float v_top = __uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3])));
+        const float v_top = fminf(fmaxf(__uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3]))),
+                                        att::pow2((int)kLeast)), att::pow2((int)kMost));
         // the 32 positions of run c that the row sees, as bits
         auto seen = [&](int c) {
           unsigned see = live ? sees32(p, r, token, j0 + c * 32) : 0u;
@@ -611,13 +626,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               if (!(see >> e & 1)) f[e] = -INFINITY;
           }
         };
-        // the largest of runs c .. c + n - 1, less `less`
+        // log2 of the largest weight times value scale of runs c .. c + n - 1, less `less`
         auto most = [&](int c, int n, float less) {
           float top = -INFINITY;
           #pragma unroll 1
           for (; n > 0; --n, ++c) {
             float f[32];
             scores(true, f, c, less, seen(c));
+            #pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(&slot.v_log[c * 32 + e]);
+              f[e] += v.x;
+              f[e + 1] += v.y;
+              f[e + 2] += v.z;
+              f[e + 3] += v.w;
+            }
             float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
             #pragma unroll
             for (int e = 4; e < 32; e += 4) {
@@ -628,10 +651,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           }
           return top;
         };
-        // sum and outputs times 2^by
-        auto raise = [&](float by, bool outputs) {
-          const float factor = by <= -126.f ? 0.f : att::ex2<false>(by);
-          sum *= factor;
+        // sum and outputs times 2^by, by <= 0, in two factors: what is left may be a normal number where 2^by is none
+        auto lower = [&](float by, bool outputs) {
+          const float f0 = att::ex2<false>(fmaxf(by, -100.f)), f1 = att::ex2<false>(fminf(by + 100.f, 0.f));
+          sum = sum * f0 * f1;
           if (!outputs) return;
           #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -641,25 +664,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
               #pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * factor);
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[16 * h + e]) * f0 * f1);
               tmem_st16(o_at + (uint32_t)(c * 32 + 16 * h), y);
             }
           }
         };
-        if (v_top > v_ref) {                                           // the same in all rows
-          // 2^e >= v_top, but e no further from the rest than fp32 can follow: shift moves by 2^122 at most.  Scales
-          // beyond have room all the same: under 2^-32 no fp16 output shows them, and in bf16 weights have fp32's range.
-          const int e = min(max((int)((__float_as_uint(v_top) + 0x007FFFFFu) >> 23) - 127, -32), 90);
-          const int by = 6 - e - shift;
-          v_ref = e == 90 ? INFINITY : att::pow2(e);
-          shift += by;
-          ref -= (float)by;
-          raise((float)by, i > 0);
-        }
-        if (__any_sync(0xffffffffu, !(sum > 0.f))) {                    // rows that have seen nothing yet
+        if (__any_sync(0xffffffffu, live && !(sum > 0.f))) {            // rows that have seen nothing yet
           const float top = most(0, S::kKeys / 32, 0.f);
           // (rounded down: a score of 2^23 and more that came out too high would leave its row without weight)
-          if (!(sum > 0.f) && top > -INFINITY) ref = top - (float)shift - fabsf(top) * 0x1p-22f;
+          if (!(sum > 0.f) && top > -INFINITY) ref = top - kAim - fabsf(top) * 0x1p-22f;
         }
         // the weights of half h, in the place of its scores
         constexpr int kRuns = S::kKeys / 64;                           // of 32 scores
@@ -667,7 +680,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
           float part;
           uint32_t hi[kRuns][S::kGroups][16], lo[kRuns][S::kGroups][16];
           auto weigh = [&](bool moved) __attribute__((always_inline)) {
-            const float cap = (float)(9 + shift);
             F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             #pragma unroll
             for (int i32 = 0; i32 < kRuns; ++i32) {
@@ -677,7 +689,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
               scores(hidden, f, c, ref, see);
               if (moved) {                                             // what the reference cannot follow (below)
                 #pragma unroll
-                for (int e = 0; e < 32; ++e) f[e] = f[e] > cap ? cap : f[e];
+                for (int e = 0; e < 32; ++e) {
+                  const float cap = kCap - slot.v_log[c * 32 + e];
+                  f[e] = f[e] > cap ? cap : f[e];
+                }
               }
               #pragma unroll
               for (int e = 0; e < 32; ++e) f[e] = att::ex2<kBf16>(f[e]);
@@ -714,16 +729,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             part = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
           };
           weigh(false);
-          const bool over = part > att::pow2(min(9 + shift, 126));
+          const bool over = part * v_top > att::pow2((int)kCap);
           if (__any_sync(0xffffffffu, over)) {                         // the scores are still there
-            const float top = most(h * kRuns, kRuns, ref + (float)shift);
-            // A reference of 2^23 and more has no room for whole numbers.  It then stays below the largest score by
-            // what the two may be off, and weights beyond the cap, of scores equal to the last bits, become the cap's.
-            const float by_most = over && top < INFINITY ? ceilf(top - (fabsf(ref) + top) * 0x1p-22f) : 0.f;
+            const float top = most(h * kRuns, kRuns, ref);
+            // A reference of 2^23 and more has no room for whole numbers.  It then stays below the largest product by
+            // what the two may be off, and what is beyond the cap, of scores equal to the last bits, becomes the cap's.
+            const float by_most = over && top < INFINITY ? ceilf(top - kAim - (fabsf(ref) + fabsf(top)) * 0x1p-22f) : 0.f;
             const float moved = __fadd_rd(ref, fmaxf(by_most, 0.f)), by = moved - ref;
             if (h > 0) wait(half_done + w, tile_steps + i, kDevErrFullWait);   // the first half is in the outputs
             gemm::tc_fence_after();
-            raise(-by, i > 0 || h > 0);
+            lower(-by, i > 0 || h > 0);
             ref = moved;
             weigh(true);
           }

@@ -67,3 +67,42 @@ def test_value_scales_from_one_end_to_the_other(low, high, q_len, bits):
     for j in range(900):
         c.v_scales[p.table[0, j // 16].long(), :, j % 16] *= 2.0 ** (low if j < 500 else high)
     p.check(p.run())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("kind,large,down", [("spread", 8, 20), ("first", 8, 20), ("late", 8, 20), ("late", 13, 24),
+                                             ("unseen", 8, 20)])
+def test_fp16_values_far_below_the_largest(kind, large, down, q_len, bits):
+    """Value scales from 2^-20 to 1 of the largest, at random; and one position that takes nearly all of every row's
+    weight and holds values 2^-20 or 2^-24 as large as the others': the first one, a late one, and beside large values that
+    most rows do not see (the new tokens' own)."""
+    n = 900
+    p = Problem([q_len], [n], 4, 2, 128, bits, 16, torch.float16, seed=33)
+    c = p.cache
+    g = torch.Generator().manual_seed(34)
+
+    def row(t, j):
+        return t[p.table[0, j // 16].long(), :, j % 16]
+
+    if kind == "spread":
+        for j in range(n):
+            row(c.v_scales, j).mul_(2.0 ** (large - down * float(torch.rand((), generator=g))))
+        p.check(p.run())
+        return
+    for j in range(n):
+        row(c.v_scales, j).mul_(2.0 ** large)
+    at = {"first": 3, "late": 777, "unseen": 3}[kind]
+    # q and the key at `at` have one sign, so that its score leads by far: about 70 beside 1.5 a standard deviation
+    p.q.abs_()
+    row(c.k_codes, at).fill_(100 if bits == 8 else 0xEE)
+    row(c.k_scales, at).fill_(0.05 if bits == 8 else 0.8)
+    row(c.v_scales, at).mul_(2.0 ** -down)
+    if kind == "unseen":
+        for j in range(n - q_len, n):
+            row(c.v_scales, j).mul_(64.0)
+        for j in range(n - q_len):
+            if j != at:
+                row(c.v_scales, j).mul_(2.0 ** -down)
+    out, lse = p.run()
+    p.check((out, lse))
