@@ -304,8 +304,10 @@ __host__ __device__ constexpr int step_add(int drow, int dchunk) {
 //     an eighth of head_dim; pairs of keys are joined by byte permutes, and
 //     the order of d within a tile of 16 is free (it only names the outputs).
 // The codes enter as exact fp16 integers.  Key scales multiply the scores
-// afterwards; bf16 queries become fp16 by a power of two per row (their 8
-// significant bits fit).  Value scales multiply the weights, which are rounded
+// afterwards; bf16 queries become fp16 by a power of two per row (8 significant
+// bits fit, down to 2^-32 of the row's largest element; a bf16 body for rows
+// that reach further, as one with a branch or as two, made every bf16 call 1 to
+// 5 % slower).  Value scales multiply the weights, which are rounded
 // to fp16 once, against a power of two that follows the largest scale seen.
 // A tile with a weight below fp16's normal range (or a hidden key) takes the
 // product in bf16 instead, the weights as a sum of two: 16 bits and fp32's
@@ -498,7 +500,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
       if constexpr (kBf16) {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = top >= 0x7F800000u ? 0 : min(max((int)(top >> 23) - 127, -126), 126);
+        // the row's largest element to 2^15 .. 2^16: what is 2^-32 of it and more keeps its 8 bits, subnormals too
+        const int e = top >= 0x7F800000u ? 0 : max((int)(top >> 23) - 127 - 15, -126);
         down = pow2(-e);
         up = pow2(e);
       }

@@ -106,3 +106,20 @@ def test_fp16_values_far_below_the_largest(kind, large, down, q_len, bits):
                 row(c.v_scales, j).mul_(2.0 ** -down)
     out, lse = p.run()
     p.check((out, lse))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("up", [12, 20])
+def test_bf16_queries_with_a_few_large_elements(up, q_len, bits):
+    """Two elements of every query 2^up times the others', where keys are zero: the others' bits decide.  (Elements keep
+    theirs down to 2^-32 of the largest, and the others are normal variates, some of them 2^-10 of their deviation.)"""
+    p = Problem([q_len], [700], 4, 2, 128, bits, 16, torch.bfloat16, seed=35)
+    for at in (3, 70):
+        p.q[..., at] *= 2.0 ** up
+        if bits == 8:
+            p.cache.k_codes[..., at] = 0
+        else:
+            byte, other = p.cache.k_codes[..., at // 2], 0x0F if at % 2 else 0xF0
+            byte.copy_((byte & other) | (0x88 & ~other & 0xFF))
+    p.check(p.run())
