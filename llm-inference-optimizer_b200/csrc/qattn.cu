@@ -191,11 +191,25 @@ int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, i
 //   2 requests of up to 3001, 256 rows:   34 / 36 | 38 / 45    (27.7 units)
 //   4 requests of up to 1500, 128 rows:   25 / 27 | 26 / 32    (17 units)
 //   1 request of 600,        512 rows:    22 / 23 | 30 / 36    (11 units)
-constexpr int64_t kTreeRows = 64, kTreeWork = 28, kItemWork = 8;
+// That is of requests alike.  A batch of few trees among single tokens has the
+// rows of its mean, not of its largest, and 256 rows for every single token cost
+// the tensor-core kernel more than they save: it is taken above kMeanRows rows
+// a request on average.  64 requests of up to 8000, 8 bits, fp16, us, streaming | tensor-core:
+//   28 heads over 4, 1 token each:                   7 rows:   71 | 201
+//                    one tree of 64, 63 tokens:     14 rows:  148 | 237
+//                    4 tokens each:                 28 rows:  194 | 220
+//                    4 trees of 64, 60 tokens:      35 rows:  290 | 253    (up to 2000: 108 | 119)
+//                    32 trees of 16, 32 tokens:     60 rows:  399 | 218
+//   32 heads over 8, 4 trees of 64, 60 tokens:      20 rows:  401 | 454
+//                    16 trees of 64, 48 tokens:     67 rows: 1009 | 468
+// The same mean tells how many rows the streaming kernel takes at once (32 heads over 8, one tree of 64 and 63
+// tokens, 8 rows: 202 us with tiles of 8, 238 with tiles of 16).
+constexpr int64_t kTreeRows = 64, kMeanRows = 32, kTreeWork = 28, kItemWork = 8;
 
 struct Attention {
   ql::att::Params p;
   int64_t max_q, max_kv, flags;
+  int64_t max_rows, mean_rows;   // of a request under one key/value head
   void* workspace;
   size_t workspace_bytes;
   void* stream;
@@ -254,12 +268,12 @@ int run_tree(const Attention& a) {
 template <typename T, int D, int BITS>
 int run_rows(const Attention& a) {
   if constexpr (D <= 128) {
-    const int64_t rows = a.max_q * a.p.group, units = cdiv(a.max_kv, ql::att::kUnitKeys) + kItemWork;
-    const double work = (double)a.p.batch * a.p.cache.heads * (double)cdiv(rows, 16) * (double)units;
-    const bool tree = rows > kTreeRows && work >= (double)(kTreeWork * a.sms);
+    const int64_t units = cdiv(a.max_kv, ql::att::kUnitKeys) + kItemWork;
+    const double work = (double)a.p.batch * a.p.cache.heads * (double)cdiv(a.mean_rows, 16) * (double)units;
+    const bool tree = a.max_rows > kTreeRows && a.mean_rows > kMeanRows && work >= (double)(kTreeWork * a.sms);
     if (!(a.flags & QL_FLAG_FORCE_GEMV) && (tree || (a.flags & QL_FLAG_FORCE_GEMM))) return run_tree<T, D, BITS>(a);
   }
-  return a.max_q * a.p.group <= 8 ? run_stream<T, D, BITS, 1>(a) : run_stream<T, D, BITS, 2>(a);
+  return a.mean_rows <= 8 ? run_stream<T, D, BITS, 1>(a) : run_stream<T, D, BITS, 2>(a);
 }
 
 template <typename T>
@@ -404,8 +418,11 @@ int ql_tree_attention(const ql_tree_attention_args* a, void* stream) {
   p.mask_words = (int)a->mask_words;
   p.scale_log2 = (float)(a->scale * 1.4426950408889634);
   p.err = dev.err_word;
-  const Attention work = {p, a->max_q, a->max_kv, a->flags, a->workspace, (size_t)std::max<int64_t>(a->workspace_bytes, 0),
-                          stream, dev.sms};
+  // the caller's bounds, where total_q and the table do not give better ones
+  const int64_t max_q = std::min(a->cu_q ? std::max<int64_t>(a->max_q, 1) : a->total_q / a->batch, a->total_q);
+  const int64_t max_kv = std::min(std::max<int64_t>(a->max_kv, 1), a->table_width * a->cache.page_size);
+  const Attention work = {p, max_q, max_kv, a->flags, max_q * p.group, cdiv(a->total_q * p.group, a->batch), a->workspace,
+                          (size_t)std::max<int64_t>(a->workspace_bytes, 0), stream, dev.sms};
   return a->dtype == QL_DTYPE_F16 ? run_attention<__half>(work, a->cache.head_dim)
                                   : run_attention<__nv_bfloat16>(work, a->cache.head_dim);
 }
