@@ -78,11 +78,29 @@ class QuantizedKVCache:
                    for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
 
     def move(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Copies the rows at slots `src` to `dst` (all read before any is
-        written): the rows of accepted drafted tokens close up behind the
-        context.  Codes move as they are, so nothing is rounded again."""
+        """Copies the rows at slots `src` (rows,) to `dst` (all read before any
+        is written): the rows of accepted drafted tokens close up behind the
+        context.  Codes move as they are, so nothing is rounded again.  A pair
+        with a negative slot is skipped, and one with a slot past the pool,
+        which is recorded as elsewhere."""
+        index_bytes(src, "src"), index_bytes(dst, "dst")
+        assert src.dim() == 1 and src.shape == dst.shape, \
+            f"src and dst must be (rows,) alike, got {tuple(src.shape)} and {tuple(dst.shape)}"
+        assert src.device == self.device and dst.device == self.device, f"src and dst must be on {self.device}"
+        if src.shape[0] == 0:
+            return
+        end, pairs = self.num_pages * self.page_size, torch.stack((src.long(), dst.long()))
+        inside = pairs < end
+        if self.device.type == "cuda":
+            read_kv(self, torch.where(inside, -1, pairs).view(-1))     # records what is past the pool
+        # no size may depend on the slots: a skipped pair repeats one that is kept, or moves row 0 to itself if none is
+        kept = (inside & (pairs >= 0)).all(0)
+        pairs = torch.where(kept, pairs, (pairs * kept).index_select(1, kept.byte().argmax(0, keepdim=True)))
+        (page, to_page), (at, to_at) = (pairs >> self.page_size.bit_length() - 1).unbind(), \
+            (pairs & self.page_size - 1).unbind()
         for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales):
-            t[dst // self.page_size, :, dst % self.page_size] = t[src // self.page_size, :, src % self.page_size]
+            rows = t.transpose(1, 2)
+            rows.index_put_((to_page, to_at), rows[page, at])
 
 
 def append_kv(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,

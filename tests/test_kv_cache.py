@@ -110,6 +110,45 @@ def test_queries_without_a_rotation_are_refused():
     assert _lib.load().ql_kv_append(_lib.KV_APPEND_ARGS.pack(*c, *args.values()), None) == _lib.QL_ERR_BAD_SHAPE
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_move_skips_slots_outside_the_pool(device, dtype):
+    """Negative slots and slots past the pool, at either end of a pair, move nothing; the other pairs of the call move."""
+    cache = QuantizedKVCache.empty(3, 16, 2, 64, 8, device=device)
+    ts = (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)
+    for n, t in enumerate(ts):
+        t.copy_((torch.arange(48)[:, None, None] + torch.arange(2)[:, None] * 48 + n).expand(48, 2, t.shape[-1])
+                .reshape(3, 16, 2, -1).transpose(1, 2).to(t.dtype))
+    before = [t.clone() for t in ts]
+
+    def rows(t):
+        return t.transpose(1, 2).flatten(0, 1)
+
+    def move(pairs):
+        cache.move(*(torch.tensor([p[i] for p in pairs], dtype=dtype, device=device) for i in (0, 1)))
+
+    for pairs in ([(-1, 3)], [(3, -1), (-1, -1)], [(5, 48)], [(48, 5), (1000, 2000)], []):
+        if device == "cuda":
+            _lib.clear_device_error()
+        move(pairs)
+        assert all(torch.equal(t, b) for t, b in zip(ts, before)), pairs
+        if device == "cuda":
+            past = any(s >= 48 for p in pairs for s in p)
+            assert _lib.device_error() == (_lib.QL_DEVICE_ERROR_BAD_INDEX if past else 0), pairs
+            _lib.clear_device_error()
+    move([(-1, 4), (20, 17), (7, 0), (18, 48), (17, 16), (9, -5)])
+    for t, b in zip(ts, before):
+        want = rows(b).clone()
+        want[17], want[0], want[16] = rows(b)[20], rows(b)[7], rows(b)[17]
+        assert torch.equal(rows(t), want)
+    if device == "cuda":
+        _lib.clear_device_error()
+    with pytest.raises(AssertionError):
+        cache.move(torch.arange(2, device=device), torch.arange(3, device=device))
+    with pytest.raises(TypeError):
+        cache.move(torch.zeros(2, device=device), torch.zeros(2, device=device))
+
+
 # ----------------------------------------------------------------------- GPU
 def stored(cache, slots):
     page, at = slots // cache.page_size, slots % cache.page_size
