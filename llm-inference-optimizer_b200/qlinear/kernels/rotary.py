@@ -16,6 +16,10 @@ import torch
 from .. import _lib
 from ._launch import activation_code, call, call_flags, index_bytes
 
+# What a model's configuration says of its rotary positions.  (mrope: the three positions of a token of text are one.)
+_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "original_max_position_embeddings",
+         "max_position_embeddings", "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow", "attention_factor",
+         "truncate", "mscale", "mscale_all_dim", "finetuned", "mrope_section", "mrope_interleaved"}
 LAYOUTS = {"half": _lib.QL_ROTARY_HALF, "interleaved": _lib.QL_ROTARY_INTERLEAVED}
 
 
@@ -34,10 +38,18 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
       step in original / wavelength between;
     * ``yarn``: pairs that turn less than ``beta_slow`` times over the original
       length divided by ``factor``, more than ``beta_fast`` times kept, a ramp
-      over the pair index between, and cos / sin times
-      ``attention_factor`` (0.1 ln(factor) + 1 unless given).
+      over the pair index between (its ends whole pairs, unless ``truncate``
+      is false), and cos / sin times ``attention_factor``; that is unless given
+      m(1) with m(x) = 0.1 x ln(factor) + 1, or m(mscale) / m(mscale_all_dim)
+      where both are.
+
+    Keys that it does not know are refused, since they may change the angles
+    (parameters by kind of layer among them: pass one kind's).
     """
-    s = dict(scaling or {})
+    s = {name: value for name, value in (scaling or {}).items() if value is not None}
+    unknown = sorted(set(s) - _KEYS)
+    if unknown:
+        raise ValueError(f"rotary scaling has keys that are not known: {', '.join(map(repr, unknown))}")
     kind = s.get("rope_type", s.get("type", "default"))
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
 
@@ -67,11 +79,21 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
             return rotary_dim * math.log(old / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
 
         fast, slow = s.get("beta_fast") or 32.0, s.get("beta_slow") or 1.0
-        lo, hi = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), rotary_dim - 1)
+        lo, hi = pair_with(fast), pair_with(slow)
+        if s.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         kept = 1.0 - ((i - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
         factor_on = s.get("attention_factor")
         if factor_on is None:
-            factor_on = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+            one, both = float(s.get("mscale") or 0.0), float(s.get("mscale_all_dim") or 0.0)
+            if both and not one or one not in (0.0, 1.0) and not both:
+                raise ValueError("rotary scaling 'yarn': mscale and mscale_all_dim go together")
+
+            def m(x):
+                return 0.1 * x * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+
+            factor_on = m(one) / m(both) if both else m(1.0)
         return f * (kept + (1.0 - kept) / factor), float(factor_on)
     raise ValueError(f"unknown rotary scaling {kind!r}")
 

@@ -61,6 +61,47 @@ def test_yarn_frequencies_and_factor():
     assert given == 0.5
 
 
+@pytest.mark.parametrize("base,old", [(1.0e4, 4096), (1.5e5, 4096), (1.0e6, 32768)])
+def test_yarn_ramp_between_fractional_pairs(base, old):
+    """truncate false: the ramp runs from the very pair that turns beta_fast times to the one that turns beta_slow times."""
+    s = {"rope_type": "yarn", "factor": 32.0, "original_max_position_embeddings": old, "beta_fast": 32.0, "beta_slow": 1.0,
+         "truncate": False}
+    f, _ = rotary_frequencies(64, base, s)
+    whole, _ = rotary_frequencies(64, base, {**s, "truncate": True})
+    default, _ = rotary_frequencies(64, base, {n: v for n, v in s.items() if n != "truncate"})
+    assert torch.equal(whole, default) and not torch.allclose(f, whole, rtol=1e-6)
+    lo, hi = (64 * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (32.0, 1.0))
+    for got, a, b in ((f, lo, hi), (whole, math.floor(lo), math.ceil(hi))):
+        for i in range(32):
+            stretched = min(max((i - a) / (b - a), 0.0), 1.0)
+            plain = base ** (-2.0 * i / 64)
+            assert got[i].item() == pytest.approx(plain * (1 - stretched) + plain / 32.0 * stretched, rel=1e-12)
+
+
+def test_yarn_factor_of_two_mscales():
+    s = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+    m = lambda x: 0.1 * x * math.log(40.0) + 1.0                                  # noqa: E731
+    assert rotary_frequencies(64, 1.0e4, {**s, "mscale": 0.707, "mscale_all_dim": 0.707})[1] == pytest.approx(1.0)
+    assert rotary_frequencies(64, 1.0e4, {**s, "mscale": 1.0, "mscale_all_dim": 0.5})[1] == pytest.approx(m(1.0) / m(0.5))
+    assert rotary_frequencies(64, 1.0e4, {**s, "mscale": 1.0})[1] == pytest.approx(m(1.0))
+    assert rotary_frequencies(64, 1.0e4, {**s, "mscale": 0.5, "mscale_all_dim": 1.0, "attention_factor": 1.25})[1] == 1.25
+    for lone in ({"mscale": 0.5}, {"mscale_all_dim": 1.0}):
+        with pytest.raises(ValueError):
+            rotary_frequencies(64, 1.0e4, {**s, **lone})
+
+
+def test_keys_that_are_not_known_are_refused():
+    with pytest.raises(ValueError, match="stretch"):
+        rotary_frequencies(64, 1.0e4, {"rope_type": "linear", "factor": 2.0, "stretch": 3.0})
+
+    class Config:                                        # parameters by kind of layer
+        hidden_size, num_attention_heads, max_position_embeddings = 1024, 16, 512
+        rope_parameters = {"full_attention": {"rope_type": "default", "rope_theta": 1.0e6},
+                           "sliding_attention": {"rope_type": "default", "rope_theta": 1.0e4}}
+    with pytest.raises(ValueError, match="full_attention"):
+        RotaryTable.from_config(Config, device="cpu")
+
+
 def test_dynamic_base_grows_only_past_the_original_length():
     s = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 4096}
     plain, _ = rotary_frequencies(64, 1.0e4)
