@@ -23,6 +23,11 @@ _KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "
 LAYOUTS = {"half": _lib.QL_ROTARY_HALF, "interleaved": _lib.QL_ROTARY_INTERLEAVED}
 
 
+def _kind(scaling: dict) -> str:
+    """The scaling's name, under its older key too."""
+    return scaling.get("rope_type") or scaling.get("type") or "default"
+
+
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None,
                        max_positions: int | None = None) -> tuple[torch.Tensor, float]:
     """Radians per position of each pair (float64 [rotary_dim / 2]) and the
@@ -50,7 +55,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     unknown = sorted(set(s) - _KEYS)
     if unknown:
         raise ValueError(f"rotary scaling has keys that are not known: {', '.join(map(repr, unknown))}")
-    kind = s.get("rope_type", s.get("type", "default"))
+    kind = _kind(s)
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
 
     def need(name):
@@ -131,8 +136,8 @@ class RotaryTable:
         ``rope_theta`` and ``rope_scaling``)."""
         s = dict(getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {})
         base = s.get("rope_theta") or getattr(config, "rope_theta", None) or 10000.0
-        if s.get("rope_type", "default") not in ("default", "linear"):
-            s.setdefault("original_max_position_embeddings", config.max_position_embeddings)
+        if _kind(s) not in ("default", "linear") and s.get("original_max_position_embeddings") is None:
+            s["original_max_position_embeddings"] = config.max_position_embeddings
         head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
         part = s.get("partial_rotary_factor") or getattr(config, "partial_rotary_factor", None) or 1.0
         return cls.build(int(head_dim * part), max_positions or config.max_position_embeddings, base, layout, s,

@@ -90,6 +90,22 @@ def test_yarn_factor_of_two_mscales():
             rotary_frequencies(64, 1.0e4, {**s, **lone})
 
 
+@pytest.mark.parametrize("kind", ["yarn", "dynamic"])
+def test_older_configurations_name_the_scaling_type(kind):
+    """`type` in the place of `rope_type`, beside rope_theta: the same table, the original length the model's own."""
+    class Config:
+        hidden_size, num_attention_heads, max_position_embeddings, rope_theta = 1024, 16, 512, 5.0e5
+
+    tables = []
+    for key in ("type", "rope_type"):
+        Config.rope_scaling = {key: kind, "factor": 2.0, "original_max_position_embeddings": None}
+        tables.append(RotaryTable.from_config(Config, max_positions=1024, device="cpu").table)
+    assert torch.equal(*tables)
+    f, factor = rotary_frequencies(64, 5.0e5, {"rope_type": kind, "factor": 2.0,
+                                               "original_max_position_embeddings": 512}, 1024)
+    assert tables[0][1000, 3, 0].item() == pytest.approx(factor * math.cos(1000 * f[3].item()), abs=2.0 ** -23)
+
+
 def test_keys_that_are_not_known_are_refused():
     with pytest.raises(ValueError, match="stretch"):
         rotary_frequencies(64, 1.0e4, {"rope_type": "linear", "factor": 2.0, "stretch": 3.0})
