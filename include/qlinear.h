@@ -350,8 +350,8 @@ int ql_allgather_f16(const void* src, int64_t lds, void* out, int64_t ldo, int64
  * out[t, h] = x[t, h] with its first rotary_dim elements turned by the angles
  * of positions[t]; out may be x.  table fp32 [max_positions][rotary_dim / 2][2]
  * holds each pair's cosine and sine (and any factor on both).  rotary_dim is
- * a multiple of 8, head_dim too (at most 2048).  inverse != 0 turns back (the direction of
- * the gradient).  A position outside the table takes its nearest row and
+ * a multiple of 8, head_dim too (at most 2048).  inverse != 0 turns by the negative angles: the
+ * gradient's direction, and back to x where the table has no factor.  A position outside the table takes its nearest row and
  * records QL_DEVICE_ERROR_BAD_INDEX.
  */
 typedef struct {

@@ -7,8 +7,8 @@
 //   y1 = x1 cos - x2 sin,   y2 = x2 cos + x1 sin,
 // with (x1, x2) = (x[i], x[i + r/2]) in the half layout and (x[2i], x[2i+1])
 // in the interleaved one; elements from r on pass through.  The inverse
-// turns by the negative angle; the rotation being orthogonal, it is also the
-// gradient's direction.  Computed in fp32 with every product and sum rounded
+// turns by the negative angle: the transpose, and so the gradient's direction,
+// whatever factor the table has on its cosines and sines.  Computed in fp32 with every product and sum rounded
 // on its own (no contraction), so that a row quantised from it has the codes
 // that the same expression gives elementwise elsewhere.
 //

@@ -111,7 +111,8 @@ def append_kv(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, slots: 
     k is turned first, in fp32; with q (tokens, q_heads, head_dim) too, q is
     turned by the same angles and returned (in `q_out`, which may be q).
     Tensors may have any strides with unit stride along head_dim, such as
-    the column slices of a fused projection's output."""
+    the column slices of a fused projection's output.  Gradients are not
+    recorded: the result is detached."""
     shape, dev = k.shape, cache.device
     tokens = shape[0]
     assert k.device == dev and k.is_cuda, f"k is on {k.device}, the cache on {dev}"

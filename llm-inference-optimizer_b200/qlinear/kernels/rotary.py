@@ -150,8 +150,11 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     positions (tokens,): the first ``rotary.rotary_dim`` elements of each head
     in ``rotary.layout``'s pairs, the rest unchanged, one rounding.  x and
     `out` may have any strides with unit stride along head_dim; ``out=x``
-    turns in place.  ``inverse=True`` turns back: it undoes the call, and maps
-    the gradient of its result to that of x."""
+    turns in place.  ``inverse=True`` turns by the negative angles: it maps the
+    gradient of the call's result to that of x, and undoes the call where the
+    table has no factor on its cosines and sines (with one, as yarn's, there and
+    back is its square times x).  Gradients are not recorded: the result is
+    detached, whatever x is."""
     shape, dev = x.shape, x.device
     assert x.is_cuda and len(shape) == 3, f"x must be a CUDA tensor (tokens, heads, head_dim), got {tuple(shape)}"
     tokens, heads, head_dim = shape

@@ -60,8 +60,8 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
       ``page_table[b, j // page_size]``;
     * kv_lens int32 (batch,): cached positions, new tokens included (they are
       the last ones);
-    * cu_q int32 (batch + 1,): request b's rows are cu_q[b] .. cu_q[b+1] - 1;
-      None gives each total_q / batch rows (one token each in plain decoding);
+    * cu_q int32 (batch + 1,): request b's rows are cu_q[b] .. cu_q[b+1] - 1
+      (rows that it does not cover are left as they are: not written); None gives each total_q / batch rows (one token each in plain decoding);
     * mask int64 (total_q, words): which of its request's new tokens a row
       sees (``pack_tree_mask``); None: those up to itself.  Every row sees all
       positions before the new tokens.  A row that sees nothing gives zeros;
@@ -71,7 +71,7 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
 
     Returns (total_q, q_heads, head_dim) in q's dtype, and with
     ``return_lse`` the rows' log-sums (total_q, q_heads) fp32 (minus infinity
-    where nothing is seen)."""
+    where nothing is seen).  Gradients are not recorded: both are detached."""
     shape, dev, dtype = q.shape, cache.device, q.dtype
     assert q.is_cuda and len(shape) == 3, f"q must be a CUDA tensor (total_q, q_heads, head_dim), got {tuple(shape)}"
     total_q, q_heads, head_dim = shape

@@ -269,6 +269,21 @@ def test_inverse_is_the_gradient(layout):
 
 
 @on_gpu
+def test_there_and_back():
+    """The inverse undoes the call without a factor; with one (yarn) there and back is its square times x."""
+    x = heads(9, 3, 64, torch.float16, 9)
+    positions = torch.arange(100, 109).cuda()
+    for scaling in (None, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}):
+        rot = RotaryTable.build(64, 256, 1.0e4, "half", scaling)
+        factor = rotary_frequencies(64, 1.0e4, scaling)[1]
+        assert (factor > 1.1) == (scaling is not None)
+        back = apply_rotary(apply_rotary(x, positions, rot), positions, rot, inverse=True).double()
+        pair = factor * x.double().abs().unflatten(-1, (2, 32)).sum(-2).repeat(1, 1, 2)
+        # rounded to fp16 there (2^-11 of |x1| + |x2|, which both of the pair take back) and back again
+        assert bool(((back - factor ** 2 * x.double()).abs() <= 3 * 2.0 ** -11 * factor * pair + 2.0 ** -22).all())
+
+
+@on_gpu
 def test_infinities_and_nan_stay_in_their_pairs():
     rot = RotaryTable.build(64, 8, 1.0e4)
     x = heads(1, 2, 64, torch.float16, 5)
