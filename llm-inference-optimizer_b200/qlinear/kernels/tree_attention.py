@@ -122,7 +122,7 @@ def tree_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.T
         if qs[2] != 1:
             q = q.contiguous()
             qs = q.stride()
-        if ts[1] != 1:
+        if ts[1] != 1 or ts[0] < width and batch > 1:        # also one row for all (expanded), or rows that overlap
             page_table = page_table.contiguous()
             ts = page_table.stride()
         if max_kv is None:

@@ -290,6 +290,26 @@ def test_strides_views_and_out():
 
 
 @on_gpu
+def test_page_tables_of_any_strides():
+    """One row of pages for all requests, as a view without a stride; rows that overlap; columns of a wider table."""
+    p = Problem([1] * 3, [70, 70, 70], 4, 2, 64, 8, 16, torch.float16, seed=22)
+    row = p.table[1]
+    want = None
+    flat = torch.cat([row, row, row])
+    for table in (row.repeat(3, 1), row.expand(3, -1), row[None].expand(3, -1), flat.as_strided((3, 5), (0, 1)),
+                  torch.stack([row, row], 1)[:, 0].expand(3, -1), flat.reshape(3, -1).t().contiguous().t()):
+        p.table = table
+        got = p.run(cu_q=None)[0]
+        p.check((got, p.run()[1]))
+        want = got if want is None else want
+        assert torch.equal(got, want)
+    p.table = torch.arange(8, dtype=torch.int32, device="cuda").as_strided((3, 5), (1, 1))     # requests a page apart
+    p.cache.k_scales.nan_to_num_(nan=0.01)
+    p.cache.v_scales.nan_to_num_(posinf=0.01)
+    p.check(p.run())
+
+
+@on_gpu
 def test_pages_outside_the_pool_are_recorded_and_hidden():
     p = Problem([1, 1], [40, 64], 4, 2, 64, 8, 16, torch.float16, seed=15)
     good = p.table.clone()
