@@ -25,7 +25,14 @@ class QuantizedKVCache:
     """One layer's pool: codes (num_pages, kv_heads, page_size, row bytes),
     int8 at 8 bits and uint8 at 4, and scales bf16 (num_pages, kv_heads,
     page_size, groups).  Pages may be strided views (a slice of a pool for
-    all layers); within a page the tensors are contiguous."""
+    all layers); within a page the tensors are contiguous.  The tensors are
+    the cache's for its life: to grow a pool, make another cache."""
+
+    # calls pass on the addresses that `fields` holds, so none may be exchanged for another tensor
+    k_codes = property(lambda self: self._tensors[0])
+    k_scales = property(lambda self: self._tensors[1])
+    v_codes = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                  v_scales: torch.Tensor):
@@ -50,7 +57,7 @@ class QuantizedKVCache:
         for t in (k_codes, k_scales, v_codes, v_scales):
             assert t.device == self.device, "codes and scales must be on one device"
             assert t[0].is_contiguous(), "codes and scales must be contiguous within a page"
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self._tensors = (k_codes, k_scales, v_codes, v_scales)
         ts = (k_codes, v_codes, k_scales, v_scales)
         strides = [t.stride(0) if self.num_pages > 1 else t[0].numel() for t in ts]
         # the C structure's fields, which stay as they are for the cache's life

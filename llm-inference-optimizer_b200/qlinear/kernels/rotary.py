@@ -104,7 +104,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
 
 
 class RotaryTable:
-    """cos and sin of every position: fp32 [max_positions, rotary_dim / 2, 2]."""
+    """cos and sin of every position: fp32 [max_positions, rotary_dim / 2, 2].
+    The tensor is the table's for its life: calls pass on its address."""
+
+    table = property(lambda self: self._table)
 
     def __init__(self, table: torch.Tensor, layout: str = "half"):
         if layout not in LAYOUTS:
@@ -115,7 +118,7 @@ class RotaryTable:
         if table.shape[0] == 0 or table.shape[1] == 0 or table.shape[1] % 4 != 0:
             raise ValueError(f"rotary_dim must be a positive multiple of 8 and the table not empty, got "
                              f"{tuple(table.shape)}")
-        self.table = table.contiguous()
+        self._table = table.contiguous()
         self.layout = layout
         self.device, self.ptr, self.layout_code = self.table.device, self.table.data_ptr(), LAYOUTS[layout]
         self.rotary_dim = 2 * table.shape[1]

@@ -48,6 +48,18 @@ def test_pool_forms_and_refusals():
         QuantizedKVCache(k[:, :, ::2], s[:, :, ::2], k[:, :, ::2], s[:, :, ::2])
 
 
+def test_tensors_are_not_exchanged():
+    """Calls pass on addresses taken once: a cache or table whose tensor was replaced would reach freed memory."""
+    c = QuantizedKVCache.empty(3, 16, 2, 128, bits=8, device="cpu")
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    t = RotaryTable.build(64, 8, 1.0e4, device="cpu")
+    with pytest.raises(AttributeError):
+        t.table = t.table.clone()
+    assert c.fields[0] == c.k_codes.data_ptr() and t.ptr == t.table.data_ptr()
+
+
 def cache_fields(**change):
     f = dict(kc=1024, ks=1024, vc=1024, vs=1024, num_pages=4, page_size=16, kv_heads=2, head_dim=64, bits=8,
              kps=2048, vps=2048, ksps=32, vsps=32)
