@@ -431,7 +431,7 @@ int ql_kv_read(const ql_kv_read_args* args, void* stream);
  * the mask's words count as clear.  A row that sees nothing gives zeros and
  * lse -inf.  lse[i, h] (optional, fp32) = log of the softmax's denominator.
  * Rows that cu_q does not cover are not written.  kv_lens is clamped to the
- * table; a page outside the pool hides its keys and records
+ * table, and to 2^31 - 512; a page outside the pool hides its keys and records
  * QL_DEVICE_ERROR_BAD_INDEX.  max_q and max_kv bound the requests' tokens and
  * lengths and only choose the launch.  flags: QL_FLAG_FORCE_GEMM (the
  * tensor-core kernel for any number of rows, where head_dim is 64 or 128) and

@@ -46,7 +46,7 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
     r.q_len = p.total_q / p.batch;
     r.q0 = b * r.q_len;
   }
-  const long long most = min((long long)p.table_width << p.cache.page_shift, 0x7FFFFFFFll);
+  const long long most = min((long long)p.table_width << p.cache.page_shift, (long long)kMostKeys);
   r.kv_len = (int)min((long long)max(p.kv_lens[b], 0), most);
   return r;
 }
@@ -66,8 +66,7 @@ constexpr int kMinUnits = 2;               // units worth a CTA of their own: 25
 
 template <int MIN_UNITS>
 __device__ __forceinline__ int item_units(const Request& r) {
-  const int n = (r.kv_len + kUnitKeys - 1) / kUnitKeys;
-  return max((n + MIN_UNITS - 1) / MIN_UNITS, 1) * MIN_UNITS;
+  return units_of(r.kv_len, MIN_UNITS);
 }
 template <int ROWS, int MIN_UNITS>
 __device__ __forceinline__ long long request_units(const Params& p, const Request& r) {

@@ -24,6 +24,16 @@ constexpr int kJoin = 16;                  // parts of an item that are joined a
 constexpr int kMaxCtas = 1024;
 constexpr int kHeaderBytes = 2 * 4 * kMaxCtas;   // counters of items and of groups of parts
 
+// The most positions of a request: the end of its last unit, at 512 keys a
+// part, is still an int.
+constexpr int kMostKeys = 0x7FFFFFFF - 511;
+
+// Units of an item over kv_len positions (0 .. kMostKeys): at least one part's, a multiple of it.
+QL_HOST_DEVICE int units_of(int kv_len, int min_units) {
+  const int n = (kv_len + kUnitKeys - 1) / kUnitKeys, parts = (n + min_units - 1) / min_units;
+  return (parts > 1 ? parts : 1) * min_units;
+}
+
 struct Work {
   long long total;     // units of the launch
   int ctas;            // CTAs that take part

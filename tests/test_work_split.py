@@ -19,6 +19,8 @@ SOURCE = r"""
 #include <utility>
 #include "qwork.h"
 using namespace ql::att;
+extern "C" int units(int kv_len, int min_units) { return units_of(kv_len, min_units); }
+extern "C" int most_keys() { return kMostKeys; }
 extern "C" int check(const int* units, int items, int min_units, int grid, int* most_parts, int* lone) {
   long long total = 0;
   for (int i = 0; i < items; ++i) total += units[i];
@@ -77,7 +79,19 @@ def check(tmp_path_factory):
         wrong = lib.check((ctypes.c_int * len(units))(*units), len(units), least, grid, ctypes.byref(parts),
                           ctypes.byref(lone))
         return wrong, parts.value, lone.value
+    run.lib = lib
     return run
+
+
+@pytest.mark.parametrize("least", [2, 4])
+def test_units_up_to_the_most_positions(check, least):
+    """As in whole numbers without an end, and the last unit's end is an int: a table of 2^15 pages of 65536 and a length
+    to match would pass it."""
+    most = check.lib.most_keys()
+    for n in (0, 1, 127, 128, 129, 128 * least, 128 * least + 1, 1 << 30, most - 513, most - 1, most):
+        units = check.lib.units(n, least)
+        assert units == items([n], 1, least)[0] and 128 * units <= (1 << 31) - 1, n
+    assert (1 << 31) - 1 - most < 512
 
 
 def items(lens, heads, least):
