@@ -43,8 +43,9 @@ class PagedDecoder:
         pages = -(-max_positions // page_size)
         self.caches = [QuantizedKVCache.empty(pages, page_size, self.kv_heads, self.head_dim, bits)
                        for _ in model.model.layers]
-        self.rotary = RotaryTable.from_config(cfg, max_positions)
+        self.rotary = RotaryTable.from_config(cfg, pages * page_size)
         self.page_table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        self.max_positions = pages * page_size
         self.length = 0                              # positions that hold accepted tokens
 
     @torch.no_grad()
@@ -53,6 +54,8 @@ class PagedDecoder:
         `depth` is each token's distance from the first (its place in the
         sequence), `mask` which of the new tokens each sees; by default a chain."""
         n = ids.shape[0]
+        if self.length + n > self.max_positions:
+            raise ValueError(f"{n} tokens behind {self.length} do not fit {self.max_positions} positions")
         slots = torch.arange(self.length, self.length + n, device="cuda")
         positions = slots if depth is None else self.length + depth
         kv_lens = torch.tensor([self.length + n], dtype=torch.int32, device="cuda")
@@ -176,7 +179,7 @@ def main() -> None:
     prompt = torch.randint(0, model.config.vocab_size, (37,), generator=torch.Generator().manual_seed(1)).cuda()
     runs = {}
     for name in ("plain", "tree"):
-        decoder = PagedDecoder(model, bits=args.bits)
+        decoder = PagedDecoder(model, bits=args.bits, max_positions=prompt.shape[0] + args.new + 64)   # and a tree
         torch.cuda.synchronize()
         t = time.perf_counter()
         if name == "plain":
