@@ -184,26 +184,26 @@ int run_append(ql::kvc::AppendParams p, int64_t chunks, int sms, void* stream, i
 // of 128 keys by 16 rows, an item's start and end counted as kItemWork of them.
 // Below, the tensor-core kernel's start and end (22 us) outweigh its rate.
 // 32 heads over 4 of 128, 8 bits, fp16 / bf16, us, streaming | tensor-core:
-//   8 requests of up to 6001, 64 rows:    45 / 47 | 46 / 56
-//                            128 rows:    75 / 78 | 47 / 58
-//   16 requests of up to 600, 72 rows:    34 / 36 | 24 / 29    (28 units)
-//   1 request of 16001,      128 rows:    46 / 48 | 45 / 50    (29 units)
-//   2 requests of up to 3001, 256 rows:   34 / 36 | 38 / 45    (27.7 units)
-//   4 requests of up to 1500, 128 rows:   25 / 27 | 26 / 32    (17 units)
-//   1 request of 600,        512 rows:    22 / 23 | 30 / 36    (11 units)
+//   8 requests of up to 6001, 64 rows:    45 / 47 | 45 / 54
+//                            128 rows:    75 / 78 | 47 / 56
+//   16 requests of up to 600, 72 rows:    33 / 35 | 23 / 28    (28 units)
+//   1 request of 16001,      128 rows:    46 / 48 | 44 / 49    (29 units)
+//   2 requests of up to 3001, 256 rows:   34 / 35 | 38 / 44    (27.7 units)
+//   4 requests of up to 1500, 128 rows:   25 / 26 | 26 / 31    (17 units)
+//   1 request of 600,        512 rows:    22 / 23 | 30 / 35    (11 units)
 // That is of requests alike.  A batch of few trees among single tokens has the
 // rows of its mean, not of its largest, and 256 rows for every single token cost
 // the tensor-core kernel more than they save: it is taken above kMeanRows rows
 // a request on average.  64 requests of up to 8000, 8 bits, fp16, us, streaming | tensor-core:
 //   28 heads over 4, 1 token each:                   7 rows:   71 | 201
 //                    one tree of 64, 63 tokens:     14 rows:  148 | 237
-//                    4 tokens each:                 28 rows:  194 | 220
-//                    4 trees of 64, 60 tokens:      35 rows:  290 | 253    (up to 2000: 108 | 119)
-//                    32 trees of 16, 32 tokens:     60 rows:  399 | 218
-//   32 heads over 8, 4 trees of 64, 60 tokens:      20 rows:  401 | 454
-//                    16 trees of 64, 48 tokens:     67 rows: 1009 | 468
+//                    4 tokens each:                 28 rows:  194 | 219
+//                    4 trees of 64, 60 tokens:      35 rows:  291 | 253    (up to 2000: 109 | 118)
+//                    32 trees of 16, 32 tokens:     60 rows:  399 | 214
+//   32 heads over 8, 4 trees of 64, 60 tokens:      20 rows:  402 | 454
+//                    16 trees of 64, 48 tokens:     67 rows: 1001 | 465
 // The same mean tells how many rows the streaming kernel takes at once (32 heads over 8, one tree of 64 and 63
-// tokens, 8 rows: 202 us with tiles of 8, 238 with tiles of 16).
+// tokens, 8 rows: 193 us with tiles of 8, 238 with tiles of 16).
 constexpr int64_t kTreeRows = 64, kMeanRows = 32, kTreeWork = 28, kItemWork = 8;
 
 struct Attention {
@@ -269,7 +269,7 @@ template <typename T, int D, int BITS>
 int run_rows(const Attention& a) {
   if constexpr (D <= 128) {
     const int64_t units = cdiv(a.max_kv, ql::att::kUnitKeys) + kItemWork;
-    const double work = (double)a.p.batch * a.p.cache.heads * (double)cdiv(a.mean_rows, 16) * (double)units;
+    const double work = (double)a.p.batch * a.p.cache.heads * (double)cdiv(a.max_rows, 16) * (double)units;
     const bool tree = a.max_rows > kTreeRows && a.mean_rows > kMeanRows && work >= (double)(kTreeWork * a.sms);
     if (!(a.flags & QL_FLAG_FORCE_GEMV) && (tree || (a.flags & QL_FLAG_FORCE_GEMM))) return run_tree<T, D, BITS>(a);
   }

@@ -38,3 +38,12 @@ def test_a_mixed_batch_goes_by_its_mean(trees, tensor, monkeypatch):
     assert not torch.equal(*sides)
     assert torch.equal(got[0], sides[tensor])
     p.check(got)
+
+
+def test_ragged_trees_go_by_the_largest_above_the_mean(monkeypatch):
+    """16 requests of up to 600 positions and 9 tokens, 57 rows on the average and 72 at most: the tensor-core kernel."""
+    p = Problem([9 - i % 5 for i in range(16)], [600 - 14 * i for i in range(16)], 32, 4, 128, 8, 16, torch.float16, "tree",
+                seed=43)
+    got, sides = p.run(max_q=9), [forced(p, monkeypatch, f, max_q=9) for f in (_lib.QL_FLAG_FORCE_GEMV, _lib.QL_FLAG_FORCE_GEMM)]
+    assert not torch.equal(*sides) and torch.equal(got[0], sides[1])
+    p.check(got)
