@@ -307,7 +307,10 @@ __host__ __device__ constexpr int step_add(int drow, int dchunk) {
 // bits fit, down to 2^-32 of the row's largest element; a bf16 body for rows
 // that reach further, as one with a branch or as two, made every bf16 call 1 to
 // 5 % slower).  Value scales multiply the weights, which are rounded
-// to fp16 once, against a power of two that follows the largest scale seen.
+// to fp16 once, against a power of two that follows the largest scale seen:
+// half the products of a sum of two, for an error against 64 bits of 0.00022 to
+// 0.00027 of an fp16 output, 0.0002 of that its own rounding, and none that shows
+// in bf16.
 // A tile with a weight below fp16's normal range (or a hidden key) takes the
 // product in bf16 instead, the weights as a sum of two: 16 bits and fp32's
 // range, so that no score far below the largest and no mixture of scales
