@@ -461,6 +461,61 @@ size_t ql_tree_attention_workspace_size(int64_t head_dim);
 uint64_t ql_capture_id(void* stream);
 int ql_tree_attention(const ql_tree_attention_args* args, void* stream);
 
+/* ------------------------------------------------------- a serving step's plan */
+/*
+ * Page tables, slots and positions of a step's new tokens, from the requests'
+ * lengths: request b is cut to its first keep[b] tokens (keep NULL: all), the
+ * pages behind them go back to the stack of free pages, and it grows by
+ * fresh[b] new tokens, whose pages come from the stack.  lens, page_table,
+ * free_pages and free_count are the state and are updated: page_table[b] holds
+ * ceil(lens[b] / page_size) pages, the first free_count[0] entries of
+ * free_pages are free.  Pages come back so that the first of them is taken
+ * first.
+ *   cu_q [batch + 1]: request b's new tokens are cu_q[b] .. cu_q[b + 1] - 1
+ *   slots, positions [max_tokens]: as ql_kv_append takes them; -1 and 0 behind
+ *     the last token.  Both 16-byte aligned.
+ * A request gets its new tokens if they fit its row of the table, if those up
+ * to and with its own fit max_tokens, and if it needs no page or the pages that
+ * requests up to and with it need are free; otherwise it is cut to keep[b], gets
+ * none, and *refused counts it.  keep is clamped to 0 .. lens[b], fresh from
+ * below to 0.  batch is at most 8192; page_size a power of two up to 65536.
+ * Nothing is followed outside the table or the stack, whatever the state holds.
+ */
+typedef struct {
+  void *page_table, *lens, *free_pages, *free_count;   /* int32 */
+  const void *keep, *fresh;                            /* int32 [batch] */
+  void *cu_q, *slots, *positions, *refused;            /* int32, int64, int32, int32 [1] */
+  int64_t batch, table_width, table_stride, num_pages, page_size, max_tokens, flags;
+} ql_plan_step_args;
+int ql_plan_step(const ql_plan_step_args* args, void* stream);
+
+/* ------------------------------------------------------------ drawing a token */
+/*
+ * ids[r] = a token of logits[r] (fp16, bf16 or fp32 [rows][row_stride], vocab
+ * of them), drawn by uniform[r] in [0, 1): with w_i = exp((x_i - max) / T), of
+ * the tokens in the order of their logits, equal ones by index, the first top_k
+ * are kept, of those the ones before which the weights come to less than top_p
+ * of their sum, of those the ones with w_i >= min_p, and the first always; the
+ * token is the first by index at which the running sum of the kept weights
+ * exceeds uniform times their sum.  Sums are in fp64.  T <= 0: the largest
+ * logit, the first of equal ones.  logprobs[r] (optional) = log of the
+ * probability with which it was drawn (0 where T <= 0).  Settings per row
+ * (fp32, top_k int32), or where the pointer is NULL the *_all for all rows;
+ * off: top_k <= 0, top_p >= 1, min_p <= 0 (and NaN).  Logits of minus infinity
+ * and NaN are hidden; with one of infinity, those alone are drawn from, alike.
+ * A row that has nothing gives -1 and minus infinity.
+ */
+#define QL_SAMPLE_MAX_VOCAB (1 << 21)
+typedef struct {
+  const void *logits, *uniform;
+  const void *temperature, *top_k, *top_p, *min_p;
+  void *ids, *logprobs;                                /* int64, fp32 [rows] */
+  int64_t rows, vocab, row_stride, dtype, top_k_all;
+  double temperature_all, top_p_all, min_p_all;
+  int64_t flags;
+} ql_sample_tokens_args;
+int ql_sample_tokens(const ql_sample_tokens_args* args, void* stream);
+
 /* ------------------------------------------------------------- diagnostics */
 const char* ql_strerror(int status);
 /* Version as (major << 16) | (minor << 8) | patch. */

@@ -514,14 +514,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         // sums it; remote store into its receive buffer, slot of this rank
         const int E = M * kRows;
         const int sz = (E + ks - 1) / ks;
-        const uint32_t me = gemm::cluster_rank();
+        const uint32_t me = cluster_rank();
         const uint32_t rbuf = smem_u32(recv);
         #pragma unroll
         for (int m = 0; m < BN; ++m) {
           if (m < M) {
             const int e = m * kRows + r;
             const int owner = e / sz;
-            gemm::st_dsmem_f32(gemm::dsmem_addr(rbuf + (uint32_t)(me * sz + (e - owner * sz)) * 4u, (uint32_t)owner),
+            st_dsmem_f32(dsmem_addr(rbuf + (uint32_t)(me * sz + (e - owner * sz)) * 4u, (uint32_t)owner),
                                acc[m]);
           }
         }
@@ -531,11 +531,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (ks > 1) {
     // ------------------------------------------------ cluster reduction
-    gemm::cluster_sync_all();                   // every member's slices are in this CTA's buffer
+    cluster_sync_all();                   // every member's slices are in this CTA's buffer
     if (warp >= 2) {
       const int E = p.M * kRows;
       const int sz = (E + ks - 1) / ks;
-      const int me = (int)gemm::cluster_rank();
+      const int me = (int)cluster_rank();
       const int e0 = me * sz, e1 = min(E, e0 + sz);
       for (int e = e0 + (int)threadIdx.x - 64; e < e1; e += kDecThreads) {
         float v = 0.f;

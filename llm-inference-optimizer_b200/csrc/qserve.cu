@@ -1,0 +1,187 @@
+// qserve.cu — C ABI of the ends of a serving step (declared in
+// include/qlinear.h): page tables and slots from request lengths, and drawing
+// tokens from logits.  Argument checks, launch shapes and launches; every
+// entry point returns a status and allocates nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/qlinear.h"
+#include "ql_host.h"
+#include "qplan.cuh"
+#include "qsample.cuh"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// One cluster of `cluster` CTAs along x after another.
+template <typename Kern, typename Params>
+int launch_clusters(Kern kernel, unsigned ctas, unsigned cluster, unsigned threads, size_t smem, void* stream,
+                    int64_t flags, const Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (flags & QL_FLAG_PDL) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return QL_ERR_CUDA;
+  }
+  return QL_OK;
+}
+
+// Lets a kernel use `smem` bytes and clusters of 16, once per device.
+template <typename Kern>
+int allow(Kern kernel, size_t smem, std::atomic<unsigned char>* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    cudaGetLastError();
+    return QL_ERR_DEVICE;
+  }
+  if (done[dev].load(std::memory_order_acquire)) return QL_OK;
+  if ((smem > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return QL_ERR_CUDA;
+  }
+  done[dev].store(1, std::memory_order_release);
+  return QL_OK;
+}
+
+// ------------------------------------------------------------------- sampling
+template <typename T, int PASSES>
+int run_sample(const ql::smp::Params& p, int ctas, void* stream, int64_t flags) {
+  auto kernel = ql::smp::sample_kernel<T, PASSES>;
+  static std::atomic<unsigned char> done[kMaxDevices];
+  const int st = allow(kernel, 0, done);
+  if (st != QL_OK) return st;
+  return launch_clusters(kernel, (unsigned)p.rows * ctas, (unsigned)ctas, ql::smp::kThreads, 0, stream, flags, p);
+}
+
+template <typename T>
+int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
+  const int64_t runs = cdiv(p.vocab, ql::smp::Type<T>::kLanes);
+  int ctas = 1;
+  while (ctas < ql::smp::kMaxCtas && cdiv(runs, (int64_t)ctas * ql::smp::kThreads) > 3) ctas *= 2;
+  switch (cdiv(runs, (int64_t)ctas * ql::smp::kThreads)) {
+    case 1: return run_sample<T, 1>(p, ctas, stream, flags);
+    case 2: return run_sample<T, 2>(p, ctas, stream, flags);
+    case 3: return run_sample<T, 3>(p, ctas, stream, flags);
+    case 4:
+    case 5: return run_sample<T, 5>(p, ctas, stream, flags);
+    default: return run_sample<T, 0>(p, ctas, stream, flags);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int ql_plan_step(const ql_plan_step_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->batch < 0 || a->batch > ql::plan::kMaxBatch || a->table_width < 0 || a->num_pages < 0 ||
+      a->num_pages > INT_MAX || a->max_tokens < 0 || a->max_tokens > INT_MAX ||
+      a->batch * std::min<int64_t>(a->table_width, INT_MAX) > INT_MAX)
+    return QL_ERR_BAD_SHAPE;
+  if (a->page_size < 1 || a->page_size > 65536 || (a->page_size & (a->page_size - 1)) != 0) return QL_ERR_UNSUPPORTED;
+  if (a->table_stride < a->table_width) return QL_ERR_BAD_STRIDE;
+  if (!a->cu_q || !a->refused || !a->free_count || (a->batch > 0 && (!a->lens || !a->fresh)) ||
+      (a->batch > 0 && a->table_width > 0 && !a->page_table) || (a->num_pages > 0 && !a->free_pages) ||
+      (a->max_tokens > 0 && (!a->slots || !a->positions)))
+    return QL_ERR_NULL_POINTER;
+  for (const void* p : {a->page_table, a->lens, a->free_pages, a->free_count, a->cu_q, a->refused})
+    if (!aligned(p, 4)) return QL_ERR_UNSUPPORTED;
+  if (!aligned(a->keep, 4) || !aligned(a->fresh, 4) || !aligned(a->slots, 16) || !aligned(a->positions, 16))
+    return QL_ERR_UNSUPPORTED;
+  ql_host::Device dev;
+  int st = ql_host::current(&dev);
+  if (st != QL_OK) return st;
+  ql::plan::Params p = {};
+  p.table = static_cast<int*>(a->page_table);
+  p.lens = static_cast<int*>(a->lens);
+  p.stack = static_cast<int*>(a->free_pages);
+  p.count = static_cast<int*>(a->free_count);
+  p.keep = static_cast<const int*>(a->keep);
+  p.fresh = static_cast<const int*>(a->fresh);
+  p.cu_q = static_cast<int*>(a->cu_q);
+  p.slots = static_cast<long long*>(a->slots);
+  p.positions = static_cast<int*>(a->positions);
+  p.refused = static_cast<int*>(a->refused);
+  p.table_stride = a->table_stride;
+  p.max_tokens = a->max_tokens;
+  p.batch = (int)a->batch;
+  p.width = (int)std::min<int64_t>(a->table_width, INT_MAX);
+  p.num_pages = (int)a->num_pages;
+  p.page_shift = __builtin_ctzll((unsigned long long)a->page_size);
+  auto kernel = ql::plan::plan_kernel;
+  static std::atomic<unsigned char> done[kMaxDevices];
+  if ((st = allow(kernel, (4 * (size_t)ql::plan::kMaxBatch + 2) * sizeof(int), done)) != QL_OK) return st;
+  const bool small = a->max_tokens <= 4096 && a->batch <= 1024;
+  const unsigned ctas = small ? 1 : 8;
+  const unsigned threads = small ? (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(std::max(a->batch, cdiv(a->max_tokens, 4)), 32) * 32, 128), ql::plan::kThreads)
+                                 : ql::plan::kThreads;
+  return launch_clusters(kernel, ctas, ctas, threads, (4 * (size_t)a->batch + 2) * sizeof(int), stream, a->flags, p);
+}
+
+int ql_sample_tokens(const ql_sample_tokens_args* a, void* stream) {
+  if (!a) return QL_ERR_NULL_POINTER;
+  if (a->rows < 0 || a->rows > INT_MAX / ql::smp::kMaxCtas || a->vocab < 1 || a->vocab > QL_SAMPLE_MAX_VOCAB)
+    return QL_ERR_BAD_SHAPE;
+  if (a->dtype != QL_DTYPE_F16 && a->dtype != QL_DTYPE_BF16 && a->dtype != QL_DTYPE_F32) return QL_ERR_UNSUPPORTED;
+  const size_t bytes = a->dtype == QL_DTYPE_F32 ? 4 : 2;
+  if (a->rows == 0) return QL_OK;
+  if (!a->logits || !a->uniform || !a->ids) return QL_ERR_NULL_POINTER;
+  if (a->row_stride < 0 || (a->rows > 1 && a->row_stride < a->vocab)) return QL_ERR_BAD_STRIDE;
+  if (!aligned(a->logits, bytes) || !aligned(a->uniform, 4) || !aligned(a->temperature, 4) || !aligned(a->top_k, 4) ||
+      !aligned(a->top_p, 4) || !aligned(a->min_p, 4) || !aligned(a->ids, 8) || !aligned(a->logprobs, 4))
+    return QL_ERR_UNSUPPORTED;
+  ql_host::Device dev;
+  const int st = ql_host::current(&dev);
+  if (st != QL_OK) return st;
+  ql::smp::Params p = {};
+  p.logits = a->logits;
+  p.uniform = static_cast<const float*>(a->uniform);
+  p.temperature = static_cast<const float*>(a->temperature);
+  p.top_k = static_cast<const int*>(a->top_k);
+  p.top_p = static_cast<const float*>(a->top_p);
+  p.min_p = static_cast<const float*>(a->min_p);
+  p.ids = static_cast<long long*>(a->ids);
+  p.logprobs = static_cast<float*>(a->logprobs);
+  p.temperature_all = a->temperature_all;
+  p.top_k_all = a->top_k_all;
+  p.top_p_all = a->top_p_all;
+  p.min_p_all = a->min_p_all;
+  p.stride = a->row_stride;
+  p.rows = (int)a->rows;
+  p.vocab = (int)a->vocab;
+  p.vec = aligned(a->logits, 16) && (a->rows == 1 || a->row_stride * (int64_t)bytes % 16 == 0);
+  switch (a->dtype) {
+    case QL_DTYPE_F16: return run_sample<__half>(p, dev.sms, stream, a->flags);
+    case QL_DTYPE_BF16: return run_sample<__nv_bfloat16>(p, dev.sms, stream, a->flags);
+    default: return run_sample<float>(p, dev.sms, stream, a->flags);
+  }
+}
+
+}  // extern "C"

@@ -40,6 +40,7 @@ QL_DEVICE_ERROR_TMEM = 4
 QL_DEVICE_ERROR_PEER_WAIT = 5
 QL_DEVICE_ERROR_BAD_INDEX = 6
 QL_XCHG_MAX_RANKS = 8
+QL_SAMPLE_MAX_VOCAB = 1 << 21
 
 QL_W4_LAYOUT_SPLIT_HALF = 0
 QL_W4_LAYOUT_ADJACENT = 1
@@ -106,6 +107,8 @@ SIGNATURES = {
     "ql_tree_attention_workspace_size": (_sz, [_i64]),
     "ql_capture_id": (ctypes.c_uint64, [_vp]),
     "ql_tree_attention": (_int, [ctypes.c_char_p, _vp]),
+    "ql_plan_step": (_int, [ctypes.c_char_p, _vp]),
+    "ql_sample_tokens": (_int, [ctypes.c_char_p, _vp]),
     "ql_strerror": (ctypes.c_char_p, [_int]),
     "ql_version": (_int, []),
     "ql_device_error": (_int, [ctypes.POINTER(_int)]),
@@ -120,6 +123,8 @@ ROTARY_ARGS = struct.Struct("18q")
 KV_APPEND_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 24}q")
 KV_READ_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 7}q")
 TREE_ATTENTION_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 18}qd3q")
+PLAN_STEP_ARGS = struct.Struct("17q")
+SAMPLE_TOKENS_ARGS = struct.Struct("13q3dq")
 
 _lock = threading.Lock()
 _lib = None
