@@ -461,6 +461,31 @@ size_t ql_tree_attention_workspace_size(int64_t head_dim);
 uint64_t ql_capture_id(void* stream);
 int ql_tree_attention(const ql_tree_attention_args* args, void* stream);
 
+/* --------------------------------------------- attention behind shared prefixes */
+/*
+ * ql_tree_attention where groups of requests begin with the same cached keys,
+ * read once for all rows of a group: row i of a request of group g sees the
+ * first prefix_lens[g] positions of pages prefix_table[g] (prefix_stride
+ * entries a row, prefix_width of them used), and then what `own` says:
+ * page_table and kv_lens there are of the request's own positions alone, which
+ * begin a page, its new tokens included.  The softmax is over both.
+ *   cu_group [groups + 1]: group g's requests are cu_group[g] ..
+ *     cu_group[g + 1] - 1, not decreasing; NULL (groups 1): all.  Requests of no
+ *     group have no prefix.
+ *   parts: ql_shared_attention_parts_size bytes, 16-byte aligned, for this
+ *     call alone until it is done; what it holds before does not matter.
+ *   max_prefix bounds the prefixes and only chooses the launch; own.max_kv is of
+ *     the requests' own positions.  own.lse is of both.
+ */
+typedef struct {
+  ql_tree_attention_args own;
+  const void *prefix_table, *prefix_lens, *cu_group;   /* int32 */
+  void* parts;
+  int64_t groups, prefix_width, prefix_stride, max_prefix, parts_bytes;
+} ql_shared_attention_args;
+size_t ql_shared_attention_parts_size(int64_t total_q, int64_t q_heads, int64_t head_dim);
+int ql_shared_attention(const ql_shared_attention_args* args, void* stream);
+
 /* ------------------------------------------------------- a serving step's plan */
 /*
  * Page tables, slots and positions of a step's new tokens, from the requests'

@@ -32,14 +32,33 @@ struct Params {
   kvc::Divisor by_group;
   float scale_log2;              // scale * log2(e): scores in units of log2
   unsigned* err;
+  // Attention behind shared prefixes takes two passes.  The first is over the prefixes: its requests are the groups
+  // that share one, every row sees every key, and what a row has (reference and sum, outputs) is left in fp32.  The
+  // second is over what the requests have of their own, and takes that in.
+  float2* early_sums;            // [total_q][q_heads]
+  float* early_out;              // [total_q][q_heads][head_dim]
+  const int* cu_group;           // the first pass: [batch + 1] requests, or null: all rows are one group's
+  int requests, first_pass;
 };
 
 struct Request {
   int q0, q_len, kv_len;
 };
+template <bool SHARED>
 __device__ __forceinline__ Request request(const Params& p, int b) {
   Request r;
-  if (p.cu_q) {
+  if (SHARED && p.first_pass && p.cu_group) {
+    const int per = p.cu_q ? 0 : p.total_q / p.requests;
+    auto row_of = [&](int request) {
+      const int at = min(max(request, 0), p.requests);
+      return p.cu_q ? min(max(p.cu_q[at], 0), p.total_q) : at * per;
+    };
+    r.q0 = row_of(p.cu_group[b]);
+    r.q_len = max(row_of(p.cu_group[b + 1]), r.q0) - r.q0;
+  } else if (SHARED && p.first_pass) {
+    r.q0 = 0;
+    r.q_len = p.total_q;
+  } else if (p.cu_q) {
     r.q0 = min(max(p.cu_q[b], 0), p.total_q);
     r.q_len = min(max(p.cu_q[b + 1], r.q0), p.total_q) - r.q0;
   } else {
@@ -50,8 +69,14 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.kv_len = (int)min((long long)max(p.kv_lens[b], 0), most);
   return r;
 }
+// Positions that every row sees: those before the request's new tokens.
+template <bool SHARED>
+__device__ __forceinline__ int context_of(const Params& p, const Request& r) {
+  return SHARED && p.first_pass ? r.kv_len : r.kv_len - r.q_len;
+}
+template <bool SHARED>
 __device__ __forceinline__ bool sees(const Params& p, const Request& r, int i, int j) {
-  const int d = j - (r.kv_len - r.q_len);        // which new token position j is
+  const int d = j - context_of<SHARED>(p, r);    // which new token position j is
   if (!p.mask) return d <= i;
   if (d < 0) return true;
   return d < 64 * p.mask_words && ((p.mask[(long long)(r.q0 + i) * p.mask_words + (d >> 6)] >> (d & 63)) & 1);
@@ -77,7 +102,7 @@ __device__ __forceinline__ long long request_units(const Params& p, const Reques
 // Sums the requests' units and finds the request that holds this CTA's first
 // unit: *b, the unit at which it begins, and its lengths.  All threads call
 // it; up to 32 requests each warp does so by itself.
-template <int ROWS, int MIN_UNITS, int THREADS>
+template <int ROWS, int MIN_UNITS, int THREADS, bool SHARED>
 __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* base, Request* r) {
   __shared__ long long warp_sum[THREADS / 32];
   __shared__ long long found_base;
@@ -96,7 +121,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
     Request mine = {0, 0, 0};
     long long units = 0;
     if (lane < p.batch) {
-      mine = request(p, lane);
+      mine = request<SHARED>(p, lane);
       units = request_units<ROWS, MIN_UNITS>(p, mine);
     }
     const long long incl = warp_scan(units);
@@ -129,7 +154,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
   long long mine = 0, incl = 0, sum;
   for (int i = 0; i < p.batch; i += THREADS) {
     const int at = i + threadIdx.x;
-    mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request(p, at)) : 0;
+    mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request<SHARED>(p, at)) : 0;
     incl = scan(mine, &sum);
     w.total += sum;
   }
@@ -140,7 +165,7 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
   for (int i = 0; i < p.batch; i += THREADS) {
     if (p.batch > THREADS) {                          // else mine, incl and sum are still these
       const int at = i + threadIdx.x;
-      mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request(p, at)) : 0;
+      mine = at < p.batch ? request_units<ROWS, MIN_UNITS>(p, request<SHARED>(p, at)) : 0;
       incl = scan(mine, &sum);
     }
     const long long from = before + incl - mine;
@@ -153,8 +178,22 @@ __device__ __forceinline__ Work find_work(const Params& p, int* b, long long* ba
   __syncthreads();
   *b = found_b;
   *base = found_base;
-  *r = request(p, *b);
+  *r = request<SHARED>(p, *b);
   return w;
+}
+
+// ------------------------------------------------- a row's parts of two passes
+// Rows that no group holds have nothing from the first pass.
+template <int THREADS>
+__device__ __forceinline__ void clear_early(const Params& p) {
+  if (!p.first_pass || !p.cu_group) return;
+  const Request first = request<true>(p, 0), last = request<true>(p, p.batch - 1);
+  const int from = first.q0, to = max(last.q0 + last.q_len, from);
+  const long long rest = (long long)(p.total_q - (to - from)) * p.q_heads;
+  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < rest; i += (long long)gridDim.x * THREADS) {
+    const long long before = (long long)from * p.q_heads;
+    p.early_sums[i < before ? i : i + (long long)(to - from) * p.q_heads] = make_float2(kLow, 0.f);
+  }
 }
 
 // ---------------------------------------------------------------- primitives
@@ -362,7 +401,7 @@ struct Shape {
   static constexpr size_t kSmem = 128 + (kRing > kJoined ? kRing : kJoined);
 };
 
-template <typename T, int D, int BITS, int NT>
+template <typename T, int D, int BITS, int NT, bool SHARED = false>
 __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     stream_kernel(const Params p, unsigned* counters, float* partials) {
   using S = Shape<D, BITS, NT>;
@@ -382,7 +421,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
   int b;
   long long base;
   Request r;
-  const Work work = find_work<S::kRows, kMinUnits, kThreads>(p, &b, &base, &r);
+  const Work work = find_work<S::kRows, kMinUnits, kThreads, SHARED>(p, &b, &base, &r);
+  if constexpr (SHARED) clear_early<kThreads>(p);
   if ((int)blockIdx.x >= work.ctas) return;
   long long u = work.first_unit(blockIdx.x);
   const long long u_end = work.first_unit(blockIdx.x + 1);
@@ -392,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     long long mine = request_units<S::kRows, kMinUnits>(p, r);
     while (u >= base + mine) {
       base += mine;
-      r = request(p, ++b);
+      r = request<SHARED>(p, ++b);
       mine = request_units<S::kRows, kMinUnits>(p, r);
     }
     const int per_item = item_units<kMinUnits>(r);
@@ -402,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     const int k_end = (int)min((long long)per_item, k_begin + (u_end - u));
     const int head = (int)Work::quotient(item, tiles), row0 = (int)(item - (long long)head * tiles) * S::kRows;
     const int rows = min(S::kRows, r.q_len * p.group - row0);
-    const int context = r.kv_len - r.q_len;             // positions that every row sees
+    const int context = context_of<SHARED>(p, r);
 
     // --------------------------------------------- this warp's tiles of 16 keys
     // tile i: keys j0(i) .. j0(i) + 15, within one page
@@ -672,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
             #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = j0 + g + (e >> 1) * 8, row = 8 * n + 2 * t + (e & 1);
-              const bool see = !hidden && j < r.kv_len && row < rows && sees(p, r, p.by_group.of(row0 + row), j);
+              const bool see = !hidden && j < r.kv_len && row < rows && sees<SHARED>(p, r, p.by_group.of(row0 + row), j);
               if (!see) d[n][e] = -INFINITY;
             }
         }
@@ -851,11 +891,27 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
     // Four neighbouring elements of a row are parked at `at`: those of lane group g = at / 4 % 8 and tiles 2 j,
     // 2 j + 1, j = at / 32, which are elements 4 j.. of its eighth (8 bits), or 4 (j % 2).. of its 8 in 64 j / 2 (4 bits).
-    auto finish = [&](int row, int place, const float4& o, float top, float sum) {
+    auto finish = [&](int row, int place, float4 o, float top, float sum) {
       const int pg = (place >> 2) & 7, j = place >> 5;
       const int d = BITS == 8 ? pg * (D / 8) + 4 * j : (j >> 1) * 64 + pg * 8 + 4 * (j & 1);
       const int token = p.by_group.of(row0 + row), qh = head * p.group + (row0 + row) - token * p.group;
       const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
+      if constexpr (SHARED) {
+        float4* early = reinterpret_cast<float4*>(p.early_out + at * D + d);
+        if (p.first_pass) {
+          *early = o;
+          if (place == 0) p.early_sums[at] = make_float2(top, sum);
+          return;
+        }
+        const float2 e = p.early_sums[at];
+        if (e.y != 0.f) {                               // there is something (a NaN too)
+          const float most = fmaxf(top, e.x), f0 = ex2<true>(top - most), f1 = ex2<true>(e.x - most);
+          const float4 v = *early;
+          top = most;
+          sum = sum * f0 + e.y * f1;
+          o = make_float4(o.x * f0 + v.x * f1, o.y * f0 + v.y * f1, o.z * f0 + v.z * f1, o.w * f0 + v.w * f1);
+        }
+      }
       const float f[4] = {o.x, o.y, o.z, o.w};
       kvc::Vec4<T> v;
       #pragma unroll

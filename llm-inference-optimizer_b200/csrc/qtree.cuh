@@ -194,8 +194,9 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 }
 
 // Which of 32 positions from j on row i of the request sees, as bits.
+template <bool SHARED>
 __device__ __forceinline__ unsigned sees32(const Params& p, const Request& r, int i, int j) {
-  const int d0 = j - (r.kv_len - r.q_len), left = r.kv_len - j;        // which new token j is; positions left
+  const int d0 = j - att::context_of<SHARED>(p, r), left = r.kv_len - j;        // which new token j is; positions left
   const auto low = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
   if (!p.mask) return low(min(left, i - d0 + 1));
   unsigned see = 0xFFFFFFFFu;
@@ -213,7 +214,7 @@ __device__ __forceinline__ unsigned sees32(const Params& p, const Request& r, in
   return see & low(left);
 }
 
-template <typename T, int D, int BITS>
+template <typename T, int D, int BITS, bool SHARED = false>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsigned* counters, float* partials) {
   using S = Shape<D, BITS>;
   using Slot = typename S::Slot;
@@ -244,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
   int b;
   long long base;
   Request r;
-  const Work work = att::find_work<kRows, kMinUnits, kThreads>(p, &b, &base, &r);
+  const Work work = att::find_work<kRows, kMinUnits, kThreads, SHARED>(p, &b, &base, &r);
+  if constexpr (SHARED) att::clear_early<kThreads>(p);
   if ((int)blockIdx.x >= work.ctas) return;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     long long mine = att::request_units<kRows, kMinUnits>(p, r);
     while (u >= base + mine) {
       base += mine;
-      r = att::request(p, ++b);
+      r = att::request<SHARED>(p, ++b);
       mine = att::request_units<kRows, kMinUnits>(p, r);
     }
     g.per_item = att::item_units<kMinUnits>(r);
@@ -588,12 +590,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
         wait(s_full + w, tile_steps + i, kDevErrFullWait);
         gemm::tc_fence_after();
         const unsigned bad = slot.bad;
-        const bool some_hidden = bad != 0 || j0 + S::kKeys > r.kv_len - r.q_len;
+        const bool some_hidden = bad != 0 || j0 + S::kKeys > att::context_of<SHARED>(p, r);
         const float v_top = fminf(fmaxf(__uint_as_float(max(max(slot.v_top[0], slot.v_top[1]), max(slot.v_top[2], slot.v_top[3]))),
                                         att::pow2((int)kLeast)), att::pow2((int)kMost));
         // the 32 positions of run c that the row sees, as bits
         auto seen = [&](int c) {
-          unsigned see = live ? sees32(p, r, token, j0 + c * 32) : 0u;
+          unsigned see = live ? sees32<SHARED>(p, r, token, j0 + c * 32) : 0u;
           if (bad >> (2 * c) & 1) see &= 0xFFFF0000u;
           if (bad >> (2 * c + 1) & 1) see &= 0x0000FFFFu;
           return see;
@@ -776,13 +778,45 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const long long out_at = (long long)(r.q0 + token) * p.q_heads + qh;
       auto finish = [&](int c, const float (&o)[32], float top, float l) {     // 32 outputs of the row
         if (!live) return;
+        float now = 1.f, then = 0.f;                        // what the two passes' outputs are taken with
+        if constexpr (SHARED) {
+          float4* early = reinterpret_cast<float4*>(p.early_out + out_at * D + c * 32);
+          if (p.first_pass) {
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) early[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            if (c == 0) p.early_sums[out_at] = make_float2(top, l);
+            return;
+          }
+          const float2 e = p.early_sums[out_at];
+          if (e.y != 0.f) {                                 // there is something (a NaN too)
+            const float most = fmaxf(top, e.x);
+            now = att::ex2<true>(top - most);
+            then = att::ex2<true>(e.x - most);
+            top = most;
+            l = l * now + e.y * then;
+          }
+        }
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        now *= inv;
+        then *= inv;
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_at * D + c * 32);
         #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float* f = o + 8 * e;
-          dst[e] = make_uint4(kvc::pack2<T>(f[0] * inv, f[1] * inv), kvc::pack2<T>(f[2] * inv, f[3] * inv),
-                              kvc::pack2<T>(f[4] * inv, f[5] * inv), kvc::pack2<T>(f[6] * inv, f[7] * inv));
+          float more[8] = {};
+          if (SHARED && then != 0.f) {
+            const float4* early = reinterpret_cast<const float4*>(p.early_out + out_at * D + c * 32 + 8 * e);
+            const float4 x = early[0], y = early[1];
+            const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) more[i] = v[i] * then;
+          }
+          uint32_t words[4];
+          #pragma unroll
+          for (int i = 0; i < 4; ++i)
+            words[i] = SHARED ? kvc::pack2<T>(fmaf(f[2 * i], now, more[2 * i]), fmaf(f[2 * i + 1], now, more[2 * i + 1]))
+                              : kvc::pack2<T>(f[2 * i] * now, f[2 * i + 1] * now);
+          dst[e] = make_uint4(words[0], words[1], words[2], words[3]);
         }
         if (p.lse && c == 0) p.lse[out_at] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.69314718056f;
       };

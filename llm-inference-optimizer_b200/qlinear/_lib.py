@@ -107,6 +107,8 @@ SIGNATURES = {
     "ql_tree_attention_workspace_size": (_sz, [_i64]),
     "ql_capture_id": (ctypes.c_uint64, [_vp]),
     "ql_tree_attention": (_int, [ctypes.c_char_p, _vp]),
+    "ql_shared_attention_parts_size": (_sz, [_i64, _i64, _i64]),
+    "ql_shared_attention": (_int, [ctypes.c_char_p, _vp]),
     "ql_plan_step": (_int, [ctypes.c_char_p, _vp]),
     "ql_sample_tokens": (_int, [ctypes.c_char_p, _vp]),
     "ql_strerror": (ctypes.c_char_p, [_int]),
@@ -123,6 +125,7 @@ ROTARY_ARGS = struct.Struct("18q")
 KV_APPEND_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 24}q")
 KV_READ_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 7}q")
 TREE_ATTENTION_ARGS = struct.Struct(f"{KV_CACHE_FIELDS + 18}qd3q")
+SHARED_ATTENTION_ARGS = struct.Struct(TREE_ATTENTION_ARGS.format + "9q")
 PLAN_STEP_ARGS = struct.Struct("17q")
 SAMPLE_TOKENS_ARGS = struct.Struct("13q3dq")
 
