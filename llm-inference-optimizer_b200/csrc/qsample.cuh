@@ -10,21 +10,34 @@
 // weights' running sum exceeds u times their sum W.  Its log-probability is
 // log(w_i / W).  T <= 0 takes the first of the order.
 //
-// All three filters keep a beginning of the order, so what is kept is known by
-// its last token: a value v and how many of the tokens equal to v are kept.
-// For top-k and top-p, v is the largest value whose measure F(v) over tokens
-// x >= v (their number; the sum of their weights) reaches a target: it is
-// searched for over the type's values in their order, which are whole numbers,
-// with four thresholds a round.  No sorting, no histogram, no atomics: each
-// thread keeps its logits in registers, and a round is a pass over those, a sum
-// over the CTA's threads and one over the cluster of CTAs that shares a row.
+// A cluster of CTAs shares a row.  Its first pass finds the largest logit; what
+// comes next depends on the row's filters:
+//   none            one pass sums the weights by blocks; the block that holds the
+//                   token is then read again.
+//   few are kept    a bound below the last token kept is found without reading the
+//                   row again: each thread's largest logit stands for the others
+//                   (k threads whose largest is >= v: k tokens are; if these tokens'
+//                   weights come to p of the sum, the kept ones lie at v and above),
+//                   and for min-p it is known.  One pass collects the tokens above
+//                   it in one CTA, which sorts them and does the rest.
+//   many are kept   all filters keep a beginning of the order, so what is kept is
+//                   known by its last token: a value v and how many of the tokens
+//                   equal to v are kept.  v is the largest value whose measure F(v)
+//                   over tokens x >= v (their number; the sum of their weights)
+//                   reaches a target: it is searched for over the type's values in
+//                   their order, which are whole numbers, with four thresholds a
+//                   round, each round a pass.
 //
-// Weights and sums are in fp64: a token is drawn, or not, by the comparison of
-// two running sums, and the sums of fp32 weights (2^-24 each) would decide one
-// row of some dozen over a large vocabulary otherwise than the definition does.
+// A token is drawn, or not, by the comparison of two running sums, so these are
+// held to more than fp32.  Sums over many weights are first taken, in fp64, of
+// weights in fp32, which says how they compare unless they come closer than
+// 2^-18.5 of themselves; then the weights are taken again in fp64.
 #pragma once
 
 #include <cuda_bf16.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "ql_common.cuh"
 
@@ -33,8 +46,10 @@ namespace smp {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;         // of a row: the largest cluster
-constexpr int kMaxPasses = 64;       // 16-byte loads a thread
+constexpr int kMaxPasses = 192;      // 16-byte loads a thread
 constexpr int kCuts = 4;             // thresholds of a round
+constexpr int kFew = 1024;           // tokens that one CTA sorts
+constexpr double kOff = 1.35e-6;     // 2^-19.5: what sums of fp32 weights may be off, of themselves
 
 struct Params {
   const void* logits;                // [rows][stride]
@@ -113,15 +128,49 @@ template <> struct Type<float> {
 __device__ __forceinline__ void st_dsmem_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
+__device__ __forceinline__ void st_dsmem_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_dsmem_u64(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t atom_dsmem_add(uint32_t addr, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+  return old;
+}
+
+// exp((x - top) / T) in fp64; infinity less itself counts as 0.
+__device__ __noinline__ double exact_weight(float x, float top, double inv_t) {
+  const double a = fmin(((double)x - (double)top) * inv_t, 0.0);
+  return a < -700.0 ? 0.0 : exp(a);
+}
 
 struct Shared {
-  double box[2][kMaxCtas][kCuts];    // what the cluster's CTAs have sent, in turn
-  double part[kWarps][kCuts];
-  double sums[kMaxCtas];
-  double block[kMaxPasses * kWarps];
-  double before;
-  long long index;
-  int owner, at;
+  union {                            // what the cluster's CTAs have sent, in turn
+    double f64[2][kMaxCtas][kCuts];
+    uint32_t u32[2][kMaxCtas][2 * kCuts];
+  } box;
+  union {
+    double f64[kWarps][kCuts];
+    uint32_t u32[kWarps][2 * kCuts];
+  } part;
+  union {
+    double block[kMaxPasses * kWarps];   // of many tokens: sums by runs of the warps
+    struct {                         // of few, in the cluster's first CTA
+      unsigned long long key[kFew];
+      double weight[kFew], upto[kFew];
+    } few;
+  };
+  double before, scan[kWarps];
+  unsigned long long found[kFew];    // tokens that this CTA has collected
+  unsigned here, at, count;          // their number, their place in the first CTA's list; the list's length
+  int owner, run, index, unsure;
 };
 
 // The CTA's part of a row, PASSES 16-byte runs a thread in registers (0: read
@@ -167,8 +216,22 @@ struct Part {
         f(v, x);
       }
     } else {
+      // four runs on their way at a time
+      constexpr int kAhead = 4;
+      int v = 0;
       #pragma unroll 1
-      for (int v = 0; v < passes; ++v) {
+      for (; v + kAhead <= passes; v += kAhead) {
+        uint4 r[kAhead];
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) r[i] = load(v + i);
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          Type<T>::decode(r[i], x);
+          f(v + i, x);
+        }
+      }
+      #pragma unroll 1
+      for (; v < passes; ++v) {
         Type<T>::decode(load(v), x);
         f(v, x);
       }
@@ -177,11 +240,8 @@ struct Part {
   __device__ __forceinline__ int index(int v) const { return first + (v * kThreads + (int)threadIdx.x) * kLanes; }
 };
 
-__device__ __forceinline__ double warp_sum(double v) {
-  #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+__device__ __forceinline__ unsigned order_of(float x) { return (unsigned)Type<float>::order(x); }
+__device__ __forceinline__ float value_of(unsigned k) { return Type<float>::value(k); }
 
 template <typename T, int PASSES>
 struct Sampler {
@@ -189,80 +249,136 @@ struct Sampler {
   Part<T, PASSES> part;
   Shared& sh;
   int rank, ctas, turn;              // turn: of the box's two sides
-  float top;                         // the row's largest logit
+  float top, mine;                   // the row's largest logit, this thread's
   double inv_t;
+  float scale_hi, scale_lo, low;     // log2(e) / T in two parts; x - top where weights end
 
-  __device__ __forceinline__ double weight(float x) const {
-    const double a = fmin(((double)x - (double)top) * inv_t, 0.0);      // infinity less itself: none
-    return a < -700.0 ? 0.0 : exp(a);
+  // ------------------------------------------------------------------ weights
+  // In fp32, 2^a with a = (x - top) log2(e) / T: a's nearest whole number n, and 2^(a - n), a - n being exact but for its
+  // last bits (two parts of the scale).  Weights end at 2^-100.  How far sums of them may be off, of themselves:
+  //   2^-22     each 2^(a - n), by ex2.approx
+  //   2^-20.5   x - top's rounding, 2^-24 |a| log(2) of each weight: over a sum that has the largest, 1, and up to 2^21 tokens
+  //             more, |a| weighs in with 16.3 at most (all of them at a = -18)
+  //   2^-22     four added in fp32, two such sums added
+  // together 1.2e-6; kOff is 1.35e-6.
+  __device__ __forceinline__ float weight(float x) const {
+    const float d = fmaxf(x - top, low);
+    const float m = fmaf(d, scale_hi, 12582912.f), n = m - 12582912.f;
+    const float rest = fmaf(d, scale_lo, fmaf(d, scale_hi, -n));
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(rest));
+    return __int_as_float(__float_as_int(w) + (__float_as_int(m) << 23));
+  }
+  template <bool EXACT>
+  __device__ __forceinline__ auto weigh(float x) const {
+    if constexpr (EXACT) return exact_weight(x, top, inv_t);
+    else return weight(x);
   }
 
-  // Sums over the cluster's threads, the same in all.  MAX: the largest instead.
-  template <int N, bool MAX = false>
-  __device__ __forceinline__ void all_sum(double (&v)[N]) {
+  // ------------------------------------------------- sums over the cluster
+  __device__ __forceinline__ void meet() {       // all threads of the cluster
+    if (ctas > 1) cluster_sync_all();
+    else __syncthreads();
+  }
+  // The same result in all threads.  `op` of a warp's 32 values, the same in all its lanes.
+  template <int N, typename Op>
+  __device__ __forceinline__ void all_u32(uint32_t (&v)[N], uint32_t none, Op op) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto add = [](double a, double b) { return MAX ? fmax(a, b) : a + b; };
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = add(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
+    for (int i = 0; i < N; ++i) v[i] = op(v[i]);
     if (lane == 0)
       #pragma unroll
-      for (int i = 0; i < N; ++i) sh.part[warp][i] = v[i];
+      for (int i = 0; i < N; ++i) sh.part.u32[warp][i] = v[i];
     __syncthreads();
     turn ^= 1;
     if (warp == 0) {
       #pragma unroll
       for (int i = 0; i < N; ++i) {
-        double s = sh.part[lane & (kWarps - 1)][i];
-        #pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) s = add(s, __shfl_xor_sync(0xffffffffu, s, o));
-        if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box[turn][rank][i]), (uint32_t)lane), s);
+        const uint32_t s = op(lane < kWarps ? sh.part.u32[lane][i] : none);
+        if (lane < ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][rank][i]), (uint32_t)lane), s);
       }
     }
-    cluster_sync_all();
+    meet();
+    #pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = op(lane < ctas ? sh.box.u32[turn][lane][i] : none);
+  }
+  template <int N>
+  __device__ __forceinline__ void all_count(uint32_t (&v)[N]) {
+    all_u32<N>(v, 0u, [](uint32_t x) { return __reduce_add_sync(0xffffffffu, x); });
+  }
+  __device__ __forceinline__ static double warp_sum(double v) {
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  template <int N>
+  __device__ __forceinline__ void all_sum(double (&v)[N]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = warp_sum(v[i]);
+      if (lane == 0) sh.part.f64[warp][i] = v[i];
+    }
+    __syncthreads();
+    turn ^= 1;
     if (warp == 0) {
       #pragma unroll
       for (int i = 0; i < N; ++i) {
-        double s = lane < ctas ? sh.box[turn][lane][i] : MAX ? -INFINITY : 0.0;
-        #pragma unroll
-        for (int o = kMaxCtas / 2; o > 0; o >>= 1) s = add(s, __shfl_xor_sync(0xffffffffu, s, o));
-        if (lane == 0) sh.sums[i] = s;
+        const double s = warp_sum(lane < kWarps ? sh.part.f64[lane][i] : 0.0);
+        if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][rank][i]), (uint32_t)lane), s);
       }
     }
-    __syncthreads();
+    meet();
     #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = sh.sums[i];
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < ctas ? sh.box.f64[turn][lane][i] : 0.0);
   }
 
-  // F at each threshold: the number of tokens x >= cut, or the sum of their weights.
-  template <bool MASS>
+  // F at each threshold: the number of tokens x >= cut, or the sum of their weights.  MINE: of the threads' largest alone.
+  template <bool MASS, bool EXACT, bool MINE = false>
   __device__ __forceinline__ void measure(const float (&cut)[kCuts], double (&f)[kCuts]) {
-    int n[kCuts] = {};
+    uint32_t n[kCuts] = {};
     #pragma unroll
     for (int i = 0; i < kCuts; ++i) f[i] = 0.0;
-    part.each([&](int, const float (&x)[kLanes]) {
+    if constexpr (MINE) {
       #pragma unroll
-      for (int e = 0; e < kLanes; ++e) {
-        const double w = MASS ? weight(x[e]) : 0.0;
+      for (int i = 0; i < kCuts; ++i)
+        if (mine >= cut[i]) {
+          ++n[i];
+          if (MASS) f[i] = (double)weight(mine);
+        }
+    } else {
+      part.each([&](int, const float (&x)[kLanes]) {
+        float s[2][kCuts] = {};
         #pragma unroll
-        for (int i = 0; i < kCuts; ++i)
-          if (x[e] >= cut[i]) {                              // not of a NaN
-            if (MASS) f[i] += w;
-            else ++n[i];
-          }
-      }
-    });
-    if (!MASS)
+        for (int e = 0; e < kLanes; ++e) {
+          const auto w = MASS ? weigh<EXACT>(x[e]) : 0.f;
+          #pragma unroll
+          for (int i = 0; i < kCuts; ++i)
+            if (x[e] >= cut[i]) {                            // not of a NaN
+              if (!MASS) ++n[i];
+              else if (EXACT) f[i] += w;
+              else s[e & 1][i] += w;
+            }
+        }
+        if (MASS && !EXACT)
+          #pragma unroll
+          for (int i = 0; i < kCuts; ++i) f[i] += (double)(s[0][i] + s[1][i]);
+      });
+    }
+    if constexpr (MASS) {
+      all_sum<kCuts>(f);
+    } else {
+      all_count<kCuts>(n);
       #pragma unroll
-      for (int i = 0; i < kCuts; ++i) f[i] = n[i];
-    all_sum<kCuts>(f);
+      for (int i = 0; i < kCuts; ++i) f[i] = (double)n[i];
+    }
   }
 
-  // The largest value whose F reaches `target`, from F(low) >= target on, and F of what lies above it.
-  template <bool MASS>
-  __device__ __forceinline__ float search(float low, double target, double* above) {
-    long long lo = Type<T>::order(low), hi = Type<T>::order(top) + 1;
+  // The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.  *unsure: a sum
+  // came too close to the target to tell.
+  template <bool MASS, bool EXACT>
+  __device__ __forceinline__ float search(float from, double target, double* above, bool* unsure) {
+    long long lo = Type<T>::order(from), hi = Type<T>::order(top) + 1;
     *above = 0.0;
     while (hi - lo > 1) {
       long long at[kCuts];
@@ -273,9 +389,10 @@ struct Sampler {
         at[i] = lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
         cut[i] = Type<T>::value(at[i]);
       }
-      measure<MASS>(cut, f);
+      measure<MASS, EXACT>(cut, f);
       #pragma unroll
       for (int i = 0; i < kCuts; ++i) {
+        if (MASS && !EXACT && fabs(f[i] - target) <= 2.0 * kOff * target) *unsure = true;
         if (f[i] >= target) {
           lo = max(lo, at[i]);
         } else if (at[i] < hi) {
@@ -287,44 +404,81 @@ struct Sampler {
     return Type<T>::value(lo);
   }
 
-  // The first token, by index, at which the running sum of weigh(x, index) exceeds target(sum), or the last
-  // that has a weight: found(index, weight, sum) in one thread of the cluster.
-  template <typename Weigh, typename Target, typename Found>
-  __device__ __forceinline__ double locate(Weigh weigh, Target target, Found found) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    part.each([&](int v, const float (&x)[kLanes]) {
-      double s = 0.0;
+  // A value v such that the threads' largest logits >= v number `target`, or weigh as much: not the largest such, but one
+  // with few of them above it.  False: there is none.
+  template <bool MASS>
+  __device__ __forceinline__ bool bound(float least, double target, float* v) {
+    long long lo = Type<T>::order(least), hi = Type<T>::order(top) + 1;
+    bool found = false;
+    for (int round = 0; round < 12; ++round) {
+      long long at[kCuts];
+      float cut[kCuts];
+      double f[kCuts];
       #pragma unroll
-      for (int e = 0; e < kLanes; ++e) s += weigh(x[e], part.index(v) + e);
-      s = warp_sum(s);
-      if (lane == 0) sh.block[v * kWarps + warp] = s;
+      for (int i = 0; i < kCuts; ++i) {
+        at[i] = round == 0 ? lo + (hi - lo) * i / kCuts : lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
+        cut[i] = Type<T>::value(at[i]);
+      }
+      measure<MASS, false, true>(cut, f);
+      double at_lo = INFINITY;
+      #pragma unroll
+      for (int i = 0; i < kCuts; ++i) {
+        if (f[i] >= target) {
+          found = true;
+          lo = max(lo, at[i]);
+          at_lo = f[i];
+        } else {
+          hi = min(hi, at[i]);
+        }
+      }
+      if (!found) return false;
+      if (hi - lo <= 1 || (MASS ? at_lo <= target * 1.01 : at_lo <= target * 1.25 + 16.0)) break;
+    }
+    *v = Type<T>::value(lo);
+    return true;
+  }
+
+  // ---------------------------------------------------------- many are kept
+  // The first token, by index, at which the running sum of weigh(x, index) exceeds target(sum), or the last that has a
+  // weight: found(index, x, sum) in one thread of the cluster.  Where a running sum comes closer to the target than sums
+  // that are `off` of themselves off can tell, sh.unsure is set in all CTAs, to be read behind the next meeting.
+  template <typename Weigh, typename Target, typename Found>
+  __device__ __forceinline__ double locate(double off, Weigh weigh, Target target, Found found) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // a block: a run of a warp
+    part.each([&](int v, const float (&x)[kLanes]) {
+      decltype(weigh(0.f, 0)) s[2] = {};
+      #pragma unroll
+      for (int e = 0; e < kLanes; ++e) s[e & 1] += weigh(x[e], part.index(v) + e);
+      const double all = warp_sum((double)(s[0] + s[1]));
+      if (lane == 0) sh.block[v * kWarps + warp] = all;
     });
     __syncthreads();
     turn ^= 1;
     const int blocks = part.passes * kWarps, per_lane = (blocks + 31) / 32;
-    double mine = 0.0, upto = 0.0;
+    double own = 0.0, upto = 0.0;
     if (warp == 0) {
       for (int i = 0; i < per_lane; ++i)
-        if (lane * per_lane + i < blocks) mine += sh.block[lane * per_lane + i];
-      upto = mine;
+        if (lane * per_lane + i < blocks) own += sh.block[lane * per_lane + i];
+      upto = own;
       #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double u = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += u;
       }
       const double all = __shfl_sync(0xffffffffu, upto, 31);
-      if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box[turn][rank][0]), (uint32_t)lane), all);
+      if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][rank][0]), (uint32_t)lane), all);
     }
-    cluster_sync_all();
+    meet();
     // each CTA finds whose part holds the token, by the same sums
+    double sum = 0.0;
+    for (int r = 0; r < ctas; ++r) sum += sh.box.f64[turn][r][0];
+    const double t = target(sum);
     if (warp == 0) {
-      double s = 0.0, before = 0.0;
-      for (int r = 0; r < ctas; ++r) s += sh.box[turn][r][0];
-      const double t = target(s);
       int owner = -1, last = 0;
-      double run = 0.0, last_before = 0.0;
+      double run = 0.0, before = 0.0, last_before = 0.0;
       for (int r = 0; r < ctas; ++r) {
-        const double w = sh.box[turn][r][0];
+        const double w = sh.box.f64[turn][r][0];
         if (w > 0.0) {
           last = r;
           last_before = run;
@@ -340,44 +494,36 @@ struct Sampler {
         before = last_before;
       }
       if (owner == rank) {
-        // of its blocks (a warp's tokens of one run), the one
-        const bool some = mine > 0.0;
-        const double from = before + (upto - mine);
-        unsigned past = __ballot_sync(0xffffffffu, some && before + upto > t), any = __ballot_sync(0xffffffffu, some);
-        const int pick = past ? __ffs(past) - 1 : 31 - __clz(any);
-        if (lane == pick) {
-          double at_sum = from, kept = from;
-          int at = -1;
+        const bool some = own > 0.0;
+        const unsigned past = __ballot_sync(0xffffffffu, some && before + upto > t), any = __ballot_sync(0xffffffffu, some);
+        if (lane == (past ? __ffs(past) - 1 : 31 - __clz(any))) {
+          double run = before + (upto - own), kept = run;
+          int at = 0;
           for (int i = lane * per_lane; i < min((lane + 1) * per_lane, blocks); ++i) {
             const double w = sh.block[i];
             if (w > 0.0) {
               at = i;
-              kept = at_sum;
-              if (at_sum + w > t) break;
+              kept = run;
+              if (run + w > t) break;
             }
-            at_sum += w;
+            run += w;
           }
-          sh.at = at;
+          sh.run = at;
           sh.before = kept;
-          sh.sums[1] = t;
         }
       }
-      if (lane == 0) {
-        sh.owner = owner;
-        sh.sums[0] = s;
-      }
+      if (lane == 0) sh.owner = owner;
     }
     __syncthreads();
-    const double sum = sh.sums[0];
-    if (sh.owner == rank && warp == sh.at % kWarps) {
-      const int v = sh.at / kWarps;
-      const double t = sh.sums[1], before = sh.before;
+    if (sh.owner == rank && warp == sh.run % kWarps) {
+      const int v = sh.run / kWarps;
+      const double before = sh.before;
       float x[kLanes];
       double w[kLanes], s = 0.0;
       Type<T>::decode(part.run(v), x);
       #pragma unroll
       for (int e = 0; e < kLanes; ++e) {
-        w[e] = weigh(x[e], part.index(v) + e);
+        w[e] = (double)weigh(x[e], part.index(v) + e);
         s += w[e];
       }
       double to = s;
@@ -388,37 +534,193 @@ struct Sampler {
       }
       const unsigned past = __ballot_sync(0xffffffffu, s > 0.0 && before + to > t), any = __ballot_sync(0xffffffffu, s > 0.0);
       if (lane == (past ? __ffs(past) - 1 : 31 - __clz(any))) {
-        double run = before + (to - s);
+        double run = before + (to - s), from = run, upto = run;
+        float x_pick = x[0];
         int pick = 0;
-        double w_pick = 0.0;
         bool done = false;
         #pragma unroll
         for (int e = 0; e < kLanes; ++e) {
           if (w[e] > 0.0 && !done) {
             pick = e;
-            w_pick = w[e];
-            done = run + w[e] > t;
+            x_pick = x[e];
+            from = run;
+            upto = run + w[e];
+            done = upto > t;
           }
           run += w[e];
         }
-        found(part.index(v) + pick, w_pick, sum);
+        if (off > 0.0 && (t - from <= 2.0 * off * t || upto - t <= 2.0 * off * t))
+          for (int r = 0; r < ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), (uint32_t)r), 1u);
+        found(part.index(v) + pick, x_pick, sum);
       }
     }
     return sum;
   }
+
+  // ----------------------------------------------------------- few are kept
+  // The tokens x >= cut, as (value, index) in the cluster's first CTA; how many there are (past kFew the list is cut off).
+  __device__ __forceinline__ unsigned collect(float cut) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) sh.here = sh.count = 0;
+    meet();
+    if (__any_sync(0xffffffffu, mine >= cut))
+      part.each([&](int v, const float (&x)[kLanes]) {
+        unsigned n = 0;
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e) n += x[e] >= cut;
+        if (!__any_sync(0xffffffffu, n > 0)) return;
+        unsigned to = n;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned u = __shfl_up_sync(0xffffffffu, to, o);
+          if (lane >= o) to += u;
+        }
+        unsigned at = 0;
+        if (lane == 31) at = atomicAdd(&sh.here, to);
+        at = __shfl_sync(0xffffffffu, at, 31) + to - n;
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e)
+          if (x[e] >= cut) {
+            if (at < kFew)
+              sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(part.index(v) + e));
+            ++at;
+          }
+      });
+    __syncthreads();
+    const uint32_t counter = dsmem_addr(smem_u32(&sh.count), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
+    if (threadIdx.x == 0 && sh.here > 0) sh.at = atom_dsmem_add(counter, sh.here);
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < sh.here && sh.at + i < kFew; i += kThreads) st_dsmem_u64(keys + (sh.at + i) * 8u, sh.found[i]);
+    meet();
+    return ld_dsmem_u32(counter);
+  }
+  // Sorts key[0 .. n), n <= kFew, from the largest down.
+  __device__ __forceinline__ void sort(unsigned n) {
+    unsigned size = 64;
+    while (size < n) size *= 2;
+    const unsigned pairs = size / 2, tid = threadIdx.x;
+    for (unsigned i = n + tid; i < size; i += kThreads) sh.few.key[i] = 0;
+    __syncthreads();
+    if (tid < 32 || pairs > 32) {
+      for (unsigned k = 2; k <= size; k *= 2)
+        for (unsigned j = k / 2; j > 0; j /= 2) {
+          if (tid < pairs) {
+            const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
+            const unsigned long long x = sh.few.key[a], y = sh.few.key[b];
+            if ((x < y) == ((a & k) == 0)) {
+              sh.few.key[a] = y;
+              sh.few.key[b] = x;
+            }
+          }
+          if (pairs > 32) __syncthreads();
+          else __syncwarp();
+        }
+    }
+    __syncthreads();
+  }
+  // Running sums of weight[0 .. n) to upto[0 .. n).
+  __device__ __forceinline__ void run_up(unsigned n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned i = 2 * threadIdx.x;
+    const double a = i < n ? sh.few.weight[i] : 0.0, b = i + 1 < n ? sh.few.weight[i + 1] : 0.0;
+    double s = a + b;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) sh.scan[warp] = s;
+    __syncthreads();
+    double before = 0.0;
+    for (int w = 0; w < warp; ++w) before += sh.scan[w];
+    if (i < n) sh.few.upto[i] = before + (s - b);
+    if (i + 1 < n) sh.few.upto[i + 1] = before + s;
+    __syncthreads();
+  }
+  // The rest, in the first CTA, of n tokens that hold all that are kept (and, where `of_few`, all whose weights the sum of
+  // top-p is over).  False: `sum` came too close to the weights before some token to tell whether that is kept.
+  __device__ __forceinline__ bool finish(unsigned n, long long top_k, double top_p, float cut, double sum, bool of_few, double off,
+                                         double u, long long* id, float* logprob) {
+    const unsigned tid = threadIdx.x;
+    const unsigned most = top_k > 0 && top_k < (long long)n ? (unsigned)top_k : n;
+    for (unsigned i = tid; i < n; i += kThreads) sh.few.weight[i] = exact_weight(value_of((unsigned)(sh.few.key[i] >> 32)), top, inv_t);
+    __syncthreads();
+    run_up(n);
+    if (of_few) sum = sh.few.upto[most - 1];
+    const double target = fmax(top_p, 0.0) * sum;
+    bool unsure = false;
+    int kept = 0;
+    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < most; ++i) {
+      const double before = i > 0 ? sh.few.upto[i - 1] : 0.0;
+      if (i > 0 && top_p < 1.0 && fabs(before - target) <= 2.0 * off * target) unsure = true;
+      if (i == 0 || ((top_p >= 1.0 || before < target) && value_of((unsigned)(sh.few.key[i] >> 32)) >= cut)) ++kept;
+    }
+    if (__syncthreads_or(unsure)) return false;
+    int all = 0;
+    {
+      const int s = (int)__reduce_add_sync(0xffffffffu, (unsigned)kept);
+      if ((tid & 31) == 0) sh.part.u32[tid >> 5][0] = (unsigned)s;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w) all += (int)sh.part.u32[w][0];
+    }
+    const double total = sh.few.upto[all - 1];
+    // what is kept, by index
+    unsigned long long mine2[2];
+    #pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const unsigned i = 2 * tid + q;
+      mine2[q] = i < (unsigned)all ? (sh.few.key[i] & 0xFFFFFFFFull) << 32 | (sh.few.key[i] >> 32) : 0ull;
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (2 * tid + q < (unsigned)all) sh.few.key[2 * tid + q] = mine2[q];
+    sort((unsigned)all);
+    for (unsigned i = tid; i < (unsigned)all; i += kThreads) sh.few.weight[i] = exact_weight(value_of((unsigned)sh.few.key[i]), top, inv_t);
+    __syncthreads();
+    run_up((unsigned)all);
+    const double t = u * total;
+    // the first whose running sum passes t, else the last that has a weight
+    unsigned pick = 0xFFFFFFFFu, last = 0;
+    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < (unsigned)all; ++i) {
+      if (sh.few.weight[i] > 0.0) {
+        last = i + 1;
+        if (sh.few.upto[i] > t) pick = min(pick, i);
+      }
+    }
+    pick = __reduce_min_sync(0xffffffffu, pick);
+    last = __reduce_max_sync(0xffffffffu, last);
+    __syncthreads();
+    if ((tid & 31) == 0) {
+      sh.part.u32[tid >> 5][0] = pick;
+      sh.part.u32[tid >> 5][1] = last;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kWarps; ++w) {
+        pick = min(pick, sh.part.u32[w][0]);
+        last = max(last, sh.part.u32[w][1]);
+      }
+      if (pick == 0xFFFFFFFFu) pick = last - 1;
+      *id = (long long)(0xFFFFFFFFu - (unsigned)(sh.few.key[pick] >> 32));
+      if (logprob) *logprob = (float)log(sh.few.weight[pick] / total);
+    }
+    return true;
+  }
 };
 
 template <typename T, int PASSES>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(const Params p) {
   __shared__ Shared sh;
   griddep_launch_dependents();
   griddep_wait();
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-  Sampler<T, PASSES> s = {{}, sh, (int)cluster_rank(), (int)ctas, 0, 0.f, 0.0};
+  Sampler<T, PASSES> s = {{}, sh, (int)cluster_rank(), (int)ctas};
   const int row = (int)(blockIdx.x / ctas);
   constexpr int kLanes = Type<T>::kLanes;
   const int runs = (p.vocab + kLanes - 1) / kLanes, mine = (runs + s.ctas - 1) / s.ctas;
+  s.turn = 0;
   s.part.first = min(s.rank * mine * kLanes, p.vocab);
   s.part.count = min(mine * kLanes, p.vocab - s.part.first);
   s.part.passes = PASSES > 0 ? PASSES : (mine + kThreads - 1) / kThreads;
@@ -427,104 +729,185 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   s.part.read();
 
   const double heat = p.temperature ? (double)p.temperature[row] : p.temperature_all;
-  double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_all;
-  double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_all;
+  const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_all;
+  const double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_all;
   const long long top_k = p.top_k ? (long long)p.top_k[row] : p.top_k_all;
-  const double u = (double)p.uniform[row];
+  const double u = fmin(fmax((double)p.uniform[row], 0.0), 1.0);
   const bool greedy = !(heat > 0.0);
+  const bool k_on = !greedy && top_k > 0 && top_k < p.vocab, p_on = !greedy && top_p < 1.0, m_on = !greedy && min_p > 0.0;
   s.inv_t = greedy ? 1.0 : 1.0 / heat;
 
-  float top = -INFINITY;
+  float most = -INFINITY;
   s.part.each([&](int, const float (&x)[kLanes]) {
     #pragma unroll
-    for (int e = 0; e < kLanes; ++e) top = fmaxf(top, x[e]);
+    for (int e = 0; e < kLanes; ++e) most = fmaxf(most, x[e]);
   });
-  double most[1] = {(double)top};
-  s.template all_sum<1, true>(most);
-  s.top = top = (float)most[0] + 0.f;
-  long long id = -1;
-  const bool empty = !(top > -INFINITY);
-  if (empty) {
+  s.mine = most = most + 0.f;
+  float least;
+  {
+    // the largest, and the least of the threads' largest (of those that have some)
+    uint32_t v[2] = {order_of(most), most > -INFINITY ? ~order_of(most) : 0u};
+    s.template all_u32<2>(v, 0u, [](uint32_t x) { return __reduce_max_sync(0xffffffffu, x); });
+    s.top = value_of(v[0]);
+    least = value_of(~v[1]);
+  }
+  const float top = s.top;
+  long long* id = p.ids + row;
+  float* logprob = p.logprobs ? p.logprobs + row : nullptr;
+  if (!(top > -INFINITY)) {
     if (s.rank == 0 && threadIdx.x == 0) {
-      p.ids[row] = -1;
-      if (p.logprobs) p.logprobs[row] = -INFINITY;
+      *id = -1;
+      if (logprob) *logprob = -INFINITY;
     }
-  } else {
-    // what is kept: x > edge, and the first `ties` tokens that equal it (all: infinity)
-    float edge = top == INFINITY ? top : Type<T>::lowest();
-    double ties = INFINITY;
-    if (greedy) {
-      edge = top;
-      ties = 1.0;
-    } else {
-      if (top_k > 0 && top_k < p.vocab) {
-        const float cut[kCuts] = {edge, top, top, top};
-        double n[kCuts];
-        s.template measure<false>(cut, n);
-        if (n[0] > (double)top_k) {
-          double above;
-          edge = s.template search<false>(edge, (double)top_k, &above);
-          ties = (double)top_k - above;
-        }
-      }
-      if (top_p < 1.0) {
-        // sums over what is kept so far: the tokens above `edge` and its ties, or all from `edge` on
-        const bool some = ties < INFINITY;
-        const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;   // NaN: nothing
-        const float cut[kCuts] = {from, top, NAN, NAN};
-        double f[kCuts], above;
-        s.template measure<true>(cut, f);
-        const double w_edge = s.weight(edge), target = fmax(top_p, 0.0) * (f[0] + (some ? ties * w_edge : 0.0));
-        if (f[1] >= target) {                            // the last one kept is one of the largest
-          edge = top;
-          ties = fmax(ceil(target), 1.0);
-        } else if (!some || f[0] >= target) {
-          edge = s.template search<true>(from, target, &above);
-          ties = fmax(ceil((target - above) / s.weight(edge)), 1.0);
-        } else {                                         // one of the ties at the edge of top-k
-          ties = fmin(ties, fmax(ceil((target - f[0]) / w_edge), 1.0));
-        }
-      }
-      if (min_p > 0.0) {
-        // w >= m where x >= max + T log m
-        const double low = (double)top + heat * log(fmin(min_p, 1.0));
-        float cut = __double2float_ru(low);
-        if (top == INFINITY) cut = top;
-        if (cut > edge) {
-          edge = cut;
-          ties = INFINITY;
-        }
-      }
+    return;                          // no CTA writes to another's shared memory any more
+  }
+  if (greedy) {
+    unsigned at = 0xFFFFFFFFu;
+    if (s.mine == top)
+      s.part.each([&](int v, const float (&x)[kLanes]) {
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e)
+          if (x[e] == top) at = min(at, (unsigned)(s.part.index(v) + e));
+      });
+    uint32_t v[1] = {at};
+    s.template all_u32<1>(v, 0xFFFFFFFFu, [](uint32_t x) { return __reduce_min_sync(0xffffffffu, x); });
+    if (s.rank == 0 && threadIdx.x == 0) {
+      *id = (long long)v[0];
+      if (logprob) *logprob = 0.f;
     }
-    // the index of the last tie kept
-    long long last = p.vocab;
-    if (ties < INFINITY) {
-      const double n = s.locate([&](float x, int i) { return x == edge ? 1.0 : 0.0; }, [&](double) { return ties - 1.0; },
-                                [&](int i, double, double) {
-                                  for (int r = 0; r < s.ctas; ++r) {
-                                    const uint32_t to = dsmem_addr(smem_u32(&sh.index), (uint32_t)r);
-                                    asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(to), "l"((long long)i) : "memory");
-                                  }
-                                });
-      cluster_sync_all();
-      if (n > ties) last = sh.index;
+    return;
+  }
+
+  const double scale = s.inv_t * 1.4426950408889634074;
+  s.scale_hi = (float)scale;
+  s.scale_lo = (float)(scale - (double)s.scale_hi);
+  s.low = fmaxf(-100.f / s.scale_hi, -3.402823466e38f);
+  // fp32 weights want a scale that fp32 can square, and no infinite logit
+  const bool fine = scale < 0x1p60 && scale > 0x1p-60 && top < INFINITY;
+  const float floor = top == INFINITY ? top : Type<T>::lowest();
+  // w >= min_p where x >= top + T log(min_p)
+  float cut = floor;
+  if (m_on && top < INFINITY) cut = fmaxf(floor, __double2float_ru((double)top + heat * log(fmin(min_p, 1.0))));
+  if (threadIdx.x == 0) sh.unsure = 0;
+
+  // ------------------------------------------------------------- few are kept
+  if (k_on || p_on || m_on) {
+    float from = floor;
+    bool known = p.vocab <= kFew;
+    double sum = 0.0, off = 0.0;
+    if (p_on && !k_on) {             // top-p's sum is over all tokens
+      const float cuts[kCuts] = {floor, NAN, NAN, NAN};
+      double f[kCuts];
+      if (fine) s.template measure<true, false>(cuts, f);
+      else s.template measure<true, true>(cuts, f);
+      sum = f[0];
+      off = fine ? kOff : 0.0;
     }
-    if (greedy) {
-      id = sh.index;
-      if (s.rank == 0 && threadIdx.x == 0) {
-        p.ids[row] = id;
-        if (p.logprobs) p.logprobs[row] = 0.f;
+    if (!known && m_on && !(k_on && p_on)) {
+      from = cut;
+      known = true;
+    }
+    unsigned n = kFew + 1;
+    if (known) n = s.collect(from);
+    if (n > kFew && k_on && top_k <= kFew / 2) {
+      known = s.template bound<false>(least, (double)top_k, &from);
+      if (known) n = s.collect(from);
+    } else if (n > kFew && p_on && !k_on && fine) {
+      known = s.template bound<true>(least, top_p * sum * (1.0 + 0x1p-16), &from);
+      if (known) n = s.collect(from);
+    }
+    if (n <= kFew) {
+      bool done = true;
+      if (s.rank == 0) {
+        s.sort(n);
+        done = s.finish(n, k_on ? top_k : 0, p_on ? top_p : 1.0, cut, sum, k_on, off, u, id, logprob);
+        if (!done && threadIdx.x == 0)
+          for (int r = 0; r < s.ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), (uint32_t)r), 1u);
       }
-    } else {
-      s.locate([&](float x, int i) { return x > edge || (x == edge && i <= last) ? s.weight(x) : 0.0; },
-               [&](double sum) { return fmin(fmax(u, 0.0), 1.0) * sum; },
-               [&](int i, double w, double sum) {
-                 p.ids[row] = i;
-                 if (p.logprobs) p.logprobs[row] = (float)log(w / sum);
-               });
+      s.meet();
+      if (off == 0.0 || !sh.unsure) return;
+      const float cuts[kCuts] = {floor, NAN, NAN, NAN};
+      double f[kCuts];
+      s.template measure<true, true>(cuts, f);
+      if (s.rank == 0) s.finish(n, 0, top_p, cut, f[0], false, 0.0, u, id, logprob);
+      return;
     }
   }
-  cluster_sync_all();                // no CTA leaves while another may write to its shared memory
+
+  // ------------------------------------------------------------ many are kept
+  // x > edge, and the first `ties` tokens that equal it (all: infinity); with weights in fp32, and once more in fp64 where
+  // these cannot tell
+  float k_edge = floor;
+  double k_ties = INFINITY, above;
+  bool unsure = false;
+  if (k_on) {
+    const float cuts[kCuts] = {floor, NAN, NAN, NAN};
+    double f[kCuts];
+    s.template measure<false, false>(cuts, f);
+    if (f[0] > (double)top_k) {
+      k_edge = s.template search<false, false>(floor, (double)top_k, &above, &unsure);
+      k_ties = (double)top_k - above;
+    }
+  }
+  auto draw = [&](auto exact) {
+    constexpr bool kExact = decltype(exact)::value;
+    const double off = kExact ? 0.0 : kOff;
+    float edge = k_edge;
+    double ties = k_ties;
+    if (p_on) {
+      // sums over what is kept so far: the tokens above `edge` and its ties, or all from `edge` on
+      const bool some = ties < INFINITY;
+      const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;     // NaN: nothing
+      const float cuts[kCuts] = {from, top, NAN, NAN};
+      double f[kCuts];
+      s.template measure<true, kExact>(cuts, f);
+      const double w_edge = exact_weight(edge, top, s.inv_t), target = fmax(top_p, 0.0) * (f[0] + (some ? ties * w_edge : 0.0));
+      auto number = [&](double mass, double w) {                       // of ties whose weights reach `mass`
+        const double n = mass / w;
+        if (!kExact && fabs(n - rint(n)) <= 4.0 * off * target / w) unsure = true;
+        return fmax(ceil(n), 1.0);
+      };
+      if (!kExact && (fabs(f[1] - target) <= 2.0 * off * target || fabs(f[0] - target) <= 2.0 * off * target)) unsure = true;
+      if (f[1] >= target) {                              // the last one kept is one of the largest
+        edge = top;
+        ties = number(target, 1.0);
+      } else if (!some || f[0] >= target) {
+        edge = s.template search<true, kExact>(from, target, &above, &unsure);
+        ties = number(target - above, exact_weight(edge, top, s.inv_t));
+      } else {                                           // one of the ties at the edge of top-k
+        ties = fmin(ties, number(target - f[0], w_edge));
+      }
+      if (unsure) return;
+    }
+    if (cut > edge) {
+      edge = cut;
+      ties = INFINITY;
+    }
+    // the index of the last tie kept
+    int last = p.vocab;
+    if (ties < INFINITY) {
+      const double n = s.locate(0.0, [&](float x, int) { return x == edge ? 1.f : 0.f; }, [&](double) { return ties - 1.0; },
+                                [&](int i, float, double) {
+                                  for (int r = 0; r < s.ctas; ++r)
+                                    st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), (uint32_t)r), (uint32_t)i);
+                                });
+      s.meet();
+      if (n > ties) last = sh.index;
+    }
+    s.locate(off, [&](float x, int i) { return x > edge || (x == edge && i <= last) ? s.template weigh<kExact>(x) : 0; },
+             [&](double sum) { return u * sum; },
+             [&](int i, float x, double sum) {
+               *id = i;
+               if (logprob) *logprob = (float)log(exact_weight(x, top, s.inv_t) / sum);
+             });
+    s.meet();
+    unsure = sh.unsure != 0;
+  };
+  if (fine) draw(std::false_type());
+  if (!fine || unsure) {
+    unsure = false;
+    draw(std::true_type());
+  }
 }
 
 }  // namespace smp

@@ -80,19 +80,20 @@ int run_sample(const ql::smp::Params& p, int ctas, void* stream, int64_t flags) 
   return launch_clusters(kernel, (unsigned)p.rows * ctas, (unsigned)ctas, ql::smp::kThreads, 0, stream, flags, p);
 }
 
+// A row's CTAs: as many as leave every SM one, up to a cluster's 16; no fewer than its passes allow.
 template <typename T>
 int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
+  constexpr bool kWide = sizeof(T) == 4;
   const int64_t runs = cdiv(p.vocab, ql::smp::Type<T>::kLanes);
+  auto passes = [&](int ctas) { return cdiv(cdiv(runs, ctas), ql::smp::kThreads); };
   int ctas = 1;
-  while (ctas < ql::smp::kMaxCtas && cdiv(runs, (int64_t)ctas * ql::smp::kThreads) > 3) ctas *= 2;
-  switch (cdiv(runs, (int64_t)ctas * ql::smp::kThreads)) {
-    case 1: return run_sample<T, 1>(p, ctas, stream, flags);
-    case 2: return run_sample<T, 2>(p, ctas, stream, flags);
-    case 3: return run_sample<T, 3>(p, ctas, stream, flags);
-    case 4:
-    case 5: return run_sample<T, 5>(p, ctas, stream, flags);
-    default: return run_sample<T, 0>(p, ctas, stream, flags);
-  }
+  while (ctas < ql::smp::kMaxCtas && ((int64_t)p.rows * ctas * 2 <= sms || passes(ctas) > ql::smp::kMaxPasses) && passes(ctas) > 1)
+    ctas *= 2;
+  const int64_t n = passes(ctas);
+  if (n <= 1) return run_sample<T, 1>(p, ctas, stream, flags);
+  if (n <= 3) return run_sample<T, 3>(p, ctas, stream, flags);
+  if (kWide && n <= 5) return run_sample<T, kWide ? 5 : 0>(p, ctas, stream, flags);
+  return run_sample<T, 0>(p, ctas, stream, flags);
 }
 
 }  // namespace
