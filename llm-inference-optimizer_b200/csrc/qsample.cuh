@@ -48,6 +48,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;         // of a row: the largest cluster
 constexpr int kMaxPasses = 192;      // 16-byte loads a thread
 constexpr int kCuts = 4;             // thresholds of a round
+constexpr int kMine = 16;            // thresholds of a round over the threads' largest logits
 constexpr int kFew = 1024;           // tokens that one CTA sorts
 constexpr double kOff = 1.35e-6;     // 2^-19.5: what sums of fp32 weights may be off, of themselves
 
@@ -151,14 +152,21 @@ __device__ __noinline__ double exact_weight(float x, float top, double inv_t) {
   return a < -700.0 ? 0.0 : exp(a);
 }
 
+// log(2)^k / k!: 2^r = sum over k of these times r^k.
+__host__ __device__ constexpr double taylor(int k) {
+  double c = 1.0;
+  for (int i = 1; i <= k; ++i) c *= 0.69314718055994530942 / i;
+  return c;
+}
+
 struct Shared {
   union {                            // what the cluster's CTAs have sent, in turn
     double f64[2][kMaxCtas][kCuts];
-    uint32_t u32[2][kMaxCtas][2 * kCuts];
+    uint32_t u32[2][kMaxCtas][kMine];
   } box;
   union {
     double f64[kWarps][kCuts];
-    uint32_t u32[kWarps][2 * kCuts];
+    uint32_t u32[kWarps][kMine];
   } part;
   union {
     double block[kMaxPasses * kWarps];   // of many tokens: sums by runs of the warps
@@ -169,8 +177,9 @@ struct Shared {
   };
   double before, scan[kWarps];
   unsigned long long found[kFew];    // tokens that this CTA has collected
-  unsigned here, at, count;          // their number, their place in the first CTA's list; the list's length
+  unsigned here[3], at, count[3];    // their number, their place in the first CTA's list; the list's length
   int owner, run, index, unsure;
+  float edge;
 };
 
 // The CTA's part of a row, PASSES 16-byte runs a thread in registers (0: read
@@ -250,8 +259,10 @@ struct Sampler {
   Shared& sh;
   int rank, ctas, turn;              // turn: of the box's two sides
   float top, mine;                   // the row's largest logit, this thread's
-  double inv_t;
-  float scale_hi, scale_lo, low;     // log2(e) / T in two parts; x - top where weights end
+  double inv_t, scale, top_scaled;   // 1 / T, log2(e) / T, and that times top
+  float scale_hi, scale_lo, low;     // log2(e) / T in two parts; x - top where fp32 weights end
+  float slow;                        // x - top below which fp64 weights take exact_weight
+  int collected;
 
   // ------------------------------------------------------------------ weights
   // In fp32, 2^a with a = (x - top) log2(e) / T: a's nearest whole number n, and 2^(a - n), a - n being exact but for its
@@ -269,9 +280,23 @@ struct Sampler {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(rest));
     return __int_as_float(__float_as_int(w) + (__float_as_int(m) << 23));
   }
+  // In fp64: the same, with the series of 2^r at |r| <= 1/2 up to r^11 (the rest is below 2^-46).  x becomes fp64 by its
+  // bits: the conversion's own instruction has a quarter of the rate.  (Numbers below fp32's normal ones, and 0, come out
+  // as one of their size: 2^-126 of a logit.)
+  __device__ __forceinline__ double weight64(float x) const {
+    if (!(x - top >= slow)) return exact_weight(x, top, inv_t);
+    const unsigned b = __float_as_uint(x);
+    const double wide = __hiloint2double((int)(((b & 0x7FFFFFFFu) >> 3) + (896u << 20) | (b & 0x80000000u)), (int)(b << 29));
+    const double a = fma(wide, scale, -top_scaled);
+    const double m = a + 6755399441055744.0, r = a - (m - 6755399441055744.0);
+    double y = taylor(11);
+    #pragma unroll
+    for (int k = 10; k >= 0; --k) y = fma(y, r, taylor(k));
+    return __hiloint2double(__double2hiint(y) + (__double2loint(m) << 20), __double2loint(y));
+  }
   template <bool EXACT>
   __device__ __forceinline__ auto weigh(float x) const {
-    if constexpr (EXACT) return exact_weight(x, top, inv_t);
+    if constexpr (EXACT) return weight64(x);
     else return weight(x);
   }
 
@@ -333,51 +358,41 @@ struct Sampler {
     for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < ctas ? sh.box.f64[turn][lane][i] : 0.0);
   }
 
-  // F at each threshold: the number of tokens x >= cut, or the sum of their weights.  MINE: of the threads' largest alone.
-  template <bool MASS, bool EXACT, bool MINE = false>
-  __device__ __forceinline__ void measure(const float (&cut)[kCuts], double (&f)[kCuts]) {
-    uint32_t n[kCuts] = {};
+  // F at each threshold: the number of tokens x >= cut, or the sum of their weights.
+  template <bool MASS, bool EXACT, int N>
+  __device__ __forceinline__ void measure(const float (&cut)[N], double (&f)[N]) {
+    uint32_t n[N] = {};
     #pragma unroll
-    for (int i = 0; i < kCuts; ++i) f[i] = 0.0;
-    if constexpr (MINE) {
+    for (int i = 0; i < N; ++i) f[i] = 0.0;
+    part.each([&](int, const float (&x)[kLanes]) {
+      float s[2][N] = {};
       #pragma unroll
-      for (int i = 0; i < kCuts; ++i)
-        if (mine >= cut[i]) {
-          ++n[i];
-          if (MASS) f[i] = (double)weight(mine);
-        }
-    } else {
-      part.each([&](int, const float (&x)[kLanes]) {
-        float s[2][kCuts] = {};
+      for (int e = 0; e < kLanes; ++e) {
+        const auto w = MASS ? weigh<EXACT>(x[e]) : 0.f;
         #pragma unroll
-        for (int e = 0; e < kLanes; ++e) {
-          const auto w = MASS ? weigh<EXACT>(x[e]) : 0.f;
-          #pragma unroll
-          for (int i = 0; i < kCuts; ++i)
-            if (x[e] >= cut[i]) {                            // not of a NaN
-              if (!MASS) ++n[i];
-              else if (EXACT) f[i] += w;
-              else s[e & 1][i] += w;
-            }
-        }
-        if (MASS && !EXACT)
-          #pragma unroll
-          for (int i = 0; i < kCuts; ++i) f[i] += (double)(s[0][i] + s[1][i]);
-      });
-    }
+        for (int i = 0; i < N; ++i)
+          if (x[e] >= cut[i]) {                            // not of a NaN
+            if (!MASS) ++n[i];
+            else if (EXACT) f[i] += w;
+            else s[e & 1][i] += w;
+          }
+      }
+      if (MASS && !EXACT)
+        #pragma unroll
+        for (int i = 0; i < N; ++i) f[i] += (double)(s[0][i] + s[1][i]);
+    });
     if constexpr (MASS) {
-      all_sum<kCuts>(f);
+      all_sum<N>(f);
     } else {
-      all_count<kCuts>(n);
+      all_count<N>(n);
       #pragma unroll
-      for (int i = 0; i < kCuts; ++i) f[i] = (double)n[i];
+      for (int i = 0; i < N; ++i) f[i] = (double)n[i];
     }
   }
 
-  // The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.  *unsure: a sum
-  // came too close to the target to tell.
-  template <bool MASS, bool EXACT>
-  __device__ __forceinline__ float search(float from, double target, double* above, bool* unsure) {
+  // The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.
+  template <bool MASS>
+  __device__ __forceinline__ float search(float from, double target, double* above) {
     long long lo = Type<T>::order(from), hi = Type<T>::order(top) + 1;
     *above = 0.0;
     while (hi - lo > 1) {
@@ -389,10 +404,9 @@ struct Sampler {
         at[i] = lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
         cut[i] = Type<T>::value(at[i]);
       }
-      measure<MASS, EXACT>(cut, f);
+      measure<MASS, MASS>(cut, f);
       #pragma unroll
       for (int i = 0; i < kCuts; ++i) {
-        if (MASS && !EXACT && fabs(f[i] - target) <= 2.0 * kOff * target) *unsure = true;
         if (f[i] >= target) {
           lo = max(lo, at[i]);
         } else if (at[i] < hi) {
@@ -405,34 +419,46 @@ struct Sampler {
   }
 
   // A value v such that the threads' largest logits >= v number `target`, or weigh as much: not the largest such, but one
-  // with few of them above it.  False: there is none.
+  // with few of them above it.  False: there is none.  Lane i looks after threshold i.
   template <bool MASS>
   __device__ __forceinline__ bool bound(float least, double target, float* v) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr float kUnit = 0x1p22f;                          // weights are counted in whole units: never too much
+    const uint32_t unit = MASS ? (uint32_t)(weight(mine) * kUnit) : 1u;
+    const double wanted = MASS ? target * (double)kUnit : target;
     long long lo = Type<T>::order(least), hi = Type<T>::order(top) + 1;
     bool found = false;
-    for (int round = 0; round < 12; ++round) {
-      long long at[kCuts];
-      float cut[kCuts];
-      double f[kCuts];
+    for (int round = 0; round < 10; ++round) {
+      const long long at = lo + (hi - lo) * (lane & (kMine - 1)) / kMine;
+      const float cut = Type<T>::value(at);
+      uint32_t f = 0;
       #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        at[i] = round == 0 ? lo + (hi - lo) * i / kCuts : lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
-        cut[i] = Type<T>::value(at[i]);
+      for (int i = 0; i < kMine; ++i) {
+        const bool over = mine >= __shfl_sync(0xffffffffu, cut, i);
+        const uint32_t n = MASS ? __reduce_add_sync(0xffffffffu, over ? unit : 0u) : __popc(__ballot_sync(0xffffffffu, over));
+        if (lane == i) f = n;
       }
-      measure<MASS, false, true>(cut, f);
-      double at_lo = INFINITY;
-      #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        if (f[i] >= target) {
-          found = true;
-          lo = max(lo, at[i]);
-          at_lo = f[i];
-        } else {
-          hi = min(hi, at[i]);
-        }
+      if (lane < kMine) sh.part.u32[warp][lane] = f;
+      __syncthreads();
+      turn ^= 1;
+      if (warp == 0 && lane < kMine) {
+        f = 0;
+        #pragma unroll
+        for (int w = 0; w < kWarps; ++w) f += sh.part.u32[w][lane];
+        for (int r = 0; r < ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][rank][lane]), (uint32_t)r), f);
       }
-      if (!found) return false;
-      if (hi - lo <= 1 || (MASS ? at_lo <= target * 1.01 : at_lo <= target * 1.25 + 16.0)) break;
+      meet();
+      double all = 0.0;
+      for (int r = 0; r < ctas; ++r) all += (double)sh.box.u32[turn][r][lane & (kMine - 1)];
+      const unsigned enough = __ballot_sync(0xffffffffu, lane < kMine && all >= wanted);
+      if (!found && !(enough & 1u)) return false;
+      found = true;                                           // of lo, and so of some threshold
+      const int pick = 31 - __clz(enough | 1u);
+      const long long next = __shfl_sync(0xffffffffu, at, (pick + 1) & (kMine - 1));
+      if (pick + 1 < kMine) hi = next;
+      lo = __shfl_sync(0xffffffffu, at, pick);
+      all = __shfl_sync(0xffffffffu, all, pick);
+      if (hi - lo <= 1 || (MASS ? all <= wanted * 1.02 : all <= wanted * 1.25 + 16.0)) break;
     }
     *v = Type<T>::value(lo);
     return true;
@@ -558,16 +584,17 @@ struct Sampler {
   }
 
   // ----------------------------------------------------------- few are kept
-  // The tokens x >= cut, as (value, index) in the cluster's first CTA; how many there are (past kFew the list is cut off).
-  __device__ __forceinline__ unsigned collect(float cut) {
+  // The tokens cut <= x < below, as (value, index) in the cluster's first CTA; how many there are (past kFew the list is
+  // cut off).  At most three times a row.
+  __device__ __forceinline__ unsigned collect(float cut, float below = NAN) {
     const int lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) sh.here = sh.count = 0;
-    meet();
+    unsigned *here = &sh.here[collected], *count = &sh.count[collected];
+    ++collected;
     if (__any_sync(0xffffffffu, mine >= cut))
       part.each([&](int v, const float (&x)[kLanes]) {
         unsigned n = 0;
         #pragma unroll
-        for (int e = 0; e < kLanes; ++e) n += x[e] >= cut;
+        for (int e = 0; e < kLanes; ++e) n += x[e] >= cut && !(x[e] >= below);
         if (!__any_sync(0xffffffffu, n > 0)) return;
         unsigned to = n;
         #pragma unroll
@@ -576,48 +603,75 @@ struct Sampler {
           if (lane >= o) to += u;
         }
         unsigned at = 0;
-        if (lane == 31) at = atomicAdd(&sh.here, to);
+        if (lane == 31) at = atomicAdd(here, to);
         at = __shfl_sync(0xffffffffu, at, 31) + to - n;
         #pragma unroll
         for (int e = 0; e < kLanes; ++e)
-          if (x[e] >= cut) {
+          if (x[e] >= cut && !(x[e] >= below)) {
             if (at < kFew)
               sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(part.index(v) + e));
             ++at;
           }
       });
     __syncthreads();
-    const uint32_t counter = dsmem_addr(smem_u32(&sh.count), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
-    if (threadIdx.x == 0 && sh.here > 0) sh.at = atom_dsmem_add(counter, sh.here);
+    const uint32_t counter = dsmem_addr(smem_u32(count), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
+    if (threadIdx.x == 0 && *here > 0) sh.at = atom_dsmem_add(counter, *here);
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < sh.here && sh.at + i < kFew; i += kThreads) st_dsmem_u64(keys + (sh.at + i) * 8u, sh.found[i]);
+    for (unsigned i = threadIdx.x; i < *here && sh.at + i < kFew; i += kThreads) st_dsmem_u64(keys + (sh.at + i) * 8u, sh.found[i]);
     meet();
     return ld_dsmem_u32(counter);
   }
-  // Sorts key[0 .. n), n <= kFew, from the largest down.
+  // Sorts key[0 .. n) from the largest down, and weight with it, n <= kFew.  Up to 128 by their ranks, four or eight threads
+  // counting the larger ones of each; else by merging (64: 1.3 us, by ranks 0.2).
   __device__ __forceinline__ void sort(unsigned n) {
-    unsigned size = 64;
-    while (size < n) size *= 2;
-    const unsigned pairs = size / 2, tid = threadIdx.x;
-    for (unsigned i = n + tid; i < size; i += kThreads) sh.few.key[i] = 0;
+    const unsigned tid = threadIdx.x;
+    auto& key = sh.few.key;
+    auto& weight = sh.few.weight;
     __syncthreads();
-    if (tid < 32 || pairs > 32) {
-      for (unsigned k = 2; k <= size; k *= 2)
-        for (unsigned j = k / 2; j > 0; j /= 2) {
-          if (tid < pairs) {
-            const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
-            const unsigned long long x = sh.few.key[a], y = sh.few.key[b];
-            if ((x < y) == ((a & k) == 0)) {
-              sh.few.key[a] = y;
-              sh.few.key[b] = x;
-            }
-          }
-          if (pairs > 32) __syncthreads();
-          else __syncwarp();
-        }
+    if (n <= kThreads / 4) {
+      const unsigned shift = n <= kThreads / 8 ? 3 : 2, i = tid >> shift, step = 1u << shift;
+      const unsigned long long k = i < n ? key[i] : 0;
+      const double w = i < n ? weight[i] : 0.0;
+      unsigned larger = 0;
+      for (unsigned j = tid & (step - 1); j < n; j += step) larger += key[j] > k;
+      #pragma unroll
+      for (unsigned o = 1; o < 4; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+      if (shift == 3) larger += __shfl_xor_sync(0xffffffffu, larger, 4);
+      __syncthreads();
+      if (i < n && (tid & (step - 1)) == 0) {
+        key[larger] = k;
+        weight[larger] = w;
+      }
+      __syncthreads();
+      return;
     }
+    unsigned size = kThreads / 2;
+    while (size < n) size *= 2;
+    for (unsigned i = n + tid; i < size; i += kThreads) key[i] = 0;
+    for (unsigned k = 2; k <= size; k *= 2)
+      for (unsigned j = k / 2; j > 0; j /= 2) {
+        __syncthreads();
+        if (tid < size / 2) {
+          const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
+          const unsigned long long x = key[a], y = key[b];
+          if ((x < y) == ((a & k) == 0)) {
+            key[a] = y;
+            key[b] = x;
+            const double w = weight[a];
+            weight[a] = weight[b];
+            weight[b] = w;
+          }
+        }
+      }
     __syncthreads();
   }
+  // Weights of key[0 .. n), and both sorted from the largest down.
+  __device__ __forceinline__ void sort_by_value(unsigned n) {
+    for (unsigned i = threadIdx.x; i < n; i += kThreads)
+      sh.few.weight[i] = weight64(value_of((unsigned)(sh.few.key[i] >> 32)));
+    sort(n);
+  }
+  __device__ __forceinline__ static int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
   // Running sums of weight[0 .. n) to upto[0 .. n).
   __device__ __forceinline__ void run_up(unsigned n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -637,74 +691,114 @@ struct Sampler {
     if (i + 1 < n) sh.few.upto[i + 1] = before + s;
     __syncthreads();
   }
-  // The rest, in the first CTA, of n tokens that hold all that are kept (and, where `of_few`, all whose weights the sum of
-  // top-p is over).  False: `sum` came too close to the weights before some token to tell whether that is kept.
+  // The sum of a count over the CTA.
+  __device__ __forceinline__ unsigned cta_count(unsigned n) {
+    n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.part.u32[threadIdx.x >> 5][0] = n;
+    __syncthreads();
+    n = 0;
+    #pragma unroll
+    for (int w = 0; w < kWarps; ++w) n += sh.part.u32[w][0];
+    return n;
+  }
+  // The rest, in the first CTA, of n tokens in order that hold all that are kept (and, where `of_few`, all whose weights the
+  // sum of top-p is over).  False: `sum` came too close to the weights before some token to tell whether that is kept.
   __device__ __forceinline__ bool finish(unsigned n, long long top_k, double top_p, float cut, double sum, bool of_few, double off,
                                          double u, long long* id, float* logprob) {
     const unsigned tid = threadIdx.x;
+    auto& key = sh.few.key;
+    auto& weight = sh.few.weight;
+    auto& upto = sh.few.upto;
     const unsigned most = top_k > 0 && top_k < (long long)n ? (unsigned)top_k : n;
-    for (unsigned i = tid; i < n; i += kThreads) sh.few.weight[i] = exact_weight(value_of((unsigned)(sh.few.key[i] >> 32)), top, inv_t);
-    __syncthreads();
     run_up(n);
-    if (of_few) sum = sh.few.upto[most - 1];
+    if (of_few) sum = upto[most - 1];
     const double target = fmax(top_p, 0.0) * sum;
     bool unsure = false;
-    int kept = 0;
+    unsigned kept = 0;
     for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < most; ++i) {
-      const double before = i > 0 ? sh.few.upto[i - 1] : 0.0;
+      const double before = i > 0 ? upto[i - 1] : 0.0;
       if (i > 0 && top_p < 1.0 && fabs(before - target) <= 2.0 * off * target) unsure = true;
-      if (i == 0 || ((top_p >= 1.0 || before < target) && value_of((unsigned)(sh.few.key[i] >> 32)) >= cut)) ++kept;
+      kept += i == 0 || ((top_p >= 1.0 || before < target) && value_of((unsigned)(key[i] >> 32)) >= cut);
     }
-    if (__syncthreads_or(unsure)) return false;
-    int all = 0;
-    {
-      const int s = (int)__reduce_add_sync(0xffffffffu, (unsigned)kept);
-      if ((tid & 31) == 0) sh.part.u32[tid >> 5][0] = (unsigned)s;
-      __syncthreads();
-      for (int w = 0; w < kWarps; ++w) all += (int)sh.part.u32[w][0];
-    }
-    const double total = sh.few.upto[all - 1];
-    // what is kept, by index
-    unsigned long long mine2[2];
-    #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const unsigned i = 2 * tid + q;
-      mine2[q] = i < (unsigned)all ? (sh.few.key[i] & 0xFFFFFFFFull) << 32 | (sh.few.key[i] >> 32) : 0ull;
-    }
-    __syncthreads();
-    #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (2 * tid + q < (unsigned)all) sh.few.key[2 * tid + q] = mine2[q];
-    sort((unsigned)all);
-    for (unsigned i = tid; i < (unsigned)all; i += kThreads) sh.few.weight[i] = exact_weight(value_of((unsigned)sh.few.key[i]), top, inv_t);
-    __syncthreads();
-    run_up((unsigned)all);
-    const double t = u * total;
+    if (__syncthreads_or(unsure && off > 0.0)) return false;
+    kept = cta_count(kept);
+    const double total = upto[kept - 1], t = u * total;
+    // by index
+    for (unsigned i = tid; i < kept; i += kThreads) key[i] = key[i] << 32;
+    sort(kept);
+    run_up(kept);
     // the first whose running sum passes t, else the last that has a weight
-    unsigned pick = 0xFFFFFFFFu, last = 0;
-    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < (unsigned)all; ++i) {
-      if (sh.few.weight[i] > 0.0) {
-        last = i + 1;
-        if (sh.few.upto[i] > t) pick = min(pick, i);
-      }
-    }
-    pick = __reduce_min_sync(0xffffffffu, pick);
-    last = __reduce_max_sync(0xffffffffu, last);
-    __syncthreads();
-    if ((tid & 31) == 0) {
-      sh.part.u32[tid >> 5][0] = pick;
-      sh.part.u32[tid >> 5][1] = last;
-    }
-    __syncthreads();
+    unsigned before = 0;
+    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= t;
+    unsigned pick = cta_count(before);
     if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) {
-        pick = min(pick, sh.part.u32[w][0]);
-        last = max(last, sh.part.u32[w][1]);
-      }
-      if (pick == 0xFFFFFFFFu) pick = last - 1;
-      *id = (long long)(0xFFFFFFFFu - (unsigned)(sh.few.key[pick] >> 32));
-      if (logprob) *logprob = (float)log(sh.few.weight[pick] / total);
+      if (pick >= kept) pick = kept - 1;
+      while (pick > 0 && !(weight[pick] > 0.0)) --pick;
+      *id = index_of(key[pick] >> 32);
+      if (logprob) *logprob = (float)log(weight[pick] / total);
     }
+    return true;
+  }
+
+  // The last token that top-p keeps of those x >= from (`more`: what top-k's ties add to their weights), where it lies among
+  // no more than kFew that fp32 weights cannot tell apart: those are collected and sorted, and the sum and what lies above
+  // them taken in fp64.  f: fp32's F(from) and F(top).  False: it does not.
+  __device__ __forceinline__ bool last_kept(float from, double more, double top_p, const double (&f)[2], float* edge, int* last) {
+    const double about = top_p * (f[0] + more), margin = 4.0 * kOff * about;
+    if (!(f[1] < about - margin) || !(f[0] > about + margin)) return false;
+    long long lo = Type<T>::order(from), hi = Type<T>::order(top);
+    for (int round = 0;; ++round) {
+      if (round >= 3 || hi - lo <= 1) {
+        const float cuts[2] = {Type<T>::value(lo), Type<T>::value(hi)};
+        double n[2];
+        measure<false, false>(cuts, n);
+        if (n[0] - n[1] <= (double)kFew) break;
+        if (hi - lo <= 1 || round >= 16) return false;
+      }
+      long long at[kCuts];
+      float cut[kCuts];
+      double g[kCuts];
+      #pragma unroll
+      for (int i = 0; i < kCuts; ++i) {
+        // first by the tokens' weights, from e^-12 to e^-1.5 of the largest
+        const long long there = round == 0 ? Type<T>::order(top - (float)((12.0 - 3.5 * i) / inv_t)) : lo + (hi - lo) * (i + 1) / (kCuts + 1);
+        at[i] = min(max(there, lo + 1), hi - 1);
+        cut[i] = Type<T>::value(at[i]);
+      }
+      measure<true, false>(cut, g);
+      bool moved = false;
+      #pragma unroll
+      for (int i = 0; i < kCuts; ++i) {
+        if (g[i] > about + margin && at[i] > lo) {
+          lo = at[i];
+          moved = true;
+        } else if (g[i] < about - margin && at[i] < hi) {
+          hi = at[i];
+          moved = true;
+        }
+      }
+      if (!moved && round >= 3) return false;                 // and more than kFew in between
+    }
+    const float cuts[2] = {from, Type<T>::value(hi)};
+    double g[2];
+    measure<true, true>(cuts, g);
+    const unsigned n = collect(Type<T>::value(lo), cuts[1]);
+    if (rank == 0) {
+      sort_by_value(n);
+      run_up(n);
+      const double target = top_p * (g[0] + more);
+      unsigned short_of = 0;
+      for (unsigned i = 2 * threadIdx.x; i < 2 * threadIdx.x + 2 && i < n; ++i) short_of += g[1] + sh.few.upto[i] < target;
+      const unsigned pick = min(cta_count(short_of), n - 1);
+      if (threadIdx.x < ctas) {
+        st_dsmem_u32(dsmem_addr(smem_u32(&sh.edge), threadIdx.x), __float_as_uint(value_of((unsigned)(sh.few.key[pick] >> 32))));
+        st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), threadIdx.x), (uint32_t)index_of(sh.few.key[pick]));
+      }
+    }
+    meet();
+    *edge = sh.edge;
+    *last = sh.index;
     return true;
   }
 };
@@ -721,6 +815,9 @@ __global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(c
   constexpr int kLanes = Type<T>::kLanes;
   const int runs = (p.vocab + kLanes - 1) / kLanes, mine = (runs + s.ctas - 1) / s.ctas;
   s.turn = 0;
+  s.collected = 0;
+  if (threadIdx.x < 3) sh.here[threadIdx.x] = sh.count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.unsure = 0;
   s.part.first = min(s.rank * mine * kLanes, p.vocab);
   s.part.count = min(mine * kLanes, p.vocab - s.part.first);
   s.part.passes = PASSES > 0 ? PASSES : (mine + kThreads - 1) / kThreads;
@@ -778,7 +875,9 @@ __global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(c
     return;
   }
 
-  const double scale = s.inv_t * 1.4426950408889634074;
+  const double scale = s.scale = s.inv_t * 1.4426950408889634074;
+  s.top_scaled = (double)top * scale;
+  s.slow = (float)(-680.0 * heat);
   s.scale_hi = (float)scale;
   s.scale_lo = (float)(scale - (double)s.scale_hi);
   s.low = fmaxf(-100.f / s.scale_hi, -3.402823466e38f);
@@ -788,126 +887,116 @@ __global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(c
   // w >= min_p where x >= top + T log(min_p)
   float cut = floor;
   if (m_on && top < INFINITY) cut = fmaxf(floor, __double2float_ru((double)top + heat * log(fmin(min_p, 1.0))));
-  if (threadIdx.x == 0) sh.unsure = 0;
+
+  double f[2] = {};                  // fp32's sums over all tokens, and over the largest
+  if (p_on && !k_on && fine) {
+    const float cuts[2] = {floor, top};
+    s.template measure<true, false>(cuts, f);
+  }
 
   // ------------------------------------------------------------- few are kept
   if (k_on || p_on || m_on) {
     float from = floor;
-    bool known = p.vocab <= kFew;
-    double sum = 0.0, off = 0.0;
-    if (p_on && !k_on) {             // top-p's sum is over all tokens
-      const float cuts[kCuts] = {floor, NAN, NAN, NAN};
-      double f[kCuts];
-      if (fine) s.template measure<true, false>(cuts, f);
-      else s.template measure<true, true>(cuts, f);
-      sum = f[0];
-      off = fine ? kOff : 0.0;
-    }
-    if (!known && m_on && !(k_on && p_on)) {
-      from = cut;
-      known = true;
-    }
     unsigned n = kFew + 1;
-    if (known) n = s.collect(from);
+    if (p.vocab <= kFew) {
+      n = s.collect(floor);
+    } else if (m_on && !(k_on && p_on)) {
+      n = s.collect(cut);
+    }
     if (n > kFew && k_on && top_k <= kFew / 2) {
-      known = s.template bound<false>(least, (double)top_k, &from);
-      if (known) n = s.collect(from);
+      if (s.template bound<false>(least, (double)top_k, &from)) n = s.collect(from);
     } else if (n > kFew && p_on && !k_on && fine) {
-      known = s.template bound<true>(least, top_p * sum * (1.0 + 0x1p-16), &from);
-      if (known) n = s.collect(from);
+      if (s.template bound<true>(least, top_p * f[0] * (1.0 + 0x1p-16), &from)) n = s.collect(from);
     }
     if (n <= kFew) {
-      bool done = true;
+      double sum = f[0], off = kOff;
+      if (p_on && !k_on && !fine) {
+        const float cuts[1] = {floor};
+        double all[1];
+        s.template measure<true, true>(cuts, all);
+        sum = all[0];
+        off = 0.0;
+      }
+      if (!p_on || k_on) off = 0.0;
       if (s.rank == 0) {
-        s.sort(n);
-        done = s.finish(n, k_on ? top_k : 0, p_on ? top_p : 1.0, cut, sum, k_on, off, u, id, logprob);
-        if (!done && threadIdx.x == 0)
-          for (int r = 0; r < s.ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), (uint32_t)r), 1u);
+        s.sort_by_value(n);
+        const bool done = s.finish(n, k_on ? top_k : 0, p_on ? top_p : 1.0, cut, sum, k_on, off, u, id, logprob);
+        if (!done && threadIdx.x < s.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), threadIdx.x), 1u);
       }
       s.meet();
       if (off == 0.0 || !sh.unsure) return;
-      const float cuts[kCuts] = {floor, NAN, NAN, NAN};
-      double f[kCuts];
-      s.template measure<true, true>(cuts, f);
-      if (s.rank == 0) s.finish(n, 0, top_p, cut, f[0], false, 0.0, u, id, logprob);
+      const float cuts[1] = {floor};
+      double all[1];
+      s.template measure<true, true>(cuts, all);
+      if (s.rank == 0) s.finish(n, 0, top_p, cut, all[0], false, 0.0, u, id, logprob);
       return;
     }
   }
 
   // ------------------------------------------------------------ many are kept
-  // x > edge, and the first `ties` tokens that equal it (all: infinity); with weights in fp32, and once more in fp64 where
-  // these cannot tell
-  float k_edge = floor;
-  double k_ties = INFINITY, above;
-  bool unsure = false;
+  // x > edge, and of the tokens that equal it the first `ties` (infinity: all), up to index `last`
+  float edge = floor;
+  double ties = INFINITY, above;
+  int last = p.vocab;
   if (k_on) {
-    const float cuts[kCuts] = {floor, NAN, NAN, NAN};
-    double f[kCuts];
-    s.template measure<false, false>(cuts, f);
-    if (f[0] > (double)top_k) {
-      k_edge = s.template search<false, false>(floor, (double)top_k, &above, &unsure);
-      k_ties = (double)top_k - above;
+    const float cuts[1] = {floor};
+    double n[1];
+    s.template measure<false, false>(cuts, n);
+    if (n[0] > (double)top_k) {
+      edge = s.template search<false>(floor, (double)top_k, &above);
+      ties = (double)top_k - above;
     }
+  }
+  if (p_on) {
+    // sums over what is kept so far: the tokens above `edge` and its ties, or all from `edge` on
+    const bool some = ties < INFINITY;
+    const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;     // NaN: nothing
+    const double w_edge = exact_weight(edge, top, s.inv_t), more = some ? ties * w_edge : 0.0;
+    const float cuts[2] = {from, top};
+    if (fine && k_on) s.template measure<true, false>(cuts, f);
+    if (fine && s.last_kept(from, more, fmax(top_p, 0.0), f, &edge, &last)) {
+      ties = INFINITY;
+    } else {
+      s.template measure<true, true>(cuts, f);
+      const double target = fmax(top_p, 0.0) * (f[0] + more);
+      if (f[1] >= target) {                              // the last one kept is one of the largest
+        edge = top;
+        ties = fmax(ceil(target), 1.0);
+      } else if (!some || f[0] >= target) {
+        edge = s.template search<true>(from, target, &above);
+        ties = fmax(ceil((target - above) / exact_weight(edge, top, s.inv_t)), 1.0);
+      } else {                                           // one of the ties at the edge of top-k
+        ties = fmin(ties, fmax(ceil((target - f[0]) / w_edge), 1.0));
+      }
+    }
+  }
+  if (cut > edge) {
+    edge = cut;
+    ties = INFINITY;
+    last = p.vocab;
+  }
+  if (ties < INFINITY) {
+    const double n = s.locate(0.0, [&](float x, int) { return x == edge ? 1.f : 0.f; }, [&](double) { return ties - 1.0; },
+                              [&](int i, float, double) {
+                                for (int r = 0; r < s.ctas; ++r)
+                                  st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), (uint32_t)r), (uint32_t)i);
+                              });
+    s.meet();
+    if (n > ties) last = sh.index;
   }
   auto draw = [&](auto exact) {
     constexpr bool kExact = decltype(exact)::value;
-    const double off = kExact ? 0.0 : kOff;
-    float edge = k_edge;
-    double ties = k_ties;
-    if (p_on) {
-      // sums over what is kept so far: the tokens above `edge` and its ties, or all from `edge` on
-      const bool some = ties < INFINITY;
-      const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;     // NaN: nothing
-      const float cuts[kCuts] = {from, top, NAN, NAN};
-      double f[kCuts];
-      s.template measure<true, kExact>(cuts, f);
-      const double w_edge = exact_weight(edge, top, s.inv_t), target = fmax(top_p, 0.0) * (f[0] + (some ? ties * w_edge : 0.0));
-      auto number = [&](double mass, double w) {                       // of ties whose weights reach `mass`
-        const double n = mass / w;
-        if (!kExact && fabs(n - rint(n)) <= 4.0 * off * target / w) unsure = true;
-        return fmax(ceil(n), 1.0);
-      };
-      if (!kExact && (fabs(f[1] - target) <= 2.0 * off * target || fabs(f[0] - target) <= 2.0 * off * target)) unsure = true;
-      if (f[1] >= target) {                              // the last one kept is one of the largest
-        edge = top;
-        ties = number(target, 1.0);
-      } else if (!some || f[0] >= target) {
-        edge = s.template search<true, kExact>(from, target, &above, &unsure);
-        ties = number(target - above, exact_weight(edge, top, s.inv_t));
-      } else {                                           // one of the ties at the edge of top-k
-        ties = fmin(ties, number(target - f[0], w_edge));
-      }
-      if (unsure) return;
-    }
-    if (cut > edge) {
-      edge = cut;
-      ties = INFINITY;
-    }
-    // the index of the last tie kept
-    int last = p.vocab;
-    if (ties < INFINITY) {
-      const double n = s.locate(0.0, [&](float x, int) { return x == edge ? 1.f : 0.f; }, [&](double) { return ties - 1.0; },
-                                [&](int i, float, double) {
-                                  for (int r = 0; r < s.ctas; ++r)
-                                    st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), (uint32_t)r), (uint32_t)i);
-                                });
-      s.meet();
-      if (n > ties) last = sh.index;
-    }
-    s.locate(off, [&](float x, int i) { return x > edge || (x == edge && i <= last) ? s.template weigh<kExact>(x) : 0; },
+    s.locate(kExact ? 0.0 : kOff,
+             [&](float x, int i) { return x > edge || (x == edge && i <= last) ? s.template weigh<kExact>(x) : 0; },
              [&](double sum) { return u * sum; },
              [&](int i, float x, double sum) {
                *id = i;
                if (logprob) *logprob = (float)log(exact_weight(x, top, s.inv_t) / sum);
              });
     s.meet();
-    unsure = sh.unsure != 0;
   };
   if (fine) draw(std::false_type());
-  if (!fine || unsure) {
-    unsure = false;
-    draw(std::true_type());
-  }
+  if (!fine || sh.unsure) draw(std::true_type());
 }
 
 }  // namespace smp
