@@ -31,7 +31,7 @@
 // A token is drawn, or not, by the comparison of two running sums, so these are
 // held to more than fp32.  Sums over many weights are first taken, in fp64, of
 // weights in fp32, which says how they compare unless they come closer than
-// 2^-18.5 of themselves; then the weights are taken again in fp64.
+// 2^-19.6 of themselves; then the weights are taken again in fp64.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -46,11 +46,13 @@ namespace smp {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;         // of a row: the largest cluster
-constexpr int kMaxPasses = 192;      // 16-byte loads a thread
 constexpr int kCuts = 4;             // thresholds of a round
 constexpr int kMine = 16;            // thresholds of a round over the threads' largest logits
 constexpr int kFew = 1024;           // tokens that one CTA sorts
-constexpr double kOff = 1.35e-6;     // 2^-19.5: what sums of fp32 weights may be off, of themselves
+constexpr int kFewer = kThreads / 4; // and those that it only compares with one another
+constexpr double kOff = 6e-7;        // what sums of fp32 weights may be off, of themselves
+constexpr int kBlocks = 3072;        // a row's part has no more than these runs of the warps
+constexpr int kStaged = 72 * 1024;   // bytes of a part that shared memory takes, two CTAs an SM
 
 struct Params {
   const void* logits;                // [rows][stride]
@@ -146,18 +148,90 @@ __device__ __forceinline__ uint32_t atom_dsmem_add(uint32_t addr, uint32_t v) {
   return old;
 }
 
-// exp((x - top) / T) in fp64; infinity less itself counts as 0.
-__device__ __noinline__ double exact_weight(float x, float top, double inv_t) {
-  const double a = fmin(((double)x - (double)top) * inv_t, 0.0);
-  return a < -700.0 ? 0.0 : exp(a);
-}
+__device__ __forceinline__ unsigned order_of(float x) { return (unsigned)Type<float>::order(x); }
+__device__ __forceinline__ float value_of(unsigned k) { return Type<float>::value(k); }
 
-// log(2)^k / k!: 2^r = sum over k of these times r^k.
-__host__ __device__ constexpr double taylor(int k) {
-  double c = 1.0;
-  for (int i = 1; i <= k; ++i) c *= 0.69314718055994530942 / i;
-  return c;
-}
+// A row's weights.  In fp32, with a = (x - top) log2(e) / T: 2^a from a whole number n near a, and 2^(a - n).  a - n is taken
+// of the unrounded product: x hi - (n + base) in one rounding, n + base being exact, plus x lo; what base leaves of top's
+// share is a factor on all of them, which sums get.  Weights end at 2^-100.  How far sums may be off, of themselves:
+//   2^-22     each 2^(a - n), by ex2.approx
+//   2^-24.5   a - n's two roundings
+//   2^-22.4   eight of them added in pairs in fp32 (fp64 from there)
+// together 4.6e-7; kOff is 6e-7.
+struct Weights {
+  float top, end;                    // the largest logit; where weights end
+  float hi, lo, bias, base;          // log2(e) / T in two parts; 1.5 * 2^23 less top's share as a whole number; that share
+  float zero;                        // where fp64 weights end: e^-700
+  double factor;                     // on sums
+  double inv_t, scale, share, high;  // 1 / T, log2(e) / T, top's share, top in fp64
+
+  __device__ __forceinline__ void set_heat(double heat) {
+    inv_t = 1.0 / heat;
+    scale = inv_t * 1.4426950408889634074;
+    hi = (float)scale;
+    lo = (float)(scale - (double)hi);
+  }
+  __device__ __forceinline__ void set_top(float largest, double heat) {
+    if (largest == INFINITY) hi = lo = 0.f, scale = inv_t = 0.0;          // the infinite ones alone, alike
+    top = largest;
+    share = largest == INFINITY ? 0.0 : (double)top * scale;
+    high = in64(top);
+    zero = fmaxf((float)((double)top - 700.0 * heat), -3.402823466e38f);
+    end = fmaxf((float)((double)top - 69.314718 * heat), -3.402823466e38f);
+    bias = 12582912.f - (float)rint(share);
+    // a multiple of so small a power of two as lets whole numbers be added exactly
+    const int e = max((__double2hiint(share) >> 20 & 0x7FF) - 1023, 7) - 21;      // (they are below 2^7)
+    const double up = __hiloint2double((1023 - e) << 20, 0), grid = __hiloint2double((1023 + e) << 20, 0);
+    base = (float)(rint(share * up) * grid);
+    factor = exp2((double)base - share);
+  }
+  // whether fp32 will do
+  __device__ __forceinline__ bool fine() const { return fabs(share) < 0x1p20 && scale < 0x1p40 && scale > 0x1p-40 && top < INFINITY; }
+
+  __device__ __forceinline__ void two(float x, float y, float& v, float& w) const {
+    const F2 m = fma2({x, y}, {hi, hi}, {bias, bias});
+    const F2 s = add2(fma2(m, {-1.f, -1.f}, {12582912.f, 12582912.f}), {-base, -base});
+    const F2 r = fma2({x, y}, {lo, lo}, fma2({x, y}, {hi, hi}, s));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(r.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(r.y));
+    v = x >= end ? __int_as_float(__float_as_int(v) + (__float_as_int(m.x) << 23)) : 0.f;      // 0 of a NaN
+    w = y >= end ? __int_as_float(__float_as_int(w) + (__float_as_int(m.y) << 23)) : 0.f;
+  }
+  __device__ __forceinline__ float one(float x) const {
+    float v, w;
+    two(x, x, v, w);
+    return v;
+  }
+  // In fp64, whose operations take eight times as long as fp32's: of (x - top) as it is, with n from fp32, and 2^(a - n) by
+  // its Chebyshev expansion up to the ninth power (2^-45; 1 of the largest, so that its ties are counted by whole numbers).
+  // Numbers become fp64 by their bits: the conversion's own instruction has a quarter of the rate.  (Numbers below fp32's
+  // normal ones, and 0, come out as one of their size: 2^-126 of a logit.)
+  __device__ __forceinline__ static double in64(float x) {
+    const unsigned b = __float_as_uint(x);
+    return __hiloint2double((int)(((b & 0x7FFFFFFFu) >> 3) + (896u << 20) | (b & 0x80000000u)), (int)(b << 29));
+  }
+  __device__ __forceinline__ double wide(float x) const {
+    const float m = fmaf(fmaxf(x - top, -3.402823466e38f), hi, 12582912.f);       // infinity less itself: a number
+    const double r = fma(in64(x) - high, scale, -in64(m - 12582912.f));
+    double y = 1.020869083593037e-07;
+    y = fma(y, r, 1.3259646250270451e-06);
+    y = fma(y, r, 1.5252657257186041e-05);
+    y = fma(y, r, 0.00015403433746224196);
+    y = fma(y, r, 0.0013333558230170627);
+    y = fma(y, r, 0.009618129193942167);
+    y = fma(y, r, 0.05550410866444768);
+    y = fma(y, r, 0.240226506956403);
+    y = fma(y, r, 0.69314718055995);
+    y = fma(y, r, 1.0);
+    return x >= zero ? __hiloint2double(__double2hiint(y) + (__float_as_int(m) << 20), __double2loint(y)) : 0.0;
+  }
+  // log(w / sum) of the weight of x: the sum's by its exponent, and the rest, 2/3 .. 4/3, in fp32 (2^-24 of at most 0.41)
+  __device__ __forceinline__ float log_chance(float x, double sum) const {
+    const int e = (__double2hiint(sum) + 0x000AAAAB >> 20) - 1023;
+    const float rest = (float)__hiloint2double(__double2hiint(sum) - (e << 20), __double2loint(sum));
+    return (float)((inv_t > 0.0 ? ((double)x - (double)top) * inv_t : 0.0) - ((double)logf(rest) + e * 0.69314718055994530942));
+  }
+};
 
 struct Shared {
   union {                            // what the cluster's CTAs have sent, in turn
@@ -169,690 +243,766 @@ struct Shared {
     uint32_t u32[kWarps][kMine];
   } part;
   union {
-    double block[kMaxPasses * kWarps];   // of many tokens: sums by runs of the warps
+    double block[kBlocks];           // of many tokens: sums by runs of the warps
     struct {                         // of few, in the cluster's first CTA
       unsigned long long key[kFew];
-      double weight[kFew], upto[kFew];
+      unsigned long long weight[kFew], upto[kFew];      // in units of 2^-52 of the largest weight
     } few;
   };
-  double before, scan[kWarps];
+  Weights weights;
+  double before;
+  unsigned long long scan[kWarps];
   unsigned long long found[kFew];    // tokens that this CTA has collected
   unsigned here[3], at, count[3];    // their number, their place in the first CTA's list; the list's length
   int owner, run, index, unsure;
   float edge;
 };
 
-// The CTA's part of a row, PASSES 16-byte runs a thread in registers (0: read
-// anew in every pass).  Run v of a thread lies v * kThreads runs behind its first.
-template <typename T, int PASSES>
-struct Part {
+__shared__ Shared sh;                // not an argument: a function that gets it as one reads it by generic addresses
+
+enum Kind { kCount, kMass, kExact }; // of a measure: the number of tokens, their weights in fp32, in fp64
+
+// What a CTA has of a row: the tokens first .. first + count - 1 at src, in 16-byte runs, of which thread t takes t,
+// t + kThreads ..; and its place in the cluster.
+template <typename T>
+struct Row {
   static constexpr int kLanes = Type<T>::kLanes;
-  uint4 raw[PASSES > 0 ? PASSES : 1];
   const T* src;
-  int first, count, passes;          // of the row: the part's first token, its tokens; runs a thread
-  bool vec;
+  int first, count, passes, rank, ctas;
+  float mine;                        // this thread's largest logit
+  bool vec;                          // runs are whole and aligned
 
   __device__ __forceinline__ uint4 load(int v) const {
     const int o = (v * kThreads + (int)threadIdx.x) * kLanes;
-    if (vec && o + kLanes <= count) return ldg_cg_v4(src + o);
+    if (vec && o + kLanes <= count) return *reinterpret_cast<const uint4*>(src + o);
     uint4 r;
     T* e = reinterpret_cast<T*>(&r);
     #pragma unroll
     for (int i = 0; i < kLanes; ++i) e[i] = o + i < count ? src[o + i] : (T)(-INFINITY);
     return r;
   }
-  __device__ __forceinline__ void read() {
-    if constexpr (PASSES > 0) {
-      #pragma unroll
-      for (int v = 0; v < PASSES; ++v) raw[v] = load(v);
-    }
-  }
-  __device__ __forceinline__ uint4 run(int v) const {
-    if constexpr (PASSES == 0) return load(v);
-    uint4 r = raw[0];
-    #pragma unroll
-    for (int i = 1; i < PASSES; ++i)
-      if (v == i) r = raw[i];
-    return r;
-  }
+  // f(run, its values), four runs on their way at a time
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {       // f(run, its values)
-    float x[kLanes];
-    if constexpr (PASSES > 0) {
+  __device__ __forceinline__ void each(F f) const {
+    constexpr int kAhead = 4;
+    #pragma unroll 1
+    for (int v = 0; v < passes; v += kAhead) {
+      uint4 r[kAhead];
       #pragma unroll
-      for (int v = 0; v < PASSES; ++v) {
-        Type<T>::decode(raw[v], x);
-        f(v, x);
-      }
-    } else {
-      // four runs on their way at a time
-      constexpr int kAhead = 4;
-      int v = 0;
-      #pragma unroll 1
-      for (; v + kAhead <= passes; v += kAhead) {
-        uint4 r[kAhead];
-        #pragma unroll
-        for (int i = 0; i < kAhead; ++i) r[i] = load(v + i);
-        #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          Type<T>::decode(r[i], x);
-          f(v + i, x);
-        }
-      }
-      #pragma unroll 1
-      for (; v < passes; ++v) {
-        Type<T>::decode(load(v), x);
-        f(v, x);
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i < passes) r[i] = load(v + i);
+      #pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (v + i >= passes) break;
+        float x[kLanes];
+        Type<T>::decode(r[i], x);
+        f(v + i, x);
       }
     }
   }
   __device__ __forceinline__ int index(int v) const { return first + (v * kThreads + (int)threadIdx.x) * kLanes; }
-};
-
-__device__ __forceinline__ unsigned order_of(float x) { return (unsigned)Type<float>::order(x); }
-__device__ __forceinline__ float value_of(unsigned k) { return Type<float>::value(k); }
-
-template <typename T, int PASSES>
-struct Sampler {
-  static constexpr int kLanes = Type<T>::kLanes;
-  Part<T, PASSES> part;
-  Shared& sh;
-  int rank, ctas, turn;              // turn: of the box's two sides
-  float top, mine;                   // the row's largest logit, this thread's
-  double inv_t, scale, top_scaled;   // 1 / T, log2(e) / T, and that times top
-  float scale_hi, scale_lo, low;     // log2(e) / T in two parts; x - top where fp32 weights end
-  float slow;                        // x - top below which fp64 weights take exact_weight
-  int collected;
-
-  // ------------------------------------------------------------------ weights
-  // In fp32, 2^a with a = (x - top) log2(e) / T: a's nearest whole number n, and 2^(a - n), a - n being exact but for its
-  // last bits (two parts of the scale).  Weights end at 2^-100.  How far sums of them may be off, of themselves:
-  //   2^-22     each 2^(a - n), by ex2.approx
-  //   2^-20.5   x - top's rounding, 2^-24 |a| log(2) of each weight: over a sum that has the largest, 1, and up to 2^21 tokens
-  //             more, |a| weighs in with 16.3 at most (all of them at a = -18)
-  //   2^-22     four added in fp32, two such sums added
-  // together 1.2e-6; kOff is 1.35e-6.
-  __device__ __forceinline__ float weight(float x) const {
-    const float d = fmaxf(x - top, low);
-    const float m = fmaf(d, scale_hi, 12582912.f), n = m - 12582912.f;
-    const float rest = fmaf(d, scale_lo, fmaf(d, scale_hi, -n));
-    float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(rest));
-    return __int_as_float(__float_as_int(w) + (__float_as_int(m) << 23));
-  }
-  // In fp64: the same, with the series of 2^r at |r| <= 1/2 up to r^11 (the rest is below 2^-46).  x becomes fp64 by its
-  // bits: the conversion's own instruction has a quarter of the rate.  (Numbers below fp32's normal ones, and 0, come out
-  // as one of their size: 2^-126 of a logit.)
-  __device__ __forceinline__ double weight64(float x) const {
-    if (!(x - top >= slow)) return exact_weight(x, top, inv_t);
-    const unsigned b = __float_as_uint(x);
-    const double wide = __hiloint2double((int)(((b & 0x7FFFFFFFu) >> 3) + (896u << 20) | (b & 0x80000000u)), (int)(b << 29));
-    const double a = fma(wide, scale, -top_scaled);
-    const double m = a + 6755399441055744.0, r = a - (m - 6755399441055744.0);
-    double y = taylor(11);
-    #pragma unroll
-    for (int k = 10; k >= 0; --k) y = fma(y, r, taylor(k));
-    return __hiloint2double(__double2hiint(y) + (__double2loint(m) << 20), __double2loint(y));
-  }
-  template <bool EXACT>
-  __device__ __forceinline__ auto weigh(float x) const {
-    if constexpr (EXACT) return weight64(x);
-    else return weight(x);
-  }
-
-  // ------------------------------------------------- sums over the cluster
-  __device__ __forceinline__ void meet() {       // all threads of the cluster
+  __device__ __forceinline__ void meet() const {             // all threads of the cluster
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
   }
-  // The same result in all threads.  `op` of a warp's 32 values, the same in all its lanes.
-  template <int N, typename Op>
-  __device__ __forceinline__ void all_u32(uint32_t (&v)[N], uint32_t none, Op op) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+};
+
+// ------------------------------------------------------- sums over the cluster
+// A warp's sums of N values (N 1, 2 or 4) with the fewest exchanges: of value i in the lanes 32 / N i .. 32 / N (i + 1) - 1.
+template <int N>
+__device__ __forceinline__ double warp_sums(const double (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  double a = v[0];
+  if constexpr (N == 4) {
+    const bool up = lane & 16, high = lane & 8;
+    const double b0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16), b1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+    const double c0 = (up ? v[2] : v[0]) + b0, c1 = (up ? v[3] : v[1]) + b1;
+    a = (high ? c1 : c0) + __shfl_xor_sync(0xffffffffu, high ? c0 : c1, 8);
+  } else if constexpr (N == 2) {
+    const bool up = lane & 16;
+    a = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+  }
+  #pragma unroll
+  for (int o = 16 / N; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
+// The same in all threads.
+template <typename T, int N>
+__device__ __forceinline__ void all_sum(const Row<T>& row, int& turn, double (&v)[N]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = lane * N / 32;
+  double s = warp_sums<N>(v);
+  if (lane % (32 / N) == 0) sh.part.f64[warp][i] = s;
+  __syncthreads();
+  turn ^= 1;
+  if (warp == 0) {
+    double w[N];
     #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = op(v[i]);
-    if (lane == 0)
-      #pragma unroll
-      for (int i = 0; i < N; ++i) sh.part.u32[warp][i] = v[i];
-    __syncthreads();
-    turn ^= 1;
-    if (warp == 0) {
-      #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t s = op(lane < kWarps ? sh.part.u32[lane][i] : none);
-        if (lane < ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][rank][i]), (uint32_t)lane), s);
-      }
+    for (int q = 0; q < N; ++q) w[q] = lane < kWarps ? sh.part.f64[lane][q] : 0.0;
+    s = warp_sums<N>(w);
+    #pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const double all = __shfl_sync(0xffffffffu, s, q * (32 / N));
+      if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][q]), (uint32_t)lane), all);
     }
-    meet();
+  }
+  row.meet();
+  double w[N];
+  #pragma unroll
+  for (int q = 0; q < N; ++q) w[q] = lane < row.ctas ? sh.box.f64[turn][lane][q] : 0.0;
+  s = warp_sums<N>(w);
+  #pragma unroll
+  for (int q = 0; q < N; ++q) v[q] = __shfl_sync(0xffffffffu, s, q * (32 / N));
+}
+// `op` of a warp's 32 values, the same in all its lanes; `none` changes nothing.
+template <typename T, int N, typename Op>
+__device__ __forceinline__ void all_u32(const Row<T>& row, int& turn, uint32_t (&v)[N], uint32_t none, Op op) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  #pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = op(v[i]);
+  if (lane == 0)
     #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = op(lane < ctas ? sh.box.u32[turn][lane][i] : none);
-  }
-  template <int N>
-  __device__ __forceinline__ void all_count(uint32_t (&v)[N]) {
-    all_u32<N>(v, 0u, [](uint32_t x) { return __reduce_add_sync(0xffffffffu, x); });
-  }
-  __device__ __forceinline__ static double warp_sum(double v) {
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  }
-  template <int N>
-  __device__ __forceinline__ void all_sum(double (&v)[N]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = 0; i < N; ++i) sh.part.u32[warp][i] = v[i];
+  __syncthreads();
+  turn ^= 1;
+  if (warp == 0) {
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = warp_sum(v[i]);
-      if (lane == 0) sh.part.f64[warp][i] = v[i];
+      const uint32_t s = op(lane < kWarps ? sh.part.u32[lane][i] : none);
+      if (lane < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][row.rank][i]), (uint32_t)lane), s);
     }
-    __syncthreads();
-    turn ^= 1;
-    if (warp == 0) {
-      #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const double s = warp_sum(lane < kWarps ? sh.part.f64[lane][i] : 0.0);
-        if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][rank][i]), (uint32_t)lane), s);
-      }
-    }
-    meet();
-    #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < ctas ? sh.box.f64[turn][lane][i] : 0.0);
   }
-
-  // F at each threshold: the number of tokens x >= cut, or the sum of their weights.
-  template <bool MASS, bool EXACT, int N>
-  __device__ __forceinline__ void measure(const float (&cut)[N], double (&f)[N]) {
-    uint32_t n[N] = {};
-    #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = 0.0;
-    part.each([&](int, const float (&x)[kLanes]) {
-      float s[2][N] = {};
+  row.meet();
+  #pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = op(lane < row.ctas ? sh.box.u32[turn][lane][i] : none);
+}
+// F at thresholds: the number of tokens x >= cut (not of a NaN), or the sum of their weights.  A function of its own for
+// each kind: the code is read from memory once a launch, and that is a good part of a short row's time.
+template <typename T, Kind KIND>
+__device__ __noinline__ double4 measure(const Row<T> row, int& turn, float4 at) {
+  constexpr int kLanes = Type<T>::kLanes;
+  const float cut[kCuts] = {at.x, at.y, at.z, at.w};
+  const Weights w = sh.weights;
+  double f[kCuts] = {};
+  if constexpr (KIND == kCount) {
+    uint32_t n[kCuts] = {};
+    row.each([&](int, const float (&x)[kLanes]) {
       #pragma unroll
-      for (int e = 0; e < kLanes; ++e) {
-        const auto w = MASS ? weigh<EXACT>(x[e]) : 0.f;
+      for (int e = 0; e < kLanes; ++e)
         #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (x[e] >= cut[i]) {                            // not of a NaN
-            if (!MASS) ++n[i];
-            else if (EXACT) f[i] += w;
-            else s[e & 1][i] += w;
-          }
-      }
-      if (MASS && !EXACT)
-        #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] += (double)(s[0][i] + s[1][i]);
+        for (int i = 0; i < kCuts; ++i) n[i] += x[e] >= cut[i];
     });
-    if constexpr (MASS) {
-      all_sum<N>(f);
-    } else {
-      all_count<N>(n);
-      #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = (double)n[i];
-    }
-  }
-
-  // The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.
-  template <bool MASS>
-  __device__ __forceinline__ float search(float from, double target, double* above) {
-    long long lo = Type<T>::order(from), hi = Type<T>::order(top) + 1;
-    *above = 0.0;
-    while (hi - lo > 1) {
-      long long at[kCuts];
-      float cut[kCuts];
-      double f[kCuts];
-      #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        at[i] = lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
-        cut[i] = Type<T>::value(at[i]);
-      }
-      measure<MASS, MASS>(cut, f);
-      #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        if (f[i] >= target) {
-          lo = max(lo, at[i]);
-        } else if (at[i] < hi) {
-          hi = at[i];
-          *above = f[i];
+    all_u32<T, kCuts>(row, turn, n, 0u, [](uint32_t v) { return __reduce_add_sync(0xffffffffu, v); });
+    return make_double4((double)n[0], (double)n[1], (double)n[2], (double)n[3]);
+  } else {
+    row.each([&](int, const float (&x)[kLanes]) {
+      if constexpr (KIND == kMass) {
+        float s[2][kCuts] = {};
+        #pragma unroll
+        for (int e = 0; e < kLanes; e += 2) {
+          float v[2];
+          w.two(x[e], x[e + 1], v[0], v[1]);
+          #pragma unroll
+          for (int i = 0; i < kCuts; ++i)
+            #pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (x[e + q] >= cut[i]) s[q][i] += v[q];
+        }
+        #pragma unroll
+        for (int i = 0; i < kCuts; ++i) f[i] += (double)(s[0][i] + s[1][i]);
+      } else {
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e) {
+          const double v = w.wide(x[e]);
+          #pragma unroll
+          for (int i = 0; i < kCuts; ++i) f[i] += x[e] >= cut[i] ? v : 0.0;
         }
       }
-    }
-    return Type<T>::value(lo);
+    });
+    all_sum<T, kCuts>(row, turn, f);
+    const double by = KIND == kMass ? w.factor : 1.0;
+    return make_double4(f[0] * by, f[1] * by, f[2] * by, f[3] * by);
   }
+}
 
-  // A value v such that the threads' largest logits >= v number `target`, or weigh as much: not the largest such, but one
-  // with few of them above it.  False: there is none.  Lane i looks after threshold i.
-  template <bool MASS>
-  __device__ __forceinline__ bool bound(float least, double target, float* v) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr float kUnit = 0x1p22f;                          // weights are counted in whole units: never too much
-    const uint32_t unit = MASS ? (uint32_t)(weight(mine) * kUnit) : 1u;
-    const double wanted = MASS ? target * (double)kUnit : target;
-    long long lo = Type<T>::order(least), hi = Type<T>::order(top) + 1;
-    bool found = false;
-    for (int round = 0; round < 10; ++round) {
-      const long long at = lo + (hi - lo) * (lane & (kMine - 1)) / kMine;
-      const float cut = Type<T>::value(at);
-      uint32_t f = 0;
-      #pragma unroll
+// The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.
+template <typename T, Kind KIND>
+__device__ __forceinline__ float search(const Row<T>& row, int& turn, float from, double target, double* above) {
+  long long lo = Type<T>::order(from), hi = Type<T>::order(sh.weights.top) + 1;
+  *above = 0.0;
+  while (hi - lo > 1) {
+    long long at[kCuts];
+    #pragma unroll
+    for (int i = 0; i < kCuts; ++i) at[i] = lo + max((hi - lo) * (i + 1) / (kCuts + 1), 1ll);
+    const double4 g = measure<T, KIND>(row, turn, make_float4(Type<T>::value(at[0]), Type<T>::value(at[1]),
+                                                                  Type<T>::value(at[2]), Type<T>::value(at[3])));
+    const double f[kCuts] = {g.x, g.y, g.z, g.w};
+    #pragma unroll
+    for (int i = 0; i < kCuts; ++i) {
+      if (f[i] >= target) {
+        lo = max(lo, at[i]);
+      } else if (at[i] < hi) {
+        hi = at[i];
+        *above = f[i];
+      }
+    }
+  }
+  return Type<T>::value(lo);
+}
+
+// A value v such that the threads' largest logits >= v number `target`, or weigh as much: not the largest such, but one
+// with few of them above it.  False: there is none.  Lane i looks after threshold i.
+template <typename T>
+__device__ __noinline__ bool bound(const Row<T> row, int& turn, bool mass, float least, double target, float* v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float top = sh.weights.top;
+  constexpr double kUnit = 0x1p22;                            // weights are counted in whole units: never too much
+  const uint32_t unit = mass ? (uint32_t)((double)sh.weights.one(row.mine) * (sh.weights.factor * kUnit)) : 1u;
+  const double wanted = mass ? target * kUnit : target, enough_of = mass ? wanted * 1.02 : wanted * 1.25 + 16.0;
+  long long lo = Type<T>::order(least), hi = Type<T>::order(top) + 1;
+  bool found = false;
+  #pragma unroll 1
+  for (int round = 0; round < 10; ++round) {
+    const long long at = lo + (hi - lo) * (lane & (kMine - 1)) / kMine;
+    const float cut = Type<T>::value(at);
+    uint32_t f = 0;
+    if (mass) {
+      #pragma unroll 4
       for (int i = 0; i < kMine; ++i) {
-        const bool over = mine >= __shfl_sync(0xffffffffu, cut, i);
-        const uint32_t n = MASS ? __reduce_add_sync(0xffffffffu, over ? unit : 0u) : __popc(__ballot_sync(0xffffffffu, over));
+        const uint32_t n = __reduce_add_sync(0xffffffffu, row.mine >= __shfl_sync(0xffffffffu, cut, i) ? unit : 0u);
         if (lane == i) f = n;
       }
-      if (lane < kMine) sh.part.u32[warp][lane] = f;
-      __syncthreads();
-      turn ^= 1;
-      if (warp == 0 && lane < kMine) {
-        f = 0;
-        #pragma unroll
-        for (int w = 0; w < kWarps; ++w) f += sh.part.u32[w][lane];
-        for (int r = 0; r < ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][rank][lane]), (uint32_t)r), f);
+    } else {
+      #pragma unroll 4
+      for (int i = 0; i < kMine; ++i) {
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, row.mine >= __shfl_sync(0xffffffffu, cut, i)));
+        if (lane == i) f = n;
       }
-      meet();
-      double all = 0.0;
-      for (int r = 0; r < ctas; ++r) all += (double)sh.box.u32[turn][r][lane & (kMine - 1)];
-      const unsigned enough = __ballot_sync(0xffffffffu, lane < kMine && all >= wanted);
-      if (!found && !(enough & 1u)) return false;
-      found = true;                                           // of lo, and so of some threshold
-      const int pick = 31 - __clz(enough | 1u);
-      const long long next = __shfl_sync(0xffffffffu, at, (pick + 1) & (kMine - 1));
-      if (pick + 1 < kMine) hi = next;
-      lo = __shfl_sync(0xffffffffu, at, pick);
-      all = __shfl_sync(0xffffffffu, all, pick);
-      if (hi - lo <= 1 || (MASS ? all <= wanted * 1.02 : all <= wanted * 1.25 + 16.0)) break;
     }
-    *v = Type<T>::value(lo);
-    return true;
-  }
-
-  // ---------------------------------------------------------- many are kept
-  // The first token, by index, at which the running sum of weigh(x, index) exceeds target(sum), or the last that has a
-  // weight: found(index, x, sum) in one thread of the cluster.  Where a running sum comes closer to the target than sums
-  // that are `off` of themselves off can tell, sh.unsure is set in all CTAs, to be read behind the next meeting.
-  template <typename Weigh, typename Target, typename Found>
-  __device__ __forceinline__ double locate(double off, Weigh weigh, Target target, Found found) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // a block: a run of a warp
-    part.each([&](int v, const float (&x)[kLanes]) {
-      decltype(weigh(0.f, 0)) s[2] = {};
-      #pragma unroll
-      for (int e = 0; e < kLanes; ++e) s[e & 1] += weigh(x[e], part.index(v) + e);
-      const double all = warp_sum((double)(s[0] + s[1]));
-      if (lane == 0) sh.block[v * kWarps + warp] = all;
-    });
+    if (lane < kMine) sh.part.u32[warp][lane] = f;
     __syncthreads();
     turn ^= 1;
-    const int blocks = part.passes * kWarps, per_lane = (blocks + 31) / 32;
-    double own = 0.0, upto = 0.0;
-    if (warp == 0) {
-      for (int i = 0; i < per_lane; ++i)
-        if (lane * per_lane + i < blocks) own += sh.block[lane * per_lane + i];
-      upto = own;
+    if (warp == 0 && lane < kMine) {
+      f = 0;
       #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double u = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += u;
-      }
-      const double all = __shfl_sync(0xffffffffu, upto, 31);
-      if (lane < ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][rank][0]), (uint32_t)lane), all);
+      for (int w = 0; w < kWarps; ++w) f += sh.part.u32[w][lane];
+      #pragma unroll
+      for (int r = 0; r < kMaxCtas; ++r)
+        if (r < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][row.rank][lane]), (uint32_t)r), f);
     }
-    meet();
-    // each CTA finds whose part holds the token, by the same sums
-    double sum = 0.0;
-    for (int r = 0; r < ctas; ++r) sum += sh.box.f64[turn][r][0];
-    const double t = target(sum);
+    row.meet();
+    unsigned long long sum = 0;
+    #pragma unroll
+    for (int r = 0; r < kMaxCtas; ++r) sum += r < row.ctas ? sh.box.u32[turn][r][lane & (kMine - 1)] : 0u;
+    double all = (double)sum;
+    const unsigned enough = __ballot_sync(0xffffffffu, lane < kMine && all >= wanted);
+    if (!found && !(enough & 1u)) return false;
+    found = true;                                             // of lo, and so of some threshold
+    const int pick = 31 - __clz(enough | 1u);
+    const long long next = __shfl_sync(0xffffffffu, at, (pick + 1) & (kMine - 1));
+    if (pick + 1 < kMine) hi = next;
+    lo = __shfl_sync(0xffffffffu, at, pick);
+    all = __shfl_sync(0xffffffffu, all, pick);
+    if (hi - lo <= 1 || all <= enough_of) break;
+  }
+  *v = Type<T>::value(lo);
+  return true;
+}
+
+// ------------------------------------------------------------ many are kept
+// The first token, by index, at which the running sum of what it counts exceeds a target, or the last that counts.  kCount:
+// the tokens equal to `edge`, and the target is `wanted`.  Else the weights of those above `edge`, and of those equal to it
+// up to index `last`, and the target is `wanted` of their sum.  found(index, x, sum) in one thread of the cluster; the sum is
+// returned.  kMass: where a running sum comes too close to the target to tell, sh.unsure is set in all CTAs, to be read
+// behind the next meeting.
+template <typename T, Kind KIND, typename Found>
+__device__ __forceinline__ double locate(const Row<T>& row, int& turn, float edge, int last, double wanted, Found found) {
+  constexpr int kLanes = Type<T>::kLanes;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Weights weights = sh.weights;
+  weights.end = fmaxf(weights.end, edge);                     // weights below the edge are 0
+  weights.zero = fmaxf(weights.zero, edge);
+  const bool whole = last == 0x7FFFFFFF;                      // all that equal `edge`
+  auto counts = [&](float x, int i) { return !(x == edge && i > last); };
+  // a block: a run of a warp; four at a time, whose sums go through the warp together
+  #pragma unroll 1
+  for (int v = 0; v < row.passes; v += 4) {
+    uint4 r[4];
+    #pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (v + q < row.passes) r[q] = row.load(v + q);
+    double s[4] = {};
+    #pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (v + q >= row.passes) continue;
+      float x[kLanes];
+      Type<T>::decode(r[q], x);
+      if constexpr (KIND == kCount) {
+        int n = 0;
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e) n += x[e] == edge;
+        s[q] = n;
+      } else if constexpr (KIND == kMass) {
+        float p[kLanes];
+        #pragma unroll
+        for (int e = 0; e < kLanes; e += 2) weights.two(x[e], x[e + 1], p[e], p[e + 1]);
+        if (!whole)
+          #pragma unroll
+          for (int e = 0; e < kLanes; ++e)
+            if (!counts(x[e], row.index(v + q) + e)) p[e] = 0.f;
+        #pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+          #pragma unroll
+          for (int e = 0; e < o; ++e) p[e] += p[e + o];
+        s[q] = p[0];
+      } else {
+        #pragma unroll
+        for (int e = 0; e < kLanes; ++e) s[q] += whole || counts(x[e], row.index(v + q) + e) ? weights.wide(x[e]) : 0.0;
+      }
+    }
+    const double all = warp_sums<4>(s);
+    if (lane % 8 == 0 && v + lane / 8 < row.passes) sh.block[(v + lane / 8) * kWarps + warp] = all;
+  }
+  __syncthreads();
+  turn ^= 1;
+  const int blocks = row.passes * kWarps, per_lane = (blocks + 31) / 32;
+  auto upto_lane = [&](double v) {
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  double own = 0.0, upto = 0.0;
+  if (warp == 0) {
+    for (int i = 0; i < per_lane; ++i)
+      if (lane * per_lane + i < blocks) own += sh.block[lane * per_lane + i];
+    upto = upto_lane(own);
+    const double all = __shfl_sync(0xffffffffu, upto, 31);
+    if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][0]), (uint32_t)lane), all);
+  }
+  row.meet();
+  // each warp finds whose part holds the token, by the same sums: first lanes, CTAs; then, in that CTA, lanes' blocks
+  const double part = lane < row.ctas ? sh.box.f64[turn][lane][0] : 0.0;
+  double to = upto_lane(part);
+  const double sum = __shfl_sync(0xffffffffu, to, 31), t = KIND == kCount ? wanted : wanted * sum;
+  auto pick = [&](bool some, bool past) {                     // the first past the target, else the last that has some
+    const unsigned any = __ballot_sync(0xffffffffu, some), over = __ballot_sync(0xffffffffu, some && past);
+    return over ? __ffs(over) - 1 : 31 - __clz(any);
+  };
+  const int owner = pick(part > 0.0, to > t);
+  if (owner == row.rank) {
+    double before = __shfl_sync(0xffffffffu, to - part, owner);
     if (warp == 0) {
-      int owner = -1, last = 0;
-      double run = 0.0, before = 0.0, last_before = 0.0;
-      for (int r = 0; r < ctas; ++r) {
-        const double w = sh.box.f64[turn][r][0];
-        if (w > 0.0) {
-          last = r;
-          last_before = run;
-          if (owner < 0 && run + w > t) {
-            owner = r;
-            before = run;
+      const int at_lane = pick(own > 0.0, before + upto > t);
+      if (lane == at_lane) {
+        double run = before + (upto - own), kept = run;
+        int at = 0;
+        for (int i = lane * per_lane; i < min((lane + 1) * per_lane, blocks); ++i) {
+          const double w = sh.block[i];
+          if (w > 0.0) {
+            at = i;
+            kept = run;
+            if (run + w > t) break;
           }
+          run += w;
         }
-        run += w;
+        sh.run = at;
+        sh.before = kept;
       }
-      if (owner < 0) {
-        owner = last;
-        before = last_before;
-      }
-      if (owner == rank) {
-        const bool some = own > 0.0;
-        const unsigned past = __ballot_sync(0xffffffffu, some && before + upto > t), any = __ballot_sync(0xffffffffu, some);
-        if (lane == (past ? __ffs(past) - 1 : 31 - __clz(any))) {
-          double run = before + (upto - own), kept = run;
-          int at = 0;
-          for (int i = lane * per_lane; i < min((lane + 1) * per_lane, blocks); ++i) {
-            const double w = sh.block[i];
-            if (w > 0.0) {
-              at = i;
-              kept = run;
-              if (run + w > t) break;
-            }
-            run += w;
-          }
-          sh.run = at;
-          sh.before = kept;
-        }
-      }
-      if (lane == 0) sh.owner = owner;
     }
     __syncthreads();
-    if (sh.owner == rank && warp == sh.run % kWarps) {
+    if (warp == sh.run % kWarps) {
       const int v = sh.run / kWarps;
-      const double before = sh.before;
+      before = sh.before;
       float x[kLanes];
       double w[kLanes], s = 0.0;
-      Type<T>::decode(part.run(v), x);
+      Type<T>::decode(row.load(v), x);
       #pragma unroll
       for (int e = 0; e < kLanes; ++e) {
-        w[e] = (double)weigh(x[e], part.index(v) + e);
+        const int i = row.index(v) + e;
+        w[e] = KIND == kCount ? (double)(x[e] == edge) : !counts(x[e], i) ? 0.0 : KIND == kMass ? (double)weights.one(x[e]) : weights.wide(x[e]);
         s += w[e];
       }
-      double to = s;
-      #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double u = __shfl_up_sync(0xffffffffu, to, o);
-        if (lane >= o) to += u;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, s > 0.0 && before + to > t), any = __ballot_sync(0xffffffffu, s > 0.0);
-      if (lane == (past ? __ffs(past) - 1 : 31 - __clz(any))) {
-        double run = before + (to - s), from = run, upto = run;
+      to = upto_lane(s);
+      const int at_lane = pick(s > 0.0, before + to > t);
+      if (lane == at_lane) {
+        double run = before + (to - s), from = run, until = run;
         float x_pick = x[0];
-        int pick = 0;
+        int e_pick = 0;
         bool done = false;
         #pragma unroll
         for (int e = 0; e < kLanes; ++e) {
           if (w[e] > 0.0 && !done) {
-            pick = e;
+            e_pick = e;
             x_pick = x[e];
             from = run;
-            upto = run + w[e];
-            done = upto > t;
+            until = run + w[e];
+            done = until > t;
           }
           run += w[e];
         }
-        if (off > 0.0 && (t - from <= 2.0 * off * t || upto - t <= 2.0 * off * t))
-          for (int r = 0; r < ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), (uint32_t)r), 1u);
-        found(part.index(v) + pick, x_pick, sum);
+        if (KIND == kMass && (t - from <= 2.0 * kOff * t || until - t <= 2.0 * kOff * t))
+          for (int r = 0; r < row.ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), (uint32_t)r), 1u);
+        found(row.index(v) + e_pick, x_pick, sum);
       }
     }
-    return sum;
   }
+  return sum;
+}
+template <typename T, Kind KIND>
+__device__ __noinline__ void draw(const Row<T> row, int& turn, float edge, int last, double u, long long* id, float* logprob) {
+  locate<T, KIND>(row, turn, edge, last, u, [&](int i, float x, double sum) {
+    *id = i;
+    if (logprob) *logprob = sh.weights.log_chance(x, sum * (KIND == kMass ? sh.weights.factor : 1.0));
+  });
+  row.meet();
+}
 
-  // ----------------------------------------------------------- few are kept
-  // The tokens cut <= x < below, as (value, index) in the cluster's first CTA; how many there are (past kFew the list is
-  // cut off).  At most three times a row.
-  __device__ __forceinline__ unsigned collect(float cut, float below = NAN) {
-    const int lane = threadIdx.x & 31;
-    unsigned *here = &sh.here[collected], *count = &sh.count[collected];
-    ++collected;
-    if (__any_sync(0xffffffffu, mine >= cut))
-      part.each([&](int v, const float (&x)[kLanes]) {
-        unsigned n = 0;
-        #pragma unroll
-        for (int e = 0; e < kLanes; ++e) n += x[e] >= cut && !(x[e] >= below);
-        if (!__any_sync(0xffffffffu, n > 0)) return;
-        unsigned to = n;
-        #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned u = __shfl_up_sync(0xffffffffu, to, o);
-          if (lane >= o) to += u;
-        }
-        unsigned at = 0;
-        if (lane == 31) at = atomicAdd(here, to);
-        at = __shfl_sync(0xffffffffu, at, 31) + to - n;
-        #pragma unroll
-        for (int e = 0; e < kLanes; ++e)
-          if (x[e] >= cut && !(x[e] >= below)) {
-            if (at < kFew)
-              sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(part.index(v) + e));
-            ++at;
-          }
-      });
-    __syncthreads();
-    const uint32_t counter = dsmem_addr(smem_u32(count), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
-    if (threadIdx.x == 0 && *here > 0) sh.at = atom_dsmem_add(counter, *here);
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < *here && sh.at + i < kFew; i += kThreads) st_dsmem_u64(keys + (sh.at + i) * 8u, sh.found[i]);
-    meet();
-    return ld_dsmem_u32(counter);
-  }
-  // Sorts key[0 .. n) from the largest down, and weight with it, n <= kFew.  Up to 128 by their ranks, four or eight threads
-  // counting the larger ones of each; else by merging (64: 1.3 us, by ranks 0.2).
-  __device__ __forceinline__ void sort(unsigned n) {
-    const unsigned tid = threadIdx.x;
-    auto& key = sh.few.key;
-    auto& weight = sh.few.weight;
-    __syncthreads();
-    if (n <= kThreads / 4) {
-      const unsigned shift = n <= kThreads / 8 ? 3 : 2, i = tid >> shift, step = 1u << shift;
-      const unsigned long long k = i < n ? key[i] : 0;
-      const double w = i < n ? weight[i] : 0.0;
-      unsigned larger = 0;
-      for (unsigned j = tid & (step - 1); j < n; j += step) larger += key[j] > k;
+// ------------------------------------------------------------- few are kept
+// The tokens cut <= x < below, as (value, index) in the cluster's first CTA; how many there are (past kFew the list is cut
+// off).  `call`: 0, 1, 2, another for each call of a row.
+template <typename T>
+__device__ __noinline__ unsigned collect(const Row<T> row, int call, float cut, float below) {
+  constexpr int kLanes = Type<T>::kLanes;
+  if (row.mine >= cut)
+    row.each([&](int v, const float (&x)[kLanes]) {
+      unsigned some = 0;
       #pragma unroll
-      for (unsigned o = 1; o < 4; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
-      if (shift == 3) larger += __shfl_xor_sync(0xffffffffu, larger, 4);
-      __syncthreads();
-      if (i < n && (tid & (step - 1)) == 0) {
-        key[larger] = k;
-        weight[larger] = w;
-      }
-      __syncthreads();
-      return;
-    }
-    unsigned size = kThreads / 2;
-    while (size < n) size *= 2;
-    for (unsigned i = n + tid; i < size; i += kThreads) key[i] = 0;
-    for (unsigned k = 2; k <= size; k *= 2)
-      for (unsigned j = k / 2; j > 0; j /= 2) {
-        __syncthreads();
-        if (tid < size / 2) {
-          const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
-          const unsigned long long x = key[a], y = key[b];
-          if ((x < y) == ((a & k) == 0)) {
-            key[a] = y;
-            key[b] = x;
-            const double w = weight[a];
-            weight[a] = weight[b];
-            weight[b] = w;
-          }
+      for (int e = 0; e < kLanes; ++e) some |= (x[e] >= cut && !(x[e] >= below)) << e;
+      if (some == 0) return;
+      unsigned at = atomicAdd(&sh.here[call], (unsigned)__popc(some));
+      #pragma unroll
+      for (int e = 0; e < kLanes; ++e)
+        if (some >> e & 1) {
+          if (at < kFew)
+            sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(row.index(v) + e));
+          ++at;
         }
-      }
+    });
+  __syncthreads();
+  const unsigned here = sh.here[call];
+  const uint32_t counter = dsmem_addr(smem_u32(&sh.count[call]), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
+  if (here > 0) {
+    if (threadIdx.x == 0) sh.at = atom_dsmem_add(counter, here);
     __syncthreads();
+    for (unsigned i = threadIdx.x; i < here && sh.at + i < kFew; i += kThreads) st_dsmem_u64(keys + (sh.at + i) * 8u, sh.found[i]);
   }
-  // Weights of key[0 .. n), and both sorted from the largest down.
-  __device__ __forceinline__ void sort_by_value(unsigned n) {
-    for (unsigned i = threadIdx.x; i < n; i += kThreads)
-      sh.few.weight[i] = weight64(value_of((unsigned)(sh.few.key[i] >> 32)));
-    sort(n);
-  }
-  __device__ __forceinline__ static int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
-  // Running sums of weight[0 .. n) to upto[0 .. n).
-  __device__ __forceinline__ void run_up(unsigned n) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned i = 2 * threadIdx.x;
-    const double a = i < n ? sh.few.weight[i] : 0.0, b = i + 1 < n ? sh.few.weight[i + 1] : 0.0;
-    double s = a + b;
-    #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == 31) sh.scan[warp] = s;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < warp; ++w) before += sh.scan[w];
-    if (i < n) sh.few.upto[i] = before + (s - b);
-    if (i + 1 < n) sh.few.upto[i + 1] = before + s;
-    __syncthreads();
-  }
-  // The sum of a count over the CTA.
-  __device__ __forceinline__ unsigned cta_count(unsigned n) {
-    n = __reduce_add_sync(0xffffffffu, n);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.part.u32[threadIdx.x >> 5][0] = n;
-    __syncthreads();
-    n = 0;
-    #pragma unroll
-    for (int w = 0; w < kWarps; ++w) n += sh.part.u32[w][0];
-    return n;
-  }
-  // The rest, in the first CTA, of n tokens in order that hold all that are kept (and, where `of_few`, all whose weights the
-  // sum of top-p is over).  False: `sum` came too close to the weights before some token to tell whether that is kept.
-  __device__ __forceinline__ bool finish(unsigned n, long long top_k, double top_p, float cut, double sum, bool of_few, double off,
-                                         double u, long long* id, float* logprob) {
-    const unsigned tid = threadIdx.x;
-    auto& key = sh.few.key;
-    auto& weight = sh.few.weight;
-    auto& upto = sh.few.upto;
-    const unsigned most = top_k > 0 && top_k < (long long)n ? (unsigned)top_k : n;
-    run_up(n);
-    if (of_few) sum = upto[most - 1];
-    const double target = fmax(top_p, 0.0) * sum;
-    bool unsure = false;
-    unsigned kept = 0;
-    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < most; ++i) {
-      const double before = i > 0 ? upto[i - 1] : 0.0;
-      if (i > 0 && top_p < 1.0 && fabs(before - target) <= 2.0 * off * target) unsure = true;
-      kept += i == 0 || ((top_p >= 1.0 || before < target) && value_of((unsigned)(key[i] >> 32)) >= cut);
-    }
-    if (__syncthreads_or(unsure && off > 0.0)) return false;
-    kept = cta_count(kept);
-    const double total = upto[kept - 1], t = u * total;
-    // by index
-    for (unsigned i = tid; i < kept; i += kThreads) key[i] = key[i] << 32;
-    sort(kept);
-    run_up(kept);
-    // the first whose running sum passes t, else the last that has a weight
-    unsigned before = 0;
-    for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= t;
-    unsigned pick = cta_count(before);
-    if (tid == 0) {
-      if (pick >= kept) pick = kept - 1;
-      while (pick > 0 && !(weight[pick] > 0.0)) --pick;
-      *id = index_of(key[pick] >> 32);
-      if (logprob) *logprob = (float)log(weight[pick] / total);
-    }
-    return true;
-  }
+  row.meet();
+  return ld_dsmem_u32(counter);
+}
 
-  // The last token that top-p keeps of those x >= from (`more`: what top-k's ties add to their weights), where it lies among
-  // no more than kFew that fp32 weights cannot tell apart: those are collected and sorted, and the sum and what lies above
-  // them taken in fp64.  f: fp32's F(from) and F(top).  False: it does not.
-  __device__ __forceinline__ bool last_kept(float from, double more, double top_p, const double (&f)[2], float* edge, int* last) {
-    const double about = top_p * (f[0] + more), margin = 4.0 * kOff * about;
-    if (!(f[1] < about - margin) || !(f[0] > about + margin)) return false;
-    long long lo = Type<T>::order(from), hi = Type<T>::order(top);
-    for (int round = 0;; ++round) {
-      if (round >= 3 || hi - lo <= 1) {
-        const float cuts[2] = {Type<T>::value(lo), Type<T>::value(hi)};
-        double n[2];
-        measure<false, false>(cuts, n);
-        if (n[0] - n[1] <= (double)kFew) break;
-        if (hi - lo <= 1 || round >= 16) return false;
-      }
-      long long at[kCuts];
-      float cut[kCuts];
-      double g[kCuts];
-      #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        // first by the tokens' weights, from e^-12 to e^-1.5 of the largest
-        const long long there = round == 0 ? Type<T>::order(top - (float)((12.0 - 3.5 * i) / inv_t)) : lo + (hi - lo) * (i + 1) / (kCuts + 1);
-        at[i] = min(max(there, lo + 1), hi - 1);
-        cut[i] = Type<T>::value(at[i]);
-      }
-      measure<true, false>(cut, g);
-      bool moved = false;
-      #pragma unroll
-      for (int i = 0; i < kCuts; ++i) {
-        if (g[i] > about + margin && at[i] > lo) {
-          lo = at[i];
-          moved = true;
-        } else if (g[i] < about - margin && at[i] < hi) {
-          hi = at[i];
-          moved = true;
+// Sums over the first CTA, the same in all its threads.
+__device__ __forceinline__ unsigned cta_count(unsigned n) {
+  n = __reduce_add_sync(0xffffffffu, n);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.part.u32[threadIdx.x >> 5][0] = n;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < kWarps ? sh.part.u32[threadIdx.x & 31][0] : 0u);
+}
+__device__ __forceinline__ unsigned long long warp_whole(unsigned long long v) {
+  #pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ unsigned long long cta_sum(unsigned long long v) {
+  v = warp_whole(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.scan[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_whole((threadIdx.x & 31) < kWarps ? sh.scan[threadIdx.x & 31] : 0ull);
+}
+__device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
+
+// Sorts key[0 .. n) from the largest down, and weight with it, n <= kFew.
+__device__ __noinline__ void sort(unsigned n) {
+  const unsigned tid = threadIdx.x;
+  auto& key = sh.few.key;
+  auto& weight = sh.few.weight;
+  unsigned size = 64;
+  while (size < n) size *= 2;
+  for (unsigned i = n + tid; i < size; i += kThreads) key[i] = 0;
+  for (unsigned k = 2; k <= size; k *= 2)
+    for (unsigned j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      if (tid < size / 2) {
+        const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
+        const unsigned long long x = key[a], y = key[b];
+        if ((x < y) == ((a & k) == 0)) {
+          key[a] = y;
+          key[b] = x;
+          const unsigned long long w = weight[a];
+          weight[a] = weight[b];
+          weight[b] = w;
         }
       }
-      if (!moved && round >= 3) return false;                 // and more than kFew in between
     }
-    const float cuts[2] = {from, Type<T>::value(hi)};
-    double g[2];
-    measure<true, true>(cuts, g);
-    const unsigned n = collect(Type<T>::value(lo), cuts[1]);
-    if (rank == 0) {
-      sort_by_value(n);
-      run_up(n);
-      const double target = top_p * (g[0] + more);
-      unsigned short_of = 0;
-      for (unsigned i = 2 * threadIdx.x; i < 2 * threadIdx.x + 2 && i < n; ++i) short_of += g[1] + sh.few.upto[i] < target;
-      const unsigned pick = min(cta_count(short_of), n - 1);
-      if (threadIdx.x < ctas) {
-        st_dsmem_u32(dsmem_addr(smem_u32(&sh.edge), threadIdx.x), __float_as_uint(value_of((unsigned)(sh.few.key[pick] >> 32))));
-        st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), threadIdx.x), (uint32_t)index_of(sh.few.key[pick]));
-      }
-    }
-    meet();
-    *edge = sh.edge;
-    *last = sh.index;
-    return true;
+  __syncthreads();
+}
+// Running sums of weight[0 .. n) to upto[0 .. n).
+__device__ __noinline__ void run_up(unsigned n) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned i = 2 * threadIdx.x;
+  const unsigned long long a = i < n ? sh.few.weight[i] : 0, b = i + 1 < n ? sh.few.weight[i + 1] : 0;
+  unsigned long long s = a + b;
+  #pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
   }
+  if (lane == 31) sh.scan[warp] = s;
+  __syncthreads();
+  const unsigned long long before = warp_whole(lane < warp ? sh.scan[lane] : 0ull);
+  if (i < n) sh.few.upto[i] = before + (s - b);
+  if (i + 1 < n) sh.few.upto[i + 1] = before + s;
+  __syncthreads();
+}
+// Weights of few tokens, as whole numbers: additions of these are exact and quick.  None but a zero becomes zero.
+constexpr double kWhole = 0x1p52;
+__device__ __forceinline__ void weigh_few(unsigned n) {
+  for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+    const double w = sh.weights.wide(value_of((unsigned)(sh.few.key[i] >> 32)));
+    const unsigned long long whole = __double2ull_rn(w * kWhole);
+    sh.few.weight[i] = whole == 0 && w > 0.0 ? 1 : whole;
+  }
+  __syncthreads();
+}
+
+struct Filters {
+  long long top_k;                   // 0: off
+  double top_p;                      // 1: off
+  float cut;                         // min-p's
 };
+// The rest, in the first CTA, of n weighted tokens that hold all that are kept (and, where top-k is on, all its tokens).
+// `sum` is what top-p is of where top-k is off, right to `off` of itself.  False: it came too close to the weights before some
+// token to tell whether that is kept; the list is as it was, or sorted.
+//
+// Up to kFewer tokens are not sorted: four or eight threads add up, for a token, the weights of those before it in the order,
+// then, of those kept, the weights up to it by index.
+__device__ __noinline__ bool finish(unsigned n, const Filters& filters, double sum, double off, double u, long long* id, float* logprob) {
+  const unsigned tid = threadIdx.x;
+  auto& key = sh.few.key;
+  auto& weight = sh.few.weight;
+  auto& upto = sh.few.upto;
+  const bool k_on = filters.top_k > 0, p_on = filters.top_p < 1.0;
+  const double top_p = fmax(filters.top_p, 0.0);
+  const unsigned most = k_on && filters.top_k < (long long)n ? (unsigned)filters.top_k : n;
+  double target = top_p * sum * kWhole, near = 2.0 * off * target;
+  // what lies before a token comes to less than the target; too close to it to tell
+  auto less = [&](unsigned long long before) { return !p_on || (double)before < target; };
+  auto close = [&](unsigned long long before) { return p_on && off > 0.0 && fabs((double)before - target) <= near; };
+  if (n <= kFewer) {
+    const unsigned shift = n <= kFewer / 2 ? 3 : 2, i = tid >> shift, step = 1u << shift, lane = tid & (step - 1);
+    const unsigned long long k = i < n ? key[i] : ~0ull, w = i < n ? weight[i] : 0;
+    auto over_step = [&](auto v) {
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (shift == 3) v += __shfl_xor_sync(0xffffffffu, v, 4);
+      return v;
+    };
+    unsigned rank = 0;
+    unsigned long long before = 0;
+    #pragma unroll 4
+    for (unsigned j = lane; j < n; j += step) {
+      const bool ahead = key[j] > k;
+      rank += ahead;
+      before += ahead ? weight[j] : 0;
+    }
+    rank = over_step(rank);
+    before = over_step(before);
+    const bool mine = lane == 0 && i < n;                     // one thread speaks for a token
+    if (k_on && p_on) target = top_p * (double)cta_sum(mine && rank < most ? w : 0);
+    const bool kept = i < n && (rank == 0 || (rank < most && less(before) && value_of((unsigned)(k >> 32)) >= filters.cut));
+    if (mine) upto[i] = kept ? w : 0;
+    if (__syncthreads_or(mine && rank > 0 && close(before))) return false;
+    const unsigned long long total = cta_sum(mine && kept ? w : 0), t = (unsigned long long)(u * (double)total);
+    unsigned long long to = 0;
+    #pragma unroll 4
+    for (unsigned j = lane; j < n; j += step) to += (unsigned)key[j] >= (unsigned)k ? upto[j] : 0;     // ~index: those up to it
+    to = over_step(to);
+    // the first whose running sum passes t, else the last that has a weight
+    const unsigned at = kept && w > 0 ? (unsigned)index_of(k) : 0xFFFFFFFFu;
+    const unsigned past = __reduce_min_sync(0xffffffffu, to > t ? at : 0xFFFFFFFFu);
+    const unsigned end = __reduce_max_sync(0xffffffffu, at + 1);          // 0: none
+    if ((tid & 31) == 0) {
+      sh.part.u32[tid >> 5][0] = past;
+      sh.part.u32[tid >> 5][1] = end;
+    }
+    __syncthreads();
+    const unsigned pick_past = __reduce_min_sync(0xffffffffu, (tid & 31) < kWarps ? sh.part.u32[tid & 31][0] : 0xFFFFFFFFu);
+    const unsigned pick_end = __reduce_max_sync(0xffffffffu, (tid & 31) < kWarps ? sh.part.u32[tid & 31][1] : 0u);
+    const unsigned pick = pick_past != 0xFFFFFFFFu ? pick_past : pick_end - 1;
+    if (mine && kept && at == pick) {
+      *id = (long long)pick;
+      if (logprob) *logprob = sh.weights.log_chance(value_of((unsigned)(k >> 32)), (double)total * (1.0 / kWhole));
+    }
+    return true;
+  }
+  sort(n);
+  run_up(n);
+  if (k_on) target = top_p * (double)upto[most - 1];
+  bool unsure = false;
+  unsigned kept = 0;
+  for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < most; ++i) {
+    const unsigned long long before = i > 0 ? upto[i - 1] : 0;
+    unsure |= i > 0 && close(before);
+    kept += i == 0 || (less(before) && value_of((unsigned)(key[i] >> 32)) >= filters.cut);
+  }
+  if (__syncthreads_or(unsure)) return false;
+  kept = cta_count(kept);
+  const unsigned long long total = upto[kept - 1], t = (unsigned long long)(u * (double)total);
+  for (unsigned i = tid; i < kept; i += kThreads) key[i] = key[i] << 32 | key[i] >> 32;       // by index
+  __syncthreads();
+  sort(kept);
+  run_up(kept);
+  unsigned before = 0;
+  for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= t;
+  unsigned pick = cta_count(before);
+  if (tid == 0) {
+    if (pick >= kept) pick = kept - 1;
+    while (pick > 0 && weight[pick] == 0) --pick;
+    *id = index_of(key[pick] >> 32);
+    if (logprob) *logprob = sh.weights.log_chance(value_of((unsigned)key[pick]), (double)total * (1.0 / kWhole));
+  }
+  return true;
+}
 
-template <typename T, int PASSES>
-__global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(const Params p) {
-  __shared__ Shared sh;
+// The last token that top-p keeps of those x >= from (`more`: what top-k's ties add to their weights), where it lies among
+// no more than kFew that fp32 weights cannot tell apart: those are collected and sorted, and the sum and what lies above
+// them taken in fp64.  all, largest: fp32's F(from) and F(top).  False: it does not.
+template <typename T>
+__device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, double more, double top_p, double all,
+                                       double largest, float* edge, int* last) {
+  const float top = sh.weights.top;
+  const double about = top_p * (all + more), margin = 4.0 * kOff * about;
+  if (!(largest < about - margin) || !(all > about + margin)) return false;
+  long long lo = Type<T>::order(from), hi = Type<T>::order(top);
+  #pragma unroll 1
+  for (int round = 0;; ++round) {
+    if (round >= 3 || hi - lo <= 1) {
+      const double4 n = measure<T, kCount>(row, turn, make_float4(Type<T>::value(lo), Type<T>::value(hi), NAN, NAN));
+      if (n.x - n.y <= (double)kFew) break;
+      if (hi - lo <= 1 || round >= 16) return false;
+    }
+    long long at[kCuts];
+    #pragma unroll
+    for (int i = 0; i < kCuts; ++i) {
+      // first by the tokens' weights, from e^-12 to e^-1.5 of the largest
+      const long long there = round == 0 ? Type<T>::order(top - (float)((12.0 - 3.5 * i) / sh.weights.inv_t)) : lo + (hi - lo) * (i + 1) / (kCuts + 1);
+      at[i] = min(max(there, lo + 1), hi - 1);
+    }
+    const double4 q = measure<T, kMass>(row, turn, make_float4(Type<T>::value(at[0]), Type<T>::value(at[1]),
+                                                                   Type<T>::value(at[2]), Type<T>::value(at[3])));
+    const double g[kCuts] = {q.x, q.y, q.z, q.w};
+    bool moved = false;
+    #pragma unroll
+    for (int i = 0; i < kCuts; ++i) {
+      if (g[i] > about + margin && at[i] > lo) {
+        lo = at[i];
+        moved = true;
+      } else if (g[i] < about - margin && at[i] < hi) {
+        hi = at[i];
+        moved = true;
+      }
+    }
+    if (!moved && round >= 3) return false;                   // and more than kFew in between
+  }
+  const float below = Type<T>::value(hi);
+  const double4 g = measure<T, kExact>(row, turn, make_float4(from, below, NAN, NAN));
+  const unsigned n = collect<T>(row, 2, Type<T>::value(lo), below);
+  if (row.rank == 0) {
+    weigh_few(n);
+    sort(n);
+    run_up(n);
+    const double target = (top_p * (g.x + more) - g.y) * kWhole;
+    unsigned short_of = 0;
+    for (unsigned i = 2 * threadIdx.x; i < 2 * threadIdx.x + 2 && i < n; ++i) short_of += (double)sh.few.upto[i] < target;
+    const unsigned pick = min(cta_count(short_of), n - 1);
+    if (threadIdx.x < row.ctas) {
+      st_dsmem_u32(dsmem_addr(smem_u32(&sh.edge), threadIdx.x), __float_as_uint(value_of((unsigned)(sh.few.key[pick] >> 32))));
+      st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), threadIdx.x), (uint32_t)index_of(sh.few.key[pick]));
+    }
+  }
+  row.meet();
+  *edge = sh.edge;
+  *last = sh.index;
+  return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int staged) {
+  extern __shared__ uint4 stage[];                            // the part, where it fits
   griddep_launch_dependents();
   griddep_wait();
+  constexpr int kLanes = Type<T>::kLanes;
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-  Sampler<T, PASSES> s = {{}, sh, (int)cluster_rank(), (int)ctas};
-  const int row = (int)(blockIdx.x / ctas);
-  constexpr int kLanes = Type<T>::kLanes;
-  const int runs = (p.vocab + kLanes - 1) / kLanes, mine = (runs + s.ctas - 1) / s.ctas;
-  s.turn = 0;
-  s.collected = 0;
+  Row<T> row;
+  row.ctas = (int)ctas;
+  row.rank = (int)cluster_rank();
+  int turn = 0;
+  const int line = (int)(blockIdx.x / ctas);
+  const int runs = (p.vocab + kLanes - 1) / kLanes, mine = (runs + row.ctas - 1) / row.ctas;
+  row.first = min(row.rank * mine * kLanes, p.vocab);
+  row.count = min(mine * kLanes, p.vocab - row.first);
+  row.passes = (mine + kThreads - 1) / kThreads;
+  row.src = static_cast<const T*>(p.logits) + (long long)line * p.stride + row.first;
+  row.vec = p.vec != 0;
   if (threadIdx.x < 3) sh.here[threadIdx.x] = sh.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.unsure = 0;
-  s.part.first = min(s.rank * mine * kLanes, p.vocab);
-  s.part.count = min(mine * kLanes, p.vocab - s.part.first);
-  s.part.passes = PASSES > 0 ? PASSES : (mine + kThreads - 1) / kThreads;
-  s.part.src = static_cast<const T*>(p.logits) + (long long)row * p.stride + s.part.first;
-  s.part.vec = p.vec != 0;
-  s.part.read();
 
-  const double heat = p.temperature ? (double)p.temperature[row] : p.temperature_all;
-  const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_all;
-  const double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_all;
-  const long long top_k = p.top_k ? (long long)p.top_k[row] : p.top_k_all;
-  const double u = fmin(fmax((double)p.uniform[row], 0.0), 1.0);
+  const double heat = p.temperature ? (double)p.temperature[line] : p.temperature_all;
+  Filters filters;
+  filters.top_p = p.top_p ? (double)p.top_p[line] : p.top_p_all;
+  filters.top_k = p.top_k ? (long long)p.top_k[line] : p.top_k_all;
+  const double min_p = p.min_p ? (double)p.min_p[line] : p.min_p_all;
+  const double u = fmin(fmax((double)p.uniform[line], 0.0), 1.0);
   const bool greedy = !(heat > 0.0);
-  const bool k_on = !greedy && top_k > 0 && top_k < p.vocab, p_on = !greedy && top_p < 1.0, m_on = !greedy && min_p > 0.0;
-  s.inv_t = greedy ? 1.0 : 1.0 / heat;
-
-  float most = -INFINITY;
-  s.part.each([&](int, const float (&x)[kLanes]) {
-    #pragma unroll
-    for (int e = 0; e < kLanes; ++e) most = fmaxf(most, x[e]);
-  });
-  s.mine = most = most + 0.f;
-  float least;
-  {
-    // the largest, and the least of the threads' largest (of those that have some)
-    uint32_t v[2] = {order_of(most), most > -INFINITY ? ~order_of(most) : 0u};
-    s.template all_u32<2>(v, 0u, [](uint32_t x) { return __reduce_max_sync(0xffffffffu, x); });
-    s.top = value_of(v[0]);
-    least = value_of(~v[1]);
+  const bool k_on = filters.top_k > 0 && filters.top_k < p.vocab, p_on = filters.top_p < 1.0, m_on = min_p > 0.0;
+  if (!k_on) filters.top_k = 0;
+  if (!p_on) filters.top_p = 1.0;
+  long long* id = p.ids + line;
+  float* logprob = p.logprobs ? p.logprobs + line : nullptr;
+  // what takes fp64's slow operations, by a thread that then waits least
+  double below = 0.0;                // min-p: w >= min_p where x >= top + T log(min_p)
+  if (threadIdx.x == kThreads - 1 && !greedy) {
+    sh.weights.set_heat(heat);
+    if (m_on) below = heat * log(fmin(min_p, 1.0));
   }
-  const float top = s.top;
-  long long* id = p.ids + row;
-  float* logprob = p.logprobs ? p.logprobs + row : nullptr;
+
+  // the largest logit; the part into shared memory, each thread its own runs
+  float most = -INFINITY;
+  {
+    constexpr int kAhead = 4;
+    #pragma unroll 1
+    for (int v = 0; v < row.passes; v += kAhead) {
+      uint4 r[kAhead];
+      #pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i < row.passes) r[i] = row.load(v + i);
+      #pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i < row.passes) {
+          if (staged) stage[(v + i) * kThreads + threadIdx.x] = r[i];
+          float x[kLanes];
+          Type<T>::decode(r[i], x);
+          #pragma unroll
+          for (int e = 0; e < kLanes; ++e) most = fmaxf(most, x[e]);
+        }
+    }
+  }
+  if (staged) {
+    row.src = reinterpret_cast<const T*>(stage);
+    row.count = row.passes * kThreads * kLanes;               // filled up with minus infinity
+    row.vec = true;
+  }
+  row.mine = most = most + 0.f;
+  // the largest, and the least of the threads' largest (of those that have some)
+  uint32_t ends[2] = {order_of(most), most > -INFINITY ? ~order_of(most) : 0u};
+  all_u32<T, 2>(row, turn, ends, 0u, [](uint32_t v) { return __reduce_max_sync(0xffffffffu, v); });
+  const float top = value_of(ends[0]), least = value_of(~ends[1]);
   if (!(top > -INFINITY)) {
-    if (s.rank == 0 && threadIdx.x == 0) {
+    if (row.rank == 0 && threadIdx.x == 0) {
       *id = -1;
       if (logprob) *logprob = -INFINITY;
     }
@@ -860,76 +1010,62 @@ __global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(c
   }
   if (greedy) {
     unsigned at = 0xFFFFFFFFu;
-    if (s.mine == top)
-      s.part.each([&](int v, const float (&x)[kLanes]) {
+    if (row.mine == top)
+      row.each([&](int v, const float (&x)[kLanes]) {
         #pragma unroll
         for (int e = 0; e < kLanes; ++e)
-          if (x[e] == top) at = min(at, (unsigned)(s.part.index(v) + e));
+          if (x[e] == top) at = min(at, (unsigned)(row.index(v) + e));
       });
     uint32_t v[1] = {at};
-    s.template all_u32<1>(v, 0xFFFFFFFFu, [](uint32_t x) { return __reduce_min_sync(0xffffffffu, x); });
-    if (s.rank == 0 && threadIdx.x == 0) {
+    all_u32<T, 1>(row, turn, v, 0xFFFFFFFFu, [](uint32_t x) { return __reduce_min_sync(0xffffffffu, x); });
+    if (row.rank == 0 && threadIdx.x == 0) {
       *id = (long long)v[0];
       if (logprob) *logprob = 0.f;
     }
     return;
   }
-
-  const double scale = s.scale = s.inv_t * 1.4426950408889634074;
-  s.top_scaled = (double)top * scale;
-  s.slow = (float)(-680.0 * heat);
-  s.scale_hi = (float)scale;
-  s.scale_lo = (float)(scale - (double)s.scale_hi);
-  s.low = fmaxf(-100.f / s.scale_hi, -3.402823466e38f);
-  // fp32 weights want a scale that fp32 can square, and no infinite logit
-  const bool fine = scale < 0x1p60 && scale > 0x1p-60 && top < INFINITY;
   const float floor = top == INFINITY ? top : Type<T>::lowest();
-  // w >= min_p where x >= top + T log(min_p)
-  float cut = floor;
-  if (m_on && top < INFINITY) cut = fmaxf(floor, __double2float_ru((double)top + heat * log(fmin(min_p, 1.0))));
-
-  double f[2] = {};                  // fp32's sums over all tokens, and over the largest
-  if (p_on && !k_on && fine) {
-    const float cuts[2] = {floor, top};
-    s.template measure<true, false>(cuts, f);
+  if (threadIdx.x == kThreads - 1) {
+    sh.weights.set_top(top, heat);
+    sh.edge = m_on && top < INFINITY ? fmaxf(floor, __double2float_ru((double)top + below)) : floor;
   }
+  __syncthreads();
+  filters.cut = sh.edge;
+  const bool fine = sh.weights.fine();
+  double4 f = {};                    // fp32's sums over all tokens, and over the largest
+  if (p_on && !k_on && fine) f = measure<T, kMass>(row, turn, make_float4(floor, top, NAN, NAN));
 
   // ------------------------------------------------------------- few are kept
   if (k_on || p_on || m_on) {
     float from = floor;
     unsigned n = kFew + 1;
     if (p.vocab <= kFew) {
-      n = s.collect(floor);
+      n = collect<T>(row, 0, floor, NAN);
     } else if (m_on && !(k_on && p_on)) {
-      n = s.collect(cut);
+      n = collect<T>(row, 0, filters.cut, NAN);
     }
-    if (n > kFew && k_on && top_k <= kFew / 2) {
-      if (s.template bound<false>(least, (double)top_k, &from)) n = s.collect(from);
-    } else if (n > kFew && p_on && !k_on && fine) {
-      if (s.template bound<true>(least, top_p * f[0] * (1.0 + 0x1p-16), &from)) n = s.collect(from);
+    if (n > kFew && ((k_on && filters.top_k <= kFew / 2) || (p_on && !k_on && fine))) {
+      if (bound<T>(row, turn, !k_on, least, k_on ? (double)filters.top_k : fmax(filters.top_p, 0.0) * f.x * (1.0 + 0x1p-16), &from))
+        n = collect<T>(row, 1, from, NAN);
     }
     if (n <= kFew) {
-      double sum = f[0], off = kOff;
+      double sum = f.x, off = p_on && !k_on ? kOff : 0.0;
       if (p_on && !k_on && !fine) {
-        const float cuts[1] = {floor};
-        double all[1];
-        s.template measure<true, true>(cuts, all);
-        sum = all[0];
+        sum = measure<T, kExact>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
         off = 0.0;
       }
-      if (!p_on || k_on) off = 0.0;
-      if (s.rank == 0) {
-        s.sort_by_value(n);
-        const bool done = s.finish(n, k_on ? top_k : 0, p_on ? top_p : 1.0, cut, sum, k_on, off, u, id, logprob);
-        if (!done && threadIdx.x < s.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), threadIdx.x), 1u);
+      #pragma unroll 1
+      for (int time = 0;; ++time) {
+        if (row.rank == 0) {
+          if (time == 0) weigh_few(n);
+          if (!finish(n, filters, sum, off, u, id, logprob) && threadIdx.x < row.ctas)
+            st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), threadIdx.x), 1u);
+        }
+        row.meet();
+        if (off == 0.0 || !sh.unsure) return;
+        sum = measure<T, kExact>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
+        off = 0.0;
       }
-      s.meet();
-      if (off == 0.0 || !sh.unsure) return;
-      const float cuts[1] = {floor};
-      double all[1];
-      s.template measure<true, true>(cuts, all);
-      if (s.rank == 0) s.finish(n, 0, top_p, cut, all[0], false, 0.0, u, id, logprob);
-      return;
     }
   }
 
@@ -937,66 +1073,53 @@ __global__ void __launch_bounds__(kThreads, PASSES == 0 ? 2 : 1) sample_kernel(c
   // x > edge, and of the tokens that equal it the first `ties` (infinity: all), up to index `last`
   float edge = floor;
   double ties = INFINITY, above;
-  int last = p.vocab;
+  int last = 0x7FFFFFFF;
   if (k_on) {
-    const float cuts[1] = {floor};
-    double n[1];
-    s.template measure<false, false>(cuts, n);
-    if (n[0] > (double)top_k) {
-      edge = s.template search<false>(floor, (double)top_k, &above);
-      ties = (double)top_k - above;
+    const double n = measure<T, kCount>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
+    if (n > (double)filters.top_k) {
+      edge = search<T, kCount>(row, turn, floor, (double)filters.top_k, &above);
+      ties = (double)filters.top_k - above;
     }
   }
   if (p_on) {
     // sums over what is kept so far: the tokens above `edge` and its ties, or all from `edge` on
     const bool some = ties < INFINITY;
     const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;     // NaN: nothing
-    const double w_edge = exact_weight(edge, top, s.inv_t), more = some ? ties * w_edge : 0.0;
-    const float cuts[2] = {from, top};
-    if (fine && k_on) s.template measure<true, false>(cuts, f);
-    if (fine && s.last_kept(from, more, fmax(top_p, 0.0), f, &edge, &last)) {
+    const double top_p = fmax(filters.top_p, 0.0);
+    const double w_edge = sh.weights.wide(edge), more = some ? ties * w_edge : 0.0;
+    if (fine && k_on) f = measure<T, kMass>(row, turn, make_float4(from, top, NAN, NAN));
+    if (fine && last_kept<T>(row, turn, from, more, top_p, f.x, f.y, &edge, &last)) {
       ties = INFINITY;
     } else {
-      s.template measure<true, true>(cuts, f);
-      const double target = fmax(top_p, 0.0) * (f[0] + more);
-      if (f[1] >= target) {                              // the last one kept is one of the largest
+      f = measure<T, kExact>(row, turn, make_float4(from, top, NAN, NAN));
+      const double target = top_p * (f.x + more);
+      if (f.y >= target) {                               // the last one kept is one of the largest
         edge = top;
         ties = fmax(ceil(target), 1.0);
-      } else if (!some || f[0] >= target) {
-        edge = s.template search<true>(from, target, &above);
-        ties = fmax(ceil((target - above) / exact_weight(edge, top, s.inv_t)), 1.0);
+      } else if (!some || f.x >= target) {
+        edge = search<T, kExact>(row, turn, from, target, &above);
+        ties = fmax(ceil((target - above) / sh.weights.wide(edge)), 1.0);
       } else {                                           // one of the ties at the edge of top-k
-        ties = fmin(ties, fmax(ceil((target - f[0]) / w_edge), 1.0));
+        ties = fmin(ties, fmax(ceil((target - f.x) / w_edge), 1.0));
       }
     }
   }
-  if (cut > edge) {
-    edge = cut;
+  if (filters.cut > edge) {
+    edge = filters.cut;
     ties = INFINITY;
-    last = p.vocab;
+    last = 0x7FFFFFFF;
   }
   if (ties < INFINITY) {
-    const double n = s.locate(0.0, [&](float x, int) { return x == edge ? 1.f : 0.f; }, [&](double) { return ties - 1.0; },
-                              [&](int i, float, double) {
-                                for (int r = 0; r < s.ctas; ++r)
-                                  st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), (uint32_t)r), (uint32_t)i);
-                              });
-    s.meet();
+    const double n = locate<T, kCount>(row, turn, edge, 0, ties - 1.0, [&](int i, float, double) {
+      for (int r = 0; r < row.ctas; ++r) st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), (uint32_t)r), (uint32_t)i);
+    });
+    row.meet();
     if (n > ties) last = sh.index;
   }
-  auto draw = [&](auto exact) {
-    constexpr bool kExact = decltype(exact)::value;
-    s.locate(kExact ? 0.0 : kOff,
-             [&](float x, int i) { return x > edge || (x == edge && i <= last) ? s.template weigh<kExact>(x) : 0; },
-             [&](double sum) { return u * sum; },
-             [&](int i, float x, double sum) {
-               *id = i;
-               if (logprob) *logprob = (float)log(exact_weight(x, top, s.inv_t) / sum);
-             });
-    s.meet();
-  };
-  if (fine) draw(std::false_type());
-  if (!fine || sh.unsure) draw(std::true_type());
+  // (weights below 2^-100 count only where the token is among the first 2^-40)
+  const bool first = fine && u >= 0x1p-40;
+  if (first) draw<T, kMass>(row, turn, edge, last, u, id, logprob);
+  if (!first || sh.unsure) draw<T, kExact>(row, turn, edge, last, u, id, logprob);
 }
 
 }  // namespace smp

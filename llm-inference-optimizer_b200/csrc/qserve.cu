@@ -23,9 +23,9 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // One cluster of `cluster` CTAs along x after another.
-template <typename Kern, typename Params>
+template <typename Kern, typename... Args>
 int launch_clusters(Kern kernel, unsigned ctas, unsigned cluster, unsigned threads, size_t smem, void* stream,
-                    int64_t flags, const Params& p) {
+                    int64_t flags, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
@@ -45,7 +45,7 @@ int launch_clusters(Kern kernel, unsigned ctas, unsigned cluster, unsigned threa
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
     cudaGetLastError();
     return QL_ERR_CUDA;
   }
@@ -71,29 +71,22 @@ int allow(Kern kernel, size_t smem, std::atomic<unsigned char>* done) {
 }
 
 // ------------------------------------------------------------------- sampling
-template <typename T, int PASSES>
-int run_sample(const ql::smp::Params& p, int ctas, void* stream, int64_t flags) {
-  auto kernel = ql::smp::sample_kernel<T, PASSES>;
-  static std::atomic<unsigned char> done[kMaxDevices];
-  const int st = allow(kernel, 0, done);
-  if (st != QL_OK) return st;
-  return launch_clusters(kernel, (unsigned)p.rows * ctas, (unsigned)ctas, ql::smp::kThreads, 0, stream, flags, p);
-}
-
-// A row's CTAs: as many as leave every SM one, up to a cluster's 16; no fewer than its passes allow.
 template <typename T>
 int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
-  constexpr bool kWide = sizeof(T) == 4;
-  const int64_t runs = cdiv(p.vocab, ql::smp::Type<T>::kLanes);
-  auto passes = [&](int ctas) { return cdiv(cdiv(runs, ctas), ql::smp::kThreads); };
+  using namespace ql::smp;
+  auto kernel = sample_kernel<T>;
+  static std::atomic<unsigned char> done[kMaxDevices];
+  const int st = allow(kernel, kStaged, done);
+  if (st != QL_OK) return st;
+  const int64_t runs = cdiv(p.vocab, Type<T>::kLanes);
+  auto passes = [&](int ctas) { return cdiv(cdiv(runs, ctas), kThreads); };
+  // as many CTAs a row as the SMs have places for; larger clusters find them less easily
+  auto room = [&](int ctas) { return ctas <= 2 ? 4 * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };
   int ctas = 1;
-  while (ctas < ql::smp::kMaxCtas && ((int64_t)p.rows * ctas * 2 <= sms || passes(ctas) > ql::smp::kMaxPasses) && passes(ctas) > 1)
-    ctas *= 2;
-  const int64_t n = passes(ctas);
-  if (n <= 1) return run_sample<T, 1>(p, ctas, stream, flags);
-  if (n <= 3) return run_sample<T, 3>(p, ctas, stream, flags);
-  if (kWide && n <= 5) return run_sample<T, kWide ? 5 : 0>(p, ctas, stream, flags);
-  return run_sample<T, 0>(p, ctas, stream, flags);
+  while (ctas < kMaxCtas && passes(ctas) > 1 && ((int64_t)p.rows * 2 * ctas <= room(2 * ctas) || passes(ctas) * kWarps > kBlocks)) ctas *= 2;
+  const size_t bytes = (size_t)passes(ctas) * kThreads * 16;
+  const int staged = bytes <= kStaged;
+  return launch_clusters(kernel, (unsigned)p.rows * ctas, (unsigned)ctas, kThreads, staged ? bytes : 0, stream, flags, p, staged);
 }
 
 }  // namespace

@@ -163,36 +163,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
       : "memory");
 }
 
-// Two fp32 operations an instruction.
-struct F2 {
-  float x, y;
-};
-__device__ __forceinline__ unsigned long long bits2(float x, float y) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ F2 floats2(unsigned long long v) {
-  F2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)), "l"(bits2(c.x, c.y)));
-  return floats2(r);
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)));
-  return floats2(r);
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a.x, a.y)), "l"(bits2(b.x, b.y)));
-  return floats2(r);
-}
-
 // Which of 32 positions from j on row i of the request sees, as bits.
 template <bool SHARED>
 __device__ __forceinline__ unsigned sees32(const Params& p, const Request& r, int i, int j) {
