@@ -33,8 +33,9 @@ struct Params {
   float scale_log2;              // scale * log2(e): scores in units of log2
   unsigned* err;
   // Attention behind shared prefixes takes two passes.  The first is over the prefixes: its requests are the groups
-  // that share one, every row sees every key, and what a row has (reference and sum, outputs) is left in fp32.  The
-  // second is over what the requests have of their own, and takes that in.
+  // that share one, every row sees every key, and what a row has (reference and sum, outputs) is left in fp32, the
+  // parts of an item joined by a kernel behind it.  The second is over what the requests have of their own, and takes
+  // that in.
   float2* early_sums;            // [total_q][q_heads]
   float* early_out;              // [total_q][q_heads][head_dim]
   const int* cu_group;           // the first pass: [batch + 1] requests, or null: all rows are one group's
@@ -400,6 +401,14 @@ struct Shape {
   static constexpr size_t kJoined = (size_t)kWarps * kRows * (kRowStride + 2) * sizeof(float);
   static constexpr size_t kSmem = 128 + (kRing > kJoined ? kRing : kJoined);
 };
+
+// Four neighbouring elements of a row are parked at `at`: those of lane group g = at / 4 % 8 and tiles 2 j,
+// 2 j + 1, j = at / 32, which are elements 4 j.. of its eighth (8 bits), or 4 (j % 2).. of its 8 in 64 j / 2 (4 bits).
+template <int D, int BITS>
+__device__ __forceinline__ int element_of(int at) {
+  const int g = (at >> 2) & 7, j = at >> 5;
+  return BITS == 8 ? g * (D / 8) + 4 * j : (j >> 1) * 64 + g * 8 + 4 * (j & 1);
+}
 
 template <typename T, int D, int BITS, int NT, bool SHARED = false>
 __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
@@ -889,11 +898,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     const long long item_begin = base + item * per_item;
     const bool whole = k_begin == 0 && k_end == per_item;
     float* mine_out = partials + (long long)(2 * blockIdx.x + (k_begin == 0)) * S::kPartial;
-    // Four neighbouring elements of a row are parked at `at`: those of lane group g = at / 4 % 8 and tiles 2 j,
-    // 2 j + 1, j = at / 32, which are elements 4 j.. of its eighth (8 bits), or 4 (j % 2).. of its 8 in 64 j / 2 (4 bits).
     auto finish = [&](int row, int place, float4 o, float top, float sum) {
-      const int pg = (place >> 2) & 7, j = place >> 5;
-      const int d = BITS == 8 ? pg * (D / 8) + 4 * j : (j >> 1) * 64 + pg * 8 + 4 * (j & 1);
+      const int d = element_of<D, BITS>(place);
       const int token = p.by_group.of(row0 + row), qh = head * p.group + (row0 + row) - token * p.group;
       const long long at = (long long)(r.q0 + token) * p.q_heads + qh;
       if constexpr (SHARED) {
@@ -947,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
         park(mine_out, row, d, o, top, sum);
     }
 
-    if (!whole) {
+    if (!whole && !(SHARED && p.first_pass)) {            // those of a first pass are joined by join_kernel
       const Join j = join_of(work, item_begin, per_item, (int)blockIdx.x);
       auto part = [&](int q) {                          // the first begins the item: its CTA's second slot
         return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * S::kPartial;
@@ -1005,6 +1011,93 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     __syncthreads();                                    // before the next segment reuses shared memory
     u += k_end - k_begin;
   }
+}
+
+// ------------------------------------------- joining the parts of a first pass
+// A first pass has few items of many parts: one CTA that joins all of an item's (some 2 MB) takes longer than the keys had
+// (64 rows of 32 heads over 8192 keys: 38 of 68 us).  So the parts stay, and this kernel, a warp a row, joins them all at
+// once.  Part: how the pass's kernel divides its work and lays a part out.
+template <int D, int BITS, int NT>
+struct StreamPart {
+  static constexpr int kRows = Shape<D, BITS, NT>::kRows, kUnits = kMinUnits, kFloats = Shape<D, BITS, NT>::kPartial;
+  // where the four outputs lie that begin at element_of(place), place a multiple of 4
+  static __device__ __forceinline__ int at(int row, int place) { return 2 * kRows + row * D + place; }
+  static __device__ __forceinline__ int element(int place) { return element_of<D, BITS>(place); }
+};
+constexpr int kJoinThreads = 256;
+
+template <typename Part, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int ctas, const float* partials) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  // units of the pass, and of the groups before the row's
+  const long long row = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  const int token = (int)(row / p.q_heads), qh = (int)(row - (long long)token * p.q_heads);
+  if (row >= (long long)p.total_q * p.q_heads) return;
+  Work work = {0, 0};
+  long long base = 0;
+  Request mine = {0, 0, 0};
+  bool found = false;
+  for (int i = 0; i < p.batch; i += 32) {
+    Request r = {0, 0, 0};
+    long long units = 0;
+    if (i + lane < p.batch) {
+      r = request<true>(p, i + lane);
+      units = request_units<Part::kRows, Part::kUnits>(p, r);
+    }
+    long long to = units;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += u;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, token >= r.q0 && token < r.q0 + r.q_len);
+    if (here && !found) {
+      const int at = __ffs(here) - 1;
+      found = true;
+      base = work.total + __shfl_sync(0xffffffffu, to - units, at);
+      mine.q0 = __shfl_sync(0xffffffffu, r.q0, at);
+      mine.q_len = __shfl_sync(0xffffffffu, r.q_len, at);
+      mine.kv_len = __shfl_sync(0xffffffffu, r.kv_len, at);
+    }
+    work.total += __shfl_sync(0xffffffffu, to, 31);
+  }
+  if (!found) return;                                         // of no group
+  work.ctas = (int)min((long long)ctas, work.total / Part::kUnits);
+  const int head = p.by_group.of(qh), in_group = (token - mine.q0) * p.group + qh - head * p.group;
+  const int tiles = (int)((unsigned)(mine.q_len * p.group + Part::kRows - 1) / Part::kRows);
+  const int per_item = item_units<Part::kUnits>(mine), tile = in_group / Part::kRows, local = in_group - tile * Part::kRows;
+  const Join j = join_of(work, base + ((long long)head * tiles + tile) * per_item, per_item, 0);
+  if (j.parts == 1) return;                                   // it is there
+  auto part = [&](int q) { return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * Part::kFloats; };
+  float top = kLow, sum = 0.f;
+  for (int q = lane; q < j.parts; q += 32) top = fmaxf(top, part(q)[local]);
+  #pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr int kEach = D / 4 > 32 ? D / 128 : 1;             // runs of four outputs a lane
+  float4 o[kEach] = {};
+  const bool live = D >= 128 || lane < D / 4;
+  #pragma unroll 4
+  for (int q = 0; q < j.parts; ++q) {
+    const float* from = part(q);
+    const float f = ex2<true>(from[local] - top);
+    sum = fmaf(from[Part::kRows + local], f, sum);
+    if (live)
+      #pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const float4 v = *reinterpret_cast<const float4*>(from + Part::at(local, (e * 32 + lane) * 4));
+        o[e].x = fmaf(v.x, f, o[e].x);
+        o[e].y = fmaf(v.y, f, o[e].y);
+        o[e].z = fmaf(v.z, f, o[e].z);
+        o[e].w = fmaf(v.w, f, o[e].w);
+      }
+  }
+  if (live)
+    #pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      *reinterpret_cast<float4*>(p.early_out + row * D + Part::element((e * 32 + lane) * 4)) = o[e];
+  if (lane == 0) p.early_sums[row] = make_float2(top, sum);
 }
 
 }  // namespace att

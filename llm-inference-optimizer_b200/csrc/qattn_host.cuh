@@ -157,6 +157,14 @@ struct Attention {
   int sms;
 };
 
+// Joins the parts of a first pass that had `ctas` CTAs.
+template <typename Part, int D>
+int run_join(const Attention& a, int ctas, const float* partials) {
+  const int64_t rows = (int64_t)a.p.total_q * a.p.q_heads;
+  return launch(ql::att::join_kernel<Part, D>, dim3((unsigned)cdiv(rows, ql::att::kJoinThreads / 32)), dim3(ql::att::kJoinThreads),
+                0, a.stream, a.flags, a.p, ctas, partials);
+}
+
 template <int D, int BITS, int NT>
 size_t stream_workspace(int sms) {
   using S = ql::att::Shape<D, BITS, NT>;
@@ -178,9 +186,12 @@ int run_stream(const Attention& a) {
   int64_t ctas = std::min<int64_t>(ql::att::kMaxCtas, (int64_t)S::kCtas * a.sms);
   const double bound = (double)a.p.batch * a.p.cache.heads * (double)tiles * (double)runs;
   if (bound < (double)ctas) ctas = std::max<int64_t>((int64_t)bound, 1);
-  return launch(kernel, dim3((unsigned)ctas), dim3(ql::att::kThreads), S::kSmem, a.stream, a.flags, a.p,
-                static_cast<unsigned*>(a.workspace),
-                reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes));
+  float* partials = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes);
+  const int status = launch(kernel, dim3((unsigned)ctas), dim3(ql::att::kThreads), S::kSmem, a.stream, a.flags, a.p,
+                            static_cast<unsigned*>(a.workspace), partials);
+  if constexpr (SHARED)
+    if (status == QL_OK && a.p.first_pass) return run_join<ql::att::StreamPart<D, BITS, NT>, D>(a, (int)ctas, partials);
+  return status;
 }
 
 template <int D, int BITS>
@@ -201,9 +212,12 @@ int run_tree(const Attention& a) {
   int64_t ctas = std::min<int64_t>(ql::att::kMaxCtas, a.sms);
   const double bound = (double)a.p.batch * a.p.cache.heads * (double)tiles * (double)runs;
   if (bound < (double)ctas) ctas = std::max<int64_t>((int64_t)bound, 1);
-  return launch(kernel, dim3((unsigned)ctas), dim3(ql::tree::kThreads), S::kSmem, a.stream, a.flags, a.p,
-                static_cast<unsigned*>(a.workspace),
-                reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes));
+  float* partials = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ql::att::kHeaderBytes);
+  const int status = launch(kernel, dim3((unsigned)ctas), dim3(ql::tree::kThreads), S::kSmem, a.stream, a.flags, a.p,
+                            static_cast<unsigned*>(a.workspace), partials);
+  if constexpr (SHARED)
+    if (status == QL_OK && a.p.first_pass) return run_join<ql::tree::TreePart<D, BITS>, D>(a, (int)ctas, partials);
+  return status;
 }
 
 template <typename T, int D, int BITS, bool SHARED>

@@ -820,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
             park(mine_out, c, o, ref, sum);
         }
       }
-      if (!whole) {
+      if (!whole && !(SHARED && p.first_pass)) {            // those of a first pass are joined by att::join_kernel
         const att::Join j = att::join_of(work, item_begin, per_item, (int)blockIdx.x);
         auto part = [&](int q) {                            // the first begins the item: its CTA's second slot
           return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * S::kPartial;
@@ -886,6 +886,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
     gemm::tmem_dealloc(tmem, 512);
   }
 }
+
+// A first pass's parts, for att::join_kernel.
+template <int D, int BITS>
+struct TreePart {
+  static constexpr int kRows = tree::kRows, kUnits = kMinUnits, kFloats = Shape<D, BITS>::kPartial;
+  static __device__ __forceinline__ int at(int row, int place) { return 2 * kRows + (place / 4 * kRows + row) * 4; }
+  static __device__ __forceinline__ int element(int place) { return place; }
+};
 
 }  // namespace tree
 }  // namespace ql
