@@ -1015,26 +1015,33 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
 
 // ------------------------------------------- joining the parts of a first pass
 // A first pass has few items of many parts: one CTA that joins all of an item's (some 2 MB) takes longer than the keys had
-// (64 rows of 32 heads over 8192 keys: 38 of 68 us).  So the parts stay, and this kernel, a warp a row, joins them all at
-// once.  Part: how the pass's kernel divides its work and lays a part out.
+// (64 rows of 32 heads over 8192 keys: 38 of 68 us).  So the parts stay, and this kernel joins them all at once.  Part: how
+// the pass's kernel divides its work and lays a part out.  Lanes go along what lies together in a part: a row's outputs
+// (a warp a row), or rows (a warp 32 rows and four outputs of each; the rows are counted by heads first, so that
+// neighbours are of one item).
 template <int D, int BITS, int NT>
 struct StreamPart {
   static constexpr int kRows = Shape<D, BITS, NT>::kRows, kUnits = kMinUnits, kFloats = Shape<D, BITS, NT>::kPartial;
-  // where the four outputs lie that begin at element_of(place), place a multiple of 4
+  static constexpr bool kLanesAreRows = false;
+  // where the four outputs lie that begin at element(place), place a multiple of 4
   static __device__ __forceinline__ int at(int row, int place) { return 2 * kRows + row * D + place; }
   static __device__ __forceinline__ int element(int place) { return element_of<D, BITS>(place); }
 };
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
 template <typename Part, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int ctas, const float* partials) {
   griddep_launch_dependents();
   griddep_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long all = (long long)p.total_q * p.q_heads;
+  long long n = Part::kLanesAreRows ? (long long)blockIdx.x * 32 + lane : (long long)blockIdx.x * kJoinWarps + warp;
+  const bool live = n < all;
+  n = live ? n : 0;
+  const int per_head = p.total_q * p.group, head = (int)(n / per_head), token = p.by_group.of((int)(n - (long long)head * per_head));
+  const int qh = (int)(n - (long long)head * per_head) - token * p.group + head * p.group;
+  const long long row = (long long)token * p.q_heads + qh;
   // units of the pass, and of the groups before the row's
-  const long long row = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-  const int token = (int)(row / p.q_heads), qh = (int)(row - (long long)token * p.q_heads);
-  if (row >= (long long)p.total_q * p.q_heads) return;
   Work work = {0, 0};
   long long base = 0;
   Request mine = {0, 0, 0};
@@ -1052,52 +1059,51 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int 
       const long long u = __shfl_up_sync(0xffffffffu, to, o);
       if (lane >= o) to += u;
     }
-    const unsigned here = __ballot_sync(0xffffffffu, token >= r.q0 && token < r.q0 + r.q_len);
-    if (here && !found) {
-      const int at = __ffs(here) - 1;
-      found = true;
-      base = work.total + __shfl_sync(0xffffffffu, to - units, at);
-      mine.q0 = __shfl_sync(0xffffffffu, r.q0, at);
-      mine.q_len = __shfl_sync(0xffffffffu, r.q_len, at);
-      mine.kv_len = __shfl_sync(0xffffffffu, r.kv_len, at);
+    for (int at = 0; at < min(32, p.batch - i); ++at) {
+      const int q0 = __shfl_sync(0xffffffffu, r.q0, at), q_len = __shfl_sync(0xffffffffu, r.q_len, at);
+      const int kv_len = __shfl_sync(0xffffffffu, r.kv_len, at);
+      const long long before = work.total + __shfl_sync(0xffffffffu, to - units, at);
+      if (!found && token >= q0 && token < q0 + q_len) {
+        found = true;
+        base = before;
+        mine = {q0, q_len, kv_len};
+      }
     }
     work.total += __shfl_sync(0xffffffffu, to, 31);
   }
-  if (!found) return;                                         // of no group
+  if (!found || !live) return;                                // of no group
   work.ctas = (int)min((long long)ctas, work.total / Part::kUnits);
-  const int head = p.by_group.of(qh), in_group = (token - mine.q0) * p.group + qh - head * p.group;
+  const int in_group = (token - mine.q0) * p.group + qh - head * p.group;
   const int tiles = (int)((unsigned)(mine.q_len * p.group + Part::kRows - 1) / Part::kRows);
   const int per_item = item_units<Part::kUnits>(mine), tile = in_group / Part::kRows, local = in_group - tile * Part::kRows;
   const Join j = join_of(work, base + ((long long)head * tiles + tile) * per_item, per_item, 0);
   if (j.parts == 1) return;                                   // it is there
   auto part = [&](int q) { return partials + (long long)(2 * (j.c_first + q) + (q == 0)) * Part::kFloats; };
   float top = kLow, sum = 0.f;
-  for (int q = lane; q < j.parts; q += 32) top = fmaxf(top, part(q)[local]);
-  #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int kEach = D / 4 > 32 ? D / 128 : 1;             // runs of four outputs a lane
+  #pragma unroll 8
+  for (int q = 0; q < j.parts; ++q) top = fmaxf(top, part(q)[local]);
+  constexpr int kEach = !Part::kLanesAreRows && D > 128 ? D / 128 : 1;   // runs of four outputs a thread
+  const int chunk = Part::kLanesAreRows ? blockIdx.y * kJoinWarps + warp : lane;
+  if (chunk >= D / 4) return;
   float4 o[kEach] = {};
-  const bool live = D >= 128 || lane < D / 4;
-  #pragma unroll 4
+  #pragma unroll 8
   for (int q = 0; q < j.parts; ++q) {
     const float* from = part(q);
     const float f = ex2<true>(from[local] - top);
     sum = fmaf(from[Part::kRows + local], f, sum);
-    if (live)
-      #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const float4 v = *reinterpret_cast<const float4*>(from + Part::at(local, (e * 32 + lane) * 4));
-        o[e].x = fmaf(v.x, f, o[e].x);
-        o[e].y = fmaf(v.y, f, o[e].y);
-        o[e].z = fmaf(v.z, f, o[e].z);
-        o[e].w = fmaf(v.w, f, o[e].w);
-      }
-  }
-  if (live)
     #pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      *reinterpret_cast<float4*>(p.early_out + row * D + Part::element((e * 32 + lane) * 4)) = o[e];
-  if (lane == 0) p.early_sums[row] = make_float2(top, sum);
+    for (int e = 0; e < kEach; ++e) {
+      const float4 v = *reinterpret_cast<const float4*>(from + Part::at(local, (e * 32 + chunk) * 4));
+      o[e].x = fmaf(v.x, f, o[e].x);
+      o[e].y = fmaf(v.y, f, o[e].y);
+      o[e].z = fmaf(v.z, f, o[e].z);
+      o[e].w = fmaf(v.w, f, o[e].w);
+    }
+  }
+  #pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    *reinterpret_cast<float4*>(p.early_out + row * D + Part::element((e * 32 + chunk) * 4)) = o[e];
+  if (chunk == 0) p.early_sums[row] = make_float2(top, sum);
 }
 
 }  // namespace att

@@ -161,8 +161,9 @@ struct Attention {
 template <typename Part, int D>
 int run_join(const Attention& a, int ctas, const float* partials) {
   const int64_t rows = (int64_t)a.p.total_q * a.p.q_heads;
-  return launch(ql::att::join_kernel<Part, D>, dim3((unsigned)cdiv(rows, ql::att::kJoinThreads / 32)), dim3(ql::att::kJoinThreads),
-                0, a.stream, a.flags, a.p, ctas, partials);
+  const dim3 grid = Part::kLanesAreRows ? dim3((unsigned)cdiv(rows, 32), (unsigned)cdiv(D / 4, ql::att::kJoinWarps))
+                                        : dim3((unsigned)cdiv(rows, ql::att::kJoinWarps));
+  return launch(ql::att::join_kernel<Part, D>, grid, dim3(ql::att::kJoinThreads), 0, a.stream, a.flags, a.p, ctas, partials);
 }
 
 template <int D, int BITS, int NT>

@@ -19,10 +19,12 @@
 //
 // All of it is prefix sums over the requests, then one lookup a token.  What
 // bounds it is a chain of latencies: the lengths' way from memory, three scans,
-// the pages' way, and for many tokens the writes (12 bytes each).  So one
-// cluster does everything in one launch: each CTA scans all requests by itself
-// (nothing has to be handed over), and a barrier of the cluster separates the
-// reading of the old state from the writing of the new.
+// the pages' way; so one launch does everything.  Many requests are scanned by
+// each CTA of a cluster for itself (nothing has to be handed over), and a barrier
+// of the cluster separates the reading of the old state from the writing of the
+// new.  Many tokens (12 bytes each to be written, more than a cluster's SMs write
+// quickly) are left to a second kernel over all SMs, which looks them up in the
+// tables as they then are.
 #pragma once
 
 #include "ql_common.cuh"
@@ -46,6 +48,7 @@ struct Params {
   int* refused;
   long long table_stride, max_tokens;
   int batch, width, num_pages, page_shift;
+  bool tokens;                     // the first kernel looks them up
 };
 
 struct Request {
@@ -107,6 +110,20 @@ __device__ __forceinline__ int holder(const int* first, int n, int i) {
     else hi = mid;
   }
   return lo;
+}
+
+// Four tokens from t0 on, a multiple of four.
+__device__ __forceinline__ void store_tokens(const Params& p, long long t0, const long long (&slot)[4], const int (&position)[4]) {
+  if (t0 + 4 <= p.max_tokens) {
+    reinterpret_cast<longlong2*>(p.slots + t0)[0] = make_longlong2(slot[0], slot[1]);
+    reinterpret_cast<longlong2*>(p.slots + t0)[1] = make_longlong2(slot[2], slot[3]);
+    *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
+  } else {
+    for (int i = 0; t0 + i < p.max_tokens; ++i) {
+      p.slots[t0 + i] = slot[i];
+      p.positions[t0 + i] = position[i];
+    }
+  }
 }
 
 __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
@@ -172,23 +189,45 @@ __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
   }
   __syncthreads();
 
-  // pages back onto the stack
+  // pages back onto the stack; several at a time, whose lookups wait together
+  constexpr int kAtOnce = 4;
   const int at = rank * threads + (int)threadIdx.x, step = ctas * threads;
-  for (long long j = at; j < back; j += step) {
-    const int b = holder(first_back, p.batch, (int)j);
-    const int k = (int)((keeps[b] + page_mask) >> p.page_shift) + (int)j - first_back[b];
-    const long long to = available - 1 - j;
-    if (to < p.num_pages) p.stack[to] = p.table[(long long)b * p.table_stride + k];
+  for (long long j0 = at; j0 < back; j0 += (long long)kAtOnce * step) {
+    int page[kAtOnce];
+    #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long j = j0 + (long long)i * step;
+      if (j >= back) continue;
+      const int b = holder(first_back, p.batch, (int)j);
+      const int k = (int)((keeps[b] + page_mask) >> p.page_shift) + (int)j - first_back[b];
+      page[i] = p.table[(long long)b * p.table_stride + k];
+    }
+    #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long to = available - 1 - (j0 + (long long)i * step);
+      if (to >= count && to < p.num_pages) p.stack[to] = page[i];         // to >= count: j < back
+    }
   }
   cluster_sync_all();               // the old lengths, count and pages have been read, the stack written
   auto page_taken = [&](int i) {
     const long long from = available - 1 - i;
     return from >= 0 && from < p.num_pages ? p.stack[from] : -1;
   };
-  for (int i = at; i < taken; i += step) {
-    const int b = holder(first_taken, p.batch, i);
-    const int k = (int)((keeps[b] + page_mask) >> p.page_shift) + i - first_taken[b];
-    p.table[(long long)b * p.table_stride + k] = page_taken(i);
+  for (long long i0 = at; i0 < taken; i0 += (long long)kAtOnce * step) {
+    int page[kAtOnce];
+    long long to[kAtOnce];
+    #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long n = i0 + (long long)i * step;
+      to[i] = -1;
+      if (n >= taken) continue;
+      const int b = holder(first_taken, p.batch, (int)n);
+      to[i] = (long long)b * p.table_stride + (int)((keeps[b] + page_mask) >> p.page_shift) + (int)n - first_taken[b];
+      page[i] = page_taken((int)n);
+    }
+    #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (to[i] >= 0) p.table[to[i]] = page[i];
   }
   for (int b = at; b <= p.batch; b += step) {
     p.cu_q[b] = first_token[b];
@@ -205,36 +244,67 @@ __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
       *p.count = (int)min(available - taken, (long long)p.num_pages);
     }
   }
-  // four neighbouring tokens a thread
-  for (long long t0 = 4ll * at; t0 < p.max_tokens; t0 += 4ll * step) {
-    int b = t0 < total ? holder(first_token, p.batch, (int)t0) : 0;
-    long long slot[4];
-    int position[4];
+  if (!p.tokens) return;
+  for (long long t0 = at; t0 < p.max_tokens; t0 += (long long)kAtOnce * step) {
+    int page[kAtOnce], position[kAtOnce];
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = (int)t0 + i;
-      slot[i] = -1;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long t = t0 + (long long)i * step;
+      page[i] = -1;
       position[i] = 0;
-      if (t < total) {
-        while (t >= first_token[b + 1]) ++b;
-        const int pos = keeps[b] + t - first_token[b];
-        const int k = pos >> p.page_shift, kept = (int)((keeps[b] + page_mask) >> p.page_shift);
-        const int page = k < kept ? p.table[(long long)b * p.table_stride + k] : page_taken(first_taken[b] + k - kept);
-        slot[i] = page < 0 ? -1 : ((long long)page << p.page_shift) + (pos & page_mask);
-        position[i] = pos;
-      }
+      if (t >= total) continue;
+      const int b = holder(first_token, p.batch, (int)t), pos = keeps[b] + (int)t - first_token[b];
+      const int k = pos >> p.page_shift, kept = (int)((keeps[b] + page_mask) >> p.page_shift);
+      const long long from = available - 1 - (first_taken[b] + k - kept);
+      const int* src = k < kept ? p.table + (long long)b * p.table_stride + k : p.stack + from;
+      if (k < kept || (from >= 0 && from < p.num_pages)) page[i] = *src;
+      position[i] = pos;
     }
-    if (t0 + 4 <= p.max_tokens) {
-      reinterpret_cast<longlong2*>(p.slots + t0)[0] = make_longlong2(slot[0], slot[1]);
-      reinterpret_cast<longlong2*>(p.slots + t0)[1] = make_longlong2(slot[2], slot[3]);
-      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
-    } else {
-      for (int i = 0; t0 + i < p.max_tokens; ++i) {
-        p.slots[t0 + i] = slot[i];
-        p.positions[t0 + i] = position[i];
-      }
+    #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long t = t0 + (long long)i * step;
+      if (t >= p.max_tokens) continue;
+      p.slots[t] = page[i] < 0 ? -1 : ((long long)page[i] << p.page_shift) + (position[i] & page_mask);
+      p.positions[t] = position[i];
     }
   }
+}
+
+// Slots and positions of four neighbouring tokens a thread, after plan_kernel.
+constexpr int kTokenThreads = 256;
+__global__ void __launch_bounds__(kTokenThreads) token_kernel(const Params p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int total = p.batch > 0 ? p.cu_q[p.batch] : 0;
+  const long long t0 = 4ll * ((long long)blockIdx.x * kTokenThreads + threadIdx.x);
+  if (t0 >= p.max_tokens) return;
+  int b = t0 < total ? holder(p.cu_q, p.batch, (int)t0) : 0;
+  long long slot[4];
+  int position[4];
+  int first = 0, end = 0, keep = 0;                           // of request b
+  if (t0 < total) {
+    first = p.cu_q[b];
+    end = p.cu_q[b + 1];
+    keep = p.lens[b] - (end - first);
+  }
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = (int)t0 + i;
+    slot[i] = -1;
+    position[i] = 0;
+    if (t < total) {
+      while (t >= end) {
+        first = end;
+        end = p.cu_q[++b + 1];
+        keep = p.lens[b] - (end - first);
+      }
+      const int pos = keep + t - first;
+      const int page = p.table[(long long)b * p.table_stride + (pos >> p.page_shift)];
+      slot[i] = page < 0 ? -1 : ((long long)page << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+      position[i] = pos;
+    }
+  }
+  store_tokens(p, t0, slot, position);
 }
 
 }  // namespace plan

@@ -70,6 +70,8 @@ int allow(Kern kernel, size_t smem, std::atomic<unsigned char>* done) {
   return QL_OK;
 }
 
+constexpr int64_t kFewRequests = 1024, kFewTokens = 8192;
+
 // ------------------------------------------------------------------- sampling
 template <typename T>
 int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
@@ -132,11 +134,17 @@ int ql_plan_step(const ql_plan_step_args* a, void* stream) {
   auto kernel = ql::plan::plan_kernel;
   static std::atomic<unsigned char> done[kMaxDevices];
   if ((st = allow(kernel, (4 * (size_t)ql::plan::kMaxBatch + 2) * sizeof(int), done)) != QL_OK) return st;
-  const bool small = a->max_tokens <= 4096 && a->batch <= 1024;
-  const unsigned ctas = small ? 1 : 8;
-  const unsigned threads = small ? (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(std::max(a->batch, cdiv(a->max_tokens, 4)), 32) * 32, 128), ql::plan::kThreads)
-                                 : ql::plan::kThreads;
-  return launch_clusters(kernel, ctas, ctas, threads, (4 * (size_t)a->batch + 2) * sizeof(int), stream, a->flags, p);
+  // One CTA as far as its threads go round the tokens and requests a few times; then a cluster (its barriers, 1 us, are
+  // worth it from some thousand requests on), and another kernel for the tokens.
+  const bool few_requests = a->batch <= kFewRequests, few_tokens = a->max_tokens <= kFewTokens;
+  p.tokens = few_tokens;
+  const int64_t wanted = std::max(a->batch, few_tokens ? a->max_tokens : cdiv(a->max_tokens, a->page_size));
+  const unsigned ctas = few_requests ? 1 : 8;
+  const unsigned threads = (unsigned)std::min<int64_t>(std::max<int64_t>(cdiv(wanted, 32) * 32, 128), ql::plan::kThreads);
+  st = launch_clusters(kernel, ctas, ctas, threads, (4 * (size_t)a->batch + 2) * sizeof(int), stream, a->flags, p);
+  if (st != QL_OK || few_tokens) return st;
+  return launch_clusters(ql::plan::token_kernel, (unsigned)cdiv(a->max_tokens, 4 * ql::plan::kTokenThreads), 1,
+                         ql::plan::kTokenThreads, 0, stream, a->flags, p);
 }
 
 int ql_sample_tokens(const ql_sample_tokens_args* a, void* stream) {

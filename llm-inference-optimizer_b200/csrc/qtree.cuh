@@ -525,19 +525,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
       const bool active = w == 0 || g.pair;
       // the warp's 32 rows of queries into shared memory, neighbouring lanes at neighbouring addresses
       if (active && steps > 0) {
-        constexpr int kChunks = D / 8;
-        #pragma unroll 8
-        for (int i = 0; i < kChunks; ++i) {
-          const int at = w * kTileRows + quarter * 32 + (i * 32 + lane) / kChunks, c = lane % kChunks;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (at < rows) {
-            const int tok = p.by_group.of(row0 + at), h = head * p.group + row0 + at - tok * p.group;
-            const kvc::Chunk k = {c * 8, c * 8 + 4, false};
-            v = kvc::load_chunk(static_cast<const T*>(p.q.p) + (long long)(r.q0 + tok) * p.q.token_stride + h * p.q.head_stride,
-                                k, p.q.vec);
+        constexpr int kChunks = D / 8, kAhead = 8;                     // loads on their way at a time
+        #pragma unroll 1
+        for (int i0 = 0; i0 < kChunks; i0 += kAhead) {
+          uint4 v[kAhead];
+          #pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const int at = w * kTileRows + quarter * 32 + ((i0 + i) * 32 + lane) / kChunks, c = lane % kChunks;
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < rows) {
+              const int tok = p.by_group.of(row0 + at), h = head * p.group + row0 + at - tok * p.group;
+              const kvc::Chunk k = {c * 8, c * 8 + 4, false};
+              v[i] = kvc::load_chunk(static_cast<const T*>(p.q.p) + (long long)(r.q0 + tok) * p.q.token_stride + h * p.q.head_stride,
+                                     k, p.q.vec);
+            }
           }
-          *reinterpret_cast<uint4*>(sm_q + ((w * S::kAtoms + (c >> 3)) * kTileRows + (at & 127)) * 128 +
-                                    (((c & 7) ^ (at & 7)) << 4)) = v;
+          #pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const int at = quarter * 32 + ((i0 + i) * 32 + lane) / kChunks, c = lane % kChunks;
+            *reinterpret_cast<uint4*>(sm_q + ((w * S::kAtoms + (c >> 3)) * kTileRows + at) * 128 + (((c & 7) ^ (at & 7)) << 4)) = v[i];
+          }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -891,6 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p, unsig
 template <int D, int BITS>
 struct TreePart {
   static constexpr int kRows = tree::kRows, kUnits = kMinUnits, kFloats = Shape<D, BITS>::kPartial;
+  static constexpr bool kLanesAreRows = true;
   static __device__ __forceinline__ int at(int row, int place) { return 2 * kRows + (place / 4 * kRows + row) * 4; }
   static __device__ __forceinline__ int element(int place) { return place; }
 };

@@ -82,8 +82,11 @@ class PageTables:
 
     def step_buffers(self, max_tokens: int) -> StepPlan:
         """Room for a step's plan, to be passed as ``out`` step after step."""
-        new = self.lens.new_empty
-        return StepPlan(new(self.batch + 1), new(max_tokens, dtype=torch.int64), new(max_tokens), self.lens, new(1))
+        dev, i32 = self.device, torch.int32
+        return StepPlan(torch.empty(self.batch + 1, dtype=i32, device=dev),
+                        torch.empty(max_tokens, dtype=torch.int64, device=dev),
+                        torch.empty(max_tokens, dtype=i32, device=dev), self._tensors[1],
+                        torch.empty(1, dtype=i32, device=dev))
 
 
 def plan_step(pages: PageTables, new_tokens: torch.Tensor, max_tokens: int, keep: torch.Tensor = None,
@@ -119,13 +122,15 @@ def plan_step(pages: PageTables, new_tokens: torch.Tensor, max_tokens: int, keep
         raise ValueError(f"max_tokens must be from 0 to 2^31 - 1, got {max_tokens}")
     if out is None:
         out = pages.step_buffers(max_tokens)
-    cu_q, slots, positions, lens, refused = out
-    if (slots.dtype, positions.dtype, cu_q.dtype, refused.dtype) != (torch.int64, torch.int32, torch.int32, torch.int32):
-        raise TypeError("out must hold cu_q, positions and refused in int32 and slots in int64")
-    assert cu_q.shape == (batch + 1,) and slots.shape == positions.shape == (max_tokens,) and refused.shape == (1,) \
-        and lens is pages.lens, f"out does not fit {batch} requests and {max_tokens} tokens"
-    for t in (cu_q, slots, positions, refused):
-        assert t.device == dev and t.is_contiguous(), f"out must be contiguous on {dev}"
+        cu_q, slots, positions, _, refused = out
+    else:
+        cu_q, slots, positions, lens, refused = out
+        if (slots.dtype, positions.dtype, cu_q.dtype, refused.dtype) != (torch.int64, torch.int32, torch.int32, torch.int32):
+            raise TypeError("out must hold cu_q, positions and refused in int32 and slots in int64")
+        assert cu_q.shape == (batch + 1,) and slots.shape == positions.shape == (max_tokens,) and refused.shape == (1,) \
+            and lens is pages.lens, f"out does not fit {batch} requests and {max_tokens} tokens"
+        for t in (cu_q, slots, positions, refused):
+            assert t.device == dev and t.is_contiguous(), f"out must be contiguous on {dev}"
     packed = _lib.PLAN_STEP_ARGS.pack(*pages._state, keep_ptr, new_tokens.data_ptr(), cu_q.data_ptr(), slots.data_ptr(),
                                       positions.data_ptr(), refused.data_ptr(), *pages._sizes, max_tokens, call_flags())
     call(_lib.load().ql_plan_step, packed, dev)
