@@ -53,7 +53,7 @@ struct Params {
 
 struct Request {
   int lens, keep, held, kept;
-  long long fresh, grow;           // asked for; 0 where the table's row has no room
+  unsigned fresh, grow;            // asked for; 0 where the table's row has no room
   bool fits;
 };
 __device__ __forceinline__ Request request(const Params& p, int b) {
@@ -66,21 +66,25 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.kept = (int)((r.keep + page) >> p.page_shift);
   const long long want = (long long)r.keep + max(p.fresh[b], 0);
   r.fits = want <= room;
-  r.fresh = r.fits ? want - r.keep : 0;
-  r.grow = r.fits ? ((want + page) >> p.page_shift) - r.kept : 0;
+  r.fresh = r.fits ? (unsigned)(want - r.keep) : 0u;
+  r.grow = r.fits ? (unsigned)((want + page) >> p.page_shift) - (unsigned)r.kept : 0u;
   return r;
 }
 
+// Sums that stop at kMost: more is never asked whether it fits.  (Associative, of what is kMost at most.)
+constexpr unsigned kMost = 0x7FFFFFFFu;
+__device__ __forceinline__ unsigned plus(unsigned a, unsigned b) { return min(a + b, kMost); }
+
 // Inclusive sums over the CTA's threads, and the CTA's.
 template <int N>
-__device__ __forceinline__ void scan(long long (&v)[N], long long (&all)[N], long long (*warp_sum)[N]) {
+__device__ __forceinline__ void scan(unsigned (&v)[N], unsigned (&all)[N], unsigned (*warp_sum)[2]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   #pragma unroll
   for (int o = 1; o < 32; o <<= 1)
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const long long u = __shfl_up_sync(0xffffffffu, v[i], o);
-      if (lane >= o) v[i] += u;
+      const unsigned u = __shfl_up_sync(0xffffffffu, v[i], o);
+      if (lane >= o) v[i] = plus(v[i], u);
     }
   __syncthreads();                 // the sums of the scan before have been read
   if (lane == 31)
@@ -89,15 +93,15 @@ __device__ __forceinline__ void scan(long long (&v)[N], long long (&all)[N], lon
   __syncthreads();
   #pragma unroll
   for (int i = 0; i < N; ++i) {
-    long long s = lane < warps ? warp_sum[lane][i] : 0;
+    unsigned s = lane < warps ? warp_sum[lane][i] : 0;
     #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
+      const unsigned u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s = plus(s, u);
     }
     all[i] = __shfl_sync(0xffffffffu, s, 31);
-    const long long before = __shfl_sync(0xffffffffu, s, (warp + 31) & 31);
-    if (warp > 0) v[i] += before;
+    const unsigned before = __shfl_sync(0xffffffffu, s, (warp + 31) & 31);
+    if (warp > 0) v[i] = plus(v[i], before);
   }
 }
 
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
   int* keeps = first_token + p.batch + 1;
   int* first_taken = keeps + p.batch;
   int* first_back = first_taken + p.batch + 1;
-  __shared__ long long warp_sum[kWarps][2];
+  __shared__ unsigned warp_sum[kWarps][2];
   griddep_launch_dependents();
   griddep_wait();
   const int rank = (int)cluster_rank(), ctas = (int)gridDim.x, threads = (int)blockDim.x;
@@ -141,39 +145,40 @@ __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
   const int count = min(max(*p.count, 0), p.num_pages);
 
   // pages that come back; the requests of the first round stay in registers
-  long long back = 0;
+  unsigned back = 0;                                          // below 2^31: the table has no more entries
   Request first = {};
   for (int i = 0; i < p.batch; i += threads) {
     const int b = i + (int)threadIdx.x;
     Request r = {};
     if (b < p.batch) r = request(p, b);
     if (i == 0) first = r;
-    long long v[1] = {r.held - r.kept}, all[1];
-    scan<1>(v, all, reinterpret_cast<long long (*)[1]>(warp_sum));
+    const unsigned mine = (unsigned)(r.held - r.kept);
+    unsigned v[1] = {mine}, all[1];
+    scan<1>(v, all, warp_sum);
     if (b < p.batch) {
       keeps[b] = r.keep;
-      first_back[b] = (int)(back + v[0] - (r.held - r.kept));
+      first_back[b] = (int)(back + v[0] - mine);
     }
     back += all[0];
   }
   // who is served, and what they get
-  const long long available = count + back;
-  long long asked[2] = {0, 0}, given[2] = {0, 0};
+  const long long available = (long long)count + back;
+  unsigned asked[2] = {0, 0}, given[2] = {0, 0};
   int refused = 0;
   for (int i = 0; i < p.batch; i += threads) {
     const int b = i + (int)threadIdx.x;
     Request r = first;
     if (i > 0 && b < p.batch) r = request(p, b);
     const bool live = b < p.batch;
-    long long v[2] = {live ? r.fresh : 0, live ? r.grow : 0}, all[2];
-    const long long fresh = v[0], grow = v[1];
+    unsigned v[2] = {live ? r.fresh : 0u, live ? r.grow : 0u}, all[2];
+    const unsigned fresh = v[0], grow = v[1];
     scan<2>(v, all, warp_sum);
-    const bool served = live && r.fits && asked[0] + v[0] <= p.max_tokens && (grow == 0 || asked[1] + v[1] <= available);
+    const bool served = live && r.fits && plus(asked[0], v[0]) <= p.max_tokens && (grow == 0 || plus(asked[1], v[1]) <= available);
     refused += live && !served && p.fresh[b] > 0;
-    asked[0] += all[0];
-    asked[1] += all[1];
-    long long w[2] = {served ? fresh : 0, served ? grow : 0};
-    const long long mine[2] = {w[0], w[1]};
+    asked[0] = plus(asked[0], all[0]);
+    asked[1] = plus(asked[1], all[1]);
+    unsigned w[2] = {served ? fresh : 0u, served ? grow : 0u};
+    const unsigned mine[2] = {w[0], w[1]};
     scan<2>(w, all, warp_sum);
     if (live) {
       first_token[b] = (int)(given[0] + w[0] - mine[0]);
@@ -275,16 +280,19 @@ constexpr int kTokenThreads = 256;
 __global__ void __launch_bounds__(kTokenThreads) token_kernel(const Params p) {
   griddep_launch_dependents();
   griddep_wait();
-  const int total = p.batch > 0 ? p.cu_q[p.batch] : 0;
+  extern __shared__ int cu[];
+  for (int i = threadIdx.x; i <= p.batch; i += kTokenThreads) cu[i] = p.cu_q[i];
+  __syncthreads();
+  const int total = cu[p.batch];
   const long long t0 = 4ll * ((long long)blockIdx.x * kTokenThreads + threadIdx.x);
   if (t0 >= p.max_tokens) return;
-  int b = t0 < total ? holder(p.cu_q, p.batch, (int)t0) : 0;
+  int b = t0 < total ? holder(cu, p.batch, (int)t0) : 0;
   long long slot[4];
   int position[4];
   int first = 0, end = 0, keep = 0;                           // of request b
   if (t0 < total) {
-    first = p.cu_q[b];
-    end = p.cu_q[b + 1];
+    first = cu[b];
+    end = cu[b + 1];
     keep = p.lens[b] - (end - first);
   }
   #pragma unroll
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(const Params p) {
     if (t < total) {
       while (t >= end) {
         first = end;
-        end = p.cu_q[++b + 1];
+        end = cu[++b + 1];
         keep = p.lens[b] - (end - first);
       }
       const int pos = keep + t - first;

@@ -70,7 +70,7 @@ int allow(Kern kernel, size_t smem, std::atomic<unsigned char>* done) {
   return QL_OK;
 }
 
-constexpr int64_t kFewRequests = 1024, kFewTokens = 8192;
+constexpr int64_t kFewRequests = 1024, kFewTokens = 2048;
 
 // ------------------------------------------------------------------- sampling
 template <typename T>
@@ -98,7 +98,7 @@ extern "C" {
 int ql_plan_step(const ql_plan_step_args* a, void* stream) {
   if (!a) return QL_ERR_NULL_POINTER;
   if (a->batch < 0 || a->batch > ql::plan::kMaxBatch || a->table_width < 0 || a->num_pages < 0 ||
-      a->num_pages > INT_MAX || a->max_tokens < 0 || a->max_tokens > INT_MAX ||
+      a->num_pages > INT_MAX || a->max_tokens < 0 || a->max_tokens >= INT_MAX ||
       a->batch * std::min<int64_t>(a->table_width, INT_MAX) > INT_MAX)
     return QL_ERR_BAD_SHAPE;
   if (a->page_size < 1 || a->page_size > 65536 || (a->page_size & (a->page_size - 1)) != 0) return QL_ERR_UNSUPPORTED;
@@ -134,8 +134,9 @@ int ql_plan_step(const ql_plan_step_args* a, void* stream) {
   auto kernel = ql::plan::plan_kernel;
   static std::atomic<unsigned char> done[kMaxDevices];
   if ((st = allow(kernel, (4 * (size_t)ql::plan::kMaxBatch + 2) * sizeof(int), done)) != QL_OK) return st;
-  // One CTA as far as its threads go round the tokens and requests a few times; then a cluster (its barriers, 1 us, are
-  // worth it from some thousand requests on), and another kernel for the tokens.
+  // One CTA for all requests as far as its threads go, else a cluster of 8, each of which scans them all.  More tokens than
+  // its threads have in two rounds go to all SMs: each lookup is a search of log2(batch) steps in shared memory, of which
+  // 6000 take one SM longer (6 us) than a launch.
   const bool few_requests = a->batch <= kFewRequests, few_tokens = a->max_tokens <= kFewTokens;
   p.tokens = few_tokens;
   const int64_t wanted = std::max(a->batch, few_tokens ? a->max_tokens : cdiv(a->max_tokens, a->page_size));
@@ -144,7 +145,7 @@ int ql_plan_step(const ql_plan_step_args* a, void* stream) {
   st = launch_clusters(kernel, ctas, ctas, threads, (4 * (size_t)a->batch + 2) * sizeof(int), stream, a->flags, p);
   if (st != QL_OK || few_tokens) return st;
   return launch_clusters(ql::plan::token_kernel, (unsigned)cdiv(a->max_tokens, 4 * ql::plan::kTokenThreads), 1,
-                         ql::plan::kTokenThreads, 0, stream, a->flags, p);
+                         ql::plan::kTokenThreads, ((size_t)a->batch + 1) * sizeof(int), stream, a->flags, p);
 }
 
 int ql_sample_tokens(const ql_sample_tokens_args* a, void* stream) {

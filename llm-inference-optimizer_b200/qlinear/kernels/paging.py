@@ -118,8 +118,8 @@ def plan_step(pages: PageTables, new_tokens: torch.Tensor, max_tokens: int, keep
         if not keep.is_contiguous():
             keep = keep.contiguous()
         keep_ptr = keep.data_ptr()
-    if max_tokens < 0 or max_tokens >= 2 ** 31:
-        raise ValueError(f"max_tokens must be from 0 to 2^31 - 1, got {max_tokens}")
+    if max_tokens < 0 or max_tokens >= 2 ** 31 - 1:
+        raise ValueError(f"max_tokens must be from 0 to 2^31 - 2, got {max_tokens}")
     if out is None:
         out = pages.step_buffers(max_tokens)
         cu_q, slots, positions, _, refused = out
