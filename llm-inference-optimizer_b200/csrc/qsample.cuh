@@ -377,51 +377,60 @@ __device__ __forceinline__ void all_u32(const Row<T>& row, int& turn, uint32_t (
 }
 // F at thresholds: the number of tokens x >= cut (not of a NaN), or the sum of their weights.  A function of its own for
 // each kind: the code is read from memory once a launch, and that is a good part of a short row's time.
-template <typename T, Kind KIND>
-__device__ __noinline__ double4 measure(const Row<T> row, int& turn, float4 at) {
+template <typename T, Kind KIND, int N>
+__device__ __noinline__ double4 measure_of(const Row<T> row, int& turn, float4 at) {
   constexpr int kLanes = Type<T>::kLanes;
   const float cut[kCuts] = {at.x, at.y, at.z, at.w};
   const Weights w = sh.weights;
-  double f[kCuts] = {};
+  double f[N] = {};
   if constexpr (KIND == kCount) {
-    uint32_t n[kCuts] = {};
+    uint32_t n[N] = {};
     row.each([&](int, const float (&x)[kLanes]) {
       #pragma unroll
       for (int e = 0; e < kLanes; ++e)
         #pragma unroll
-        for (int i = 0; i < kCuts; ++i) n[i] += x[e] >= cut[i];
+        for (int i = 0; i < N; ++i) n[i] += x[e] >= cut[i];
     });
-    all_u32<T, kCuts>(row, turn, n, 0u, [](uint32_t v) { return __reduce_add_sync(0xffffffffu, v); });
-    return make_double4((double)n[0], (double)n[1], (double)n[2], (double)n[3]);
+    all_u32<T, N>(row, turn, n, 0u, [](uint32_t v) { return __reduce_add_sync(0xffffffffu, v); });
+    return make_double4((double)n[0], (double)n[1], N > 2 ? (double)n[N - 2] : 0.0, N > 2 ? (double)n[N - 1] : 0.0);
   } else {
     row.each([&](int, const float (&x)[kLanes]) {
       if constexpr (KIND == kMass) {
-        float s[2][kCuts] = {};
+        float s[2][N] = {};
         #pragma unroll
         for (int e = 0; e < kLanes; e += 2) {
           float v[2];
           w.two(x[e], x[e + 1], v[0], v[1]);
           #pragma unroll
-          for (int i = 0; i < kCuts; ++i)
+          for (int i = 0; i < N; ++i)
             #pragma unroll
             for (int q = 0; q < 2; ++q)
               if (x[e + q] >= cut[i]) s[q][i] += v[q];
         }
         #pragma unroll
-        for (int i = 0; i < kCuts; ++i) f[i] += (double)(s[0][i] + s[1][i]);
+        for (int i = 0; i < N; ++i) f[i] += (double)(s[0][i] + s[1][i]);
       } else {
         #pragma unroll
         for (int e = 0; e < kLanes; ++e) {
           const double v = w.wide(x[e]);
           #pragma unroll
-          for (int i = 0; i < kCuts; ++i) f[i] += x[e] >= cut[i] ? v : 0.0;
+          for (int i = 0; i < N; ++i) f[i] += x[e] >= cut[i] ? v : 0.0;
         }
       }
     });
-    all_sum<T, kCuts>(row, turn, f);
+    all_sum<T, N>(row, turn, f);
     const double by = KIND == kMass ? w.factor : 1.0;
-    return make_double4(f[0] * by, f[1] * by, f[2] * by, f[3] * by);
+    return make_double4(f[0] * by, f[1] * by, N > 2 ? f[N - 2] * by : 0.0, N > 2 ? f[N - 1] * by : 0.0);
   }
+}
+template <typename T, Kind KIND>
+__device__ __forceinline__ double4 measure(const Row<T>& row, int& turn, float4 at) {
+  return measure_of<T, KIND, kCuts>(row, turn, at);
+}
+template <typename T, Kind KIND>
+__device__ __forceinline__ double2 measure(const Row<T>& row, int& turn, float2 at) {
+  const double4 f = measure_of<T, KIND, 2>(row, turn, make_float4(at.x, at.y, NAN, NAN));
+  return make_double2(f.x, f.y);
 }
 
 // The largest value whose F reaches `target`, from F(from) >= target on; *above: F of what lies above it.
@@ -880,7 +889,7 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
   #pragma unroll 1
   for (int round = 0;; ++round) {
     if (round >= 3 || hi - lo <= 1) {
-      const double4 n = measure<T, kCount>(row, turn, make_float4(Type<T>::value(lo), Type<T>::value(hi), NAN, NAN));
+      const double2 n = measure<T, kCount>(row, turn, make_float2(Type<T>::value(lo), Type<T>::value(hi)));
       if (n.x - n.y <= (double)kFew) break;
       if (hi - lo <= 1 || round >= 16) return false;
     }
@@ -908,7 +917,7 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
     if (!moved && round >= 3) return false;                   // and more than kFew in between
   }
   const float below = Type<T>::value(hi);
-  const double4 g = measure<T, kExact>(row, turn, make_float4(from, below, NAN, NAN));
+  const double2 g = measure<T, kExact>(row, turn, make_float2(from, below));
   const unsigned n = collect<T>(row, 2, Type<T>::value(lo), below);
   if (row.rank == 0) {
     weigh_few(n);
@@ -1032,8 +1041,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
   __syncthreads();
   filters.cut = sh.edge;
   const bool fine = sh.weights.fine();
-  double4 f = {};                    // fp32's sums over all tokens, and over the largest
-  if (p_on && !k_on && fine) f = measure<T, kMass>(row, turn, make_float4(floor, top, NAN, NAN));
+  double2 f = {};                    // fp32's sums over all tokens, and over the largest
+  if (p_on && !k_on && fine) f = measure<T, kMass>(row, turn, make_float2(floor, top));
 
   // ------------------------------------------------------------- few are kept
   if (k_on || p_on || m_on) {
@@ -1051,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
     if (n <= kFew) {
       double sum = f.x, off = p_on && !k_on ? kOff : 0.0;
       if (p_on && !k_on && !fine) {
-        sum = measure<T, kExact>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
+        sum = measure<T, kExact>(row, turn, make_float2(floor, NAN)).x;
         off = 0.0;
       }
       #pragma unroll 1
@@ -1063,7 +1072,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
         }
         row.meet();
         if (off == 0.0 || !sh.unsure) return;
-        sum = measure<T, kExact>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
+        sum = measure<T, kExact>(row, turn, make_float2(floor, NAN)).x;
         off = 0.0;
       }
     }
@@ -1075,7 +1084,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
   double ties = INFINITY, above;
   int last = 0x7FFFFFFF;
   if (k_on) {
-    const double n = measure<T, kCount>(row, turn, make_float4(floor, NAN, NAN, NAN)).x;
+    const double n = measure<T, kCount>(row, turn, make_float2(floor, NAN)).x;
     if (n > (double)filters.top_k) {
       edge = search<T, kCount>(row, turn, floor, (double)filters.top_k, &above);
       ties = (double)filters.top_k - above;
@@ -1087,11 +1096,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
     const float from = !some ? edge : edge < top ? Type<T>::value(Type<T>::order(edge) + 1) : NAN;     // NaN: nothing
     const double top_p = fmax(filters.top_p, 0.0);
     const double w_edge = sh.weights.wide(edge), more = some ? ties * w_edge : 0.0;
-    if (fine && k_on) f = measure<T, kMass>(row, turn, make_float4(from, top, NAN, NAN));
+    if (fine && k_on) f = measure<T, kMass>(row, turn, make_float2(from, top));
     if (fine && last_kept<T>(row, turn, from, more, top_p, f.x, f.y, &edge, &last)) {
       ties = INFINITY;
     } else {
-      f = measure<T, kExact>(row, turn, make_float4(from, top, NAN, NAN));
+      f = measure<T, kExact>(row, turn, make_float2(from, top));
       const double target = top_p * (f.x + more);
       if (f.y >= target) {                               // the last one kept is one of the largest
         edge = top;

@@ -16,6 +16,12 @@ from .kv_cache import QuantizedKVCache
 from .tree_attention import _workspace
 
 
+def parts_size(total_q: int, q_heads: int, head_dim: int) -> int:
+    """ql_shared_attention_parts_size, without the call: the rows' sums up to a multiple of 16 bytes, then their outputs."""
+    rows = total_q * q_heads
+    return (8 * rows + 15 & -16) + 4 * rows * head_dim
+
+
 def _index(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise TypeError(f"{what} must be int32, got {t.dtype}")
@@ -108,14 +114,15 @@ def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKVCache, prefix_tab
             qs = q.stride()
         lib, ws = _lib.load(), _workspace(dev)
         # of this call alone: the allocator hands it on only to what the stream runs later
-        parts = torch.empty(lib.ql_shared_attention_parts_size(total_q, q_heads, head_dim), dtype=torch.uint8, device=dev)
+        nbytes = parts_size(total_q, q_heads, head_dim)
+        parts = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         packed = _lib.SHARED_ATTENTION_ARGS.pack(
             *cache.fields, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(),
             kv_lens.data_ptr(), cu_ptr, mask_ptr, batch, total_q, q_heads, qs[0], qs[1], width, stride, words, max_q,
             width * cache.page_size if max_kv is None else max_kv, code, head_dim ** -0.5 if scale is None else scale,
             ws.data_ptr(), ws.numel(), call_flags(), prefix_table.data_ptr(), prefix_lens.data_ptr(), group_ptr,
             parts.data_ptr(), groups, prefix_width, prefix_stride,
-            prefix_width * cache.page_size if max_prefix is None else max_prefix, parts.numel())
+            prefix_width * cache.page_size if max_prefix is None else max_prefix, nbytes)
         call(lib.ql_shared_attention, packed, dev)
     return (out, lse) if return_lse else out
 

@@ -357,3 +357,9 @@ def test_refusals():
                        ((q, c, first, prefix, t, kv), dict(mask=torch.zeros(2, 1, dtype=torch.int32, device="cuda")))):
         with pytest.raises(TypeError):
             run(*args, **(dict(cu_group=cu) | more))
+
+
+def test_parts_size_is_the_librarys():
+    from qlinear.kernels.shared_attention import parts_size
+    for total_q, q_heads, head_dim in ((0, 4, 64), (1, 1, 64), (3, 5, 128), (77, 28, 256), (100000, 64, 128)):
+        assert parts_size(total_q, q_heads, head_dim) == _lib.load().ql_shared_attention_parts_size(total_q, q_heads, head_dim)
