@@ -910,9 +910,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
           return;
         }
         const float2 e = p.early_sums[at];
+        const float4 v = *early;                        // whatever it is, where there is nothing
         if (e.y != 0.f) {                               // there is something (a NaN too)
           const float most = fmaxf(top, e.x), f0 = ex2<true>(top - most), f1 = ex2<true>(e.x - most);
-          const float4 v = *early;
           top = most;
           sum = sum * f0 + e.y * f1;
           o = make_float4(o.x * f0 + v.x * f1, o.y * f0 + v.y * f1, o.z * f0 + v.z * f1, o.w * f0 + v.w * f1);

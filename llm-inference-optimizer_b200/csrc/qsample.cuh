@@ -151,6 +151,13 @@ __device__ __forceinline__ uint32_t atom_dsmem_add(uint32_t addr, uint32_t v) {
 __device__ __forceinline__ unsigned order_of(float x) { return (unsigned)Type<float>::order(x); }
 __device__ __forceinline__ float value_of(unsigned k) { return Type<float>::value(k); }
 
+// 2^(i / 16).  In shared memory, where 16 of them take each bank once: lanes never wait for one another.
+__constant__ const double kRoots[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721,
+                                        1.241857812073484, 1.2968395546510096, 1.3542555469368927, 1.4142135623730951,
+                                        1.4768261459394993, 1.5422108254079407, 1.6104903319492543, 1.681792830507429,
+                                        1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+__shared__ double roots[16];
+
 // A row's weights.  In fp32, with a = (x - top) log2(e) / T: 2^a from a whole number n near a, and 2^(a - n).  a - n is taken
 // of the unrounded product: x hi - (n + base) in one rounding, n + base being exact, plus x lo; what base leaves of top's
 // share is a factor on all of them, which sums get.  Weights end at 2^-100.  How far sums may be off, of themselves:
@@ -202,28 +209,25 @@ struct Weights {
     two(x, x, v, w);
     return v;
   }
-  // In fp64, whose operations take eight times as long as fp32's: of (x - top) as it is, with n from fp32, and 2^(a - n) by
-  // its Chebyshev expansion up to the ninth power (2^-45; 1 of the largest, so that its ties are counted by whole numbers).
-  // Numbers become fp64 by their bits: the conversion's own instruction has a quarter of the rate.  (Numbers below fp32's
-  // normal ones, and 0, come out as one of their size: 2^-126 of a logit.)
+  // In fp64, whose operations take eight times as long as fp32's: of (x - top) as it is, 16 a as a whole number m (from fp32)
+  // and a rest r; 2^(m / 16) from a table of 16 and the exponent, 2^(r / 16) by its Chebyshev expansion up to the fifth power
+  // (2^-46; 1 of the largest, so that its ties are counted by whole numbers).  Numbers become fp64 by their bits: the
+  // conversion's own instruction has a quarter of the rate.  (Numbers below fp32's normal ones, and 0, come out as one of
+  // their size: 2^-126 of a logit.)
   __device__ __forceinline__ static double in64(float x) {
     const unsigned b = __float_as_uint(x);
     return __hiloint2double((int)(((b & 0x7FFFFFFFu) >> 3) + (896u << 20) | (b & 0x80000000u)), (int)(b << 29));
   }
   __device__ __forceinline__ double wide(float x) const {
-    const float m = fmaf(fmaxf(x - top, -3.402823466e38f), hi, 12582912.f);       // infinity less itself: a number
-    const double r = fma(in64(x) - high, scale, -in64(m - 12582912.f));
-    double y = 1.020869083593037e-07;
-    y = fma(y, r, 1.3259646250270451e-06);
-    y = fma(y, r, 1.5252657257186041e-05);
-    y = fma(y, r, 0.00015403433746224196);
-    y = fma(y, r, 0.0013333558230170627);
-    y = fma(y, r, 0.009618129193942167);
-    y = fma(y, r, 0.05550410866444768);
-    y = fma(y, r, 0.240226506956403);
-    y = fma(y, r, 0.69314718055995);
-    y = fma(y, r, 1.0);
-    return x >= zero ? __hiloint2double(__double2hiint(y) + (__float_as_int(m) << 20), __double2loint(y)) : 0.0;
+    const float m = fmaf(fmaxf(x - top, -3.402823466e38f), 16.f * hi, 12582912.f);       // infinity less itself: a number
+    const double r = fma(in64(x) - high, 16.0 * scale, -in64(m - 12582912.f));
+    double y = 1.2716120543908984e-09;
+    y = fma(y, r, 1.4676444622018903e-07);
+    y = fma(y, r, 1.355080777639003e-05);
+    y = fma(y, r, 0.0009383847924862057);
+    y = fma(y, r, 0.04332169878499668);
+    y = fma(y, r, 1.0) * roots[__float_as_int(m) & 15];
+    return x >= zero ? __hiloint2double(__double2hiint(y) + (__float_as_int(m) - 0x4B400000 >> 4 << 20), __double2loint(y)) : 0.0;
   }
   // log(w / sum) of the weight of x: the sum's by its exponent, and the rest, 2/3 .. 4/3, in fp32 (2^-24 of at most 0.41)
   __device__ __forceinline__ float log_chance(float x, double sum) const {
@@ -957,6 +961,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
   row.passes = (mine + kThreads - 1) / kThreads;
   row.src = static_cast<const T*>(p.logits) + (long long)line * p.stride + row.first;
   row.vec = p.vec != 0;
+  if (threadIdx.x < 16) roots[threadIdx.x] = kRoots[threadIdx.x];
   if (threadIdx.x < 3) sh.here[threadIdx.x] = sh.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.unsure = 0;
 
