@@ -1059,7 +1059,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int 
       const long long u = __shfl_up_sync(0xffffffffu, to, o);
       if (lane >= o) to += u;
     }
-    for (int at = 0; at < min(32, p.batch - i); ++at) {
+    // most are none of this warp's rows
+    const int from = __reduce_min_sync(0xffffffffu, i + lane < p.batch ? r.q0 : 0x7FFFFFFF);
+    const int end = __reduce_max_sync(0xffffffffu, r.q0 + r.q_len);
+    const bool near = __any_sync(0xffffffffu, !found && token >= from && token < end);
+    for (int at = 0; near && at < min(32, p.batch - i); ++at) {
       const int q0 = __shfl_sync(0xffffffffu, r.q0, at), q_len = __shfl_sync(0xffffffffu, r.q_len, at);
       const int kv_len = __shfl_sync(0xffffffffu, r.kv_len, at);
       const long long before = work.total + __shfl_sync(0xffffffffu, to - units, at);

@@ -175,7 +175,7 @@ struct Weights {
   __device__ __forceinline__ void set_heat(double heat) {
     inv_t = 1.0 / heat;
     scale = inv_t * 1.4426950408889634074;
-    hi = (float)scale;
+    hi = (float)fmin(scale, 1e37);                            // (no infinity, of which nothing could be taken 0 times)
     lo = (float)(scale - (double)hi);
   }
   __device__ __forceinline__ void set_top(float largest, double heat) {

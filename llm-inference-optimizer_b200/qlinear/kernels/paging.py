@@ -40,7 +40,9 @@ class PageTables:
     * free_pages int32 (num_pages,) and free_count int32 (1,): the first
       free_count entries are the free pages, the last of them taken first.
 
-    The tensors are the object's for its life, and calls change them."""
+    The tensors are the object's for its life, and calls change them: calls that
+    share some (two tables over one stack of free pages, say) must follow one
+    another, as they do on one stream."""
 
     page_table = property(lambda self: self._tensors[0])
     lens = property(lambda self: self._tensors[1])

@@ -72,6 +72,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     k, k_ptr, k_all = _setting(0 if top_k is None else top_k, rows, torch.int32, dev, "top_k")
     p, p_ptr, p_all = _setting(1.0 if top_p is None else top_p, rows, torch.float32, dev, "top_p")
     m, m_ptr, m_all = _setting(0.0 if min_p is None else min_p, rows, torch.float32, dev, "min_p")
+    if not isinstance(k_all, int):
+        raise TypeError(f"top_k must be a whole number, got {k_all!r}")
     if not 0.0 <= heat_all < float("inf") or not p_all >= 0.0 or not 0.0 <= m_all <= 1.0:
         raise ValueError(f"temperature must be finite and not negative, top_p not negative, min_p from 0 to 1: got "
                          f"{heat_all}, {p_all}, {m_all}")

@@ -150,6 +150,15 @@ def test_cut_and_grown_again_a_request_has_its_own_pages():
 
 
 @on_gpu
+def test_keep_may_be_the_lengths_themselves():
+    for batch, most in ((5, 64), (1500, 9000)):
+        pages, plain = PageTables.empty(batch, 8, 8 * batch, 16), Plain(batch, 8, 8 * batch, 16)
+        for i in range(3):
+            new = [(3 * b + i) % 9 for b in range(batch)]
+            agree(pages, plan_step(pages, ints(new), most, keep=pages.lens), plain, plain.step(new, most), most)
+
+
+@on_gpu
 def test_empty_calls():
     pages = PageTables.empty(0, 4, 8, 16)
     plan = plan_step(pages, ints([]), 5)

@@ -207,6 +207,20 @@ def test_hidden_and_infinite(dtype):
 
 
 @on_gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_temperatures_at_the_ends(dtype):
+    """So cold that only the largest have a weight, so hot that all have nearly the same; fp32's smallest and infinity."""
+    logits, uniform = rows_of(10, 4099, dtype, 15)
+    logits[3, [7, 4000]] = 30.0                            # two largest
+    for heat in (1e-45, 1e-38, 1e-30, 1e-12, 1e-4, 50.0, 1e6, 1e30, 3e38):
+        heats = torch.full((10,), heat, device="cuda")
+        for f in (dict(), dict(top_p=0.5), dict(top_k=20, top_p=0.9), dict(min_p=0.5)):
+            agree(logits, uniform, temperature=heats, **f)
+    hot = torch.full((10,), math.inf, device="cuda")       # all alike
+    assert torch.equal(sample_tokens(logits, uniform, temperature=hot), (uniform.double() * 4099).long())
+
+
+@on_gpu
 def test_random_numbers_at_the_ends():
     logits, _ = rows_of(6, 5000, torch.float16, 11)
     logits[:, 0] = -math.inf
@@ -283,5 +297,7 @@ def test_refusals():
                 dict(top_p=math.nan)):
         with pytest.raises(ValueError):
             sample_tokens(x, u, **bad)
+    with pytest.raises(TypeError, match="whole number"):
+        sample_tokens(x, u, top_k=2.0)
     with pytest.raises(AssertionError, match="out"):
         sample_tokens(x, u, out=torch.zeros(3, dtype=torch.int32, device="cuda"))

@@ -197,6 +197,29 @@ def test_empty_prefixes_groups_and_requests_outside(family):
 
 
 @on_gpu
+def test_prefix_tables_without_pages(family):
+    """Lengths are clamped to the table: there is no prefix."""
+    p = Problem([90], [0, 3], [2, 1, 4], [30, 9, 50], 8, 2, 64, 8, 16, torch.float16, seed=16)
+    p.first = p.first[:, :0]
+    got = p.run(cu_group=None)
+    p.prefixes = [0]
+    p.check(got)
+
+
+@on_gpu
+def test_many_groups(family):
+    """More groups than a warp's lanes; some of them empty, lengths from 0 to several units."""
+    n = 75
+    groups = [0]
+    for i in range(n):
+        groups.append(groups[-1] + (i * 7) % 3)
+    batch = groups[-1] + 2
+    p = Problem([(i * 97) % 700 for i in range(n)], groups, [1 + b % 3 for b in range(batch)], [3 + (b * 31) % 90 for b in range(batch)],
+                8, 2, 64, 8, 16, torch.float16, seed=17)
+    p.check(p.run())
+
+
+@on_gpu
 def test_rows_that_see_nothing_of_their_own(family):
     """Own lengths of zero and masks without a bit: the prefix alone; with a prefix of nothing: zeros."""
     for prefix in (400, 0):
