@@ -473,25 +473,35 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, BITS, NT>::kCtas))
     };
     int page_now = fetch_page(0), page_next = fetch_page(32), pages_at = 0;   // of tiles 32 pages_at ..
     // rows g of the queries, on their way while the pages are looked up and the first tiles copied
+    // (zeros first, then the loads: lanes that wrote zeros beside others' loads would wait for each of these)
     kvc::Vec8<T> q_raw[NT][S::kChunks][2];
     #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 8 * n + g;
-      const bool live = 8 * n + g < rows;
-      const int token = live ? p.by_group.of(row) : 0, qh = head * p.group + (live ? row - token * p.group : 0);
-      const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride;
+    for (int n = 0; n < NT; ++n)
       #pragma unroll
       for (int c = 0; c < S::kChunks; ++c)
         #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const T* at = src + c * 64 + t * 16 + h * 8;
-          if (live && p.q.vec) {
-            q_raw[n][c][h] = *reinterpret_cast<const kvc::Vec8<T>*>(at);
-          } else {
+        for (int h = 0; h < 2; ++h)
+          #pragma unroll
+          for (int i = 0; i < 8; ++i) q_raw[n][c][h].v[i] = kvc::from_f<T>(0.f);
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + 8 * n + g;
+      if (8 * n + g >= rows) continue;
+      const int token = p.by_group.of(row), qh = head * p.group + row - token * p.group;
+      const T* src = static_cast<const T*>(p.q.p) + (long long)(r.q0 + token) * p.q.token_stride + qh * p.q.head_stride + t * 16;
+      if (p.q.vec) {
+        #pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) q_raw[n][c][h] = *reinterpret_cast<const kvc::Vec8<T>*>(src + c * 64 + h * 8);
+      } else {
+        #pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h)
             #pragma unroll
-            for (int i = 0; i < 8; ++i) q_raw[n][c][h].v[i] = live ? at[i] : kvc::from_f<T>(0.f);
-          }
-        }
+            for (int i = 0; i < 8; ++i) q_raw[n][c][h].v[i] = src[c * 64 + h * 8 + i];
+      }
     }
     page_now = check_page(page_now);
     page_next = check_page(page_next);
