@@ -365,9 +365,9 @@ __host__ __device__ constexpr int step_add(int drow, int dchunk) {
 // does not matter.
 //
 // 64 requests of 3152 to 8192 positions, one token, 32 heads over 8 of 128, 8
-// bits: 129 us, 5.9 TB/s, 90 % of a plain copy's rate.  Repeated for seconds,
+// bits: 127 us, 6.0 TB/s, 91 % of a plain copy's rate.  Repeated for seconds,
 // that draws the GPU's 1000 W; the SM clock falls from 1965 to about 1700 MHz
-// and the time rises to 147.  At 4 bits half the bytes want as many
+// and the time rises to 143.  At 4 bits half the bytes want as many
 // instructions (about 400 per warp and tile of 16 keys), which bound it: one
 // token over 130001 positions, 28 heads over 4: 31 us, of which the tiles take
 // 18, the rest being a CTA's start and the joining of parts.

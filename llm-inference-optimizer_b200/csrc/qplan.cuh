@@ -25,6 +25,9 @@
 // new.  Many tokens (12 bytes each to be written, more than a cluster's SMs write
 // quickly) are left to a second kernel over all SMs, which looks them up in the
 // tables as they then are.
+//
+// One request: 3.8 us; 64 requests with trees (2100 tokens) 7.0; 1000 requests, 5900 tokens: 10.7 (one kernel: 12.9); 23
+// prompts, 131000 tokens: 10.7 (by the cluster's SMs alone: 23), of which the tokens' writes need 0.4.
 #pragma once
 
 #include "ql_common.cuh"

@@ -82,7 +82,11 @@ int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
   if (st != QL_OK) return st;
   const int64_t runs = cdiv(p.vocab, Type<T>::kLanes);
   auto passes = [&](int ctas) { return cdiv(cdiv(runs, ctas), kThreads); };
-  // as many CTAs a row as the SMs have places for; larger clusters find them less easily
+  // As many CTAs a row as the SMs have places for (two on each), and fewer of the larger clusters, which find their places
+  // less easily.  151936 logits, fp16, device us by CTAs a row 1 | 2 | 4 | 8 | 16:
+  //   top-k 50, top-p 0.95:   1 row  33 | 24 | 19 | 15 | 16     16 rows 35 | 26 | 21 | 19 | 34     64 rows 41 | 32 | 25 | 40 | 89
+  //   all of them:            1 row  27 | 17 | 12 |  9 |  8     16 rows 61 | 36 | 25 | 19 | 19     64 rows 85 | 54 | 38 | 38 | 55
+  //                         128 rows 98 | 61 | 55 | 64 | 102   256 rows 127 | 88 | 90 | 120 | 200
   auto room = [&](int ctas) { return ctas <= 2 ? 4 * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };
   int ctas = 1;
   while (ctas < kMaxCtas && passes(ctas) > 1 && ((int64_t)p.rows * 2 * ctas <= room(2 * ctas) || passes(ctas) * kWarps > kBlocks)) ctas *= 2;

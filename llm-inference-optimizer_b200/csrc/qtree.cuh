@@ -32,11 +32,12 @@
 // without meaning, and the device error word tells.
 //
 // 16 trees of 64 tokens after up to 8133 positions, 28 heads over 4 of 128, 8
-// bits, fp16: 158 us, 411 TFLOP/s (bf16: 213 us), a quarter of the tensor cores' rate.  A step
+// bits, fp16: 139 us, 467 TFLOP/s (bf16: 216 us), 28 % of the tensor cores' rate.  A step
 // of 128 keys takes some 4900 cycles, of which its products alone would be
 // 2048: P V reads its weights and scores leave through the same TMEM, decode
 // and products share the shared memory's ports, and the halves of the softmax
-// wait for one another.  About 30 us go into a CTA's start, queries and join.
+// wait for one another.  About 12 us go into a CTA's start, queries and join (30 while each of a thread's 16 loads of
+// queries waited for the one before).
 #pragma once
 
 #include "qattend.cuh"

@@ -11,6 +11,9 @@ SriramL1/LLM-inference-optimizer:
     qlinear.kernels.rotary          rotary positions (new)
     qlinear.kernels.kv_cache        quantised paged key/value cache (new)
     qlinear.kernels.tree_attention  attention of tokens, chains and trees over it (new)
+    qlinear.kernels.shared_attention  the same where requests share prefixes (new)
+    qlinear.kernels.paging          a batch's page tables, slots and positions (new)
+    qlinear.kernels.sampling        drawing tokens from logits (new)
 
 The compute runs in libqlinear.so (hand-written CUDA for sm_100a, C ABI in
 include/qlinear.h), bound through ctypes in ``qlinear._lib``.

@@ -2,9 +2,10 @@
 
     python -m qlinear._build            (from llm-inference-optimizer_b200/)
 
-The library is two translation units (csrc/qlinear.cu, the linear layers, and
-csrc/qattn.cu, the attention side; both include their kernel headers) linked
-against a static CUDA runtime, so the .so next to this file is all a GPU
+The library is four translation units (csrc/qlinear.cu, the linear layers;
+csrc/qattn.cu, the attention side; csrc/qshared.cu, attention behind shared
+prefixes; csrc/qserve.cu, a serving step's plan and sampling; all include their
+kernel headers) linked against a static CUDA runtime, so the .so next to this file is all a GPU
 machine needs.
 """
 from __future__ import annotations
