@@ -39,8 +39,9 @@
 // among them) and, of spread-out logits, the few rows that want fp64: 100 cycles
 // a logit and warp.  151936 logits, fp16, device: one row, top-k 50 and top-p
 // 0.95: 14.5 us; the largest: 4.2; 64 rows, the same: 23 and 8.2; 256 rows of
-// spread-out logits, all of them: 89 us (reading them: 12), of which 15 to 20 rows'
-// fp64 take about 45; 64 such rows under top-p alone, 50000 tokens kept: 189.
+// spread-out logits, all of them: 87 us (reading them: 12), and 53 where the given
+// numbers leave no row to fp64, which 7 in 100 want (64 rows: 39 and 18); 64 such
+// rows under top-p alone, 50000 tokens kept: 189.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -60,7 +61,7 @@ constexpr int kMine = 16;            // thresholds of a round over the threads' 
 constexpr int kFew = 1024;           // tokens that one CTA sorts
 constexpr int kFewer = kThreads / 4; // and those that it only compares with one another
 constexpr double kOff = 6e-7;        // what sums of fp32 weights may be off, of themselves
-constexpr int kBlocks = 3072;        // a row's part has no more than these runs of the warps
+constexpr int kBlocks = 3 * kFew;    // a row's part has no more than these runs of the warps
 constexpr int kStaged = 72 * 1024;   // bytes of a part that shared memory takes, two CTAs an SM
 
 struct Params {
