@@ -975,13 +975,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
   if (threadIdx.x < 3) sh.here[threadIdx.x] = sh.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.unsure = 0;
 
-  const double heat = p.temperature ? (double)p.temperature[line] : p.temperature_all;
+  double heat = p.temperature ? (double)p.temperature[line] : p.temperature_all;
   Filters filters;
   filters.top_p = p.top_p ? (double)p.top_p[line] : p.top_p_all;
   filters.top_k = p.top_k ? (long long)p.top_k[line] : p.top_k_all;
   const double min_p = p.min_p ? (double)p.min_p[line] : p.min_p_all;
   const double u = fmin(fmax((double)p.uniform[line], 0.0), 1.0);
   const bool greedy = !(heat > 0.0);
+  if (!greedy) heat = fmax(heat, 1e-200);      // its inverse is a number; no two fp32 logits are as near as 700 of it
   const bool k_on = filters.top_k > 0 && filters.top_k < p.vocab, p_on = filters.top_p < 1.0, m_on = min_p > 0.0;
   if (!k_on) filters.top_k = 0;
   if (!p_on) filters.top_p = 1.0;

@@ -221,6 +221,26 @@ def test_temperatures_at_the_ends(dtype):
 
 
 @on_gpu
+def test_temperatures_of_64_bits():
+    """Numbers, not tensors: down to those whose inverse is no number, and up to the largest."""
+    logits, uniform = rows_of(6, 4099, torch.float32, 16)
+    logits[3, [7, 4000]] = 30.0
+    for heat in (5e-324, 1e-310, 1e-308, 1e-250, 1e-199, 1e-100):
+        for f in (dict(), dict(top_p=0.5), dict(top_k=20, top_p=0.9), dict(min_p=0.5)):
+            ids, logprobs = sample_tokens(logits, uniform, heat, return_logprobs=True, **f)
+            want = sample_tokens(logits, uniform, 0.0)
+            if f.get("top_p") != 0.5 and uniform[3] >= 0.5:          # the second of two
+                want[3] = 4000
+            assert torch.equal(ids, want)
+            chance = torch.zeros(6, device="cuda")
+            if f.get("top_p") != 0.5:
+                chance[3] = -math.log(2.0)
+            assert torch.allclose(logprobs, chance, rtol=2.0 ** -19, atol=0)
+    for heat in (1e300, 1.7e308):                                    # all alike
+        assert torch.equal(sample_tokens(logits, uniform, heat), (uniform.double() * 4099).long())
+
+
+@on_gpu
 def test_random_numbers_at_the_ends():
     logits, _ = rows_of(6, 5000, torch.float16, 11)
     logits[:, 0] = -math.inf
