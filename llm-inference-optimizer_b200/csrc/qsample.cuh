@@ -61,6 +61,7 @@ constexpr int kMine = 16;            // thresholds of a round over the threads' 
 constexpr int kFew = 1024;           // tokens that one CTA sorts
 constexpr int kFewer = kThreads / 4; // and those that it only compares with one another
 constexpr double kOff = 6e-7;        // what sums of fp32 weights may be off, of themselves
+constexpr int kBins = 4096;          // of a histogram
 constexpr int kBlocks = 3 * kFew;    // a row's part has no more than these runs of the warps
 constexpr int kStaged = 72 * 1024;   // bytes of a part that shared memory takes, two CTAs an SM
 
@@ -258,6 +259,7 @@ struct Shared {
   } part;
   union {
     double block[kBlocks];           // of many tokens: sums by runs of the warps
+    unsigned bins[kBins];
     struct {                         // of few, in the cluster's first CTA
       unsigned long long key[kFew];
       unsigned long long weight[kFew], upto[kFew];      // in units of 2^-52 of the largest weight
@@ -265,11 +267,15 @@ struct Shared {
   };
   Weights weights;
   double before;
-  unsigned long long scan[kWarps];
+  unsigned long long scan[kWarps], sums[kWarps][2];
   unsigned long long found[kFew];    // tokens that this CTA has collected
   unsigned here[3], at, count[3];    // their number, their place in the first CTA's list; the list's length
   int owner, run, index, unsure;
   float edge;
+  // where a histogram's running sum crosses a target: its bins just below and just above that, -1 for none; what lies above
+  // the one and up to the other
+  int bin_above, bin_below;
+  unsigned long long mass_above, units_above, units_below;
 };
 
 __shared__ Shared sh;                // not an argument: a function that gets it as one reads it by generic addresses
@@ -890,6 +896,140 @@ __device__ __noinline__ bool finish(unsigned n, const Filters& filters, double s
   return true;
 }
 
+// Narrows lo <= x < hi (as Type::order), where F crosses `target`, right to `margin`, by a histogram of these tokens' weights;
+// *above: F(hi), in units of 2^-42 of the largest.  Returns no less than the number of tokens that are left, or infinity where
+// that is not known.
+//
+// A bin is a step of 1 / per in log2 of the weight, and counts units of 2^-bits of the weight in its middle: 2^-t of a token's
+// distance t from there, |t| <= 1/80, is 1 - t ln 2 + (t ln 2)^2 / 2 to 2^-23, so the units say both the weights and, to 1 in
+// 100, the number, and take no ex2.  bits: as many as let 32 hold a CTA's tokens.  Bins are found by one rounding of a product and a difference, which never falls where x rises: each is a range of values.
+constexpr double kPart = 0x1p42;
+template <typename T>
+__device__ __noinline__ double narrow(const Row<T> row, int& turn, double target, double margin, long long* lo, long long* hi,
+                                      unsigned long long* above, int bits, bool wide) {
+  constexpr int kLanes = Type<T>::kLanes;
+  constexpr float kMagic = 12582912.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float low = Type<T>::value(*lo), high = Type<T>::value(*hi);
+  const double scale = sh.weights.scale, octaves = ((double)high - (double)low) * scale;
+  // 32 octaves, below which few weights reach so far that top-p's target is there; less where less is left
+  const double per = fmin(fmax((kBins - 1) / octaves, wide ? kBins / 32.0 : 0.0), 0x1p24);
+  const float h = (float)(per * scale), off = (float)(per * scale * (double)high), one = (float)(1 << bits);
+  const float slope = (float)(one * 0.6931471805599453 / per), curve = (float)(0.5 * 0.6931471805599453 * 0.6931471805599453 * one / (per * per));
+  auto place = [&](float x) { return fmaxf(fmaf(x, -h, off), 0.f) + kMagic; };
+  auto bin_of = [&](float place) { return __float_as_int(place) - 0x4B400000; };
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.bin_above = sh.bin_below = -1;
+  row.each([&](int, const float (&x)[kLanes]) {
+    #pragma unroll
+    for (int e = 0; e < kLanes; ++e) {
+      const float f = fmaxf(fmaf(x[e], -h, off), 0.f), m = f + kMagic, t = f - (m - kMagic);
+      const float units = fmaf(t, fmaf(t, curve, -slope), one + kMagic);
+      const int bin = bin_of(m);
+      if (x[e] >= low && x[e] < high && bin < kBins) atomicAdd(&sh.bins[bin], (unsigned)(__float_as_int(units) - 0x4B400000));
+    }
+  });
+  row.meet();
+  // each CTA takes a run of the bins, each thread some of that
+  const int each = kBins / row.ctas, run = max(each / kThreads, 1), first = row.rank * each + (int)threadIdx.x * run;
+  const bool live = (int)threadIdx.x * run < each;
+  auto units_of = [&](int bin) {
+    unsigned long long u = 0;
+    for (int r = 0; r < row.ctas; ++r) u += ld_dsmem_u32(dsmem_addr(smem_u32(&sh.bins[bin]), (uint32_t)r));
+    return u;
+  };
+  const float middle = (float)(((double)high - (double)sh.weights.top) * scale), step = (float)(1.0 / per);
+  auto mass_of = [&](int bin, unsigned long long units) {
+    return __double2ull_rn((double)units * (double)(exp2f(fmaf((float)bin, -step, middle)) * (float)kPart / one));
+  };
+  unsigned long long mass = 0, units = 0;
+  if (live)
+    for (int i = 0; i < run; ++i) {
+      const unsigned long long u = units_of(first + i);
+      units += u;
+      mass += mass_of(first + i, u);
+    }
+  auto up = [&](unsigned long long& v) {
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+  };
+  unsigned long long mass_to = mass, units_to = units;
+  up(mass_to);
+  up(units_to);
+  if (lane == 31) {
+    sh.sums[warp][0] = mass_to;
+    sh.sums[warp][1] = units_to;
+  }
+  __syncthreads();
+  unsigned long long all = 0, all_units = 0, mass_at = *above, units_at = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) {
+      mass_at += sh.sums[i][0];
+      units_at += sh.sums[i][1];
+    }
+    all += sh.sums[i][0];
+    all_units += sh.sums[i][1];
+  }
+  turn ^= 1;
+  if ((int)threadIdx.x < row.ctas) {
+    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][0]), threadIdx.x), all);
+    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][1]), threadIdx.x), all_units);
+  }
+  row.meet();
+  unsigned long long everything = *above;
+  for (int r = 0; r < row.ctas; ++r) {
+    const unsigned long long m = (unsigned long long)__double_as_longlong(sh.box.f64[turn][r][0]);
+    everything += m;
+    if (r >= row.rank) continue;
+    mass_at += m;
+    units_at += (unsigned long long)__double_as_longlong(sh.box.f64[turn][r][1]);
+  }
+  mass_at += mass_to - mass;
+  units_at += units_to - units;
+  const unsigned long long least = (unsigned long long)((target - margin) * kPart), most = (unsigned long long)((target + margin) * kPart);
+  // the bin that reaches `least` first, and the one that passes `most`
+  if (live && mass_at <= most && mass_at + mass >= least) {
+    for (int i = 0; i < run; ++i) {
+      const unsigned long long u = units_of(first + i), m = mass_of(first + i, u);
+      if (mass_at < least && mass_at + m >= least)
+        for (int r = 0; r < row.ctas; ++r) {
+          st_dsmem_u32(dsmem_addr(smem_u32(&sh.bin_above), (uint32_t)r), (uint32_t)(first + i));
+          st_dsmem_u64(dsmem_addr(smem_u32(&sh.mass_above), (uint32_t)r), mass_at);
+          st_dsmem_u64(dsmem_addr(smem_u32(&sh.units_above), (uint32_t)r), units_at);
+        }
+      if (mass_at <= most && mass_at + m > most)
+        for (int r = 0; r < row.ctas; ++r) {
+          st_dsmem_u32(dsmem_addr(smem_u32(&sh.bin_below), (uint32_t)r), (uint32_t)(first + i));
+          st_dsmem_u64(dsmem_addr(smem_u32(&sh.units_below), (uint32_t)r), units_at + u);
+        }
+      mass_at += m;
+      units_at += u;
+    }
+  }
+  row.meet();
+  // the smallest value of a bin and those above it
+  auto value_from = [&](int bin) {
+    long long a = *lo, b = *hi;
+    if (bin_of(place(low)) <= bin) return a;
+    while (b - a > 1) {
+      const long long mid = (a + b) >> 1;
+      if (bin_of(place(Type<T>::value(mid))) <= bin) b = mid;
+      else a = mid;
+    }
+    return b;
+  };
+  const int bin_above = sh.bin_above, bin_below = sh.bin_below;
+  const long long to = bin_above < 0 ? value_from(kBins - 1) : bin_above > 0 ? value_from(bin_above - 1) : *hi;
+  if (bin_below >= 0) *lo = value_from(bin_below);
+  *hi = to;
+  *above = bin_above < 0 ? everything : sh.mass_above;
+  return bin_above < 0 || bin_below < 0 ? INFINITY : (double)(sh.units_below - sh.units_above) * 1.01 / (double)one;
+}
+
 // The last token that top-p keeps of those x >= from (`more`: what top-k's ties add to their weights), where it lies among
 // no more than kFew that fp32 weights cannot tell apart: those are collected and sorted, and the sum and what lies above
 // them taken in fp64.  all, largest: fp32's F(from) and F(top).  False: it does not.
@@ -899,10 +1039,19 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
   const float top = sh.weights.top;
   const double about = top_p * (all + more), margin = 4.0 * kOff * about;
   if (!(largest < about - margin) || !(all > about + margin)) return false;
-  long long lo = Type<T>::order(from), hi = Type<T>::order(top);
+  long long lo = Type<T>::order(fmaxf(from, sh.weights.end)), hi = Type<T>::order(top);
+  // How far a histogram's sums may be off, of themselves: by the units' rounding, the bins' weights (2^-18, exp2f of up to 100)
+  // and, as the product's factor and the bins' origin are rounded, by 2^-23 of the largest token's share.
+  const int bits = min(__clz(row.passes * kThreads * Type<T>::kLanes - 1) - 1, 20);
+  const double loose = 1.1 * about * (__hiloint2double((1023 - bits - 1) << 20, 0) + 0x1p-17 + fabs(sh.weights.share) * 0x1p-23);
+  double left = INFINITY;
+  unsigned long long above = (unsigned long long)(largest * kPart);
   #pragma unroll 1
-  for (int round = 0;; ++round) {
-    if (round >= 3 || hi - lo <= 1) {
+  for (int time = 0; time < 3 && left > (double)kFew && hi - lo > 1 && (double)above < (about - loose) * kPart; ++time)
+    left = narrow<T>(row, turn, about, loose, &lo, &hi, &above, bits, time == 0);
+  #pragma unroll 1
+  for (int round = 0; left > (double)kFew; ++round) {
+    if (round >= 2 || hi - lo <= 1) {
       const double2 n = measure<T, kCount>(row, turn, make_float2(Type<T>::value(lo), Type<T>::value(hi)));
       if (n.x - n.y <= (double)kFew) break;
       if (hi - lo <= 1 || round >= 16) return false;
@@ -910,9 +1059,7 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
     long long at[kCuts];
     #pragma unroll
     for (int i = 0; i < kCuts; ++i) {
-      // first by the tokens' weights, from e^-12 to e^-1.5 of the largest
-      const long long there = round == 0 ? Type<T>::order(top - (float)((12.0 - 3.5 * i) / sh.weights.inv_t)) : lo + (hi - lo) * (i + 1) / (kCuts + 1);
-      at[i] = min(max(there, lo + 1), hi - 1);
+      at[i] = min(max(lo + (hi - lo) * (i + 1) / (kCuts + 1), lo + 1), hi - 1);
     }
     const double4 q = measure<T, kMass>(row, turn, make_float4(Type<T>::value(at[0]), Type<T>::value(at[1]),
                                                                    Type<T>::value(at[2]), Type<T>::value(at[3])));
