@@ -936,7 +936,9 @@ __device__ __noinline__ double narrow(const Row<T> row, int& turn, double target
   const bool live = (int)threadIdx.x * run < each;
   auto units_of = [&](int bin) {
     unsigned long long u = 0;
-    for (int r = 0; r < row.ctas; ++r) u += ld_dsmem_u32(dsmem_addr(smem_u32(&sh.bins[bin]), (uint32_t)r));
+    #pragma unroll
+    for (int r = 0; r < kMaxCtas; ++r)                        // all on their way together
+      if (r < row.ctas) u += ld_dsmem_u32(dsmem_addr(smem_u32(&sh.bins[bin]), (uint32_t)r));
     return u;
   };
   const float middle = (float)(((double)high - (double)sh.weights.top) * scale), step = (float)(1.0 / per);
@@ -1012,13 +1014,16 @@ __device__ __noinline__ double narrow(const Row<T> row, int& turn, double target
   }
   row.meet();
   // the smallest value of a bin and those above it
-  auto value_from = [&](int bin) {
+  auto value_from = [&](int bin) {                            // 33 parts a round, of which lanes tell
     long long a = *lo, b = *hi;
     if (bin_of(place(low)) <= bin) return a;
     while (b - a > 1) {
-      const long long mid = (a + b) >> 1;
-      if (bin_of(place(Type<T>::value(mid))) <= bin) b = mid;
-      else a = mid;
+      const long long mid = a + max((b - a) * (lane + 1) / 33, 1ll);
+      const unsigned in = __ballot_sync(0xffffffffu, mid >= b || bin_of(place(Type<T>::value(mid))) <= bin);
+      const int pick = in ? __ffs(in) - 1 : 32;
+      const long long below = __shfl_sync(0xffffffffu, mid, max(pick - 1, 0)), to = __shfl_sync(0xffffffffu, mid, min(pick, 31));
+      if (pick > 0) a = below;
+      if (pick < 32) b = min(b, to);
     }
     return b;
   };
