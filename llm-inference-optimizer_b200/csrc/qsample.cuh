@@ -743,29 +743,44 @@ __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v) {
 }
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
 
-// Sorts key[0 .. n) from the largest down, and weight with it, n <= kFew.
+// Sorts key[0 .. n) from the largest down, n <= kFew; upto is lost.  A bitonic network over registers, one key a thread, two
+// above kThreads: partners within a warp exchange by shuffles, others through key and upto in turn, one barrier a step.  (256
+// keys: 6 such steps of 36; all steps through shared memory, with a barrier each, took 11700 cycles.)
 __device__ __noinline__ void sort(unsigned n) {
   const unsigned tid = threadIdx.x;
-  auto& key = sh.few.key;
-  auto& weight = sh.few.weight;
   unsigned size = 64;
   while (size < n) size *= 2;
-  for (unsigned i = n + tid; i < size; i += kThreads) key[i] = 0;
+  const bool live = tid < size, two = size > kThreads;
+  __syncthreads();
+  unsigned long long a = tid < n ? sh.few.key[tid] : 0, b = tid + kThreads < n ? sh.few.key[tid + kThreads] : 0;
+  unsigned long long *at = sh.few.upto, *next = sh.few.key;
+  auto keep = [&](unsigned long long mine, unsigned long long other, bool larger) { return (mine < other) == larger ? other : mine; };
+  #pragma unroll 1
   for (unsigned k = 2; k <= size; k *= 2)
+    #pragma unroll 1
     for (unsigned j = k / 2; j > 0; j /= 2) {
-      __syncthreads();
-      if (tid < size / 2) {
-        const unsigned a = 2 * tid - (tid & (j - 1)), b = a + j;
-        const unsigned long long x = key[a], y = key[b];
-        if ((x < y) == ((a & k) == 0)) {
-          key[a] = y;
-          key[b] = x;
-          const unsigned long long w = weight[a];
-          weight[a] = weight[b];
-          weight[b] = w;
-        }
+      const bool low = (tid & j) == 0, a_larger = low == ((tid & k) == 0), b_larger = low == ((tid + kThreads & k) == 0);
+      if (j == kThreads) {
+        const unsigned long long most = max(a, b);
+        b = min(a, b);
+        a = most;
+      } else if (j >= 32) {
+        if (live) at[tid] = a;
+        if (two) at[tid + kThreads] = b;
+        __syncthreads();
+        if (live) a = keep(a, at[tid ^ j], a_larger);
+        if (two) b = keep(b, at[(tid ^ j) + kThreads], b_larger);
+        unsigned long long* swap = at;
+        at = next;
+        next = swap;
+      } else if (live) {
+        a = keep(a, __shfl_xor_sync(0xffffffffu, a, j), a_larger);
+        if (two) b = keep(b, __shfl_xor_sync(0xffffffffu, b, j), b_larger);
       }
     }
+  __syncthreads();
+  if (live) sh.few.key[tid] = a;
+  if (two) sh.few.key[tid + kThreads] = b;
   __syncthreads();
 }
 // Running sums of weight[0 .. n) to upto[0 .. n).
@@ -788,9 +803,9 @@ __device__ __noinline__ void run_up(unsigned n) {
 }
 // Weights of few tokens, as whole numbers: additions of these are exact and quick.  None but a zero becomes zero.
 constexpr double kWhole = 0x1p52;
-__device__ __forceinline__ void weigh_few(unsigned n) {
+__device__ __noinline__ void weigh_few(unsigned n, int value_at = 32) {      // where keys have the value
   for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-    const double w = sh.weights.wide(value_of((unsigned)(sh.few.key[i] >> 32)));
+    const double w = sh.weights.wide(value_of((unsigned)(sh.few.key[i] >> value_at)));
     const unsigned long long whole = __double2ull_rn(w * kWhole);
     sh.few.weight[i] = whole == 0 && w > 0.0 ? 1 : whole;
   }
@@ -868,6 +883,7 @@ __device__ __noinline__ bool finish(unsigned n, const Filters& filters, double s
     return true;
   }
   sort(n);
+  weigh_few(n);
   run_up(n);
   if (k_on) target = top_p * (double)upto[most - 1];
   bool unsure = false;
@@ -883,6 +899,7 @@ __device__ __noinline__ bool finish(unsigned n, const Filters& filters, double s
   for (unsigned i = tid; i < kept; i += kThreads) key[i] = key[i] << 32 | key[i] >> 32;       // by index
   __syncthreads();
   sort(kept);
+  weigh_few(kept, 0);
   run_up(kept);
   unsigned before = 0;
   for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= t;
@@ -1086,8 +1103,8 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
   const double2 g = measure<T, kExact>(row, turn, make_float2(from, below));
   const unsigned n = collect<T>(row, 2, Type<T>::value(lo), below);
   if (row.rank == 0) {
-    weigh_few(n);
     sort(n);
+    weigh_few(n);
     run_up(n);
     const double target = (top_p * (g.x + more) - g.y) * kWhole;
     unsigned short_of = 0;
@@ -1234,7 +1251,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
       #pragma unroll 1
       for (int time = 0;; ++time) {
         if (row.rank == 0) {
-          if (time == 0) weigh_few(n);
+          if (time == 0 && n <= kFewer) weigh_few(n);
           if (!finish(n, filters, sum, off, u, id, logprob) && threadIdx.x < row.ctas)
             st_dsmem_u32(dsmem_addr(smem_u32(&sh.unsure), threadIdx.x), 1u);
         }
