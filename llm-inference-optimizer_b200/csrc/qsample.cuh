@@ -292,8 +292,8 @@ struct Row {
   float mine;                        // this thread's largest logit
   bool vec;                          // runs are whole and aligned
 
-  __device__ __forceinline__ uint4 load(int v) const {
-    const int o = (v * kThreads + (int)threadIdx.x) * kLanes;
+  __device__ __forceinline__ uint4 load(int v, int thread) const {
+    const int o = (v * kThreads + thread) * kLanes;
     if (vec && o + kLanes <= count) return *reinterpret_cast<const uint4*>(src + o);
     uint4 r;
     T* e = reinterpret_cast<T*>(&r);
@@ -301,6 +301,7 @@ struct Row {
     for (int i = 0; i < kLanes; ++i) e[i] = o + i < count ? src[o + i] : (T)(-INFINITY);
     return r;
   }
+  __device__ __forceinline__ uint4 load(int v) const { return load(v, (int)threadIdx.x); }
   // f(run, its values), four runs on their way at a time
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
@@ -320,7 +321,8 @@ struct Row {
       }
     }
   }
-  __device__ __forceinline__ int index(int v) const { return first + (v * kThreads + (int)threadIdx.x) * kLanes; }
+  __device__ __forceinline__ int index(int v, int thread) const { return first + (v * kThreads + thread) * kLanes; }
+  __device__ __forceinline__ int index(int v) const { return index(v, (int)threadIdx.x); }
   __device__ __forceinline__ void meet() const {             // all threads of the cluster
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
@@ -491,7 +493,10 @@ __device__ __noinline__ bool bound(const Row<T> row, int& turn, bool mass, float
   bool found = false;
   #pragma unroll 1
   for (int round = 0; round < 10; ++round) {
-    const long long at = lo + (hi - lo) * (lane & (kMine - 1)) / kMine;
+    // even in value, where the values are that near; else even in their order
+    const float from = Type<T>::value(lo), span = Type<T>::value(hi) - from;
+    long long at = lo + (hi - lo) * (lane & (kMine - 1)) / kMine;
+    if (span < 1024.f) at = min(max(Type<T>::order(fmaf(span, (float)(lane & (kMine - 1)) / kMine, from) + 0.f), lo), hi - 1);
     const float cut = Type<T>::value(at);
     uint32_t f = 0;
     if (mass) {
@@ -531,7 +536,8 @@ __device__ __noinline__ bool bound(const Row<T> row, int& turn, bool mass, float
     if (pick + 1 < kMine) hi = next;
     lo = __shfl_sync(0xffffffffu, at, pick);
     all = __shfl_sync(0xffffffffu, all, pick);
-    if (hi - lo <= 1 || all <= enough_of) break;
+    // (weights: what lies within 2^(1/32) of the last is not told apart, however few are above)
+    if (hi - lo <= 1 || all <= enough_of || (mass && (double)(Type<T>::value(hi) - Type<T>::value(lo)) * sh.weights.scale < 0.03125)) break;
   }
   *v = Type<T>::value(lo);
   return true;
@@ -694,21 +700,33 @@ __device__ __noinline__ void draw(const Row<T> row, int& turn, float edge, int l
 template <typename T>
 __device__ __noinline__ unsigned collect(const Row<T> row, int call, float cut, float below) {
   constexpr int kLanes = Type<T>::kLanes;
-  if (row.mine >= cut)
-    row.each([&](int v, const float (&x)[kLanes]) {
-      unsigned some = 0;
-      #pragma unroll
-      for (int e = 0; e < kLanes; ++e) some |= (x[e] >= cut && !(x[e] >= below)) << e;
-      if (some == 0) return;
-      unsigned at = atomicAdd(&sh.here[call], (unsigned)__popc(some));
-      #pragma unroll
-      for (int e = 0; e < kLanes; ++e)
-        if (some >> e & 1) {
-          if (at < kFew)
-            sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(row.index(v) + e));
-          ++at;
-        }
-    });
+  auto take = [&](const float (&x)[kLanes], int index) {
+    unsigned some = 0;
+    #pragma unroll
+    for (int e = 0; e < kLanes; ++e) some |= (x[e] >= cut && !(x[e] >= below)) << e;
+    if (some == 0) return;
+    unsigned at = atomicAdd(&sh.here[call], (unsigned)__popc(some));
+    #pragma unroll
+    for (int e = 0; e < kLanes; ++e)
+      if (some >> e & 1) {
+        if (at < kFew) sh.found[at] = (unsigned long long)order_of(x[e] + 0.f) << 32 | (0xFFFFFFFFu - (unsigned)(index + e));
+        ++at;
+      }
+  };
+  unsigned holders = __ballot_sync(0xffffffffu, row.mine >= cut);
+  if (__popc(holders) * ((row.passes + 31) / 32) < row.passes) {
+    // few threads of the warp have any: their runs one thread after another, a run a lane
+    for (; holders; holders &= holders - 1) {
+      const int thread = (int)(threadIdx.x & ~31u) + __ffs(holders) - 1;
+      for (int v = threadIdx.x & 31; v < row.passes; v += 32) {
+        float x[kLanes];
+        Type<T>::decode(row.load(v, thread), x);
+        take(x, row.index(v, thread));
+      }
+    }
+  } else if (row.mine >= cut) {
+    row.each([&](int v, const float (&x)[kLanes]) { take(x, row.index(v)); });
+  }
   __syncthreads();
   const unsigned here = sh.here[call];
   const uint32_t counter = dsmem_addr(smem_u32(&sh.count[call]), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
