@@ -762,8 +762,22 @@ __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v) {
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
 
 // Sorts key[0 .. n) from the largest down, n <= kFew; upto is lost.  A bitonic network over registers, one key a thread, two
-// above kThreads: partners within a warp exchange by shuffles, others through key and upto in turn, one barrier a step.  (256
-// keys: 6 such steps of 36; all steps through shared memory, with a barrier each, took 11700 cycles.)
+// above kThreads: partners within a warp exchange by shuffles, others through upto and key in turn, one barrier a step.
+template <int J>
+__device__ __forceinline__ void exchange(unsigned long long& v, bool larger) {
+  const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, J);
+  v = (larger == ((threadIdx.x & J) == 0)) ? max(v, other) : min(v, other);
+}
+// the steps within a warp of blocks of k
+template <int J>
+__device__ __forceinline__ void exchanges(unsigned long long& v, unsigned index, unsigned k) {
+  const bool larger = (index & k) == 0;
+  if constexpr (J >= 16) exchange<16>(v, larger);
+  if constexpr (J >= 8) exchange<8>(v, larger);
+  if constexpr (J >= 4) exchange<4>(v, larger);
+  if constexpr (J >= 2) exchange<2>(v, larger);
+  exchange<1>(v, larger);
+}
 __device__ __noinline__ void sort(unsigned n) {
   const unsigned tid = threadIdx.x;
   unsigned size = 64;
@@ -772,30 +786,44 @@ __device__ __noinline__ void sort(unsigned n) {
   __syncthreads();
   unsigned long long a = tid < n ? sh.few.key[tid] : 0, b = tid + kThreads < n ? sh.few.key[tid + kThreads] : 0;
   unsigned long long *at = sh.few.upto, *next = sh.few.key;
-  auto keep = [&](unsigned long long mine, unsigned long long other, bool larger) { return (mine < other) == larger ? other : mine; };
+  auto first = [&](unsigned long long& v) {
+    exchanges<1>(v, tid, 2);
+    exchanges<2>(v, tid, 4);
+    exchanges<4>(v, tid, 8);
+    exchanges<8>(v, tid, 16);
+    exchanges<16>(v, tid, 32);
+  };
+  if (live) first(a);
+  if (two) first(b);
   #pragma unroll 1
-  for (unsigned k = 2; k <= size; k *= 2)
+  for (unsigned k = 64; k <= size; k *= 2) {
     #pragma unroll 1
-    for (unsigned j = k / 2; j > 0; j /= 2) {
-      const bool low = (tid & j) == 0, a_larger = low == ((tid & k) == 0), b_larger = low == ((tid + kThreads & k) == 0);
+    for (unsigned j = k / 2; j >= 32; j /= 2) {
       if (j == kThreads) {
         const unsigned long long most = max(a, b);
         b = min(a, b);
         a = most;
-      } else if (j >= 32) {
-        if (live) at[tid] = a;
-        if (two) at[tid + kThreads] = b;
-        __syncthreads();
-        if (live) a = keep(a, at[tid ^ j], a_larger);
-        if (two) b = keep(b, at[(tid ^ j) + kThreads], b_larger);
-        unsigned long long* swap = at;
-        at = next;
-        next = swap;
-      } else if (live) {
-        a = keep(a, __shfl_xor_sync(0xffffffffu, a, j), a_larger);
-        if (two) b = keep(b, __shfl_xor_sync(0xffffffffu, b, j), b_larger);
+        continue;
       }
+      if (live) at[tid] = a;
+      if (two) at[tid + kThreads] = b;
+      __syncthreads();
+      const bool low = (tid & j) == 0;
+      if (live) {
+        const unsigned long long other = at[tid ^ j];
+        a = low == ((tid & k) == 0) ? max(a, other) : min(a, other);
+      }
+      if (two) {
+        const unsigned long long other = at[(tid ^ j) + kThreads];
+        b = low == ((tid + kThreads & k) == 0) ? max(b, other) : min(b, other);
+      }
+      unsigned long long* swap = at;
+      at = next;
+      next = swap;
     }
+    if (live) exchanges<16>(a, tid, k);
+    if (two) exchanges<16>(b, tid + kThreads, k);
+  }
   __syncthreads();
   if (live) sh.few.key[tid] = a;
   if (two) sh.few.key[tid + kThreads] = b;
