@@ -24,9 +24,10 @@
 //                   known by its last token: a value v and how many of the tokens
 //                   equal to v are kept.  v is the largest value whose measure F(v)
 //                   over tokens x >= v (their number; the sum of their weights)
-//                   reaches a target: it is searched for over the type's values in
-//                   their order, which are whole numbers, with four thresholds a
-//                   round, each round a pass.
+//                   reaches a target.  For weights a histogram narrows it down to
+//                   the tokens that one CTA sorts; else it is searched for over the
+//                   type's values in their order, which are whole numbers, with
+//                   four thresholds a round, each round a pass.
 //
 // A token is drawn, or not, by the comparison of two running sums, so these are
 // held to more than fp32.  Sums over many weights are first taken, in fp64, of
@@ -34,14 +35,14 @@
 // 2^-19.6 of themselves; then the weights are taken again in fp64.
 //
 // What bounds it: for few rows the chain of passes and meetings of the cluster (a
-// meeting 0.5 us, each function's first run its way from memory), for many the
-// instructions of the weights (a dozen a logit, ex2 at a quarter of the rate
-// among them) and, of spread-out logits, the few rows that want fp64: 100 cycles
-// a logit and warp.  151936 logits, fp16, device: one row, top-k 50 and top-p
-// 0.95: 14.5 us; the largest: 4.2; 64 rows, the same: 23 and 8.2; 256 rows of
-// spread-out logits, all of them: 87 us (reading them: 12), and 53 where the given
-// numbers leave no row to fp64, which 7 in 100 want (64 rows: 39 and 18); 64 such
-// rows under top-p alone, 50000 tokens kept: 189.
+// meeting 0.5 us, each function's first run its way from memory: less code is
+// quicker than unrolled code), for many the instructions of the weights (a dozen a
+// logit, ex2 at a quarter of the rate among them) and, of spread-out logits, the
+// few rows that want fp64: some 40 instructions a logit.  151936 logits, fp16,
+// device: one row, top-k 50 and top-p 0.95: 12.4 us; the largest: 4.1; 64 rows, the
+// same: 20 and 8.5; 256 rows of spread-out logits, all of them: 86 us (reading them:
+// 12), and 53 where the given numbers leave no row to fp64, which 7 in 100 want (64
+// rows: 38 and 18); 64 such rows under top-p alone, 50000 tokens kept: 103.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -220,7 +221,7 @@ struct Weights {
     two(x, x, v, w);
     return v;
   }
-  // In fp64, whose operations take eight times as long as fp32's: of (x - top) as it is, 16 a as a whole number m (from fp32)
+  // In fp64, some 40 instructions: of (x - top) as it is, 16 a as a whole number m (from fp32)
   // and a rest r; 2^(m / 16) from a table of 16 and the exponent, 2^(r / 16) by its Chebyshev expansion up to the fifth power
   // (2^-46; 1 of the largest, so that its ties are counted by whole numbers).  Numbers become fp64 by their bits: the
   // conversion's own instruction has a quarter of the rate.  (Numbers below fp32's normal ones, and 0, come out as one of
@@ -316,6 +317,24 @@ struct Row {
   }
   __device__ __forceinline__ int index(int v, int thread) const { return first + (v * kThreads + thread) * kLanes; }
   __device__ __forceinline__ int index(int v) const { return index(v, (int)threadIdx.x); }
+  // f(values, index of the first) of the runs of those threads whose `holds` is set.  Where they are few of a warp, its lanes
+  // take these one thread after another, a run a lane.
+  template <typename F>
+  __device__ __forceinline__ void each_of(bool holds, F f) const {
+    unsigned holders = __ballot_sync(0xffffffffu, holds);
+    if (__popc(holders) * ((passes + 31) / 32) < passes) {
+      for (; holders; holders &= holders - 1) {
+        const int thread = (int)(threadIdx.x & ~31u) + __ffs(holders) - 1;
+        for (int v = threadIdx.x & 31; v < passes; v += 32) {
+          float x[kLanes];
+          Type<T>::decode(load(v, thread), x);
+          f(x, index(v, thread));
+        }
+      }
+    } else if (holds) {
+      each([&](int v, const float (&x)[kLanes]) { f(x, index(v)); });
+    }
+  }
   __device__ __forceinline__ void meet() const {             // all threads of the cluster
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
@@ -706,20 +725,7 @@ __device__ __noinline__ unsigned collect(const Row<T> row, int call, float cut, 
         ++at;
       }
   };
-  unsigned holders = __ballot_sync(0xffffffffu, row.mine >= cut);
-  if (__popc(holders) * ((row.passes + 31) / 32) < row.passes) {
-    // few threads of the warp have any: their runs one thread after another, a run a lane
-    for (; holders; holders &= holders - 1) {
-      const int thread = (int)(threadIdx.x & ~31u) + __ffs(holders) - 1;
-      for (int v = threadIdx.x & 31; v < row.passes; v += 32) {
-        float x[kLanes];
-        Type<T>::decode(row.load(v, thread), x);
-        take(x, row.index(v, thread));
-      }
-    }
-  } else if (row.mine >= cut) {
-    row.each([&](int v, const float (&x)[kLanes]) { take(x, row.index(v)); });
-  }
+  row.each_of(row.mine >= cut, take);
   __syncthreads();
   const unsigned here = sh.here[call];
   const uint32_t counter = dsmem_addr(smem_u32(&sh.count[call]), 0), keys = dsmem_addr(smem_u32(&sh.few.key[0]), 0);
@@ -755,7 +761,8 @@ __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v) {
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
 
 // Sorts key[0 .. n) from the largest down, n <= kFew; upto is lost.  A bitonic network over registers, one key a thread, two
-// above kThreads: partners within a warp exchange by shuffles, others through upto and key in turn, one barrier a step.
+// above kThreads: partners within a warp exchange by shuffles, others through upto and key in turn, one barrier a step.  200
+// keys take 3900 cycles, 1024 12800; all steps in shared memory, with a barrier each, took 11700 and 18000.
 template <int J>
 __device__ __forceinline__ void exchange(unsigned long long& v, bool larger) {
   const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, J);
@@ -1243,12 +1250,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
   }
   if (greedy) {
     unsigned at = 0xFFFFFFFFu;
-    if (row.mine == top)
-      row.each([&](int v, const float (&x)[kLanes]) {
-        #pragma unroll
-        for (int e = 0; e < kLanes; ++e)
-          if (x[e] == top) at = min(at, (unsigned)(row.index(v) + e));
-      });
+    row.each_of(row.mine == top, [&](const float (&x)[kLanes], int index) {
+      #pragma unroll
+      for (int e = 0; e < kLanes; ++e)
+        if (x[e] == top) at = min(at, (unsigned)(index + e));
+    });
     uint32_t v[1] = {at};
     all_u32<T, 1>(row, turn, v, 0xFFFFFFFFu, [](uint32_t x) { return __reduce_min_sync(0xffffffffu, x); });
     if (row.rank == 0 && threadIdx.x == 0) {

@@ -74,7 +74,7 @@ constexpr int64_t kFewRequests = 1024, kFewTokens = 2048;
 
 // ------------------------------------------------------------------- sampling
 template <typename T>
-int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
+int run_sample(const ql::smp::Params& p, bool few, int sms, void* stream, int64_t flags) {
   using namespace ql::smp;
   auto kernel = sample_kernel<T>;
   static std::atomic<unsigned char> done[kMaxDevices];
@@ -84,10 +84,13 @@ int run_sample(const ql::smp::Params& p, int sms, void* stream, int64_t flags) {
   auto passes = [&](int ctas) { return cdiv(cdiv(runs, ctas), kThreads); };
   // As many CTAs a row as the SMs have places for (two on each), and fewer of the larger clusters, which find their places
   // less easily.  151936 logits, fp16, device us by CTAs a row 1 | 2 | 4 | 8 | 16:
-  //   top-k 50, top-p 0.95:   1 row  33 | 24 | 19 | 15 | 16     16 rows 35 | 26 | 21 | 19 | 34     64 rows 41 | 32 | 25 | 40 | 89
-  //   all of them:            1 row  27 | 17 | 12 |  9 |  8     16 rows 61 | 36 | 25 | 19 | 19     64 rows 85 | 54 | 38 | 38 | 55
-  //                         128 rows 98 | 61 | 55 | 64 | 102   256 rows 127 | 88 | 90 | 120 | 200
-  auto room = [&](int ctas) { return ctas <= 2 ? 4 * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };
+  //   top-k 50, top-p 0.95:   1 row  20 | 16 | 14 | 13 | 12     16 rows 23 | 18 | 17 | 16 | 27     64 rows 26 | 22 | 20 | 33 | 74
+  //   all of them:            1 row  26 | 17 | 12 |  9 |  8     16 rows 62 | 37 | 25 | 18 | 18     64 rows 83 | 54 | 37 | 35 | 53
+  //                         128 rows 97 | 62 | 56 | 61 |  98   256 rows 120 | 86 | 89 | 114 | 192
+  //   top-p 0.9:              1 row 156 | 95 | 64 | 44 | 40     64 rows 224 | 143 | 104 | 124 | 226   256 rows 298 | 300 | 346 | 459 | 845
+  // Where all rows are known to keep few, one CTA is less to start and to meet:
+  //   top-k 50, top-p 0.95: 128 rows 33 | 25 | 39     256 rows 38 | 47 | 74        the largest: 128 rows 21 | 15     256 rows 24 | 28
+  auto room = [&](int ctas) { return ctas <= 2 ? (few ? 2 : 4) * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };
   int ctas = 1;
   while (ctas < kMaxCtas && passes(ctas) > 1 && ((int64_t)p.rows * 2 * ctas <= room(2 * ctas) || passes(ctas) * kWarps > kBlocks)) ctas *= 2;
   const size_t bytes = (size_t)passes(ctas) * kThreads * 16;
@@ -184,10 +187,11 @@ int ql_sample_tokens(const ql_sample_tokens_args* a, void* stream) {
   p.rows = (int)a->rows;
   p.vocab = (int)a->vocab;
   p.vec = aligned(a->logits, 16) && (a->rows == 1 || a->row_stride * (int64_t)bytes % 16 == 0);
+  const bool few = (!a->temperature && !(a->temperature_all > 0.0)) || (!a->top_k && a->top_k_all > 0 && a->top_k_all <= ql::smp::kFew / 2);
   switch (a->dtype) {
-    case QL_DTYPE_F16: return run_sample<__half>(p, dev.sms, stream, a->flags);
-    case QL_DTYPE_BF16: return run_sample<__nv_bfloat16>(p, dev.sms, stream, a->flags);
-    default: return run_sample<float>(p, dev.sms, stream, a->flags);
+    case QL_DTYPE_F16: return run_sample<__half>(p, few, dev.sms, stream, a->flags);
+    case QL_DTYPE_BF16: return run_sample<__nv_bfloat16>(p, few, dev.sms, stream, a->flags);
+    default: return run_sample<float>(p, few, dev.sms, stream, a->flags);
   }
 }
 
