@@ -40,7 +40,7 @@
 // logit, ex2 at a quarter of the rate among them) and, of spread-out logits, the
 // few rows that want fp64: some 40 instructions a logit.  151936 logits, fp16,
 // device: one row, top-k 50 and top-p 0.95: 12.4 us; the largest: 4.1; 64 rows, the
-// same: 20 and 8.5; 256 rows of spread-out logits, all of them: 86 us (reading them:
+// same: 20 and 7.3; 256 rows of spread-out logits, all of them: 86 us (reading them:
 // 12), and 53 where the given numbers leave no row to fp64, which 7 in 100 want (64
 // rows: 38 and 18); 64 such rows under top-p alone, 50000 tokens kept: 103.
 #pragma once

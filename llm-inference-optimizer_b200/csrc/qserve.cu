@@ -89,7 +89,7 @@ int run_sample(const ql::smp::Params& p, bool few, int sms, void* stream, int64_
   //                         128 rows 97 | 62 | 56 | 61 |  98   256 rows 120 | 86 | 89 | 114 | 192
   //   top-p 0.9:              1 row 156 | 95 | 64 | 44 | 40     64 rows 224 | 143 | 104 | 124 | 226   256 rows 298 | 300 | 346 | 459 | 845
   // Where all rows are known to keep few, one CTA is less to start and to meet:
-  //   top-k 50, top-p 0.95: 128 rows 33 | 25 | 39     256 rows 38 | 47 | 74        the largest: 128 rows 21 | 15     256 rows 24 | 28
+  //   top-k 50, top-p 0.95: 128 rows 34 | 25 | 40     256 rows 39 | 48 | 75        the largest: 128 rows 15 | 12     256 rows 18 | 22
   auto room = [&](int ctas) { return ctas <= 2 ? (few ? 2 : 4) * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };
   int ctas = 1;
   while (ctas < kMaxCtas && passes(ctas) > 1 && ((int64_t)p.rows * 2 * ctas <= room(2 * ctas) || passes(ctas) * kWarps > kBlocks)) ctas *= 2;

@@ -152,6 +152,31 @@ def test_vocabularies_past_the_registers(dtype):
     agree(logits, uniform)
 
 
+MANY = {
+    "spread": lambda g, n: 2.2 * torch.randn(n, generator=g),
+    "even": lambda g, n: torch.rand(n, generator=g),                                  # thousands within a small step
+    "steps": lambda g, n: torch.randint(0, 6, (n,), generator=g).float(),             # thousands of each value
+    "two heaps": lambda g, n: torch.where(torch.rand(n, generator=g) < 0.1, 5.0, -9.0) + 0.3 * torch.randn(n, generator=g),
+    "long": lambda g, n: 40.0 * torch.rand(n, generator=g) - 1000.0,                  # all of 58 octaves alike
+    "one above": lambda g, n: torch.cat([torch.tensor([60000.0]), 59990.0 + 0.0 * torch.randn(n - 1, generator=g)]),
+}
+
+
+@on_gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", MANY)
+def test_many_tokens_kept(dtype, kind):
+    """top-p's border among thousands of tokens: near its ends, behind top-k, of a large vocabulary and of a part of it."""
+    g = torch.Generator().manual_seed(71)
+    for vocab in (2500, 50021) + ((151936,) if kind == "spread" else ()):
+        x = torch.stack([MANY[kind](g, vocab) for _ in range(3)])
+        x[1, torch.rand(vocab, generator=g) < 0.5] = -math.inf
+        x, u = x.to(dtype).cuda(), torch.rand(3, generator=g).cuda()
+        for f in (dict(top_p=0.3), dict(top_p=0.9, temperature=1.3), dict(top_p=0.99, temperature=0.6), dict(top_p=0.99999),
+                  dict(top_p=0.9, top_k=2000), dict(top_p=0.97, min_p=1e-3), dict(top_p=1e-6)):
+            agree(x, u, **f)
+
+
 @on_gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_settings_of_each_row(dtype):
