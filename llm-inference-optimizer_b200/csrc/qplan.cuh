@@ -26,7 +26,7 @@
 // quickly) are left to a second kernel over all SMs, which looks them up in the
 // tables as they then are.
 //
-// One request: 3.8 us; 64 requests with trees (2100 tokens) 7.0; 1000 requests, 5900 tokens: 10.7 (one kernel: 12.9); 23
+// One request: 3.7 us; 64 requests with trees (2100 tokens) 7.0; 1000 requests, 5900 tokens: 10.7 (one kernel: 12.9); 23
 // prompts, 131000 tokens: 10.7 (by the cluster's SMs alone: 23), of which the tokens' writes need 0.4.
 #pragma once
 
@@ -253,28 +253,16 @@ __global__ void __launch_bounds__(kThreads, 1) plan_kernel(const Params p) {
     }
   }
   if (!p.tokens) return;
-  for (long long t0 = at; t0 < p.max_tokens; t0 += (long long)kAtOnce * step) {
-    int page[kAtOnce], position[kAtOnce];
-    #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const long long t = t0 + (long long)i * step;
-      page[i] = -1;
-      position[i] = 0;
-      if (t >= total) continue;
-      const int b = holder(first_token, p.batch, (int)t), pos = keeps[b] + (int)t - first_token[b];
-      const int k = pos >> p.page_shift, kept = (int)((keeps[b] + page_mask) >> p.page_shift);
-      const long long from = available - 1 - (first_taken[b] + k - kept);
-      const int* src = k < kept ? p.table + (long long)b * p.table_stride + k : p.stack + from;
-      if (k < kept || (from >= 0 && from < p.num_pages)) page[i] = *src;
-      position[i] = pos;
+  for (long long t = at; t < p.max_tokens; t += step) {       // one at a time: they are few, and so is the code
+    int page = -1, position = 0;
+    if (t < total) {
+      const int b = holder(first_token, p.batch, (int)t);
+      position = keeps[b] + (int)t - first_token[b];
+      const int k = position >> p.page_shift, kept = (int)((keeps[b] + page_mask) >> p.page_shift);
+      page = k < kept ? p.table[(long long)b * p.table_stride + k] : page_taken(first_taken[b] + k - kept);
     }
-    #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const long long t = t0 + (long long)i * step;
-      if (t >= p.max_tokens) continue;
-      p.slots[t] = page[i] < 0 ? -1 : ((long long)page[i] << p.page_shift) + (position[i] & page_mask);
-      p.positions[t] = position[i];
-    }
+    p.slots[t] = page < 0 ? -1 : ((long long)page << p.page_shift) + (position & page_mask);
+    p.positions[t] = position;
   }
 }
 

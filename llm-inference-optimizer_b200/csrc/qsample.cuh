@@ -1148,6 +1148,7 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
   const float below = Type<T>::value(hi);
   const double2 g = measure<T, kExact>(row, turn, make_float2(from, below));
   const unsigned n = collect<T>(row, 2, Type<T>::value(lo), below);
+  if (n == 0 || n > kFew) return false;                       // (neither, by the bounds above)
   if (row.rank == 0) {
     sort(n);
     weigh_few(n);
