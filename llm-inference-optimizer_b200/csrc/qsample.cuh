@@ -250,10 +250,13 @@ struct Weights {
 };
 
 struct Shared {
-  union {                            // what the cluster's CTAs have sent, in turn
-    double f64[2][kMaxCtas][kCuts];
-    uint32_t u32[2][kMaxCtas][kMine];
-  } box;
+  // What the cluster's CTAs have sent, in turn: a meeting's values to one half, the next one's to the other.  A CTA writes a
+  // half again only behind the meeting in between, at which all have read what it held.  Sums and counts share the halves, of
+  // which each is a union of its own: halves of different sizes in one union would lie over each other.
+  union {
+    double f64[kMaxCtas][kCuts];
+    uint32_t u32[kMaxCtas][kMine];
+  } box[2];
   union {
     double f64[kWarps][kCuts];
     uint32_t u32[kWarps][kMine];
@@ -376,13 +379,13 @@ __device__ __forceinline__ void all_sum(const Row<T>& row, int& turn, double (&v
     #pragma unroll
     for (int q = 0; q < N; ++q) {
       const double all = __shfl_sync(0xffffffffu, s, q * (32 / N));
-      if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][q]), (uint32_t)lane), all);
+      if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box[turn].f64[row.rank][q]), (uint32_t)lane), all);
     }
   }
   row.meet();
   double w[N];
   #pragma unroll
-  for (int q = 0; q < N; ++q) w[q] = lane < row.ctas ? sh.box.f64[turn][lane][q] : 0.0;
+  for (int q = 0; q < N; ++q) w[q] = lane < row.ctas ? sh.box[turn].f64[lane][q] : 0.0;
   s = warp_sums<N>(w);
   #pragma unroll
   for (int q = 0; q < N; ++q) v[q] = __shfl_sync(0xffffffffu, s, q * (32 / N));
@@ -402,12 +405,12 @@ __device__ __forceinline__ void all_u32(const Row<T>& row, int& turn, uint32_t (
     #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t s = op(lane < kWarps ? sh.part.u32[lane][i] : none);
-      if (lane < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][row.rank][i]), (uint32_t)lane), s);
+      if (lane < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box[turn].u32[row.rank][i]), (uint32_t)lane), s);
     }
   }
   row.meet();
   #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = op(lane < row.ctas ? sh.box.u32[turn][lane][i] : none);
+  for (int i = 0; i < N; ++i) v[i] = op(lane < row.ctas ? sh.box[turn].u32[lane][i] : none);
 }
 // F at thresholds: the number of tokens x >= cut (not of a NaN), or the sum of their weights.  A function of its own for
 // each kind: the code is read from memory once a launch, and that is a good part of a short row's time.
@@ -533,12 +536,12 @@ __device__ __noinline__ bool bound(const Row<T> row, int& turn, bool mass, float
       for (int w = 0; w < kWarps; ++w) f += sh.part.u32[w][lane];
       #pragma unroll
       for (int r = 0; r < kMaxCtas; ++r)
-        if (r < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box.u32[turn][row.rank][lane]), (uint32_t)r), f);
+        if (r < row.ctas) st_dsmem_u32(dsmem_addr(smem_u32(&sh.box[turn].u32[row.rank][lane]), (uint32_t)r), f);
     }
     row.meet();
     unsigned long long sum = 0;
     #pragma unroll
-    for (int r = 0; r < kMaxCtas; ++r) sum += r < row.ctas ? sh.box.u32[turn][r][lane & (kMine - 1)] : 0u;
+    for (int r = 0; r < kMaxCtas; ++r) sum += r < row.ctas ? sh.box[turn].u32[r][lane & (kMine - 1)] : 0u;
     double all = (double)sum;
     const unsigned enough = __ballot_sync(0xffffffffu, lane < kMine && all >= wanted);
     if (!found && !(enough & 1u)) return false;
@@ -626,11 +629,11 @@ __device__ __forceinline__ double locate(const Row<T>& row, int& turn, float edg
       if (lane * per_lane + i < blocks) own += sh.block[lane * per_lane + i];
     upto = upto_lane(own);
     const double all = __shfl_sync(0xffffffffu, upto, 31);
-    if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][0]), (uint32_t)lane), all);
+    if (lane < row.ctas) st_dsmem_f64(dsmem_addr(smem_u32(&sh.box[turn].f64[row.rank][0]), (uint32_t)lane), all);
   }
   row.meet();
   // each warp finds whose part holds the token, by the same sums: first lanes, CTAs; then, in that CTA, lanes' blocks
-  const double part = lane < row.ctas ? sh.box.f64[turn][lane][0] : 0.0;
+  const double part = lane < row.ctas ? sh.box[turn].f64[lane][0] : 0.0;
   double to = upto_lane(part);
   const double sum = __shfl_sync(0xffffffffu, to, 31), t = KIND == kCount ? wanted : wanted * sum;
   auto pick = [&](bool some, bool past) {                     // the first past the target, else the last that has some
@@ -1041,17 +1044,17 @@ __device__ __noinline__ double narrow(const Row<T> row, int& turn, double target
   }
   turn ^= 1;
   if ((int)threadIdx.x < row.ctas) {
-    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][0]), threadIdx.x), all);
-    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box.f64[turn][row.rank][1]), threadIdx.x), all_units);
+    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box[turn].f64[row.rank][0]), threadIdx.x), all);
+    st_dsmem_u64(dsmem_addr(smem_u32(&sh.box[turn].f64[row.rank][1]), threadIdx.x), all_units);
   }
   row.meet();
   unsigned long long everything = *above;
   for (int r = 0; r < row.ctas; ++r) {
-    const unsigned long long m = (unsigned long long)__double_as_longlong(sh.box.f64[turn][r][0]);
+    const unsigned long long m = (unsigned long long)__double_as_longlong(sh.box[turn].f64[r][0]);
     everything += m;
     if (r >= row.rank) continue;
     mass_at += m;
-    units_at += (unsigned long long)__double_as_longlong(sh.box.f64[turn][r][1]);
+    units_at += (unsigned long long)__double_as_longlong(sh.box[turn].f64[r][1]);
   }
   mass_at += mass_to - mass;
   units_at += units_to - units;
