@@ -1175,10 +1175,11 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int staged) {
   extern __shared__ uint4 stage[];                            // the part, where it fits
   griddep_launch_dependents();
-  griddep_wait();
-  constexpr int kLanes = Type<T>::kLanes;
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  if (ctas > 1) cluster_arrive_relaxed();                     // waited for where the logits have been read
+  griddep_wait();
+  constexpr int kLanes = Type<T>::kLanes;
   Row<T> row;
   row.ctas = (int)ctas;
   row.rank = (int)cluster_rank();
@@ -1241,7 +1242,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p, int
     row.vec = true;
   }
   row.mine = most = most + 0.f;
-  // the largest, and the least of the threads' largest (of those that have some)
+  // the largest, and the least of the threads' largest (of those that have some); the row's other CTAs run by now
+  if (ctas > 1) cluster_wait();
   uint32_t ends[2] = {order_of(most), most > -INFINITY ? ~order_of(most) : 0u};
   all_u32<T, 2>(row, turn, ends, 0u, [](uint32_t v) { return __reduce_max_sync(0xffffffffu, v); });
   const float top = value_of(ends[0]), least = value_of(~ends[1]);
