@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (ks > 1) cluster_arrive_relaxed();                // waited for before the first store to a member's buffer
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full + s, 1);
@@ -472,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (m < M) comb[m * kRows + r] = acc[m];
     }
     named_bar_sync(1, kDecThreads);
+    if (ks > 1) cluster_wait();                    // all members run
     if (set == 0) {
       if (WBITS == 4) {
         #pragma unroll
@@ -531,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (ks > 1) {
     // ------------------------------------------------ cluster reduction
+    if (warp < 2) cluster_wait();         // (the others have)
     cluster_sync_all();                   // every member's slices are in this CTA's buffer
     if (warp >= 2) {
       const int E = p.M * kRows;
