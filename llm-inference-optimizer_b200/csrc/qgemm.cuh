@@ -334,6 +334,8 @@ __global__ void __launch_bounds__(Layout<WBITS, BN>::kThreads, 1)
   // accumulator at TMEM column q * BN
   const int nissuers = (L::kTwoIssuers && nk > 1) ? 2 : 1;
 
+  // waited for before the first store to a member's buffer
+  if (gridDim.z > 1 && L::kPush) cluster_arrive_relaxed();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(wfull + s, 1);
@@ -631,6 +633,7 @@ __global__ void __launch_bounds__(Layout<WBITS, BN>::kThreads, 1)
       // Split-K, push: element e = m*128 + r of the partial belongs to
       // member e / sz, which sums it; store it straight into that member's
       // receive buffer, slot of this CTA's rank (remote stores, no reply)
+      cluster_wait();                      // all members run
       const int ks = (int)gridDim.z;
       const int sz = (BN * kTileN + ks - 1) / ks;
       const uint32_t me = cluster_rank();
@@ -669,6 +672,7 @@ __global__ void __launch_bounds__(Layout<WBITS, BN>::kThreads, 1)
 
   if (gridDim.z > 1 && L::kPush) {
     // ------------------------------------------ cluster reduction (push)
+    if (warp < 2 || warp == kIssuer1Warp) cluster_wait();   // (the others have)
     cluster_sync_all();                 // every member's slices are in this CTA's receive buffer
     if (warp >= 2 && warp < kIssuer1Warp) {
       const int ks = (int)gridDim.z;

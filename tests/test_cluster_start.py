@@ -22,7 +22,8 @@ def body(file: str, kernel: str) -> str:
 
 
 @pytest.mark.parametrize("file,kernel,store", [("qsample.cuh", "sample_kernel", r"all_u32<"),
-                                               ("qdec.cuh", "qdec_kernel", r"st_dsmem_f32\(")])
+                                               ("qdec.cuh", "qdec_kernel", r"st_dsmem_f32\("),
+                                               ("qgemm.cuh", "qgemm_kernel", r"st_dsmem_f32\(")])
 def test_all_run_before_the_first_store(file, kernel, store):
     text = body(file, kernel)
     at = [re.search(pattern, text) for pattern in (r"cluster_arrive_relaxed\(\)", r"cluster_wait\(\)", store)]
