@@ -1159,13 +1159,17 @@ __device__ __noinline__ bool last_kept(const Row<T> row, int& turn, float from, 
     const double target = (top_p * (g.x + more) - g.y) * kWhole;
     unsigned short_of = 0;
     for (unsigned i = 2 * threadIdx.x; i < 2 * threadIdx.x + 2 && i < n; ++i) short_of += (double)sh.few.upto[i] < target;
-    const unsigned pick = min(cta_count(short_of), n - 1);
+    const unsigned pick = cta_count(short_of);
+    // exact sums say whether the border lies among these tokens at all, whatever the bounds above are worth
+    const bool among = target > 0.0 && pick < n;
+    const unsigned long long key = sh.few.key[among ? pick : 0];
     if (threadIdx.x < row.ctas) {
-      st_dsmem_u32(dsmem_addr(smem_u32(&sh.edge), threadIdx.x), __float_as_uint(value_of((unsigned)(sh.few.key[pick] >> 32))));
-      st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), threadIdx.x), (uint32_t)index_of(sh.few.key[pick]));
+      st_dsmem_u32(dsmem_addr(smem_u32(&sh.edge), threadIdx.x), __float_as_uint(value_of((unsigned)(key >> 32))));
+      st_dsmem_u32(dsmem_addr(smem_u32(&sh.index), threadIdx.x), among ? (uint32_t)index_of(key) : 0xFFFFFFFFu);
     }
   }
   row.meet();
+  if (sh.index < 0) return false;
   *edge = sh.edge;
   *last = sh.index;
   return true;
