@@ -138,17 +138,23 @@ class BatchDecoder:
 def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
     """Runs all prompts, each for its number of tokens; returns their tokens and the number of steps.  Where the running
     requests wait for one another's pages, the last one begins again later."""
-    g = torch.Generator(device="cuda").manual_seed(seed)
+    device = decoder.tokens.device
+    g = torch.Generator(device=device).manual_seed(seed)
     waiting, at, out = list(range(len(prompts))), [None] * decoder.batch, [[] for _ in prompts]
     steps, short = 0, False
     while waiting or any(r is not None for r in at):
+        refused = False
         for place, running in enumerate(at):
             if running is None and waiting and not short:
-                draw = torch.rand(1, generator=g, device="cuda")
+                draw = torch.rand(1, generator=g, device=device)
                 if decoder.start(place, prompts[waiting[0]], draw):
                     at[place] = waiting.pop(0)
                     out[at[place]].append(int(decoder.tokens[place]))
-        tokens, served = (t.tolist() for t in decoder.step(torch.rand(decoder.batch, generator=g, device="cuda")))
+                else:
+                    refused = True
+        if refused and all(r is None for r in at):
+            raise ValueError(f"the pool is too small for request {waiting[0]}'s prompt alone")
+        tokens, served = (t.tolist() for t in decoder.step(torch.rand(decoder.batch, generator=g, device=device)))
         steps += 1
         running = [place for place, r in enumerate(at) if r is not None]
         short = not all(served[place] for place in running)
@@ -166,7 +172,7 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
             decoder.end(place)
             waiting.insert(0, at[place])
             out[at[place]], at[place] = [], None
-    decoder.step(torch.zeros(decoder.batch, device="cuda"))          # the last ones' pages
+    decoder.step(torch.zeros(decoder.batch, device=device))          # the last ones' pages
     return out, steps
 
 

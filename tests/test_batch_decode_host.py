@@ -1,0 +1,60 @@
+"""examples/batch_decode.py without a GPU: how requests are served by a decoder that only counts, and what becomes of a row
+that had nothing to draw."""
+import sys
+from pathlib import Path
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+
+
+class Counter:
+    """A decoder of `batch` places and `room` tokens, whose requests' tokens count up from their prompt's length."""
+
+    def __init__(self, batch: int, room: int):
+        self.batch, self.room = batch, room
+        self.tokens = torch.zeros(batch + 1, dtype=torch.int64)
+        self.held, self.left = [0] * batch, 200
+
+    def start(self, place, ids, uniform):
+        self.left -= 1
+        assert self.left > 0, "serve goes on without end"
+        if sum(self.held) + len(ids) > self.room:
+            return False
+        self.held[place], self.tokens[place] = len(ids), len(ids)
+        return True
+
+    def end(self, place):
+        self.held[place] = 0
+
+    def step(self, uniform):
+        self.left -= 1
+        assert self.left > 0, "serve goes on without end"
+        served = torch.zeros(self.batch, dtype=torch.bool)
+        for place in range(self.batch):
+            if self.held[place] and sum(self.held) < self.room:
+                self.held[place] += 1
+                self.tokens[place] += 1
+                served[place] = True
+        return self.tokens[:self.batch], served
+
+
+def prompts(*lengths):
+    return [torch.zeros(n, dtype=torch.int64) for n in lengths]
+
+
+def test_requests_wait_for_one_another():
+    from batch_decode import serve
+    out, _ = serve(Counter(2, 12), prompts(3, 2, 4), [5, 9, 4])
+    assert out == [list(range(3, 8)), list(range(2, 11)), list(range(4, 8))]
+
+
+def test_a_request_that_never_fits_is_refused():
+    """Behind others that do, or at once: nothing runs whose end could make room."""
+    from batch_decode import serve
+    with pytest.raises(ValueError, match="too small"):
+        serve(Counter(2, 10), prompts(3, 11), [2, 2])
+    with pytest.raises(ValueError, match="too small"):
+        serve(Counter(1, 10), prompts(11), [2])
