@@ -140,7 +140,7 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
     requests wait for one another's pages, the last one begins again later."""
     device = decoder.tokens.device
     g = torch.Generator(device=device).manual_seed(seed)
-    waiting, at, out = list(range(len(prompts))), [None] * decoder.batch, [[] for _ in prompts]
+    waiting, at, out = [r for r, n in enumerate(lengths) if n > 0], [None] * decoder.batch, [[] for _ in prompts]
     steps, short = 0, False
     while waiting or any(r is not None for r in at):
         refused = False
@@ -150,6 +150,9 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
                 if decoder.start(place, prompts[waiting[0]], draw):
                     at[place] = waiting.pop(0)
                     out[at[place]].append(int(decoder.tokens[place]))
+                    if lengths[at[place]] == 1:
+                        decoder.end(place)
+                        at[place] = None
                 else:
                     refused = True
         if refused and all(r is None for r in at):

@@ -58,3 +58,12 @@ def test_a_request_that_never_fits_is_refused():
         serve(Counter(2, 10), prompts(3, 11), [2, 2])
     with pytest.raises(ValueError, match="too small"):
         serve(Counter(1, 10), prompts(11), [2])
+
+
+def test_as_many_tokens_as_asked_for():
+    """The first comes with the prompt: a request for one token has no step, one for none does not begin."""
+    from batch_decode import serve
+    out, steps = serve(Counter(2, 40), prompts(3, 5, 6, 7), [1, 0, 2, 1])
+    assert out == [[3], [], [6, 7], [7]]
+    out, _ = serve(Counter(1, 5), prompts(5, 4, 5), [1, 1, 1])          # no room for a step
+    assert out == [[5], [4], [5]]
