@@ -50,7 +50,10 @@ class BatchDecoder:
                                  torch.zeros(1, dtype=torch.int32, device="cuda"), self.pages.free_pages,
                                  self.pages.free_count, page_size)
         self.prompt_len = prompt.shape[0]
-        self._fill(prompt, plan_step(self.prefix, self._ints([self.prompt_len]), self.prompt_len), self.prefix, None)
+        plan = plan_step(self.prefix, self._ints([self.prompt_len]), self.prompt_len)
+        if int(plan.refused):
+            raise ValueError(f"a prompt of {self.prompt_len} tokens needs {room} pages, the pool has {num_pages}")
+        self._fill(prompt, plan, self.prefix, None)
         # a step's buffers, which the graph reads and writes
         self.new = torch.zeros(batch, dtype=torch.int32, device="cuda")
         self.keep = torch.zeros(batch, dtype=torch.int32, device="cuda")

@@ -67,3 +67,21 @@ def test_as_many_tokens_as_asked_for():
     assert out == [[3], [], [6, 7], [7]]
     out, _ = serve(Counter(1, 5), prompts(5, 4, 5), [1, 1, 1])          # no room for a step
     assert out == [[5], [4], [5]]
+
+
+def test_a_prompt_that_does_not_fit_the_pool(monkeypatch):
+    """Its plan has no tokens, and all requests would be answered without it."""
+    import batch_decode
+    refused = SimpleNamespace(refused=torch.tensor([1], dtype=torch.int32))
+    monkeypatch.setattr(batch_decode, "plan_step", lambda *args, **kwargs: refused)
+    monkeypatch.setattr(batch_decode.BatchDecoder, "_fill", lambda *args: pytest.fail("goes on without its prompt"))
+    monkeypatch.setattr(batch_decode.BatchDecoder, "_ints", staticmethod(lambda v: torch.tensor(v, dtype=torch.int32)))
+    monkeypatch.setattr(batch_decode.QuantizedKVCache, "empty", lambda *args, **kwargs: None)
+    monkeypatch.setattr(batch_decode.RotaryTable, "from_config", lambda *args, **kwargs: None)
+    empty, zeros = batch_decode.PageTables.empty, torch.zeros
+    monkeypatch.setattr(batch_decode.PageTables, "empty", lambda *args: empty(*args, device="cpu"))
+    monkeypatch.setattr(torch, "zeros", lambda *args, device="cpu", **kwargs: zeros(*args, **kwargs))
+    config = SimpleNamespace(hidden_size=128, num_attention_heads=2, num_key_value_heads=1)
+    model = SimpleNamespace(config=config, model=SimpleNamespace(layers=[]))
+    with pytest.raises(ValueError, match="prompt"):
+        batch_decode.BatchDecoder(model, torch.arange(70), 2, num_pages=4, pages_each=2)
