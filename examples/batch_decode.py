@@ -77,7 +77,7 @@ class BatchDecoder:
         """Logits of tokens ids at the plan's slots and positions, these counted from `offset`."""
         inner = self.model.model
         positions = plan.positions + offset
-        h = inner.embed_tokens(ids)
+        h = inner.embed_tokens(ids.clamp(min=0))              # -1: a row that had nothing to draw
         for layer, cache in zip(inner.layers, self.caches):
             attn = layer.self_attn
             q, k, v = (t.unflatten(-1, (-1, self.head_dim)) for t in attn.qkv_proj(layer.input_layernorm(h)))
@@ -145,6 +145,11 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
     g = torch.Generator(device=device).manual_seed(seed)
     waiting, at, out = [r for r, n in enumerate(lengths) if n > 0], [None] * decoder.batch, [[] for _ in prompts]
     steps, short = 0, False
+
+    def take(r: int, token: int) -> None:
+        if token < 0:
+            raise ValueError(f"request {r} has nothing to draw from after {len(out[r])} tokens: are its logits NaN?")
+        out[r].append(token)
     while waiting or any(r is not None for r in at):
         refused = False
         for place, running in enumerate(at):
@@ -152,7 +157,7 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
                 draw = torch.rand(1, generator=g, device=device)
                 if decoder.start(place, prompts[waiting[0]], draw):
                     at[place] = waiting.pop(0)
-                    out[at[place]].append(int(decoder.tokens[place]))
+                    take(at[place], int(decoder.tokens[place]))
                     if lengths[at[place]] == 1:
                         decoder.end(place)
                         at[place] = None
@@ -167,7 +172,7 @@ def serve(decoder: BatchDecoder, prompts, lengths, seed: int = 0):
         for place in running:
             r = at[place]
             if served[place]:
-                out[r].append(tokens[place])
+                take(r, tokens[place])
             if len(out[r]) >= lengths[r]:
                 decoder.end(place)
                 at[place] = None

@@ -85,3 +85,33 @@ def test_a_prompt_that_does_not_fit_the_pool(monkeypatch):
     model = SimpleNamespace(config=config, model=SimpleNamespace(layers=[]))
     with pytest.raises(ValueError, match="prompt"):
         batch_decode.BatchDecoder(model, torch.arange(70), 2, num_pages=4, pages_each=2)
+
+
+def test_a_row_with_nothing_to_draw():
+    """sample_tokens gives -1 for it (all of its logits NaN): no index of the embedding, where it would end the process on
+    a GPU, and no token for the user either."""
+    from batch_decode import BatchDecoder, serve
+    d = BatchDecoder.__new__(BatchDecoder)
+    inner = SimpleNamespace(embed_tokens=torch.nn.Embedding(5, 4), layers=[], norm=lambda h: h)
+    d.model, d.caches = SimpleNamespace(model=inner, lm_head=lambda h: h), []
+    plan = SimpleNamespace(positions=torch.zeros(3, dtype=torch.int32))
+    got = d._layers(torch.tensor([1, -1, 4]), plan, None, 0)
+    assert torch.equal(got, inner.embed_tokens.weight[[1, 0, 4]])
+
+    class Nothing(Counter):
+        def step(self, uniform):
+            tokens, served = super().step(uniform)
+            tokens[0] = -1
+            return tokens, served
+
+    with pytest.raises(ValueError, match="nothing to draw"):
+        serve(Nothing(2, 40), prompts(3, 5), [4, 4])
+
+    class AtOnce(Counter):
+        def start(self, place, ids, uniform):
+            started = super().start(place, ids, uniform)
+            self.tokens[place] = -1
+            return started
+
+    with pytest.raises(ValueError, match="nothing to draw"):
+        serve(AtOnce(2, 40), prompts(3, 5), [4, 4])
