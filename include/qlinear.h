@@ -522,13 +522,15 @@ int ql_plan_step(const ql_plan_step_args* args, void* stream);
  * are kept, of those the ones before which the weights come to less than top_p
  * of their sum, of those the ones with w_i >= min_p, and the first always; the
  * token is the first by index at which the running sum of the kept weights
- * exceeds uniform times their sum.  Sums are in fp64.  T <= 0: the largest
- * logit, the first of equal ones.  logprobs[r] (optional) = log of the
- * probability with which it was drawn (0 where T <= 0).  Settings per row
+ * exceeds uniform times their sum.  Which tokens are kept and which is drawn is
+ * decided as by sums in fp64.  T <= 0: the largest logit, the first of equal
+ * ones.  logprobs[r] (optional) = log of the probability with which it was drawn
+ * (0 where T <= 0): fp32, of a sum that may be one of fp32 weights where these
+ * decide, so off by up to 6e-7 absolute and fp32's rounding.  Settings per row
  * (fp32, top_k int32), or where the pointer is NULL the *_all for all rows;
  * off: top_k <= 0, top_p >= 1, min_p <= 0 (and NaN).  Logits of minus infinity
  * and NaN are hidden; with one of infinity, those alone are drawn from, alike.
- * A row that has nothing gives -1 and minus infinity.
+ * A row that has nothing gives -1, which is no index, and minus infinity.
  */
 #define QL_SAMPLE_MAX_VOCAB (1 << 21)
 typedef struct {

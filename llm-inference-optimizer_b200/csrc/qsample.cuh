@@ -32,7 +32,8 @@
 // A token is drawn, or not, by the comparison of two running sums, so these are
 // held to more than fp32.  Sums over many weights are first taken, in fp64, of
 // weights in fp32, which says how they compare unless they come closer than
-// 2^-19.6 of themselves; then the weights are taken again in fp64.
+// 2^-19.6 of themselves; then the weights are taken again in fp64.  The
+// log-probability is of the sum that decided, off by up to 6e-7 (kOff).
 //
 // What bounds it: for few rows the chain of passes and meetings of the cluster (a
 // meeting 0.5 us, each function's first run its way from memory: less code is

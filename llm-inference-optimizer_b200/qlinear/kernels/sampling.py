@@ -43,14 +43,18 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     * the first is always kept.
 
     The token is the first, by index, at which the running sum of the kept
-    weights exceeds uniform times their sum; sums are in fp64.  temperature 0
+    weights exceeds uniform times their sum; what is kept and which token it is
+    are decided as by sums in fp64.  temperature 0
     (and less) takes the largest logit, the first of equal ones.  Each setting
     is a number, or a tensor (rows,) of fp32 (top_k: int32).  Logits of minus
     infinity or NaN are never drawn; where some are infinite, only those are.
 
     Returns ids (rows,) int64, in ``out`` if given: -1 for a row with nothing to
-    draw.  With ``return_logprobs``, also the log of the probability with which
-    each was drawn, fp32 (0 at temperature 0, minus infinity for -1)."""
+    draw, which is no index of an embedding.  With ``return_logprobs``, also the
+    log of the probability with which each was drawn, fp32 (0 at temperature 0,
+    minus infinity for -1); its sum may be one of fp32 weights, so it is off by up
+    to 6e-7 absolute, beside fp32's rounding: more than the value itself where a
+    token is all but certain."""
     assert logits.is_cuda and logits.dim() == 2, f"logits must be a CUDA tensor (rows, vocab), got {tuple(logits.shape)}"
     code = _DTYPES.get(logits.dtype)
     if code is None:
