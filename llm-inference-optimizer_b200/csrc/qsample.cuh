@@ -250,6 +250,19 @@ struct Weights {
   }
 };
 
+// What a row's CTAs hold and send one another.  A meeting is a barrier of all of them (Row::meet); no store to another CTA
+// comes before all have started.  What keeps one use from the next:
+//   box    all_sum, all_u32, bound, locate, narrow send to a half, meet, read it; the other half is next (`turn`).
+//   part   written, __syncthreads, read; then the call's meeting, or in the first CTA's own steps (cta_count, finish) a
+//          __syncthreads before the next writing.  scan, sums alike.
+//   block  locate: each CTA its own, read by itself before and behind the call's meeting; a meeting follows each call.
+//   bins   narrow: each CTA adds to its own; a meeting; all read all CTAs' (twice); a meeting.
+//   few    collect: all CTAs store keys in the first one's; a meeting; then the first CTA alone (finish, last_kept), until the
+//          meeting behind that.
+// So whoever begins with one member of the union comes from a meeting behind which nobody touches another.
+//   found, here, at   collect: the CTA's own, here one for each call; its meeting follows.  count: added to by all CTAs, read
+//          behind that meeting, before the next one.
+//   edge, index, unsure, bin_*, mass_above, units_*   sent by one thread before a meeting, read behind it.
 struct Shared {
   // What the cluster's CTAs have sent, in turn: a meeting's values to one half, the next one's to the other.  A CTA writes a
   // half again only behind the meeting in between, at which all have read what it held.  Sums and counts share the halves, of
@@ -275,7 +288,7 @@ struct Shared {
   unsigned long long scan[kWarps], sums[kWarps][2];
   unsigned long long found[kFew];    // tokens that this CTA has collected
   unsigned here[3], at, count[3];    // their number, their place in the first CTA's list; the list's length
-  int owner, run, index, unsure;
+  int run, index, unsure;
   float edge;
   // where a histogram's running sum crosses a target: its bins just below and just above that, -1 for none; what lies above
   // the one and up to the other
