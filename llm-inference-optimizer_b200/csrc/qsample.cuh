@@ -37,13 +37,16 @@
 //
 // What bounds it: for few rows the chain of passes and meetings of the cluster (a
 // meeting 0.5 us, each function's first run its way from memory: less code is
-// quicker than unrolled code), for many the instructions of the weights (a dozen a
-// logit, ex2 at a quarter of the rate among them) and, of spread-out logits, the
-// few rows that want fp64: some 40 instructions a logit.  151936 logits, fp16,
-// device: one row, top-k 50 and top-p 0.95: 12.4 us; the largest: 4.1; 64 rows, the
-// same: 20 and 7.3; 256 rows of spread-out logits, all of them: 86 us (reading them:
-// 12), and 53 where the given numbers leave no row to fp64, which 7 in 100 want (64
-// rows: 38 and 18); 64 such rows under top-p alone, 50000 tokens kept: 103.
+// quicker than unrolled code).  For many it is waiting too: a row's passes follow
+// one another, first the largest logit and then the weights, a meeting behind each,
+// and 256 rows of two CTAs are 1.73 rounds of the SMs' places; the instructions (a
+// dozen a logit) take half of the issue slots.  Of spread-out logits 7 rows in 100
+// want fp64, some 40 instructions a logit, when most others are done.  151936
+// logits, fp16, device: one row, top-k 50 and top-p 0.95: 12.2 us; the largest: 4.1;
+// 64 rows, the same: 20 and 7.0; 256 rows of spread-out logits, all of them: 87 us
+// (reading them: 12; 28.7 M warp instructions: 25), and 52 where the given numbers
+// leave no row to fp64 (64 rows: 38 and 18); 64 such rows under top-p alone, 50000
+// tokens kept: 104.
 #pragma once
 
 #include <cuda_bf16.h>

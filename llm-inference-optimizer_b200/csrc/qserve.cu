@@ -88,6 +88,12 @@ int run_sample(const ql::smp::Params& p, bool few, int sms, void* stream, int64_
   //   all of them:            1 row  26 | 17 | 12 |  9 |  8     16 rows 62 | 37 | 25 | 18 | 18     64 rows 83 | 54 | 37 | 35 | 53
   //                         128 rows 97 | 62 | 56 | 61 |  98   256 rows 120 | 86 | 89 | 114 | 192
   //   top-p 0.9:              1 row 156 | 95 | 64 | 44 | 40     64 rows 224 | 143 | 104 | 124 | 226   256 rows 298 | 300 | 346 | 459 | 845
+  // fp32 and smaller vocabularies, as the rule has it | the best:
+  //   151936 fp32, top-p 0.9: 1 row 42 | 42   64 rows 116 | 116  128 rows 198 | 197  256 rows 350 | 350
+  //     all of them:                          64 rows  43 | 42   128 rows  72 | 61   256 rows 109 | 100
+  //    32003 fp16, top-p 0.9: 1 row 33 | 33   64 rows  48 | 48   128 rows  61 | 61   256 rows 110 | 85
+  //    32003 fp32, top-p 0.9: 1 row 34 | 31   64 rows  49 | 49   128 rows  64 | 64   256 rows 118 | 106
+  //     4099 fp16, top-p 0.9: 1 row 15 | 14   64 rows  37 | 37   128 rows  39 | 39   256 rows  55 | 44
   // Where all rows are known to keep few, one CTA is less to start and to meet:
   //   top-k 50, top-p 0.95: 128 rows 34 | 25 | 40     256 rows 39 | 48 | 75        the largest: 128 rows 15 | 12     256 rows 18 | 22
   auto room = [&](int ctas) { return ctas <= 2 ? (few ? 2 : 4) * sms : ctas <= 4 ? 2 * sms : ctas <= 8 ? sms : sms / 2; };

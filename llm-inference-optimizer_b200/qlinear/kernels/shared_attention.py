@@ -60,7 +60,8 @@ def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKVCache, prefix_tab
     * page_table int32 (batch, pages), kv_lens int32 (batch,): the requests' own
       positions behind the prefix, new tokens included; they begin a page;
     * cu_q, mask, max_q, scale: as in ``tree_attention``; the mask is over the
-      new tokens;
+      new tokens, and rows of q behind the last request's are left as they are
+      in the output (not written: pass ``out`` to say what they hold);
     * max_prefix, max_kv: the most positions of any prefix, and of any request's
       own, where the caller knows them; they only help to choose the launch.
 
