@@ -640,6 +640,11 @@ __device__ __forceinline__ double locate(const Row<T>& row, int& turn, float edg
     }
     return v;
   };
+  // what lies before a lane, of sums up to it: not those less its own, of which a weight of 1 leaves nothing below 2^-53
+  auto before_lane = [&](double to) {
+    const double b = __shfl_up_sync(0xffffffffu, to, 1);
+    return lane > 0 ? b : 0.0;
+  };
   double own = 0.0, upto = 0.0;
   if (warp == 0) {
     for (int i = 0; i < per_lane; ++i)
@@ -659,11 +664,12 @@ __device__ __forceinline__ double locate(const Row<T>& row, int& turn, float edg
   };
   const int owner = pick(part > 0.0, to > t);
   if (owner == row.rank) {
-    double before = __shfl_sync(0xffffffffu, to - part, owner);
+    double before = __shfl_sync(0xffffffffu, before_lane(to), owner);
     if (warp == 0) {
       const int at_lane = pick(own > 0.0, before + upto > t);
+      const double lanes = before_lane(upto);
       if (lane == at_lane) {
-        double run = before + (upto - own), kept = run;
+        double run = before + lanes, kept = run;
         int at = 0;
         for (int i = lane * per_lane; i < min((lane + 1) * per_lane, blocks); ++i) {
           const double w = sh.block[i];
@@ -693,8 +699,9 @@ __device__ __forceinline__ double locate(const Row<T>& row, int& turn, float edg
       }
       to = upto_lane(s);
       const int at_lane = pick(s > 0.0, before + to > t);
+      const double lanes = before_lane(to);
       if (lane == at_lane) {
-        double run = before + (to - s), from = run, until = run;
+        double run = before + lanes, from = run, until = run;
         float x_pick = x[0];
         int e_pick = 0;
         bool done = false;
