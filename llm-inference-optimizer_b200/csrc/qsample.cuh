@@ -874,15 +874,28 @@ __device__ __noinline__ void run_up(unsigned n) {
   if (i + 1 < n) sh.few.upto[i + 1] = before + s;
   __syncthreads();
 }
-// Weights of few tokens, as whole numbers: additions of these are exact and quick.  None but a zero becomes zero.
+// Weights of few tokens, as whole numbers: additions of these are exact and quick.  What is less than half a unit is nothing,
+// as beside 1 in fp64 (lifted to a unit it would be drawn where u falls between two tokens to the bit).
 constexpr double kWhole = 0x1p52;
-__device__ __noinline__ void weigh_few(unsigned n, int value_at = 32) {      // where keys have the value
-  for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-    const double w = sh.weights.wide(value_of((unsigned)(sh.few.key[i] >> value_at)));
-    const unsigned long long whole = __double2ull_rn(w * kWhole);
-    sh.few.weight[i] = whole == 0 && w > 0.0 ? 1 : whole;
-  }
+__device__ __forceinline__ unsigned long long whole(double w, double per) { return __double2ull_rn(fmin(w * per, kWhole)); }
+__device__ __noinline__ void weigh_few(unsigned n, int value_at = 32, double per = kWhole) {      // where keys have the value
+  for (unsigned i = threadIdx.x; i < n; i += kThreads)
+    sh.few.weight[i] = whole(sh.weights.wide(value_of((unsigned)(sh.few.key[i] >> value_at))), per);
   __syncthreads();
+}
+// How the token is drawn of the kept weights, whose sum is `total` units of 2^-52: in units of 1 / per, with t of them the
+// target.  From u = 2^-12 on they are the same units, whose rounding is 2^-31 of the target at most (half a unit of 1024
+// tokens).  Below, small weights come to matter: units so fine that the target is 2^51 of them, larger weights than it cut off
+// at 2^52.  At the ends each token that has a weight counts, however small: the first is drawn, or the last.
+struct Draw {
+  double per;
+  unsigned long long t;
+  bool same;
+};
+__device__ __forceinline__ Draw draw_of(double u, unsigned long long total) {
+  if (u >= 0x1p-12 && u < 1.0) return {kWhole, (unsigned long long)(u * (double)total), true};
+  if (u <= 0.0 || u >= 1.0) return {0x1p1023, u <= 0.0 ? 0ull : ~0ull, false};      // (weights end at e^-700)
+  return {0x1p103 / (u * (double)total), 1ull << 51, false};
 }
 
 struct Filters {
@@ -932,14 +945,21 @@ __device__ __noinline__ bool finish(unsigned n, const Filters& filters, double s
     const bool kept = i < n && (rank == 0 || (rank < most && less(before) && value_of((unsigned)(k >> 32)) >= filters.cut));
     if (mine) upto[i] = kept ? w : 0;
     if (__syncthreads_or(mine && rank > 0 && close(before))) return false;
-    const unsigned long long total = cta_sum(mine && kept ? w : 0), t = (unsigned long long)(u * (double)total);
+    const unsigned long long total = cta_sum(mine && kept ? w : 0);
+    const Draw draw = draw_of(u, total);
+    unsigned long long share = w;                             // in the draw's units
+    if (!draw.same) {
+      share = i < n ? whole(sh.weights.wide(value_of((unsigned)(k >> 32))), draw.per) : 0;
+      if (mine) upto[i] = kept ? share : 0;
+      __syncthreads();
+    }
     unsigned long long to = 0;
     #pragma unroll 4
     for (unsigned j = lane; j < n; j += step) to += (unsigned)key[j] >= (unsigned)k ? upto[j] : 0;     // ~index: those up to it
     to = over_step(to);
     // the first whose running sum passes t, else the last that has a weight
-    const unsigned at = kept && w > 0 ? (unsigned)index_of(k) : 0xFFFFFFFFu;
-    const unsigned past = __reduce_min_sync(0xffffffffu, to > t ? at : 0xFFFFFFFFu);
+    const unsigned at = kept && share > 0 ? (unsigned)index_of(k) : 0xFFFFFFFFu;
+    const unsigned past = __reduce_min_sync(0xffffffffu, to > draw.t ? at : 0xFFFFFFFFu);
     const unsigned end = __reduce_max_sync(0xffffffffu, at + 1);          // 0: none
     if ((tid & 31) == 0) {
       sh.part.u32[tid >> 5][0] = past;
@@ -968,14 +988,15 @@ __device__ __noinline__ bool finish(unsigned n, const Filters& filters, double s
   }
   if (__syncthreads_or(unsure)) return false;
   kept = cta_count(kept);
-  const unsigned long long total = upto[kept - 1], t = (unsigned long long)(u * (double)total);
+  const unsigned long long total = upto[kept - 1];
+  const Draw draw = draw_of(u, total);
   for (unsigned i = tid; i < kept; i += kThreads) key[i] = key[i] << 32 | key[i] >> 32;       // by index
   __syncthreads();
   sort(kept);
-  weigh_few(kept, 0);
+  weigh_few(kept, 0, draw.per);
   run_up(kept);
   unsigned before = 0;
-  for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= t;
+  for (unsigned i = 2 * tid; i < 2 * tid + 2 && i < kept; ++i) before += upto[i] <= draw.t;
   unsigned pick = cta_count(before);
   if (tid == 0) {
     if (pick >= kept) pick = kept - 1;
