@@ -893,7 +893,10 @@ struct Draw {
   bool same;
 };
 __device__ __forceinline__ Draw draw_of(double u, unsigned long long total) {
-  if (u >= 0x1p-12 && u < 1.0) return {kWhole, (unsigned long long)(u * (double)total), true};
+  if (u >= 0x1p-12 && u < 1.0) {     // u is fp32: whole in units of 2^-36; the product to its last bit, so that ties are ties
+    const unsigned long long m = (unsigned long long)(u * 0x1p36);
+    return {kWhole, __umul64hi(m, total) << 28 | m * total >> 36, true};
+  }
   if (u <= 0.0 || u >= 1.0) return {0x1p1023, u <= 0.0 ? 0ull : ~0ull, false};      // (weights end at e^-700)
   return {0x1p103 / (u * (double)total), 1ull << 51, false};
 }

@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from qlinear.kernels.sampling import sample_tokens
 from test_sampling import TYPES, agree, on_gpu
 
 COUNTS = [40, 128, 129, 700, 1024]         # one CTA compares up to 128 tokens, sorts up to 1024
@@ -97,3 +98,21 @@ def test_small_random_numbers_under_top_k(n):
         # every token left out is e^-200, beneath all sums here; shares are 2^-15 of the sum and more
         for f in (dict(top_k=n + 20 - len(set(out[0].tolist()))), dict(top_k=n, min_p=1e-40)):
             agree(x.cuda(), u.cuda(), **f)
+
+
+@on_gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 6, 40, 128, 130, 700, 1024])
+def test_exact_halves(dtype, n):
+    """The second half's tokens weigh what the first half's do: 1/2 of the sum is not exceeded by the first half, whatever
+    the weights are and however they are rounded; the next token is drawn."""
+    g = torch.Generator().manual_seed(n)
+    half = 3.0 * torch.randn(200, n // 2, generator=g)
+    other = half.gather(1, torch.rand(half.shape, generator=g).argsort(1))
+    x = torch.cat([half, other], 1).to(dtype).cuda()
+    uniform = torch.full((200,), 0.5, device="cuda")
+    more = torch.cat([x, torch.full_like(x[:, :1], -60000.0)], 1)
+    for logits, f in ((more, dict(top_k=n)), (x, dict(min_p=1e-12)), (more[:, :n], dict(top_p=1.0 - 2.0 ** -53))):
+        if logits.shape[1] > 1024:
+            continue
+        assert bool((sample_tokens(logits, uniform, **f) == n // 2).all()), f
