@@ -42,7 +42,7 @@
 // and 256 rows of two CTAs are 1.73 rounds of the SMs' places; the instructions (a
 // dozen a logit) take half of the issue slots.  Of spread-out logits 7 rows in 100
 // want fp64, some 40 instructions a logit, when most others are done.  151936
-// logits, fp16, device: one row, top-k 50 and top-p 0.95: 12.2 us; the largest: 4.1;
+// logits, fp16, device: one row, top-k 50 and top-p 0.95: 12.5 us; the largest: 4.1;
 // 64 rows, the same: 20 and 7.0; 256 rows of spread-out logits, all of them: 87 us
 // (reading them: 12; 28.7 M warp instructions: 25), and 52 where the given numbers
 // leave no row to fp64 (64 rows: 38 and 18); 64 such rows under top-p alone, 50000
